@@ -9,7 +9,7 @@
 
 Head layouts, widths and expert counts are the ones of the library's layer classes (16 query and 2 KV heads of 256; 256
 experts, 8 picked, 512 wide, model width 2048) and generic ones beside them. The cache: codes int8, keys
-[page, head, token, dim], values [page, head, token / 16, dim, 16], scales float32 [page, head].
+[page, head, token, dim], values [page, head, token / 8, dim, 8], scales float32 [page, head].
 """
 
 from __future__ import annotations
@@ -207,7 +207,7 @@ def _filled_cache(r, pages, heads, dim, page):
         x /= s.view(shape[0], shape[1], *([1] * (len(shape) - 2)))
         return x.round_().to(torch.int8), s
     k, ks = codes((pages, heads, page, dim), (2, 3))
-    v, vs = codes((pages, heads, page // 16, dim, 16), (2, 3, 4))
+    v, vs = codes((pages, heads, page // 8, dim, 8), (2, 3, 4))
     return {"k": k, "v": v, "ks": ks, "vs": vs}
 
 
@@ -262,9 +262,10 @@ def _plan_plain(s):
     c, n = s["cached"].long(), s["fresh"].long()
     start = torch.cat([torch.zeros(1, dtype=torch.int64, device=DEV), n.cumsum(0)])
     first = (c + page - 1) // page
-    need = torch.where(n > 0, (c + n + page - 1) // page - first, torch.zeros_like(n))
+    room = (c + n <= page * table.shape[1]) & (start[1:] <= s["rows"])
+    need = torch.where((n > 0) & room, (c + n + page - 1) // page - first, torch.zeros_like(n))
     upto = need.cumsum(0)
-    fits = (upto <= s["free"].numel() - head) & (c + n <= page * table.shape[1])
+    fits = room & ((need == 0) | (upto <= s["free"].numel() - head))
     j = torch.arange(table.shape[1], device=DEV)
     fresh_page = fits[:, None] & (j >= first[:, None]) & (j < (first + need)[:, None])
     take = (head + (upto - need)[:, None] + j - first[:, None]).clamp(0, s["free"].numel() - 1)
@@ -276,7 +277,7 @@ def _plan_plain(s):
     slot = table[b, (pos // page).clamp(max=table.shape[1] - 1)].long() * page + pos % page
     slot = torch.where(real & fits[b], slot, torch.full_like(slot, -1))
     kv_len = torch.where(fits, c + n, torch.zeros_like(c))
-    used = head + torch.where(fits, upto, torch.zeros_like(upto)).amax()
+    used = head + torch.where(fits & (need > 0), upto, torch.zeros_like(upto)).amax()
     return {"table": table, "start": start.to(I32), "len": kv_len.to(I32), "slots": slot.to(I32), "pos": pos.to(I32),
             "head": used.to(I32)}
 
@@ -300,8 +301,8 @@ def _store_one(codes, scales, x, slots, page):
 
 
 def _values_by_token(v):
-    """[page, head, token / 16, dim, 16] -> [page, head, token, dim]."""
-    return v.transpose(3, 4).reshape(v.shape[0], v.shape[1], v.shape[2] * 16, v.shape[3])
+    """[page, head, token / 8, dim, 8] -> [page, head, token, dim]."""
+    return v.transpose(3, 4).reshape(v.shape[0], v.shape[1], v.shape[2] * 8, v.shape[3])
 
 
 def _store_plain(s):
@@ -309,7 +310,7 @@ def _store_plain(s):
     v = _values_by_token(s["v"]).clone(memory_format=torch.contiguous_format)
     _store_one(s["k"], s["ks"], s["new_k"], s["slots"], page)
     _store_one(v, s["vs"], s["new_v"], s["slots"], page)
-    s["v"].copy_(v.view(v.shape[0], v.shape[1], page // 16, 16, v.shape[3]).transpose(3, 4))
+    s["v"].copy_(v.view(v.shape[0], v.shape[1], page // 8, 8, v.shape[3]).transpose(3, 4))
     pid, off = s["read"].long() // page, s["read"].long() % page
     return {"k": s["k"][pid, :, off].float() * s["ks"][pid][:, :, None],
             "v": v[pid, :, off].float() * s["vs"][pid][:, :, None], "k_scale": s["ks"], "v_scale": s["vs"]}
@@ -444,12 +445,13 @@ def _exact_plan(s):
     start, lens, slots, pos, wanted, used = [0], [], [], [], head, head
     for b, (c, n) in enumerate(zip(cached, fresh)):
         have = -(-c // page)
-        need = -(-(c + n) // page) - have if n else 0
+        room = c + n <= page * len(table[b]) and start[-1] + n <= s["rows"]
+        need = -(-(c + n) // page) - have if n and room else 0
         wanted += need
-        good = wanted <= len(free) and c + n <= page * len(table[b])
-        if good:
+        good = room and (need == 0 or wanted <= len(free))
+        if good and need:
             table[b][have:have + need] = free[wanted - need:wanted]
-            used = max(used, wanted)
+            used = wanted
         lens.append(c + n if good else 0)
         start.append(start[-1] + n)
         for t in range(c, c + n):
@@ -496,7 +498,7 @@ def _exact_attn(s):
         for h in range(s["q_heads"]):
             g = h // group
             k = s["k"][pid, g, off].double() * s["ks"][pid, g].double()[:, None]
-            v = s["v"][pid, g, off // 16, :, off % 16].double() * s["vs"][pid, g].double()[:, None]
+            v = s["v"][pid, g, off // 8, :, off % 8].double() * s["vs"][pid, g].double()[:, None]
             score = (q[:, h] @ k.T / math.sqrt(dim)).masked_fill(hidden, -math.inf)
             o[:, h] = torch.softmax(score, dim=1) @ v
         outs.append(o)
