@@ -317,6 +317,66 @@ int qwen_attn_decode_noalloc(const float* q, const float* k_cache, const float* 
                              const float* gate, float* out, int heads, int kv_heads, int dim,
                              int pos, void* stream);
 
+/* ====================================================================== several requests: a paged 8-bit KV cache
+ * One step of a batch of requests, prompts and single tokens mixed. The reference serves one sequence from a contiguous
+ * fp32 cache (src/layer_attn.cpp:44-46, 99-105); these entry points have no counterpart there.
+ *
+ * The cache is `pages` pages of page_size tokens (a power of two from 8 to 1024), caller-owned device arrays:
+ *   k_codes int8 [pages][kv_heads][page_size][dim], v_codes int8 [pages][kv_heads][page_size / 8][dim][8] (16-byte
+ *   aligned), k_scale, v_scale float [pages][kv_heads]; a value is code * scale. dim is 64, 128 or 256.
+ * A token's slot is page * page_size + its index in the page; pages * page_size < 2^31. A request's block table row
+ * holds the ids of its pages, token t in page t / page_size. Ids and slots are device data: one outside the cache is
+ * never followed (see the calls for what it gives). requests <= 4096. */
+
+/* The bookkeeping of a step: pages for the fresh tokens, and where every row of the step goes. For request b with
+ * cached[b] tokens in the cache and fresh[b] new ones (0: idle; negative counts are taken as 0):
+ *   row_start [requests + 1]  prefix sums of fresh: its rows are row_start[b] .. row_start[b + 1] - 1
+ *   block_table [requests x max_pages], in place: the ids of the pages it needs beyond its ceil(cached / page_size) ones,
+ *     taken from free_pages [n_free] in request order from index free_head[0] on; free_head_out[0] = the next index
+ *     (may be free_head itself: the call then runs as one workgroup)
+ *   kv_len [requests]         cached + fresh
+ *   slots [rows], pos [rows]  slot and position of each row; -1 and 0 behind the last request's rows
+ * A request is not granted its step if the free pages do not reach for it (then no later request that needs a page is
+ * either), its tokens exceed the table row, or its rows exceed `rows`: it takes no page, its kv_len is 0 and its
+ * slots are -1 (pos is still written). max_pages * page_size < 2^31. */
+int qwen_kv8_plan(const int32_t* cached, const int32_t* fresh, int requests, int32_t* block_table, int max_pages,
+                  const int32_t* free_pages, int n_free, const int32_t* free_head, int32_t* free_head_out,
+                  int page_size, int rows, int32_t* row_start, int32_t* kv_len, int32_t* slots, int32_t* pos,
+                  void* stream);
+
+/* Rows of keys and values, [rows] x [kv_heads x dim] with row strides k_stride, v_stride (elements), quantized into the
+ * slots. Rows whose slot is negative or past the cache are skipped. Neighbouring rows with neighbouring slots of a page
+ * are one run; a call holds at most one run of a page (what a second one would leave in that page is not defined). For
+ * each run, page and head:
+ *   scale' = max(scale, RN(max |x| / 127), 2^-100), the old scale counting as 0 if the run starts at the page's first
+ *   token; codes of tokens before the run become rne(code * RN(scale / scale')), the run's codes are rne(x / scale');
+ *   codes behind the run are not defined.
+ * An infinity or NaN makes the scale of its page and head NaN (every later read of them is NaN) until the page is begun
+ * again. */
+int qwen_kv8_store_rows(const float* k, const float* v, int64_t k_stride, int64_t v_stride, const int32_t* slots,
+                        int rows, int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale, int pages,
+                        int page_size, int kv_heads, int dim, void* stream);
+
+/* Slots back as fp32 rows k, v [rows x kv_heads x dim] (16-byte aligned): zeros for a negative slot, NaN for one past
+ * the cache. */
+int qwen_kv8_read_rows(const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                       int pages, int page_size, int kv_heads, int dim, const int32_t* slots, int rows, float* k,
+                       float* v, void* stream);
+
+/* Attention of the step's rows: q, out [rows x heads x dim], gate like out or NULL. Row i of request b's n rows stands at
+ * position p = kv_len[b] - n + i and sees keys 0 .. p:
+ *   out = sum_t softmax_t(q . k_t / sqrt(dim)) v_t  (* sigmoid(gate)), fp32 accuracy over the codes' exact values.
+ * Zeros where p < 0; a page id outside the cache, or a table row too short, makes the rows that see it NaN. Rows behind
+ * row_start[requests] are left as they were. heads a multiple of kv_heads, rows * heads <= 2^24; out must not overlap
+ * q. workspace: device memory, 16-byte aligned, of at least qwen_attn_kv8_workspace_bytes() bytes, for one call at a
+ * time; nothing in it is kept between calls. */
+size_t qwen_attn_kv8_workspace_bytes(int rows, int requests, int heads, int kv_heads, int dim);
+int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
+                       const float* v_scale, int pages, int page_size, const int32_t* block_table, int max_pages,
+                       const int32_t* row_start, const int32_t* kv_len, int requests, const float* gate, float* out,
+                       int rows, int heads, int kv_heads, int dim, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 /* ====================================================================== MoE routing
  * The reference picks experts on the device, copies them to the host and syncs
  * (src/layer_moe.cpp:98-106); these entry points keep the routing on the device. */

@@ -1,0 +1,768 @@
+// Attention over the paged 8-bit cache (kv8_common.hpp) on gfx950: the rows of several requests in one call, single
+// tokens and prompts mixed. Row i of a request with n rows and kv_len keys stands at position kv_len - n + i and sees
+// keys 0 .. position:
+//   out = sum_t softmax_t(q . k_t / sqrt(D)) v_t  (x sigmoid(gate)),  zeros where no key is seen.
+// The reference has the one-token form over an fp32 cache (src/cuda/attn_kernels.cu:72-195, src/layer_attn.cpp:103-108).
+//
+// Both products run on v_mfma_f32_16x16x32_f16 with an fp32 dot product's accuracy: a code is exact in fp16, and the
+// other operand (a query row scaled by a power of two; the softmax weights) is two fp16 parts, 22 bits. Both are
+// computed transposed, scores^T = K q^T and out^T = V^T p^T, because then the scores that a lane holds (4 tokens of one
+// row in each tile) are already the p^T operand of the second product: with key row lr of tile `half` standing for token
+// 8 (lr / 4) + 4 half + lr % 4, lane group lk holds tokens 8 lk .. 8 lk + 7, whose value codes of one dim are 8
+// neighbouring bytes of the cache. Nothing crosses lanes or LDS between the products.
+//
+// Scales: score = S * (2^-e / sqrt(D) log2(e) * k_scale); the value scale rides on the weights, w = p * v_scale, so that
+// tokens of pages with different scales share one accumulator. The running reference m of the exponentials therefore
+// bounds score + log2(v_scale); it moves, and the sums are rescaled, only when a score passes it by 8 (weights up to
+// 2^8 are as exact as weights up to 1).
+//
+// Two kernels. split_kernel (few rows per request): bound by the cache's bytes. A workgroup takes 8 (row, head) pairs
+// that share a KV head - 16 columns: 8 rows x 2 fp16 parts - and a range of 32-token tiles, its 4 waves every fourth tile,
+// straight from the cache to operand registers. The ranges are cut so that the whole call, ragged requests and all, is
+// about kTargetItems equal pieces; every workgroup works that out from the lengths, so nothing is planned on the host.
+// combine_kernel joins the pieces. prompt_kernel (many rows): bound by the MFMAs. 128 rows per workgroup, both parts of
+// a row in its column, the codes turned to fp16 once per workgroup into LDS.
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "capi_common.hpp"
+#include "device_common.hpp"
+#include "kv8_common.hpp"
+
+namespace qk {
+namespace {
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kTile = 32;              // tokens of a step
+constexpr int kSplitWaves = 4;
+constexpr int kSplitBlock = kSplitWaves * kWave;
+constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
+constexpr int kTargetItems = 1024;     // pieces of the whole call
+constexpr int kMinTiles = 8;           // of a piece: two steps per wave
+constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take the split kernel
+constexpr int kPromptWaves = 8;
+constexpr int kPromptRows = 16 * kPromptWaves;
+constexpr float kMoves = 8.0f;         // a score past the reference by more moves it
+constexpr float kWeightUp = 64.0f;     // weights (up to 2^8) enter fp16 times 2^6
+
+struct AttnArgs {
+    const float* q;
+    const float* gate;   // or null
+    float* out;
+    Kv8Cache c;
+    const int32_t* table;
+    const int32_t* row_start;
+    const int32_t* kv_len;
+    int max_pages, page_shift, requests, rows, heads, group;
+    int split_all;       // every request takes the split kernel
+    float* part;         // [item][kRows][D] sums
+    float2* stat;        // [item][kRows] (m, l)
+    int2* info;          // [row][head] (first item * kRows + row in item, pieces)
+    int items;           // capacity: the split kernel's grid
+    float scale;         // log2(e) / sqrt(D)
+};
+
+// A request as the kernels see it, whatever the arrays hold: rows inside q, lengths from 0 to what the table row holds
+// (`bad` marks a longer one, whose rows come out NaN).
+struct Request {
+    int first, n, len;
+    bool bad;
+};
+__device__ __forceinline__ Request request(const AttnArgs& a, int b) {
+    const int s = min(max(a.row_start[b], 0), a.rows), e = min(max(a.row_start[b + 1], s), a.rows);
+    const int len = a.kv_len[b], most = a.max_pages << a.page_shift;
+    return Request{s, e - s, min(max(len, 0), most), len > most};
+}
+__device__ __forceinline__ bool takes_split(const AttnArgs& a, const Request& r) {
+    return a.split_all || static_cast<int64_t>(r.n) * a.group <= kSplitMax;
+}
+
+// Inclusive prefix over the wave.
+__device__ __forceinline__ int64_t wave_prefix(int64_t v, int lane) {
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int64_t up = __shfl_up(v, o);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+
+// Piece `item` of the call: request, which of its units (KV head, row block), which piece of the unit's tiles. Every wave
+// finds it by itself from the lengths (64 requests at a time).
+struct Piece {
+    int b, unit, split, splits, tiles;   // tiles: of one piece
+};
+__device__ __forceinline__ int tiles_of(const Request& r) { return max(1, (r.len + kTile - 1) / kTile); }
+__device__ __forceinline__ int64_t units_of(const AttnArgs& a, const Request& r) {
+    return takes_split(a, r) ? (static_cast<int64_t>(r.n) * a.group + kRows - 1) / kRows * a.c.heads : 0;
+}
+__device__ bool find_piece(const AttnArgs& a, int64_t item, Piece& p) {
+    const int lane = threadIdx.x & 63;
+    int64_t total = 0;
+    for (int b = lane; b < a.requests; b += kWave) {
+        const Request r = request(a, b);
+        total += units_of(a, r) * tiles_of(r);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
+    const int64_t cut = max(static_cast<int64_t>(kMinTiles), (total + kTargetItems - 1) / kTargetItems);
+    p.tiles = static_cast<int>(min(cut, static_cast<int64_t>(0x7fffffff)));
+    for (int b0 = 0; b0 < a.requests; b0 += kWave) {
+        const int b = b0 + lane;
+        int64_t n = 0;
+        int splits = 0;
+        if (b < a.requests) {
+            const Request r = request(a, b);
+            splits = static_cast<int>((tiles_of(r) + cut - 1) / cut);
+            n = units_of(a, r) * splits;
+        }
+        const int64_t upto = wave_prefix(n, lane);
+        const uint64_t hit = __ballot(item < upto);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            const int64_t local = item - (__shfl(upto, l) - __shfl(n, l));
+            p.b = __builtin_amdgcn_readfirstlane(b0 + l);
+            p.splits = __builtin_amdgcn_readfirstlane(__shfl(splits, l));
+            p.unit = __builtin_amdgcn_readfirstlane(static_cast<int>(local / p.splits));
+            p.split = __builtin_amdgcn_readfirstlane(static_cast<int>(local - static_cast<int64_t>(p.unit) * p.splits));
+            return true;
+        }
+        item -= __shfl(upto, 63);
+    }
+    return false;
+}
+
+// 8 codes -> the fp16 operand: byte u = code + 128 under 0x64 is the fp16 1024 + u.
+__device__ __forceinline__ f16x8_t codes8(uint32_t a, uint32_t b) {
+    const uint32_t x[2] = {a ^ 0x80808080u, b ^ 0x80808080u};
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        w[2 * i] = __builtin_amdgcn_perm(0x64646464u, x[i], 0x04010400u);
+        w[2 * i + 1] = __builtin_amdgcn_perm(0x64646464u, x[i], 0x04030402u);
+    }
+    f16x8_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, w[i]) - f16x2_t{(_Float16)1152.0f, (_Float16)1152.0f};
+        r[2 * i] = h[0];
+        r[2 * i + 1] = h[1];
+    }
+    return r;
+}
+
+__device__ __forceinline__ float max_over_lk(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+
+// A lane's 16 (D / 64) elements of query row `row` (dims 64 j + 16 lk ..), scaled by 2^e so that the row's largest
+// magnitude is in [2^14, 2^15). Returns the factor from products to log2 scores; NaN for a row with infinities or NaNs.
+template <int D>
+__device__ __forceinline__ float load_query(const float* __restrict__ row, int lk, float scale, float (&f)[D / 4]) {
+    float m = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float v = row[64 * j + 16 * lk + i];
+            f[16 * j + i] = v;
+            m = fmaxf(m, fabsf(v));
+            bad |= !(fabsf(v) <= FLT_MAX);
+        }
+    m = max_over_lk(bad ? INFINITY : m);
+    int e = 0;
+    if (m > 0.f && m <= FLT_MAX) {
+        int em;
+        frexpf(m, &em);
+        e = 15 - em;
+    }
+    const bool ok = m <= FLT_MAX;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) f[i] = ok ? ldexpf(f[i], e) : 0.f;
+    return ok ? ldexpf(scale, -e) : __builtin_nanf("");
+}
+
+// The fp32 product behind a value that is then split in two fp16 parts: kept from being fused into the conversion
+// (v_fma_mixlo_f16 rounds once where the other part's subtraction has rounded twice, and the parts miss by an fp16 ulp
+// of one weight in some thousands).
+__device__ __forceinline__ float rounded(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+__device__ __forceinline__ float low_part(float v) { return v - static_cast<float>(static_cast<_Float16>(v)); }
+
+// Where the octet of tokens that starts at token t lies: the page's first code (of one head) and the two scales. Tokens
+// from `seen` on are not looked up (page 0, scales 0: their weights are 0); a page id outside the cache has scale NaN.
+struct Octet {
+    size_t base;   // (page, head) index
+    bool live, bad;
+};
+__device__ __forceinline__ Octet octet(const AttnArgs& a, int b, int h, int t, int seen) {
+    Octet o{static_cast<size_t>(h), t < seen, false};
+    if (!o.live) return o;
+    const int j = t >> a.page_shift;
+    const int id = j < a.max_pages ? a.table[static_cast<size_t>(b) * a.max_pages + j] : -1;
+    o.bad = id < 0 || id >= a.c.pages;
+    if (!o.bad) o.base = static_cast<size_t>(id) * a.c.heads + h;
+    return o;
+}
+
+// ------------------------------------------------------------------ few rows
+template <int D>
+__global__ __launch_bounds__(kSplitBlock, 2) void split_kernel(const AttnArgs a) {
+    constexpr int NJ = D / 64, ND = D / 32, LD = D + 2;
+    __shared__ float sums[kSplitWaves][kRows * LD];
+    __shared__ float stat[kSplitWaves][kRows][2];
+    Piece pc;
+    if (!find_piece(a, blockIdx.x, pc)) return;   // the whole workgroup
+    const Request r = request(a, pc.b);
+    const int G = a.group, pairs = r.n * G;
+    const int blocks = (pairs + kRows - 1) / kRows;
+    const int h = pc.unit / blocks, rb = pc.unit - h * blocks;
+    const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4, part = lr & 1;
+    const int wv = wave_in_block();
+    const int rr = min(rb * kRows + (lr >> 1), pairs - 1);   // columns past the last pair repeat it
+    const int ti = rr / G, head = h * G + (rr - ti * G);
+    const int limit = r.len - r.n + ti;                      // this column's last key
+    const int first_limit = r.len - r.n + rb * kRows / G;    // the smallest of the workgroup
+    const int seen = max(r.len - r.n + min(rb * kRows + kRows - 1, pairs - 1) / G + 1, 0);   // keys that some column sees
+    const int t_end = min((pc.split + 1) * pc.tiles, (seen + kTile - 1) / kTile);
+    int t = pc.split * pc.tiles + wv;
+    const int P = a.c.page;
+    const size_t block = static_cast<size_t>(P) * D;
+
+    struct Where {
+        const int8_t* k;
+        const int8_t* v;
+        const float* ks;
+        const float* vs;
+        bool live, bad;
+    };
+    auto where = [&](int tile) {   // this lane's addresses: key rows of octet lr / 4, values and scales of octet lk
+        const int t0 = tile * kTile;
+        const int tk = t0 + 8 * (lr >> 2), tv = t0 + 8 * lk;
+        const Octet ok = octet(a, pc.b, h, tk, seen), ov = octet(a, pc.b, h, tv, seen);
+        Where w;
+        w.k = a.c.k + ok.base * block + static_cast<size_t>((tk & (P - 1)) + (lr & 3)) * D + 16 * lk;
+        w.v = a.c.v + ov.base * block + (static_cast<size_t>((tv & (P - 1)) >> 3) * D + 2 * lr) * 8;
+        w.ks = a.c.ks + ov.base;
+        w.vs = a.c.vs + ov.base;
+        w.live = ov.live;
+        w.bad = ov.bad;
+        return w;
+    };
+    uint4 K[2][NJ], V[ND];
+    float ksc, vsc;
+    auto load_k = [&](const Where& w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) K[half][j] = ld16(w.k + 4 * half * D + 64 * j);
+    };
+    auto load_v = [&](const Where& w) {
+#pragma unroll
+        for (int m = 0; m < ND; ++m) V[m] = ld16(w.v + 32 * 8 * m);
+        ksc = *w.ks;
+        vsc = *w.vs;
+        if (!w.live) ksc = vsc = 0.f;
+        if (w.bad) ksc = __builtin_nanf("");
+    };
+    const bool any = t < t_end;
+    Where next{};
+    if (any) {
+        const Where w = where(t);
+        load_k(w);
+        load_v(w);
+        if (t + kSplitWaves < t_end) next = where(t + kSplitWaves);
+    }
+    f16x8_t Q[2 * NJ];
+    float factor;
+    {
+        float f[D / 4];
+        factor = load_query<D>(a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D, lk, a.scale, f);
+#pragma unroll
+        for (int d = 0; d < 2 * NJ; ++d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = f[8 * d + i];
+                Q[d][i] = static_cast<_Float16>(part ? low_part(v) : v);
+            }
+    }
+    f32x4_t acc[ND][2];
+#pragma unroll
+    for (int m = 0; m < ND; ++m) acc[m][0] = acc[m][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float mu = -FLT_MAX, l = 0.f;
+    for (; t < t_end; t += kSplitWaves) {
+        const bool more = t + kSplitWaves < t_end;
+        f32x4_t S[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            S[half] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const uint4 w = K[half][j];
+                S[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(w.x, w.y), Q[2 * j], S[half], 0, 0, 0);
+                S[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(w.z, w.w), Q[2 * j + 1], S[half], 0, 0, 0);
+            }
+        }
+        if (more) load_k(next);
+        const float f = factor * ksc;
+        float sv = vsc;
+        float s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = S[i >> 2][i & 3];
+            s[i] = (v + dpp_move<0xB1>(v)) * f;   // both fp16 parts of the query
+        }
+        if (t * kTile + kTile - 1 > first_limit) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (t * kTile + 8 * lk + i > limit) s[i] = -INFINITY;
+            if (t * kTile + 8 * lk > limit) sv = 0.f;   // a page that the row does not see may be marked: no 0 * NaN
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
+        top += __builtin_amdgcn_logf(fmaxf(sv, kKv8Floor));   // log2
+        if (__ballot(top > mu + kMoves)) {
+            const float now = fmaxf(mu, max_over_lk(top));
+            const float shrink = __builtin_amdgcn_exp2f(mu - now);
+            mu = now;
+            l *= shrink;
+#pragma unroll
+            for (int m = 0; m < ND; ++m)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[m][e][i] *= shrink;
+        }
+        f16x8_t W;
+        const float up = sv * kWeightUp;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p = __builtin_amdgcn_exp2f(s[i] - mu);
+            l += p;
+            const float w = rounded(p * up);
+            W[i] = static_cast<_Float16>(part ? low_part(w) : w);
+        }
+#pragma unroll
+        for (int m = 0; m < ND; ++m) {
+            const uint4 w = V[m];
+            acc[m][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(w.x, w.y), W, acc[m][0], 0, 0, 0);
+            acc[m][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(w.z, w.w), W, acc[m][1], 0, 0, 0);
+        }
+        if (more) {
+            load_v(next);
+            if (t + 2 * kSplitWaves < t_end) next = where(t + 2 * kSplitWaves);
+        }
+    }
+    // The waves' sums meet in LDS; the two parts of a row are neighbouring columns, each lane of a pair writes every
+    // other dim of both.
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    float* mine = sums[wv] + (lr >> 1) * LD;
+#pragma unroll
+    for (int m = 0; m < ND; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float e0 = acc[m][0][i] + dpp_move<0xB1>(acc[m][0][i]);
+            const float e1 = acc[m][1][i] + dpp_move<0xB1>(acc[m][1][i]);
+            mine[32 * m + 8 * lk + 2 * i + part] = part ? e1 : e0;
+        }
+    if (lane < 16 && part == 0) {
+        stat[wv][lr >> 1][0] = mu;
+        stat[wv][lr >> 1][1] = l;
+    }
+    __syncthreads();
+    const int rows = min(kRows, pairs - rb * kRows);
+    for (int i = threadIdx.x; i < rows * D; i += kSplitBlock) {
+        const int row = i / D, d = i - row * D;
+        float m = stat[0][row][0];
+#pragma unroll
+        for (int w = 1; w < kSplitWaves; ++w) m = fmaxf(m, stat[w][row][0]);
+        float sum = 0.f, tot = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSplitWaves; ++w) {
+            const float k = __builtin_amdgcn_exp2f(stat[w][row][0] - m);
+            sum += k * sums[w][row * LD + d];
+            tot += k * stat[w][row][1];
+        }
+        if (r.bad) tot = __builtin_nanf("");
+        const int at = rb * kRows + row, tok = at / G;
+        const size_t o = (static_cast<size_t>(r.first + tok) * a.heads + h * G + (at - tok * G)) * D + d;
+        if (pc.splits == 1) {
+            float v = tot == 0.f ? 0.f : sum / kWeightUp / tot;
+            if (a.gate) v *= sigmoid(a.gate[o]);
+            a.out[o] = v;
+        } else {
+            a.part[(static_cast<size_t>(blockIdx.x) * kRows + row) * D + d] = sum;
+            if (d == 0) a.stat[static_cast<size_t>(blockIdx.x) * kRows + row] = make_float2(m, tot);
+        }
+        if (d == 0 && pc.split == 0) a.info[o / D] = make_int2(static_cast<int>(blockIdx.x) * kRows + row, pc.splits);
+    }
+}
+
+// ------------------------------------------------------------------ join
+// One workgroup of NW waves per (row, head): wave w takes pieces w, w + NW, ...; lanes the dims.
+template <int D, int NW>
+__global__ __launch_bounds__(NW * kWave) void combine_kernel(const AttnArgs a) {
+    constexpr int V = D / kWave;
+    __shared__ float sums[NW][D], ls[NW], ms[NW];
+    const int row = static_cast<int>(blockIdx.x) / a.heads;
+    if (row >= a.row_start[a.requests]) return;   // behind the last request
+    const int2 in = a.info[blockIdx.x];
+    const int pieces = in.y, slot = in.x % kRows, first = in.x / kRows;
+    if (pieces <= 1 || in.x < 0 || pieces > a.items - first) return;
+    const int wv = wave_in_block(), lane = threadIdx.x & 63;
+    float m = -FLT_MAX, l = 0.f, s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = 0.f;
+    auto at = [&](int p) { return static_cast<size_t>(first + p) * kRows + slot; };
+    constexpr int U = 4;   // pieces in flight
+    for (int p0 = wv; p0 < pieces; p0 += U * NW) {
+        float2 st[U];
+        float x[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t k = at(min(p0 + u * NW, pieces - 1));
+            st[u] = a.stat[k];
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[u][i] = a.part[k * D + V * lane + i];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (p0 + u * NW >= pieces) break;
+            const float now = fmaxf(m, st[u].x);
+            const float was = __builtin_amdgcn_exp2f(m - now), k = __builtin_amdgcn_exp2f(st[u].x - now);
+            m = now;
+            l = l * was + st[u].y * k;
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * k;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
+    if (lane == 0) {
+        ms[wv] = m;
+        ls[wv] = l;
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += NW * kWave) {
+        float top = ms[0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, ms[w]);
+        float sum = 0.f, tot = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float k = __builtin_amdgcn_exp2f(ms[w] - top);
+            sum += k * sums[w][d];
+            tot += k * ls[w];
+        }
+        const size_t o = static_cast<size_t>(blockIdx.x) * D + d;
+        float v = tot == 0.f ? 0.f : sum / kWeightUp / tot;
+        if (a.gate) v *= sigmoid(a.gate[o]);
+        a.out[o] = v;
+    }
+}
+
+// ------------------------------------------------------------------ many rows
+template <int D>
+__global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const AttnArgs a) {
+    constexpr int NJ = D / 64, ND = D / 32, NT = D == 64 ? 128 : 64, NTH = kPromptWaves * kWave;
+    constexpr int UK = NT * (D / 16) / NTH;   // 16-byte pieces of keys (and of values) per thread and step
+    static_assert(UK >= 1 && NT * (D / 16) % NTH == 0, "shape");
+    // fp16 operands in the order in which a wave reads them: [16-token tile or 32-token group][depth or dim tile][lane]
+    __shared__ __align__(16) f16x8_t ks[2][NT / 16][2 * NJ][kWave];
+    __shared__ __align__(16) f16x8_t vs[2][NT / 32][2 * ND][kWave];
+    __shared__ float scl[2][2][NT / 8];   // [slot][key, value][octet]
+    // which request, KV head and row tile: the last row tiles (the longest rows) first
+    const int G = a.group, lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4;
+    int b = -1;
+    int64_t item = blockIdx.x;
+    for (int b0 = 0; b0 < a.requests && b < 0; b0 += kWave) {
+        int64_t n = 0;
+        if (b0 + lane < a.requests) {
+            const Request r = request(a, b0 + lane);
+            if (!takes_split(a, r)) n = (static_cast<int64_t>(r.n) * G + kPromptRows - 1) / kPromptRows * a.c.heads;
+        }
+        const int64_t upto = wave_prefix(n, lane);
+        const uint64_t hit = __ballot(item < upto);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            item -= __shfl(upto, l) - __shfl(n, l);
+            b = __builtin_amdgcn_readfirstlane(b0 + l);
+        } else {
+            item -= __shfl(upto, 63);
+        }
+    }
+    if (b < 0) return;   // the whole workgroup
+    const Request r = request(a, b);
+    const int pairs = r.n * G, tiles = (pairs + kPromptRows - 1) / kPromptRows;
+    const int unit = __builtin_amdgcn_readfirstlane(static_cast<int>(item));
+    const int h = unit % a.c.heads, rt = tiles - 1 - unit / a.c.heads;
+    const int wv = wave_in_block(), tid = threadIdx.x;
+    const int mine = rt * kPromptRows + 16 * wv + lr;
+    const int rr = min(mine, pairs - 1);
+    const int ti = rr / G, head = h * G + (rr - ti * G);
+    const int limit = r.len - r.n + ti;
+    const int wave_first = r.len - r.n + min(rt * kPromptRows + 16 * wv, pairs - 1) / G;
+    const int wave_seen = r.len - r.n + min(rt * kPromptRows + 16 * wv + 15, pairs - 1) / G + 1;
+    const int seen = max(r.len - r.n + min(rt * kPromptRows + kPromptRows - 1, pairs - 1) / G + 1, 0);
+    const int steps = (seen + NT - 1) / NT;
+    const int P = a.c.page;
+    const size_t block = static_cast<size_t>(P) * D;
+
+    uint4 kr[UK], vr[UK];
+    float sr = 0.f;
+    auto load = [&](int st) {
+        const int t0 = st * NT;
+#pragma unroll
+        for (int i = 0; i < UK; ++i) {
+            const int u = tid + i * NTH;
+            const int tok = u / (D / 16), ch = u % (D / 16);          // keys: token, 16-dim piece
+            const Octet o = octet(a, b, h, (t0 + tok) & ~7, seen);
+            kr[i] = ld16(a.c.k + o.base * block + static_cast<size_t>((t0 + tok) & (P - 1)) * D + 16 * ch);
+            const int oc = u / (D / 2), dp = u % (D / 2);             // values: octet, pair of dims
+            const Octet ov = octet(a, b, h, t0 + 8 * oc, seen);
+            vr[i] = ld16(a.c.v + ov.base * block + (static_cast<size_t>(((t0 + 8 * oc) & (P - 1)) >> 3) * D + 2 * dp) * 8);
+        }
+        if (tid < 2 * (NT / 8)) {
+            const Octet o = octet(a, b, h, t0 + 8 * (tid % (NT / 8)), seen);
+            sr = (tid < NT / 8 ? a.c.ks : a.c.vs)[o.base];
+            if (!o.live) sr = 0.f;
+            if (o.bad) sr = __builtin_nanf("");
+        }
+    };
+    auto store = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < UK; ++i) {
+            const int u = tid + i * NTH;
+            const int tok = u / (D / 16), ch = u % (D / 16);
+            // token 8 o + 4 half + x of a 32-token group is row 4 o + x of the group's tile `half`
+            const int tile = 2 * (tok >> 5) + ((tok >> 2) & 1), row = 4 * ((tok >> 3) & 3) + (tok & 3);
+            const int j = ch >> 2, g = ch & 3;
+            ks[slot][tile][2 * j][16 * g + row] = codes8(kr[i].x, kr[i].y);
+            ks[slot][tile][2 * j + 1][16 * g + row] = codes8(kr[i].z, kr[i].w);
+            const int oc = u / (D / 2), dp = u % (D / 2);
+            const int m = dp >> 4;
+            vs[slot][oc >> 2][2 * m][16 * (oc & 3) + (dp & 15)] = codes8(vr[i].x, vr[i].y);
+            vs[slot][oc >> 2][2 * m + 1][16 * (oc & 3) + (dp & 15)] = codes8(vr[i].z, vr[i].w);
+        }
+        if (tid < 2 * (NT / 8)) scl[slot][tid / (NT / 8)][tid % (NT / 8)] = sr;
+    };
+
+    f16x8_t Qh[2 * NJ], Ql[2 * NJ];
+    float factor;
+    {
+        float f[D / 4];
+        factor = load_query<D>(a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D, lk, a.scale, f);
+#pragma unroll
+        for (int d = 0; d < 2 * NJ; ++d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                Qh[d][i] = static_cast<_Float16>(f[8 * d + i]);
+                Ql[d][i] = static_cast<_Float16>(low_part(f[8 * d + i]));
+            }
+    }
+    f32x4_t acc[ND][2];
+#pragma unroll
+    for (int m = 0; m < ND; ++m) acc[m][0] = acc[m][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float mu = -FLT_MAX, l = 0.f;
+    if (steps > 0) {
+        load(0);
+        store(0);
+        if (steps > 1) load(1);
+    }
+    for (int st = 0; st < steps; ++st) {
+        __syncthreads();   // slot st % 2 is whole; the other one has been read
+        if (st + 1 < steps) {
+            store((st + 1) & 1);
+            if (st + 2 < steps) load(st + 2);
+        }
+        const int slot = st & 1;
+#pragma unroll 1
+        for (int g = 0; g < NT / 32; ++g) {
+            const int t0 = st * NT + 32 * g;
+            if (t0 >= wave_seen) break;   // the wave's rows see nothing from here on
+            f32x4_t S[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                S[half] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int d = 0; d < 2 * NJ; ++d) {
+                    const f16x8_t A = ks[slot][2 * g + half][d][lane];
+                    S[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Qh[d], S[half], 0, 0, 0);
+                    S[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Ql[d], S[half], 0, 0, 0);
+                }
+            }
+            const float f = factor * scl[slot][0][4 * g + lk];
+            float sv = scl[slot][1][4 * g + lk];
+            float s[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = S[i >> 2][i & 3] * f;
+            if (t0 + 31 > wave_first) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (t0 + 8 * lk + i > limit) s[i] = -INFINITY;
+                if (t0 + 8 * lk > limit) sv = 0.f;
+            }
+            float top = s[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
+            top += __builtin_amdgcn_logf(fmaxf(sv, kKv8Floor));
+            if (__ballot(top > mu + kMoves)) {
+                const float now = fmaxf(mu, max_over_lk(top));
+                const float shrink = __builtin_amdgcn_exp2f(mu - now);
+                mu = now;
+                l *= shrink;
+#pragma unroll
+                for (int m = 0; m < ND; ++m)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[m][e][i] *= shrink;
+            }
+            f16x8_t Wh, Wl;
+            const float up = sv * kWeightUp;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float p = __builtin_amdgcn_exp2f(s[i] - mu);
+                l += p;
+                const float w = rounded(p * up);
+                Wh[i] = static_cast<_Float16>(w);
+                Wl[i] = static_cast<_Float16>(low_part(w));
+            }
+#pragma unroll
+            for (int m = 0; m < ND; ++m)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const f16x8_t A = vs[slot][g][2 * m + e][lane];
+                    acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Wh, acc[m][e], 0, 0, 0);
+                    acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Wl, acc[m][e], 0, 0, 0);
+                }
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (mine >= pairs) return;
+    if (r.bad) l = __builtin_nanf("");
+    const size_t o = (static_cast<size_t>(r.first + ti) * a.heads + head) * D;
+    const float inv = kWeightUp * l;
+#pragma unroll
+    for (int m = 0; m < ND; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)   // dims 32 m + 2 (4 lk + i) + e
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int d = 32 * m + 8 * lk + 2 * i + e;
+                float v = l == 0.f ? 0.f : acc[m][e][i] / inv;
+                if (a.gate) v *= sigmoid(a.gate[o + d]);
+                a.out[o + d] = v;
+            }
+    if (lk == 0) a.info[o / D] = make_int2(0, 1);
+}
+
+// ------------------------------------------------------------------ host
+// Pieces are at most kTargetItems plus one per unit, and units at most one per 8 pairs plus one per request that has rows.
+int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
+    const int64_t pairs = static_cast<int64_t>(rows) * (heads / kv_heads);
+    return (pairs / kRows + std::min(rows, requests)) * kv_heads;
+}
+size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
+
+struct Layout {
+    int64_t items;
+    size_t stat, info, bytes;
+};
+Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
+    Layout l;
+    l.items = kTargetItems + unit_bound(rows, requests, heads, kv_heads);
+    l.stat = align_up(static_cast<size_t>(l.items) * kRows * dim * 4);
+    l.info = l.stat + align_up(static_cast<size_t>(l.items) * kRows * 8);
+    l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);
+    return l;
+}
+
+template <int D>
+void launch(const AttnArgs& a, hipStream_t s) {
+    split_kernel<D><<<static_cast<unsigned>(a.items), kSplitBlock, 0, s>>>(a);
+    if (!a.split_all) {
+        const int64_t pairs = static_cast<int64_t>(a.rows) * a.group;
+        const int64_t tiles = (pairs / kPromptRows + std::min<int64_t>(a.requests, pairs / kSplitMax + 1)) * a.c.heads;
+        prompt_kernel<D><<<static_cast<unsigned>(tiles), kPromptWaves * kWave, 0, s>>>(a);
+    }
+    const unsigned grid = static_cast<unsigned>(a.rows) * static_cast<unsigned>(a.heads);
+    if (grid <= 128)   // few rows: many pieces each
+        combine_kernel<D, 16><<<grid, 16 * kWave, 0, s>>>(a);
+    else
+        combine_kernel<D, 4><<<grid, 4 * kWave, 0, s>>>(a);
+}
+
+}  // namespace
+}  // namespace qk
+
+using namespace qk;
+
+extern "C" {
+
+size_t qwen_attn_kv8_workspace_bytes(int rows, int requests, int heads, int kv_heads, int dim) {
+    if (rows <= 0 || requests <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || dim <= 0) return 0;
+    return layout(rows, requests, heads, kv_heads, dim).bytes;
+}
+
+int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
+                       const float* v_scale, int pages, int page_size, const int32_t* block_table, int max_pages,
+                       const int32_t* row_start, const int32_t* kv_len, int requests, const float* gate, float* out, int rows,
+                       int heads, int kv_heads, int dim, void* workspace, size_t workspace_bytes, void* stream) {
+    const Kv8Cache c{const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes), const_cast<float*>(k_scale),
+                     const_cast<float*>(v_scale), pages, page_size, kv_heads, dim};
+    if (const int rc = kv8_check("attn_kv8_rows", c)) return rc;
+    QK_REQUIRE(heads > 0 && heads % kv_heads == 0, "attn_kv8_rows: %d query heads over %d KV heads", heads, kv_heads);
+    QK_REQUIRE(rows >= 0 && requests >= 0 && max_pages >= 0, "attn_kv8_rows: negative size");
+    QK_REQUIRE(requests <= kKv8MaxRequests, "attn_kv8_rows: %d requests (at most %d)", requests, kKv8MaxRequests);
+    QK_REQUIRE(static_cast<int64_t>(max_pages) * page_size <= 0x7fffffff, "attn_kv8_rows: table rows of %d pages", max_pages);
+    if (rows == 0 || requests == 0) return ok();
+    QK_REQUIRE(q && out && row_start && kv_len && (block_table || max_pages == 0), "attn_kv8_rows: null pointer");
+    QK_REQUIRE(static_cast<int64_t>(rows) * heads <= (int64_t{1} << 24), "attn_kv8_rows: %d rows of %d heads exceed one call",
+               rows, heads);
+    QK_REQUIRE(out != q, "attn_kv8_rows: out is q");
+    const Layout l = layout(rows, requests, heads, kv_heads, dim);
+    QK_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= l.bytes,
+               "attn_kv8_rows: workspace of %zu bytes, need %zu (16-byte aligned)", workspace_bytes, l.bytes);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    AttnArgs a;
+    a.q = q;
+    a.gate = gate;
+    a.out = out;
+    a.c = c;
+    a.table = block_table;
+    a.row_start = row_start;
+    a.kv_len = kv_len;
+    a.max_pages = max_pages;
+    a.page_shift = __builtin_ctz(static_cast<unsigned>(page_size));
+    a.requests = requests;
+    a.rows = rows;
+    a.heads = heads;
+    a.group = heads / kv_heads;
+    a.split_all = static_cast<int64_t>(rows) * a.group <= kSplitMax;   // no request can have more
+    a.part = reinterpret_cast<float*>(ws);
+    a.stat = reinterpret_cast<float2*>(ws + l.stat);
+    a.info = reinterpret_cast<int2*>(ws + l.info);
+    a.items = static_cast<int>(l.items);
+    a.scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(dim)));
+    const hipStream_t s = as_stream(stream);
+    if (dim == 64)
+        launch<64>(a, s);
+    else if (dim == 128)
+        launch<128>(a, s);
+    else
+        launch<256>(a, s);
+    return check_launch("attn_kv8_rows");
+}
+
+}  // extern "C"

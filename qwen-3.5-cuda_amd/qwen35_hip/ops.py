@@ -12,6 +12,7 @@ torch is used for device memory and streams only.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -525,6 +526,136 @@ def attn_decode_noalloc(q, k_cache, v_cache, heads, kv_heads, dim, pos, gate=Non
     _dev(out, dtype=torch.float32)
     check(load().qwen_attn_decode_noalloc(_p(q), _p(k_cache), _p(v_cache), _p(gate), _p(out), heads, kv_heads, dim,
                                           pos, _stream(stream)))
+    return out
+
+
+# ------------------------------------------------------------------ several requests: a paged 8-bit KV cache
+class Kv8Cache(NamedTuple):
+    """int8 codes and float32 scales of a paged cache (qwen35_hip.h): k [pages, kv_heads, page, dim],
+    v [pages, kv_heads, page / 8, dim, 8], k_scale, v_scale [pages, kv_heads]."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def kv8_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv8Cache:
+    """An empty cache."""
+    codes = dict(dtype=torch.int8, device=device)
+    scales = dict(dtype=torch.float32, device=device)
+    return Kv8Cache(torch.zeros((pages, kv_heads, page_size, dim), **codes),
+                    torch.zeros((pages, kv_heads, page_size // 8, dim, 8), **codes),
+                    torch.zeros((pages, kv_heads), **scales), torch.zeros((pages, kv_heads), **scales))
+
+
+def _kv8_check(cache):
+    _dev(cache.k, cache.v, dtype=torch.int8)
+    _dev(cache.k_scale, cache.v_scale, dtype=torch.float32)
+    if cache.k.dim() != 4:
+        raise ValueError("cache keys must be [pages, kv_heads, page, dim]")
+    pages, heads, page, dim = cache.k.shape
+    _same((pages, heads, page // 8, dim, 8), cache.v)
+    _same((pages, heads), cache.k_scale, cache.v_scale)
+    return pages, page, heads, dim
+
+
+def kv8_plan(cached, fresh, block_table, free_pages, free_head, page_size, rows, free_head_out=None, row_start=None,
+             kv_len=None, slots=None, pos=None, stream=None):
+    """The bookkeeping of a step of several requests: cached, fresh int32 [requests]; block_table int32
+    [requests, max_pages] in place; free_pages int32 [n], free_head int32 [1]
+    -> (row_start [requests + 1], kv_len [requests], slots [rows], pos [rows], free_head_out [1])."""
+    _dev(cached, fresh, block_table, free_pages, free_head, dtype=torch.int32)
+    n = cached.numel()
+    _same((n,), cached, fresh)
+    if block_table.dim() != 2 or block_table.shape[0] != n:
+        raise ValueError("block_table must be [requests, max_pages]")
+    _same((1,), free_head)
+    i32 = dict(dtype=torch.int32, device=cached.device)
+    free_head_out = torch.empty(1, **i32) if free_head_out is None else free_head_out
+    row_start = torch.empty(n + 1, **i32) if row_start is None else row_start
+    kv_len = torch.empty(n, **i32) if kv_len is None else kv_len
+    slots = torch.empty(rows, **i32) if slots is None else slots
+    pos = torch.empty(rows, **i32) if pos is None else pos
+    _dev(free_head_out, row_start, kv_len, slots, pos, dtype=torch.int32)
+    _same((1,), free_head_out)
+    _same((n + 1,), row_start)
+    _same((n,), kv_len)
+    _same((rows,), slots, pos)
+    check(load().qwen_kv8_plan(_p(cached), _p(fresh), n, _p(block_table), block_table.shape[1], _p(free_pages),
+                               free_pages.numel(), _p(free_head), _p(free_head_out), page_size, rows, _p(row_start),
+                               _p(kv_len), _p(slots), _p(pos), _stream(stream)))
+    return row_start, kv_len, slots, pos, free_head_out
+
+
+def _kv_rows(x, heads, dim):
+    """Row stride of x [rows, kv_heads, dim]: rows may lie apart (a slice of wider rows), each in one piece."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.float32:
+        raise ValueError("expected a float32 device tensor")
+    if x.dim() != 3 or tuple(x.shape[1:]) != (heads, dim):
+        raise ValueError(f"expected [rows, {heads}, {dim}], got {tuple(x.shape)}")
+    if x.shape[0] and (x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim)):
+        raise ValueError("expected rows of kv_heads x dim in one piece")
+    return x.stride(0) if x.shape[0] > 1 else heads * dim
+
+
+def kv8_store_rows(k, v, slots, cache: Kv8Cache, stream=None):
+    """k, v [rows, kv_heads, dim] (rows may be strided) quantized into `slots` int32 [rows] of the cache, in place."""
+    pages, page, heads, dim = _kv8_check(cache)
+    ks, vs = _kv_rows(k, heads, dim), _kv_rows(v, heads, dim)
+    _dev(slots, dtype=torch.int32)
+    _same((k.shape[0],), slots)
+    _same(k.shape, v)
+    check(load().qwen_kv8_store_rows(_p(k), _p(v), ks, vs, _p(slots), k.shape[0], _p(cache.k), _p(cache.v),
+                                     _p(cache.k_scale), _p(cache.v_scale), pages, page, heads, dim, _stream(stream)))
+    return cache
+
+
+def kv8_read_rows(cache: Kv8Cache, slots, k=None, v=None, stream=None):
+    """The values of `slots` int32 [rows] -> k, v float32 [rows, kv_heads, dim]."""
+    pages, page, heads, dim = _kv8_check(cache)
+    _dev(slots, dtype=torch.int32)
+    shape = (slots.numel(), heads, dim)
+    k = torch.empty(shape, dtype=torch.float32, device=slots.device) if k is None else k
+    v = torch.empty(shape, dtype=torch.float32, device=slots.device) if v is None else v
+    _dev(k, v, dtype=torch.float32)
+    _same(shape, k, v)
+    check(load().qwen_kv8_read_rows(_p(cache.k), _p(cache.v), _p(cache.k_scale), _p(cache.v_scale), pages, page, heads,
+                                    dim, _p(slots), slots.numel(), _p(k), _p(v), _stream(stream)))
+    return k, v
+
+
+def attn_kv8_workspace_bytes(rows, requests, heads, kv_heads, dim) -> int:
+    return int(load().qwen_attn_kv8_workspace_bytes(rows, requests, heads, kv_heads, dim))
+
+
+def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None, workspace=None, out=None, stream=None):
+    """q [rows, heads, dim] of several requests (rows row_start[b] .. row_start[b + 1] - 1 are the last positions of
+    request b's kv_len[b] tokens, in the pages block_table[b]) -> out [rows, heads, dim] (x sigmoid(gate)), causal."""
+    pages, page, kv_heads, dim = _kv8_check(cache)
+    _dev(q, dtype=torch.float32)
+    if q.dim() != 3 or q.shape[2] != dim:
+        raise ValueError(f"q must be [rows, heads, {dim}], got {tuple(q.shape)}")
+    rows, heads, _ = q.shape
+    _dev(block_table, row_start, kv_len, dtype=torch.int32)
+    n = kv_len.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != n:
+        raise ValueError("block_table must be [requests, max_pages]")
+    _same((n,), kv_len)
+    _same((n + 1,), row_start)
+    if gate is not None:
+        _dev(gate, dtype=torch.float32)
+        _same(q.shape, gate)
+    out = torch.empty_like(q) if out is None else out
+    _dev(out, dtype=torch.float32)
+    _same(q.shape, out)
+    if workspace is None:
+        workspace = torch.empty(max(16, attn_kv8_workspace_bytes(rows, n, heads, kv_heads, dim)), dtype=torch.uint8,
+                                device=q.device)
+    _dev(workspace)
+    check(load().qwen_attn_kv8_rows(_p(q), _p(cache.k), _p(cache.v), _p(cache.k_scale), _p(cache.v_scale), pages, page,
+                                    _p(block_table), block_table.shape[1], _p(row_start), _p(kv_len), n, _p(gate),
+                                    _p(out), rows, heads, kv_heads, dim, _p(workspace),
+                                    workspace.numel() * workspace.element_size(), _stream(stream)))
     return out
 
 
