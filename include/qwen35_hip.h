@@ -419,6 +419,27 @@ int qwen_moe_expert_gate_up(const void* w_gate, const void* w_up, int type, uint
                             uint64_t expert_stride, int n_experts, const int32_t* idx, int n_sel,
                             const float* x, float* gate_out, float* up_out, int M, int K, void* stream);
 
+/* The (token, pick) pairs of many tokens grouped by expert: idx [pairs] holds the experts' ids (moe_topk_rows' idx, pair
+ * p = t k + j) -> order [pairs], the pairs sorted by id, equal ids in their order, and starts [n_experts + 1]: expert
+ * e's pairs are order[starts[e]] .. order[starts[e + 1] - 1]. Pairs whose id is outside [0, n_experts) come last, behind
+ * starts[n_experts]. pairs <= 2^24, n_experts <= 1024. No counterpart in the reference. */
+int qwen_moe_group_rows(const int32_t* idx, int pairs, int n_experts, int32_t* order, int32_t* starts, void* stream);
+
+/* The routed experts of many tokens: x [rows x width], weights [rows x top], order and starts as qwen_moe_group_rows
+ * gives them for the rows * top ids;
+ *   out[t] = sum_j weights[t][j] * Wd_e (SiLU(Wg_e x_t) * (Wu_e x_t)),  e = the id of pair t top + j
+ * written to out [rows x width]. w_gate and w_up (one type) hold n_experts matrices of inter x width one after the
+ * other, w_down n_experts of width x inter: Q4_K or Q6_K, width and inter multiples of 256; every pointer 16-byte
+ * aligned, out apart from x, rows * top <= 2^24. The products have an fp32 dot product's accuracy (qwen_matmul_rows). A
+ * token with an id outside the experts has a NaN row. workspace: at least qwen_moe_experts_rows_workspace_bytes() bytes
+ * (0 for sizes that the call refuses), for one call at a time.
+ * ref: src/layer_moe.cpp:127-142, token by token there */
+size_t qwen_moe_experts_rows_workspace_bytes(int rows, int top, int n_experts, int width, int inter);
+int qwen_moe_experts_rows(const void* w_gate, const void* w_up, int type, const void* w_down, int down_type,
+                          int n_experts, const int32_t* order, const int32_t* starts, const float* weights, int top,
+                          const float* x, int rows, int width, int inter, float* out, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 /* The SwiGLU hidden rows of a MoE layer's decode step in one launch
  * (src/layer_moe.cpp:131-133 per routed expert, :146-148 for the shared expert):
  *   hidden[j]     = SiLU(Wg_e x) * (Wu_e x)       e = idx[j] (on the device), j < n_sel

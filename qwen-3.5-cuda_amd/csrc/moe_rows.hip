@@ -1,0 +1,607 @@
+// The routed experts of many tokens on gfx950: (token, pick) pairs grouped by expert, then
+//   hidden[p] = SiLU(Wg_e x_t) * (Wu_e x_t),  out[t] = sum_j w[t][j] Wd_e hidden[t k + j],   p = t k + j, e = idx[p]
+// with K-quant weights of n_experts matrices each. The reference runs the experts of one token one after the other
+// (src/layer_moe.cpp:127-142), five launches each; here every expert's rows go through it together.
+//
+// The products are gemm.hip's: x as two fp16 parts per row, weights as exact small integers in fp16, block scales in fp32
+// (the mathematics stands there). What differs is the shape of the work: 256 products with a few to a few hundred rows
+// each. A tile is up to 16 WT pairs of one expert, a table of tiles is written by the first launch from the experts'
+// starts, and a workgroup takes a tile and a slice of the expert's rows. Rows of x are gathered by pair: their fp16 parts
+// lie row by row, 128 bytes per depth of 32 elements, so a gathered operand is still whole cache lines. The hidden rows
+// are kept in the order of the groups, so the down products read neighbouring rows and only the last step scatters.
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
+#include "capi_common.hpp"
+#include "device_common.hpp"
+#include "gemm_common.hpp"
+#include "ggml_common.hpp"
+
+namespace qk {
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kGroupBlock = 1024;
+
+// ------------------------------------------------------------------ grouping
+// A stable counting sort in one launch: workgroup w places pairs [1024 w, 1024 w + 1024), one to a thread. Each counts
+// all pairs' experts itself (LDS counters: integer sums, the same in any order), and those of the pairs before its own, so no
+// workgroup waits for another; ranks among its own pairs come from ballots on the bits of the id (lanes of the wave with
+// the same expert) and per-wave counts. Ids outside [0, n) go behind the last group.
+__global__ __launch_bounds__(kGroupBlock) void group_kernel(const int32_t* __restrict__ idx, int pairs, int n,
+                                                            int32_t* __restrict__ order, int32_t* __restrict__ starts) {
+    __shared__ int all[kMaxExperts + 1], before[kMaxExperts + 1];
+    __shared__ uint16_t mine[kGroupBlock / kWave][kMaxExperts + 2];
+    __shared__ int part[kGroupBlock / kWave];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int first = blockIdx.x * kGroupBlock;
+    for (int e = tid; e <= n; e += kGroupBlock) all[e] = before[e] = 0;
+    for (int e = lane; e <= n; e += kWave) mine[wv][e] = 0;
+    __syncthreads();
+    auto bucket = [&](int i) {
+        const int e = idx[i];
+        return e >= 0 && e < n ? e : n;
+    };
+    for (int i = tid; i < pairs; i += kGroupBlock) {
+        const int e = bucket(i);
+        atomicAdd(&all[e], 1);
+        if (i < first) atomicAdd(&before[e], 1);
+    }
+    const int p = first + tid;
+    const bool in = p < pairs;
+    const int e = in ? bucket(p) : n + 1;   // n + 1: no pair
+    uint64_t same = ~0ull;
+    for (int bit = 0; (1 << bit) <= n + 1; ++bit) {
+        const uint64_t set = __ballot((e >> bit) & 1);
+        same &= (e >> bit) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    if (in && rank == 0) mine[wv][e] = static_cast<uint16_t>(__popcll(same));
+    __syncthreads();
+    // exclusive prefix of all[0 .. n], a bucket to a thread (n <= 1024; bucket n needs only the sum before it)
+    const int c = tid < n ? all[tid] : 0;
+    int inc = c;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int up = __shfl_up(inc, o);
+        if (lane >= o) inc += up;
+    }
+    if (lane == 63) part[wv] = inc;
+    __syncthreads();
+    int base = 0, total = 0;
+    for (int w = 0; w < kGroupBlock / kWave; ++w) {
+        if (w < wv) base += part[w];
+        total += part[w];
+    }
+    if (tid < n) all[tid] = base + inc - c;
+    if (tid == 0) all[n] = total;
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int i = tid; i <= n; i += kGroupBlock) starts[i] = all[i];
+    if (!in) return;
+    int at = all[e] + before[e] + rank;
+    for (int w = 0; w < wv; ++w) at += mine[w][e];
+    order[at] = p;
+}
+
+// ------------------------------------------------------------------ tiles, x in two fp16 parts
+struct Tile {
+    int expert, first, n;   // pairs order[first .. first + n)
+};
+
+// Tiles of up to `size` pairs, expert by expert; the count in tiles[-1].expert. One wave.
+__device__ void write_tiles(const int32_t* __restrict__ starts, int experts, int pairs, int size, Tile* __restrict__ tiles,
+                            int most) {
+    const int lane = threadIdx.x & 63;
+    int at = 0;
+    for (int e0 = 0; e0 < experts; e0 += kWave) {
+        const int e = e0 + lane;
+        int s = 0, n = 0;
+        if (e < experts) {
+            s = min(max(starts[e], 0), pairs);
+            n = min(max(starts[e + 1], s), pairs) - s;
+        }
+        const int k = (n + size - 1) / size;
+        int inc = k;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int up = __shfl_up(inc, o);
+            if (lane >= o) inc += up;
+        }
+        for (int i = 0; i < k; ++i) {
+            const int slot = at + inc - k + i;
+            if (slot < most) tiles[slot] = Tile{e, s + i * size, min(size, n - i * size)};
+        }
+        at += __shfl(inc, 63);
+    }
+    if (lane == 0) tiles[-1] = Tile{min(at, most), 0, 0};
+}
+
+// Pair at a place of the order, inside the call's pairs whatever the array holds.
+__device__ __forceinline__ int pair_at(const int32_t* __restrict__ order, int pos, int pairs) {
+    return min(max(order[pos], 0), pairs - 1);
+}
+
+// A wave per row: exponent, group sums and parts, [row][depth of 32][part][lk][8 elements] (gemm.hip's order of the
+// elements in a block). The last workgroup of the first launch (x) writes the table of tiles, the one of the second
+// launch (hidden rows) marks the tokens that have a pair behind the last group: their output is NaN.
+struct Grouping {
+    const int32_t* order;
+    const int32_t* starts;
+    Tile* tiles;
+    int* lost;   // per token
+    int experts, pairs, top, size, most;
+};
+template <bool FIRST>
+__global__ __launch_bounds__(256) void rows_prep(const float* __restrict__ x, int rows, int K, int* __restrict__ ex,
+                                                 float* __restrict__ sx, uint8_t* __restrict__ xp, const Grouping gr) {
+    const int wv = wave_in_block(), lane = threadIdx.x & 63;
+    if (blockIdx.x == gridDim.x - 1) {
+        if constexpr (FIRST) {
+            if (wv == 0) write_tiles(gr.starts, gr.experts, gr.pairs, gr.size, gr.tiles, gr.most);
+        } else {
+            for (int q = max(gr.starts[gr.experts], 0) + static_cast<int>(threadIdx.x); q < gr.pairs; q += 256)
+                gr.lost[pair_at(gr.order, q, gr.pairs) / gr.top] = 1;
+        }
+        return;
+    }
+    const int r = blockIdx.x * 4 + wv;
+    if (r >= rows) return;
+    if (FIRST && lane == 0) gr.lost[r] = 0;
+    const float* row = x + static_cast<size_t>(r) * K;
+    float m = 0.f;
+    for (int k = 8 * lane; k < K; k += 512) m = max_abs4(max_abs4(m, ld4(row + k)), ld4(row + k + 4));
+    const int e = prep_exponent(wave_max_abs(m)), es = e == kRowNonFinite ? 0 : e;
+    if (lane == 0) ex[r] = e;
+    const int c = lane & 31;   // chunk of 8 in the block: 16 (lk / 2) + 4 u + 2 (lk % 2) + j, depth 2 u + j
+    const int depth = 2 * ((c >> 2) & 3) + (c & 1), lk = 2 * (c >> 4) + ((c >> 1) & 1);
+    uint8_t* out = xp + static_cast<size_t>(r) * K * 4 + 128 * depth + 16 * lk;
+    for (int k = 8 * lane; k < K; k += 512) {
+        uint32_t h[4], l[4];
+        float s = split8(ld4(row + k), ld4(row + k + 4), es, h, l);
+        uint8_t* o = out + 1024 * (k >> 8);
+        st16(o, make_uint4(h[0], h[1], h[2], h[3]));
+        st16(o + 64, make_uint4(l[0], l[1], l[2], l[3]));
+        s += __shfl_xor(s, 1);
+        s += __shfl_xor(s, 2);
+        if ((lane & 3) == 0) sx[static_cast<size_t>(r) * (K >> 5) + (k >> 5)] = s;
+    }
+}
+
+// ------------------------------------------------------------------ the products
+struct RowsArgs {
+    const uint8_t* w[2];   // gate and up, or down
+    const Tile* tiles;     // tiles[-1].expert: how many
+    const int32_t* order;
+    const int* ex;
+    const float* sx;
+    const uint8_t* xp;
+    const float* x;        // the rows in fp32, for those with an infinity
+    float* y;
+    int M, K, top, pairs, column_blocks;   // M: rows of an expert's matrix; top: pairs per row of x (gate and up)
+};
+
+// 8 waves: RW row groups x KW slices of K; a wave owns 16 WT pairs x 32 weight rows of its slice: 16 gate and the same
+// 16 up rows (SWIGLU), or 32 down rows. Pipeline, operands and epilogue as gemm_kquant's (gemm.hip).
+template <int WT, int KW, bool SWIGLU>
+struct RowsShape {
+    static constexpr int RW = 8 / KW, FR = WT * KW * 4, XF = FR / 8, tokens = 16 * WT, cols = (SWIGLU ? 16 : 32) * RW;
+    static constexpr size_t ring = size_t{4} * FR * 1024, fold = KW > 1 ? size_t{8} * WT * 2 * 1024 : 0;
+    static constexpr size_t lds = ring > fold ? ring : fold;
+    static_assert(FR % 8 == 0, "shape");
+};
+
+template <int TYPE, int WT, int KW, bool SWIGLU>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void rows_kernel(const RowsArgs a) {
+    using G = RowsShape<WT, KW, SWIGLU>;
+    constexpr int BB = TYPE == kQ4_K ? 144 : 210, NB = TYPE == kQ4_K ? 1 : 2, WR = 2;
+    __shared__ __align__(16) uint8_t smem[G::lds];
+    uint4* xs = reinterpret_cast<uint4*>(smem);
+    const int tile = static_cast<int>(blockIdx.x) / a.column_blocks, cb = static_cast<int>(blockIdx.x) - tile * a.column_blocks;
+    if (tile >= a.tiles[-1].expert) return;   // the whole workgroup
+    const Tile tl = a.tiles[tile];
+    const int M = a.M, K = a.K, n = tl.n;
+    const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4;
+    const int wv = wave_in_block();
+    const int kw = wv / G::RW, rw = wv % G::RW;
+    const int nb = K >> 8, nbk = nb / KW, steps = 4 * nbk, nst = K >> 5;
+    const int c0 = cb * G::cols, r0 = c0 + (SWIGLU ? 16 : 32) * rw;   // the workgroup's and the wave's first row
+    const uint64_t eb = (static_cast<uint64_t>(tl.expert) * M + c0) * nb + static_cast<uint64_t>(kw) * nbk;
+    const uint8_t* wbase[WR];
+    uint32_t wo[WR];
+#pragma unroll
+    for (int rt = 0; rt < WR; ++rt) {
+        wbase[rt] = a.w[SWIGLU ? rt : 0] + eb * BB;
+        wo[rt] = static_cast<uint32_t>(min(r0 + (SWIGLU ? 0 : 16 * rt) + lr, M - 1) - c0) * static_cast<uint32_t>(nb) * BB;
+    }
+    auto xrow = [&](int i) {   // row of x of the tile's pair i (the last one again past the end)
+        const int pos = tl.first + min(i, n - 1);
+        return SWIGLU ? pair_at(a.order, pos, a.pairs) / a.top : pos;
+    };
+    const uint8_t* xb[G::XF];   // this wave's fragments of a step: fragment id -> (slice, tile, (depth, part))
+#pragma unroll
+    for (int i = 0; i < G::XF; ++i) {
+        const int id = wv * G::XF + i;
+        const int ti = id / 4 % WT, ks = id / (4 * WT);
+        xb[i] = a.xp + static_cast<size_t>(xrow(16 * ti + lr)) * K * 4 + ks * nbk * 1024 + 64 * (id % 4) + 16 * lk;
+    }
+    uint4 xr[2][G::XF];
+    auto x_load = [&](uint4 (&d)[G::XF], int st) {
+#pragma unroll
+        for (int i = 0; i < G::XF; ++i) d[i] = ld16(xb[i] + 256u * static_cast<uint32_t>(min(st, steps - 1)));
+    };
+    auto x_store = [&](const uint4 (&d)[G::XF], int slot) {
+#pragma unroll
+        for (int i = 0; i < G::XF; ++i) xs[(slot * G::FR + wv * G::XF + i) * 64 + lane] = d[i];
+    };
+    const uint4* as = xs + kw * WT * 4 * 64 + lane;
+    constexpr int PT = WT < 2 ? WT : 2;
+    f16x8_t An[PT][2];
+    auto a_load = [&](f16x8_t (&d)[PT][2], int slot, int j, int t0) {
+#pragma unroll
+        for (int i = 0; i < PT; ++i)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                d[i][p] = *reinterpret_cast<const f16x8_t*>(&as[(slot * G::FR + 4 * min(t0 + i, WT - 1) + 2 * j + p) * 64]);
+    };
+    auto barrier = []() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const float* sg_row[WT];
+#pragma unroll
+    for (int tt = 0; tt < WT; ++tt) sg_row[tt] = a.sx + static_cast<size_t>(xrow(16 * tt + lr)) * nst + 8 * kw * nbk + 2 * lk;
+
+    f32x4_t acc[WT][WR], C[WT][WR];
+#pragma unroll
+    for (int tt = 0; tt < WT; ++tt)
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) acc[tt][rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    uint32_t k64 = 0x64006400u;
+    asm volatile("" : "+v"(k64));
+    WBlock<TYPE> wc[WR], wn[WR];
+    WScale<TYPE> sc[WR];
+    f16x8_t B[2][WR][NB];
+    auto w_load = [&](int b) {
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) wn[rt].load(wbase[rt] + static_cast<size_t>(min(b, nbk - 1)) * BB, wo[rt], lk);
+    };
+    auto w_take = [&]() {
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) wc[rt] = wn[rt];
+    };
+    auto b_make = [&](auto dI) {
+        constexpr int D = decltype(dI)::value;
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) {
+            if constexpr ((D & 1) == 0) sc[rt].template set<(D >> 1)>(wc[rt], lk);
+            decode<(D >> 1), (D & 1)>(wc[rt], sc[rt], k64, B[D & 1][rt]);
+        }
+    };
+    w_load(0);
+    x_load(xr[0], 0);
+    x_load(xr[1], 1);
+    w_take();
+    w_load(1);
+    x_store(xr[0], 0);
+    x_load(xr[0], 2);
+    x_store(xr[1], 1);
+    x_load(xr[1], 3);
+    b_make(IC<0>{});
+    barrier();
+    a_load(An, 0, 0, 0);
+    for (int b = 0; b < nbk; ++b) {
+        f16x4_t Bm[WR];
+        float dsc[WR], dmn[WR];
+        float2 sg[WT];
+        if constexpr (TYPE == kQ4_K) {
+#pragma unroll
+            for (int rt = 0; rt < WR; ++rt) {
+                Bm[rt] = min_weights(wc[rt].hd, lk);
+                dsc[rt] = opaque(half_bits(wc[rt].hd.x & 0xffffu));
+                dmn[rt] = opaque(-32.0f * half_bits(wc[rt].hd.x >> 16));
+            }
+#pragma unroll
+            for (int tt = 0; tt < WT; ++tt) sg[tt] = *reinterpret_cast<const float2*>(sg_row[tt] + 8 * b);
+        } else {
+#pragma unroll
+            for (int rt = 0; rt < WR; ++rt) dsc[rt] = opaque(half_bits(wc[rt].d));
+        }
+        static_for<8>([&](auto dI) {
+            constexpr int D = decltype(dI)::value, U = D >> 1, J = D & 1;
+            const int st = 4 * b + U;
+            if constexpr (D == 7) {
+                w_take();
+                w_load(b + 2);
+            }
+            if constexpr (J == 0) {
+                x_store(xr[U & 1], (U + 2) & 3);
+                x_load(xr[U & 1], st + 4);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            b_make(IC<(D + 1) & 7>{});
+            static_for<(WT + 1) / 2>([&](auto pI) {
+                constexpr int P0 = 2 * decltype(pI)::value, PN = P0 + 2 <= WT ? 2 : 1;
+                f16x8_t A[2][2];
+#pragma unroll
+                for (int i = 0; i < PN; ++i) {
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) A[i][p] = An[i][p];
+                }
+                if constexpr (P0 + 2 < WT)
+                    a_load(An, U, J, P0 + 2);
+                else
+                    a_load(An, J == 0 ? U : (U + 1) & 3, J ^ 1, 0);
+#pragma unroll
+                for (int i = 0; i < PN; ++i)
+#pragma unroll
+                    for (int rt = 0; rt < WR; ++rt)
+                        C[P0 + i][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            A[i][0], B[J][rt][0], D == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : C[P0 + i][rt], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < PN; ++i)
+#pragma unroll
+                    for (int rt = 0; rt < WR; ++rt)
+                        C[P0 + i][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[i][1], B[J][rt][0], C[P0 + i][rt], 0, 0, 0);
+                if constexpr (NB == 2) {
+#pragma unroll
+                    for (int i = 0; i < PN; ++i)
+#pragma unroll
+                        for (int rt = 0; rt < WR; ++rt)
+                            C[P0 + i][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[i][0], B[J][rt][NB - 1], C[P0 + i][rt], 0, 0, 0);
+                }
+#pragma unroll
+                for (int tt = P0; D == 7 && tt < P0 + PN; ++tt) {
+                    f16x4_t As;
+                    if constexpr (TYPE == kQ4_K) As = min_operand(sg[tt]);
+#pragma unroll
+                    for (int rt = 0; rt < WR; ++rt) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[tt][rt][i] = __builtin_fmaf(dsc[rt], C[tt][rt][i], acc[tt][rt][i]);
+                        if constexpr (TYPE == kQ4_K) {
+                            const f32x4_t pm =
+                                __builtin_amdgcn_mfma_f32_16x16x16f16(As, Bm[rt], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[tt][rt][i] = __builtin_fmaf(dmn[rt], pm[i], acc[tt][rt][i]);
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            if constexpr (J == 1) barrier();
+        });
+    }
+
+    // lane: pairs 4 lk + i of token tile tt, row lr of each row tile
+    auto finite = [&](const f32x4_t& v, int i, int rt, int row, int xr_, int e) {
+        if (e != kRowNonFinite) return ldexpf(v[i], -e);
+        return row_dot_per_element(a.w[SWIGLU ? rt : 0], TYPE, (static_cast<uint64_t>(tl.expert) * M + row) * K,
+                                   a.x + static_cast<size_t>(xr_) * K, K);
+    };
+    auto put = [&](int tt, const f32x4_t (&v)[WR]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 16 * tt + 4 * lk + i;
+            if (t >= n) continue;
+            const int pos = tl.first + t, xi = xrow(t), e = a.ex[xi];
+            if constexpr (SWIGLU) {
+                const int row = r0 + lr;
+                if (row < M) {
+                    const float g = finite(v[0], i, 0, row, xi, e), u = finite(v[1], i, 1, row, xi, e);
+                    a.y[static_cast<size_t>(pos) * M + row] = silu(g) * u;
+                }
+            } else {
+                float* y = a.y + static_cast<size_t>(pair_at(a.order, pos, a.pairs)) * M;
+#pragma unroll
+                for (int rt = 0; rt < WR; ++rt)
+                    if (r0 + 16 * rt + lr < M) y[r0 + 16 * rt + lr] = finite(v[rt], i, rt, r0 + 16 * rt + lr, xi, e);
+            }
+        }
+    };
+    if constexpr (KW == 1) {
+#pragma unroll
+        for (int tt = 0; tt < WT; ++tt) put(tt, acc[tt]);
+    } else {   // every slice's sums to LDS; wave kw of a row group adds the token tiles tt = kw (mod KW) in slice order
+        f32x4_t* part = reinterpret_cast<f32x4_t*>(smem);
+        auto at = [&](int slice, int tt, int rt) { return (((slice * G::RW + rw) * WT + tt) * WR + rt) * 64 + lane; };
+        barrier();
+#pragma unroll
+        for (int tt = 0; tt < WT; ++tt)
+#pragma unroll
+            for (int rt = 0; rt < WR; ++rt) part[at(kw, tt, rt)] = acc[tt][rt];
+        barrier();
+#pragma unroll
+        for (int tt = 0; tt < WT; ++tt) {
+            if (tt % KW != kw) continue;
+            f32x4_t v[WR];
+#pragma unroll
+            for (int rt = 0; rt < WR; ++rt) {
+                v[rt] = part[at(0, tt, rt)];
+#pragma unroll
+                for (int sl = 1; sl < KW; ++sl) v[rt] += part[at(sl, tt, rt)];
+            }
+            put(tt, v);
+        }
+    }
+}
+
+// out[t] = sum_j w[t][j] y[t k + j], j in order; NaN for a token one of whose pairs has no expert (y has no row of it).
+__global__ __launch_bounds__(256) void rows_combine(const float* __restrict__ y, const float* __restrict__ w,
+                                                    const int* __restrict__ lost, int rows, int k, int dim4,
+                                                    float* __restrict__ out) {
+    const int64_t n = static_cast<int64_t>(rows) * dim4;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int t = static_cast<int>(i / dim4), d4 = static_cast<int>(i - static_cast<int64_t>(t) * dim4);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* yt = y + (static_cast<size_t>(t) * k * dim4 + d4) * 4;
+        for (int j = 0; j < k; ++j) {
+            const float4 v = ld4(yt + static_cast<size_t>(j) * dim4 * 4);
+            const float a = w[static_cast<size_t>(t) * k + j];
+            o.x = __builtin_fmaf(a, v.x, o.x);
+            o.y = __builtin_fmaf(a, v.y, o.y);
+            o.z = __builtin_fmaf(a, v.z, o.z);
+            o.w = __builtin_fmaf(a, v.w, o.w);
+        }
+        if (lost[t]) o = make_float4(__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""));
+        st4(out + 4 * i, o);
+    }
+}
+
+// ------------------------------------------------------------------ host
+size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
+
+// Pairs of a tile by the mean group size.
+int tile_pairs(int64_t pairs, int experts) {
+    const double mean = static_cast<double>(pairs) / std::min<int64_t>(pairs, experts);
+    return mean <= 8 ? 16 : mean <= 20 ? 32 : 64;
+}
+int64_t tile_bound(int64_t pairs, int experts, int size) { return pairs / size + std::min<int64_t>(pairs, experts); }
+
+struct Layout {
+    int64_t tiles;
+    size_t table, lost, ex, sx, xp, hidden, hex, hsx, hxp, y, bytes;
+};
+Layout layout(int rows, int top, int experts, int width, int inter) {
+    const size_t pairs = static_cast<size_t>(rows) * top;
+    Layout l;
+    l.tiles = tile_bound(pairs, experts, tile_pairs(pairs, experts));
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += align_up(n);
+        return here;
+    };
+    l.table = take(sizeof(Tile) * (l.tiles + 1));
+    l.lost = take(4 * static_cast<size_t>(rows));
+    l.ex = take(4 * static_cast<size_t>(rows));
+    l.sx = take(static_cast<size_t>(rows) * (width / 32) * 4);
+    l.xp = take(static_cast<size_t>(rows) * width * 4);
+    l.hidden = take(pairs * inter * 4);
+    l.hex = take(4 * pairs);
+    l.hsx = take(pairs * (inter / 32) * 4);
+    l.hxp = take(pairs * inter * 4);
+    l.y = take(pairs * width * 4);
+    l.bytes = at;
+    return l;
+}
+
+template <int TYPE, int WT, int KW, bool SWIGLU>
+void launch_rows(RowsArgs a, int64_t tiles, hipStream_t s) {
+    using G = RowsShape<WT, KW, SWIGLU>;
+    a.column_blocks = static_cast<int>(blocks_for(a.M, G::cols));
+    rows_kernel<TYPE, WT, KW, SWIGLU><<<static_cast<unsigned>(tiles * a.column_blocks), 512, 0, s>>>(a);
+}
+
+template <int TYPE, bool SWIGLU>
+void launch_type(const RowsArgs& a, int size, int64_t tiles, hipStream_t s) {
+    const int nb = a.K / 256;
+    if (size == 16) {
+        if (nb % 4 == 0)
+            launch_rows<TYPE, 1, 4, SWIGLU>(a, tiles, s);
+        else if (nb % 2 == 0)
+            launch_rows<TYPE, 1, 2, SWIGLU>(a, tiles, s);
+        else
+            launch_rows<TYPE, 2, 1, SWIGLU>(a, tiles, s);   // half of the tile unused
+    } else if (size == 32) {
+        if (nb % 2 == 0)
+            launch_rows<TYPE, 2, 2, SWIGLU>(a, tiles, s);
+        else
+            launch_rows<TYPE, 2, 1, SWIGLU>(a, tiles, s);
+    } else {
+        launch_rows<TYPE, 4, 1, SWIGLU>(a, tiles, s);
+    }
+}
+
+template <bool SWIGLU>
+void launch_product(int type, const RowsArgs& a, int size, int64_t tiles, hipStream_t s) {
+    if (type == kQ4_K)
+        launch_type<kQ4_K, SWIGLU>(a, size, tiles, s);
+    else
+        launch_type<kQ6_K, SWIGLU>(a, size, tiles, s);
+}
+
+}  // namespace
+}  // namespace qk
+
+using namespace qk;
+
+extern "C" {
+
+int qwen_moe_group_rows(const int32_t* idx, int pairs, int n_experts, int32_t* order, int32_t* starts, void* stream) {
+    QK_REQUIRE(pairs >= 0 && pairs <= (1 << 24), "moe_group_rows: %d pairs", pairs);
+    QK_REQUIRE(n_experts > 0 && n_experts <= kMaxExperts, "moe_group_rows: %d experts (1 to %d)", n_experts, kMaxExperts);
+    QK_REQUIRE(starts && (pairs == 0 || (idx && order)), "moe_group_rows: null pointer");
+    group_kernel<<<std::max(blocks_for(pairs, kGroupBlock), 1u), kGroupBlock, 0, as_stream(stream)>>>(idx, pairs, n_experts,
+                                                                                                   order, starts);
+    return check_launch("moe_group_rows");
+}
+
+size_t qwen_moe_experts_rows_workspace_bytes(int rows, int top, int n_experts, int width, int inter) {
+    if (rows <= 0 || top <= 0 || n_experts <= 0 || width <= 0 || inter <= 0 || width % 256 || inter % 256) return 0;
+    return layout(rows, top, n_experts, width, inter).bytes;
+}
+
+int qwen_moe_experts_rows(const void* w_gate, const void* w_up, int type, const void* w_down, int down_type, int n_experts,
+                          const int32_t* order, const int32_t* starts, const float* weights, int top, const float* x, int rows,
+                          int width, int inter, float* out, void* workspace, size_t workspace_bytes, void* stream) {
+    QK_REQUIRE(w_gate && w_up && w_down, "moe_experts_rows: tensor is not loaded");
+    if ((type != kQ4_K && type != kQ6_K) || (down_type != kQ4_K && down_type != kQ6_K))
+        return fail(QWEN_STATUS_UNSUPPORTED_TYPE, "moe_experts_rows: GGML types %d, %d (Q4_K and Q6_K)", type, down_type);
+    QK_REQUIRE(width > 0 && inter > 0 && width % 256 == 0 && inter % 256 == 0,
+               "moe_experts_rows: widths %d and %d are not multiples of 256", width, inter);
+    QK_REQUIRE(n_experts > 0 && n_experts <= kMaxExperts, "moe_experts_rows: %d experts (1 to %d)", n_experts, kMaxExperts);
+    QK_REQUIRE(rows >= 0 && top > 0 && static_cast<int64_t>(rows) * top <= (1 << 24), "moe_experts_rows: %d rows of %d picks",
+               rows, top);
+    if (rows == 0) return ok();
+    QK_REQUIRE(order && starts && weights && x && out, "moe_experts_rows: null pointer");
+    QK_REQUIRE(aligned16(w_gate) && aligned16(w_up) && aligned16(w_down) && aligned16(x) && aligned16(out),
+               "moe_experts_rows: tensors must be 16-byte aligned");
+    QK_REQUIRE(out != x, "moe_experts_rows: out is x");
+    const Layout l = layout(rows, top, n_experts, width, inter);
+    QK_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= l.bytes,
+               "moe_experts_rows: workspace of %zu bytes, need %zu (16-byte aligned)", workspace_bytes, l.bytes);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const hipStream_t s = as_stream(stream);
+    const int pairs = rows * top, size = tile_pairs(pairs, n_experts);
+    Tile* tiles = reinterpret_cast<Tile*>(ws + l.table) + 1;
+    int* lost = reinterpret_cast<int*>(ws + l.lost);
+    const Grouping gr{order, starts, tiles, lost, n_experts, pairs, top, size, static_cast<int>(l.tiles)};
+    int *ex = reinterpret_cast<int*>(ws + l.ex), *hex = reinterpret_cast<int*>(ws + l.hex);
+    float *sx = reinterpret_cast<float*>(ws + l.sx), *hsx = reinterpret_cast<float*>(ws + l.hsx);
+    float *hidden = reinterpret_cast<float*>(ws + l.hidden), *y = reinterpret_cast<float*>(ws + l.y);
+    rows_prep<true><<<blocks_for(rows, 4) + 1, 256, 0, s>>>(x, rows, width, ex, sx, ws + l.xp, gr);
+    RowsArgs a{};
+    a.w[0] = static_cast<const uint8_t*>(w_gate);
+    a.w[1] = static_cast<const uint8_t*>(w_up);
+    a.tiles = tiles;
+    a.order = order;
+    a.ex = ex;
+    a.sx = sx;
+    a.xp = ws + l.xp;
+    a.x = x;
+    a.y = hidden;
+    a.M = inter;
+    a.K = width;
+    a.top = top;
+    a.pairs = pairs;
+    launch_product<true>(type, a, size, l.tiles, s);
+    rows_prep<false><<<blocks_for(pairs, 4) + 1, 256, 0, s>>>(hidden, pairs, inter, hex, hsx, ws + l.hxp, gr);
+    a.w[0] = static_cast<const uint8_t*>(w_down);
+    a.w[1] = nullptr;
+    a.ex = hex;
+    a.sx = hsx;
+    a.xp = ws + l.hxp;
+    a.x = hidden;
+    a.y = y;
+    a.M = width;
+    a.K = inter;
+    launch_product<false>(down_type, a, size, l.tiles, s);
+    const int64_t n4 = static_cast<int64_t>(rows) * (width / 4);
+    rows_combine<<<static_cast<unsigned>(std::min<int64_t>((n4 + 255) / 256, 8192)), 256, 0, s>>>(
+        y, weights, lost, rows, top, width / 4, out);
+    return check_launch("moe_experts_rows");
+}
+
+}  // extern "C"

@@ -854,6 +854,59 @@ def moe_down_combine(w_down, down_type, down_elements, expert_stride, n_experts,
     return out
 
 
+# ------------------------------------------------------------------ MoE, many tokens
+GGML_BLOCK_BYTES = {12: 144, 14: 210}   # of 256 elements: Q4_K, Q6_K
+
+
+def moe_group_rows(idx, n_experts: int, order=None, starts=None, stream=None):
+    """idx int32 [rows, k] (moe_topk_rows) -> order int32 [rows * k]: the pairs t * k + j sorted by expert, equal ones in
+    their order; starts int32 [n_experts + 1]: where each expert's pairs begin."""
+    _dev(idx, dtype=torch.int32)
+    n = idx.numel()
+    order = torch.empty(n, dtype=torch.int32, device=idx.device) if order is None else order
+    starts = torch.empty(n_experts + 1, dtype=torch.int32, device=idx.device) if starts is None else starts
+    _dev(order, starts, dtype=torch.int32)
+    _same((n,), order)
+    _same((n_experts + 1,), starts)
+    check(load().qwen_moe_group_rows(_p(idx), n, n_experts, _p(order), _p(starts), _stream(stream)))
+    return order, starts
+
+
+def moe_experts_rows_workspace_bytes(rows, top, n_experts, width, inter) -> int:
+    return int(load().qwen_moe_experts_rows_workspace_bytes(rows, top, n_experts, width, inter))
+
+
+def moe_experts_rows(w_gate, w_up, ggml_type, w_down, down_type, n_experts, order, starts, weights, x, inter, out=None,
+                     workspace=None, stream=None):
+    """x [rows, width], weights [rows, k], order / starts of moe_group_rows -> out [rows, width]:
+    out[t] = sum_j weights[t, j] Wd_e (SiLU(Wg_e x_t) * (Wu_e x_t)), e the expert of pair t * k + j."""
+    _dev(w_gate, w_up, w_down, dtype=torch.uint8)
+    _dev(order, starts, dtype=torch.int32)
+    _dev(weights, x, dtype=torch.float32)
+    if x.dim() != 2 or weights.dim() != 2 or weights.shape[0] != x.shape[0]:
+        raise ValueError("x must be [rows, width] and weights [rows, k]")
+    rows, width = x.shape
+    top = weights.shape[1]
+    _same((rows * top,), order)
+    _same((n_experts + 1,), starts)
+    t, td = (GGML_TYPES[v] if isinstance(v, str) else int(v) for v in (ggml_type, down_type))
+    blocks = n_experts * inter * width // 256
+    for w, ty in ((w_gate, t), (w_up, t), (w_down, td)):
+        if w.numel() < blocks * GGML_BLOCK_BYTES.get(ty, 0):
+            raise ValueError(f"{n_experts} experts of {inter} x {width} exceed a tensor of {w.numel()} bytes")
+    out = torch.empty_like(x) if out is None else out
+    _dev(out, dtype=torch.float32)
+    _same(x.shape, out)
+    if workspace is None:
+        workspace = torch.empty(max(16, moe_experts_rows_workspace_bytes(rows, top, n_experts, width, inter)),
+                                dtype=torch.uint8, device=x.device)
+    _dev(workspace)
+    check(load().qwen_moe_experts_rows(_p(w_gate), _p(w_up), t, _p(w_down), td, n_experts, _p(order), _p(starts),
+                                       _p(weights), top, _p(x), rows, width, inter, _p(out), _p(workspace),
+                                       workspace.numel() * workspace.element_size(), _stream(stream)))
+    return out
+
+
 # ------------------------------------------------------------------ MoE
 def moe_silu_mul(g, u, out=None, stream=None):
     _dev(g, u, dtype=torch.float32)
