@@ -134,10 +134,10 @@ __global__ __launch_bounds__(kPlanBlock) void kv8_plan_kernel(
 // ------------------------------------------------------------------ store
 // A workgroup takes the runs that start in its share of the rows (a run: neighbouring rows with neighbouring slots of
 // one page), for one head and for keys or values: it alone writes that page's codes and scale, so no order of workgroups
-// shows in the result. Two passes over the run's fp32 rows (largest magnitude; codes): the second finds them in the
-// caches, 64 KB at 64 tokens of 256. A thread's item is 8 tokens x 4 dims: 16-byte loads, 4-byte stores of keys, 32
-// bytes in a row of values.
-constexpr int kStoreBlock = 256;
+// shows in the result. A thread's item is an octet of tokens x 4 dims: 16-byte loads, kept in registers between the
+// largest magnitude and the codes (what does not fit, past 64 tokens of 256, is read again), 4-byte stores of keys, 32
+// bytes in a row of values. Bound by latency: one round of loads, one reduction, the stores.
+constexpr int kStoreBlock = 512;
 
 template <bool ALIGNED>
 __device__ __forceinline__ float4 row4(const float* p) {
@@ -156,80 +156,99 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
                  kv8_rescale(code_of(w, 3), ratio));
 }
 
-template <bool ALIGNED, bool VALUES>
+template <int BLOCK, bool ALIGNED, bool VALUES>
 __device__ void store_run(const float* __restrict__ x, int64_t stride, int n, int8_t* __restrict__ codes, float* scale,
                           int off, int dim, uint32_t* red) {
-    const int tid = threadIdx.x, d4s = dim >> 2;
-    const int lane_d = tid % d4s, lane_t = tid / d4s, t_step = kStoreBlock / d4s;   // dim 64, 128 or 256
+    const int tid = threadIdx.x, d_shift = __builtin_ctz(dim) - 2, d4s = 1 << d_shift;   // dim 64, 128 or 256
+    const int end = off + n, o0 = off >> 3, items = (((end + 7) >> 3) - o0) << d_shift;
+    const int first_o = o0 + (tid >> d_shift), d4 = tid & (d4s - 1), o_step = BLOCK >> d_shift;
+    float4 f[8];
+    auto load = [&](int o) {   // tokens of octet o that are not in the run come out 0
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const int at = 8 * o + t - off;
+            f[t] = at >= 0 && at < n ? row4<ALIGNED>(x + at * stride + 4 * d4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
     // the run's largest magnitude, as bits: infinities and NaNs come out above every finite value
     uint32_t m = 0;
-    for (int t = lane_t; t < n; t += t_step) {
-        const float4 v = row4<ALIGNED>(x + t * stride + 4 * lane_d);
-        m = max(max(m, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu)),
-                max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+    auto take = [&]() {
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+            m = max(max(m, max(__float_as_uint(f[t].x) & 0x7fffffffu, __float_as_uint(f[t].y) & 0x7fffffffu)),
+                    max(__float_as_uint(f[t].z) & 0x7fffffffu, __float_as_uint(f[t].w) & 0x7fffffffu));
+    };
+    const bool single = items <= BLOCK;
+    if (single) {
+        load(first_o);   // past the run's end: zeros
+        take();
+    } else {
+        for (int i = tid, o = first_o; i < items; i += BLOCK, o += o_step) {
+            load(o);
+            take();
+        }
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o)));
     const float was = off ? *scale : 0.0f;   // read before the barrier that the one write comes after
     if ((tid & 63) == 0) red[tid >> 6] = m;
     __syncthreads();
-    m = max(max(red[0], red[1]), max(red[2], red[3]));
+    m = red[0];
+#pragma unroll
+    for (int w = 1; w < BLOCK / kWave; ++w) m = max(m, red[w]);
     const bool bad = m >= 0x7f800000u || was != was;
     const float s = bad ? __builtin_nanf("") : fmaxf(fmaxf(was, __uint_as_float(m) / 127.0f), kKv8Floor);
     const float rs = 1.0f / s;
     const bool again = off > 0 && !bad && s > was;   // kept codes change
     const float ratio = was / s;
-    const int end = off + n;
-    if constexpr (VALUES) {
-        for (int o = (again ? 0 : off >> 3) + lane_t; 8 * o < end; o += t_step) {
-            uint4* p = reinterpret_cast<uint4*>(codes + (static_cast<size_t>(o) * dim + 4 * lane_d) * 8);
+    auto code = [&](float v) { return static_cast<uint32_t>(static_cast<int>(kv8_code(v, s, rs))) & 0xffu; };
+    for (int i = tid, o = first_o; i < items; i += BLOCK, o += o_step) {
+        if (!single) load(o);
+        if constexpr (VALUES) {
+            uint4* p = reinterpret_cast<uint4*>(codes + (static_cast<size_t>(o) * dim + 4 * d4) * 8);
             uint32_t w[8] = {};   // [dim][tokens 0-3, 4-7]
             if (8 * o < off) {
                 const uint4 a = p[0], b = p[1];
                 const uint32_t old[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = again ? rescale4(old[i], ratio) : old[i];
+                for (int k = 0; k < 8; ++k) w[k] = again ? rescale4(old[k], ratio) : old[k];
             }
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                const int at = 8 * o + t;
-                if (at < off || at >= end) continue;
-                const float4 v = row4<ALIGNED>(x + (at - off) * stride + 4 * lane_d);
-                const float f[4] = {v.x, v.y, v.z, v.w};
+                if (8 * o + t < off || 8 * o + t >= end) continue;
+                const float v[4] = {f[t].x, f[t].y, f[t].z, f[t].w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t c = bad ? 0u : static_cast<uint32_t>(static_cast<int>(kv8_code(f[i], s, rs))) & 0xffu;
+                for (int k = 0; k < 4; ++k) {
                     const int sh = 8 * (t & 3);
-                    w[2 * i + (t >> 2)] = (w[2 * i + (t >> 2)] & ~(0xffu << sh)) | (c << sh);
+                    w[2 * k + (t >> 2)] = (w[2 * k + (t >> 2)] & ~(0xffu << sh)) | ((bad ? 0u : code(v[k])) << sh);
                 }
             }
             p[0] = make_uint4(w[0], w[1], w[2], w[3]);
             p[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+            uint32_t* p = reinterpret_cast<uint32_t*>(codes) + (static_cast<size_t>(8 * o) << d_shift) + d4;
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                if (8 * o + t >= off && 8 * o + t < end)
+                    p[t << d_shift] = bad ? 0u : code(f[t].x) | (code(f[t].y) << 8) | (code(f[t].z) << 16) | (code(f[t].w) << 24);
         }
-    } else {
-        uint32_t* p = reinterpret_cast<uint32_t*>(codes) + lane_d;
-        for (int t = (again ? 0 : off) + lane_t; t < end; t += t_step) {
-            uint32_t w = 0;
-            if (t < off) {
-                w = rescale4(p[static_cast<size_t>(t) * d4s], ratio);
-            } else if (!bad) {
-                const float4 v = row4<ALIGNED>(x + (t - off) * stride + 4 * lane_d);
-                w = pack4(kv8_code(v.x, s, rs), kv8_code(v.y, s, rs), kv8_code(v.z, s, rs), kv8_code(v.w, s, rs));
-            }
-            p[static_cast<size_t>(t) * d4s] = w;
-        }
+    }
+    if (again) {   // the page's tokens before the run (values: its octets; a shared octet has been written above)
+        uint32_t* p = reinterpret_cast<uint32_t*>(codes);
+        const int words = VALUES ? (o0 << d_shift) * 8 : off << d_shift;
+        for (int i = tid; i < words; i += BLOCK) p[i] = rescale4(p[i], ratio);
     }
     if (tid == 0) *scale = s;
     __syncthreads();   // red is used again by the next run
 }
 
 // Grid: x = shares of `share` rows (at most 64), y = head, z = keys, values.
-template <bool ALIGNED>
-__global__ __launch_bounds__(kStoreBlock) void kv8_store_kernel(const float* __restrict__ k, const float* __restrict__ v,
+template <int BLOCK, bool ALIGNED>
+__global__ __launch_bounds__(BLOCK) void kv8_store_kernel(const float* __restrict__ k, const float* __restrict__ v,
                                                                 int64_t k_stride, int64_t v_stride,
                                                                 const int32_t* __restrict__ slots, int rows, int share,
                                                                 const Kv8Cache c) {
-    __shared__ uint32_t red[kStoreBlock / kWave];
+    __shared__ uint32_t red[BLOCK / kWave];
     const int lane = threadIdx.x & 63, h = blockIdx.y, P = c.page;
     const int total = c.pages * P;
     const int r0 = blockIdx.x * share;
@@ -257,9 +276,9 @@ __global__ __launch_bounds__(kStoreBlock) void kv8_store_kernel(const float* __r
         }
         const size_t at = static_cast<size_t>(pg) * c.heads + h, block = static_cast<size_t>(P) * c.dim;
         if (blockIdx.z == 0)
-            store_run<ALIGNED, false>(k + first * k_stride + h * c.dim, k_stride, n, c.k + at * block, c.ks + at, off, c.dim, red);
+            store_run<BLOCK, ALIGNED, false>(k + first * k_stride + h * c.dim, k_stride, n, c.k + at * block, c.ks + at, off, c.dim, red);
         else
-            store_run<ALIGNED, true>(v + first * v_stride + h * c.dim, v_stride, n, c.v + at * block, c.vs + at, off, c.dim, red);
+            store_run<BLOCK, ALIGNED, true>(v + first * v_stride + h * c.dim, v_stride, n, c.v + at * block, c.vs + at, off, c.dim, red);
     }
 }
 
@@ -269,18 +288,18 @@ __global__ __launch_bounds__(kStoreBlock) void kv8_store_kernel(const float* __r
 // group, from L1 where the tokens are neighbours.
 __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Cache c, const int32_t* __restrict__ slots, int rows,
                                                        float* __restrict__ k, float* __restrict__ v) {
-    const int d4s = c.dim >> 2, per_row = c.heads * d4s;
-    const int64_t n = static_cast<int64_t>(rows) * per_row;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int r = static_cast<int>(i / per_row), rest = static_cast<int>(i - static_cast<int64_t>(r) * per_row);
-        const int h = rest / d4s, d4 = rest - h * d4s;
+    const int d_shift = __builtin_ctz(c.dim) - 2, p_shift = __builtin_ctz(c.page);
+    const uint32_t per_row = static_cast<uint32_t>(c.heads) << d_shift, n = static_cast<uint32_t>(rows) * per_row;   // below 2^31
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
+        const uint32_t r = i / per_row, rest = i - r * per_row;
+        const int h = static_cast<int>(rest >> d_shift), d4 = static_cast<int>(rest) & ((1 << d_shift) - 1);
         const int s = slots[r];
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
         if (s >= c.pages * c.page) {
             const float nan = __builtin_nanf("");
             a = b = make_float4(nan, nan, nan, nan);
         } else if (s >= 0) {
-            const int pg = s / c.page, t = s - pg * c.page;
+            const int pg = s >> p_shift, t = s & (c.page - 1);
             const size_t at = static_cast<size_t>(pg) * c.heads + h;
             const int8_t* kc = c.k + (at * c.page + t) * c.dim + 4 * d4;
             const int8_t* vc = c.v + at * c.page * c.dim + (static_cast<size_t>(t >> 3) * c.dim + 4 * d4) * 8 + (t & 7);
@@ -290,8 +309,8 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Cache c, const i
             b = make_float4(static_cast<float>(vc[0]) * vs, static_cast<float>(vc[8]) * vs, static_cast<float>(vc[16]) * vs,
                             static_cast<float>(vc[24]) * vs);
         }
-        st4(k + 4 * i, a);
-        st4(v + 4 * i, b);
+        st4(k + 4 * static_cast<size_t>(i), a);
+        st4(v + 4 * static_cast<size_t>(i), b);
     }
 }
 
@@ -333,13 +352,12 @@ int qwen_kv8_store_rows(const float* k, const float* v, int64_t k_stride, int64_
     QK_REQUIRE(rows == 1 || (k_stride >= width && v_stride >= width), "kv8_store_rows: row strides below kv_heads x dim");
     // Steps of single tokens: every row starts a run, a workgroup each. Longer ones: 16 rows to a workgroup, of which a
     // page's first row lies in one.
-    const int share = rows <= 1024 ? 1 : 16;
+    const int share = rows <= 512 ? 1 : 16;
     const dim3 grid(blocks_for(rows, share), static_cast<unsigned>(kv_heads), 2);
     const hipStream_t s = as_stream(stream);
-    if (aligned16(k) && aligned16(v) && k_stride % 4 == 0 && v_stride % 4 == 0)
-        kv8_store_kernel<true><<<grid, kStoreBlock, 0, s>>>(k, v, k_stride, v_stride, slots, rows, share, c);
-    else
-        kv8_store_kernel<false><<<grid, kStoreBlock, 0, s>>>(k, v, k_stride, v_stride, slots, rows, share, c);
+    const bool vec = aligned16(k) && aligned16(v) && k_stride % 4 == 0 && v_stride % 4 == 0;
+    const auto launch = vec ? kv8_store_kernel<kStoreBlock, true> : kv8_store_kernel<kStoreBlock, false>;
+    launch<<<grid, kStoreBlock, 0, s>>>(k, v, k_stride, v_stride, slots, rows, share, c);
     return check_launch("kv8_store_rows");
 }
 
@@ -353,6 +371,7 @@ int qwen_kv8_read_rows(const int8_t* k_codes, const int8_t* v_codes, const float
     QK_REQUIRE(slots && k && v, "kv8_read_rows: null pointer");
     QK_REQUIRE(aligned16(k) && aligned16(v), "kv8_read_rows: outputs must be 16-byte aligned");
     const int64_t items = static_cast<int64_t>(rows) * kv_heads * (dim / 4);
+    QK_REQUIRE(items <= 0x7fffffff, "kv8_read_rows: %d rows exceed one call", rows);
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((items + 255) / 256, 8192));
     kv8_read_kernel<<<grid, 256, 0, as_stream(stream)>>>(c, slots, rows, k, v);
     return check_launch("kv8_read_rows");

@@ -42,7 +42,8 @@ constexpr int kSplitBlock = kSplitWaves * kWave;
 constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
 constexpr int kTargetItems = 1024;     // pieces of the whole call
 constexpr int kMinTiles = 8;           // of a piece: two steps per wave
-constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take the split kernel
+constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take the split kernel;
+                                       // a single row always does
 constexpr int kPromptWaves = 8;
 constexpr int kPromptRows = 16 * kPromptWaves;
 constexpr float kMoves = 8.0f;         // a score past the reference by more moves it
@@ -77,7 +78,7 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int b) {
     return Request{s, e - s, min(max(len, 0), most), len > most};
 }
 __device__ __forceinline__ bool takes_split(const AttnArgs& a, const Request& r) {
-    return a.split_all || static_cast<int64_t>(r.n) * a.group <= kSplitMax;
+    return a.split_all || static_cast<int64_t>(r.n) * a.group <= max(kSplitMax, a.group);
 }
 
 // Inclusive prefix over the wave.
@@ -408,65 +409,82 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split_kernel(const AttnArgs a)
 }
 
 // ------------------------------------------------------------------ join
-// One workgroup of NW waves per (row, head): wave w takes pieces w, w + NW, ...; lanes the dims.
+// A workgroup of NW waves joins the pieces of `per` neighbouring (row, head) pairs, one after the other: wave w takes
+// pieces w, w + NW, ...; lanes the dims. Pairs in one piece (and rows of the many-row kernel) are there already: in a
+// prompt's call most workgroups only look, so they look at 16 pairs at once (a workgroup per pair took 29 us at 5000 rows
+// of 16 heads).
 template <int D, int NW>
-__global__ __launch_bounds__(NW * kWave) void combine_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(NW * kWave) void combine_kernel(const AttnArgs a, int per) {
     constexpr int V = D / kWave;
     __shared__ float sums[NW][D], ls[NW], ms[NW];
-    const int row = static_cast<int>(blockIdx.x) / a.heads;
-    if (row >= a.row_start[a.requests]) return;   // behind the last request
-    const int2 in = a.info[blockIdx.x];
-    const int pieces = in.y, slot = in.x % kRows, first = in.x / kRows;
-    if (pieces <= 1 || in.x < 0 || pieces > a.items - first) return;
     const int wv = wave_in_block(), lane = threadIdx.x & 63;
-    float m = -FLT_MAX, l = 0.f, s[V];
+    const int live = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;   // pairs of the requests' rows
+    const int pair0 = static_cast<int>(blockIdx.x) * per;
+    int2 in = make_int2(0, 0);
+    if (lane < per && pair0 + lane < live) in = a.info[pair0 + lane];
+    const bool join = in.y > 1 && in.x >= 0 && in.y <= a.items - in.x / kRows;
+    uint64_t todo = __ballot(join);   // the same in every wave
+    while (todo) {
+        const int k = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int pieces = __builtin_amdgcn_readlane(in.y, k), where = __builtin_amdgcn_readlane(in.x, k);
+        const int slot = where % kRows, first = where / kRows;
+        float m = -FLT_MAX, l = 0.f, s[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = 0.f;
-    auto at = [&](int p) { return static_cast<size_t>(first + p) * kRows + slot; };
-    constexpr int U = 4;   // pieces in flight
-    for (int p0 = wv; p0 < pieces; p0 += U * NW) {
-        float2 st[U];
-        float x[U][V];
+        for (int i = 0; i < V; ++i) s[i] = 0.f;
+        auto at = [&](int p) { return static_cast<size_t>(first + p) * kRows + slot; };
+        constexpr int U = 4;   // pieces in flight
+        for (int p0 = wv; p0 < pieces; p0 += U * NW) {
+            float2 st[U];
+            float x[U][V];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const size_t k = at(min(p0 + u * NW, pieces - 1));
-            st[u] = a.stat[k];
+            for (int u = 0; u < U; ++u) {
+                const size_t q = at(min(p0 + u * NW, pieces - 1));
+                st[u] = a.stat[q];
+                if constexpr (V == 4) {
+                    const float4 f = ld4(a.part + q * D + 4 * lane);
+                    x[u][0] = f.x, x[u][1] = f.y, x[u][2] = f.z, x[u][3] = f.w;
+                } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[u][i] = a.part[k * D + V * lane + i];
+                    for (int i = 0; i < V; ++i) x[u][i] = a.part[q * D + V * lane + i];
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p0 + u * NW >= pieces) break;
+                const float now = fmaxf(m, st[u].x);
+                const float was = __builtin_amdgcn_exp2f(m - now), f = __builtin_amdgcn_exp2f(st[u].x - now);
+                m = now;
+                l = l * was + st[u].y * f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
+            }
         }
+        __syncthreads();   // the last pair's sums have been read
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (p0 + u * NW >= pieces) break;
-            const float now = fmaxf(m, st[u].x);
-            const float was = __builtin_amdgcn_exp2f(m - now), k = __builtin_amdgcn_exp2f(st[u].x - now);
-            m = now;
-            l = l * was + st[u].y * k;
-#pragma unroll
-            for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * k;
+        for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
+        if (lane == 0) {
+            ms[wv] = m;
+            ls[wv] = l;
         }
-    }
+        __syncthreads();
+        for (int d = threadIdx.x; d < D; d += NW * kWave) {
+            float top = ms[0];
 #pragma unroll
-    for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
-    if (lane == 0) {
-        ms[wv] = m;
-        ls[wv] = l;
-    }
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += NW * kWave) {
-        float top = ms[0];
+            for (int w = 1; w < NW; ++w) top = fmaxf(top, ms[w]);
+            float sum = 0.f, tot = 0.f;
 #pragma unroll
-        for (int w = 1; w < NW; ++w) top = fmaxf(top, ms[w]);
-        float sum = 0.f, tot = 0.f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float k = __builtin_amdgcn_exp2f(ms[w] - top);
-            sum += k * sums[w][d];
-            tot += k * ls[w];
+            for (int w = 0; w < NW; ++w) {
+                const float f = __builtin_amdgcn_exp2f(ms[w] - top);
+                sum += f * sums[w][d];
+                tot += f * ls[w];
+            }
+            const size_t o = static_cast<size_t>(pair0 + k) * D + d;
+            float v = tot == 0.f ? 0.f : sum / kWeightUp / tot;
+            if (a.gate) v *= sigmoid(a.gate[o]);
+            a.out[o] = v;
         }
-        const size_t o = static_cast<size_t>(blockIdx.x) * D + d;
-        float v = tot == 0.f ? 0.f : sum / kWeightUp / tot;
-        if (a.gate) v *= sigmoid(a.gate[o]);
-        a.out[o] = v;
     }
 }
 
@@ -668,10 +686,12 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
 }
 
 // ------------------------------------------------------------------ host
-// Pieces are at most kTargetItems plus one per unit, and units at most one per 8 pairs plus one per request that has rows.
+// Pieces are at most kTargetItems plus one per unit; units at most one per 8 pairs plus one per request that has rows, and
+// at most one per 8 of the pairs with which a request still takes this kernel.
 int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
-    const int64_t pairs = static_cast<int64_t>(rows) * (heads / kv_heads);
-    return (pairs / kRows + std::min(rows, requests)) * kv_heads;
+    const int group = heads / kv_heads;
+    const int64_t pairs = static_cast<int64_t>(rows) * group, busy = std::min(rows, requests);
+    return std::min(pairs / kRows + busy, busy * blocks_for(std::max(kSplitMax, group), kRows)) * kv_heads;
 }
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
@@ -696,11 +716,13 @@ void launch(const AttnArgs& a, hipStream_t s) {
         const int64_t tiles = (pairs / kPromptRows + std::min<int64_t>(a.requests, pairs / kSplitMax + 1)) * a.c.heads;
         prompt_kernel<D><<<static_cast<unsigned>(tiles), kPromptWaves * kWave, 0, s>>>(a);
     }
-    const unsigned grid = static_cast<unsigned>(a.rows) * static_cast<unsigned>(a.heads);
-    if (grid <= 128)   // few rows: many pieces each
-        combine_kernel<D, 16><<<grid, 16 * kWave, 0, s>>>(a);
+    const unsigned pairs = static_cast<unsigned>(a.rows) * static_cast<unsigned>(a.heads);
+    if (pairs <= 128)   // few rows: many pieces each
+        combine_kernel<D, 16><<<pairs, 16 * kWave, 0, s>>>(a, 1);
+    else if (pairs <= 2048)
+        combine_kernel<D, 4><<<pairs, 4 * kWave, 0, s>>>(a, 1);
     else
-        combine_kernel<D, 4><<<grid, 4 * kWave, 0, s>>>(a);
+        combine_kernel<D, 4><<<blocks_for(pairs, 16), 4 * kWave, 0, s>>>(a, 16);
 }
 
 }  // namespace
@@ -749,7 +771,7 @@ int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_co
     a.rows = rows;
     a.heads = heads;
     a.group = heads / kv_heads;
-    a.split_all = static_cast<int64_t>(rows) * a.group <= kSplitMax;   // no request can have more
+    a.split_all = rows == 1 || static_cast<int64_t>(rows) * a.group <= kSplitMax;   // no request can have more
     a.part = reinterpret_cast<float*>(ws);
     a.stat = reinterpret_cast<float2*>(ws + l.stat);
     a.info = reinterpret_cast<int2*>(ws + l.info);

@@ -170,6 +170,13 @@ __global__ __launch_bounds__(256) void rows_prep(const float* __restrict__ x, in
 }
 
 // ------------------------------------------------------------------ the products
+// v[rt][i] = f, rt and i not known at compile time (a register array).
+__device__ __forceinline__ void replace(f32x4_t (&v)[2], int rt, int i, float f) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+        if (q == 4 * rt + i) v[q >> 2][q & 3] = f;
+}
+
 struct RowsArgs {
     const uint8_t* w[2];   // gate and up, or down
     const Tile* tiles;     // tiles[-1].expert: how many
@@ -375,28 +382,36 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 
     // lane: pairs 4 lk + i of token tile tt, row lr of each row tile
-    auto finite = [&](const f32x4_t& v, int i, int rt, int row, int xr_, int e) {
-        if (e != kRowNonFinite) return ldexpf(v[i], -e);
-        return row_dot_per_element(a.w[SWIGLU ? rt : 0], TYPE, (static_cast<uint64_t>(tl.expert) * M + row) * K,
-                                   a.x + static_cast<size_t>(xr_) * K, K);
-    };
-    auto put = [&](int tt, const f32x4_t (&v)[WR]) {
+    auto put = [&](int tt, f32x4_t (&v)[WR]) {
+        int bad = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = a.ex[xrow(16 * tt + 4 * lk + i)];
+            bad |= (e == kRowNonFinite) << i;
+#pragma unroll
+            for (int rt = 0; rt < WR; ++rt) v[rt][i] = ldexpf(v[rt][i], e == kRowNonFinite ? 0 : -e);
+        }
+        if (__ballot(bad != 0)) {   // a row of x with an infinity: its outputs element by element
+#pragma unroll 1
+            for (int q = 0; q < 4 * WR; ++q) {
+                const int i = q & 3, rt = q >> 2, row = r0 + (SWIGLU ? 0 : 16 * rt) + lr;
+                if (!((bad >> i) & 1) || row >= M) continue;
+                replace(v, rt, i, row_dot_per_element(a.w[SWIGLU ? rt : 0], TYPE, (static_cast<uint64_t>(tl.expert) * M + row) * K,
+                                                      a.x + static_cast<size_t>(xrow(16 * tt + 4 * lk + i)) * K, K));
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int t = 16 * tt + 4 * lk + i;
             if (t >= n) continue;
-            const int pos = tl.first + t, xi = xrow(t), e = a.ex[xi];
+            const int pos = tl.first + t;
             if constexpr (SWIGLU) {
-                const int row = r0 + lr;
-                if (row < M) {
-                    const float g = finite(v[0], i, 0, row, xi, e), u = finite(v[1], i, 1, row, xi, e);
-                    a.y[static_cast<size_t>(pos) * M + row] = silu(g) * u;
-                }
+                if (r0 + lr < M) a.y[static_cast<size_t>(pos) * M + r0 + lr] = silu(v[0][i]) * v[1][i];
             } else {
                 float* y = a.y + static_cast<size_t>(pair_at(a.order, pos, a.pairs)) * M;
 #pragma unroll
                 for (int rt = 0; rt < WR; ++rt)
-                    if (r0 + 16 * rt + lr < M) y[r0 + 16 * rt + lr] = finite(v[rt], i, rt, r0 + 16 * rt + lr, xi, e);
+                    if (r0 + 16 * rt + lr < M) y[r0 + 16 * rt + lr] = v[rt][i];
             }
         }
     };
@@ -427,13 +442,204 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 }
 
+// ------------------------------------------------------------------ small groups
+// Tiles of up to 8 or 16 pairs, rows of up to 8 blocks (K <= 2048): bound by the weights, each expert's read about once. A
+// workgroup's waves split the blocks of a row, KW waves a block each, so that they read a row tile whole, 16 rows of
+// neighbouring memory, at one time, and a wave keeps its block's operands of x in registers for all row tiles of a tile of
+// pairs. (Waves that went through 32 rows a block at a time, 144 bytes here and there, took 100 us for the gate and up
+// products of 77 tokens, of which 67 were the weight loads by themselves and 30 the repeated loads of x.) 8 / KW row groups;
+// a turn is one row tile of each - 16 gate and the same 16 up rows, or 32 down rows - whose blocks' sums meet in LDS, two
+// turns' worth, one barrier a turn; the waves of a group take turns in adding them up and writing.
+// The grid is one workgroup a CU, and each has an equal part of all tiles' turns: its weights are requested AHEAD turns
+// ahead, over the border of a tile too, where only the operands of x are loaded anew. (A workgroup per tile and share of its
+// rows: two rounds of some 45 us at 77 tokens. Two workgroups a CU of 128 registers, two turns ahead: 92 us against 65.)
+// Of up to 8 pairs both fp16 parts enter one operand, rows 0-7 the high ones and 8-15 the low ones: half the products, and
+// a sum of two lanes at the end (5 tokens 20.5 and 12.4 us for the two products, 22.2 and 13.6 with tiles of 16).
+// Without its arithmetic the kernel takes 57 us at 77 tokens (202 MB), 65 with it; 8 us are the start.
+template <int TYPE, int TP, int KW, bool SWIGLU>
+__global__ __launch_bounds__(512, 2) void strip_kernel(const RowsArgs a) {
+    constexpr int BB = TYPE == kQ4_K ? 144 : 210, NB = TYPE == kQ4_K ? 1 : 2, WR = 2, RW = 8 / KW;
+    constexpr int RT = SWIGLU ? 16 : 32;              // rows of a row tile
+    constexpr int NP = TP == 8 ? 1 : 2;               // operands of x per depth
+    constexpr int AHEAD = 4;                          // turns of weights in flight
+    __shared__ f32x4_t part[2][8][WR][kWave];
+    __shared__ int exps[2][TP];                       // of the rows of this tile and the one before
+    const int M = a.M, K = a.K, nb = K >> 8;
+    const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4;
+    const int wv = wave_in_block(), kw = wv % KW, rw = wv / KW;
+    const int row_tiles = (M + RT - 1) / RT, groups = (row_tiles + RW - 1) / RW;   // turns of a tile
+    const int tiles = a.tiles[-1].expert;
+    const int64_t total = static_cast<int64_t>(tiles) * groups;
+    const int64_t from = total * blockIdx.x / gridDim.x;
+    const int count = static_cast<int>(total * (blockIdx.x + 1) / gridDim.x - from);
+    if (count <= 0) return;                           // the whole workgroup
+    const int kb = min(kw, nb - 1);                   // a wave past the row's blocks repeats the last one, and adds nothing
+    const bool active = kw < nb;
+    int tile = static_cast<int>(from / groups), group = static_cast<int>(from - static_cast<int64_t>(tile) * groups);
+    // the weights' cursor
+    int lt = tile, lg = group, ln = 0;
+    const uint8_t* wexp[WR];
+    auto w_expert = [&]() {
+        const int e = a.tiles[lt].expert;
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) wexp[rt] = a.w[SWIGLU ? rt : 0] + (static_cast<uint64_t>(e) * M * nb + kb) * BB;
+    };
+    auto w_load = [&](WBlock<TYPE> (&d)[WR]) {        // past the end the last one again: nothing waits for it
+        const int r0 = min(lg * RW + rw, row_tiles - 1) * RT;
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) {
+            const uint32_t r = static_cast<uint32_t>(min(r0 + (SWIGLU ? 0 : 16 * rt) + lr, M - 1));
+            d[rt].load(wexp[rt] + static_cast<size_t>(r) * nb * BB, 0u, lk);
+        }
+        if (++ln < count && ++lg == groups) {
+            lg = 0;
+            ++lt;
+            w_expert();
+        }
+    };
+    WBlock<TYPE> w[AHEAD][WR];
+    w_expert();
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        w_load(w[i]);
+        __builtin_amdgcn_sched_barrier(0);   // in this order, which the waits of the loop below count on
+    }
+    uint32_t k64 = 0x64006400u;
+    asm volatile("" : "+v"(k64));
+    Tile tl{};
+    f16x8_t A[8][NP];
+    f16x4_t As;
+    auto row_of = [&](const Tile& q, int i) {   // row of x of a tile's pair i (the last one again past the end)
+        const int pos = q.first + min(i, q.n - 1);
+        return SWIGLU ? pair_at(a.order, pos, a.pairs) / a.top : pos;
+    };
+    int next_row = row_of(a.tiles[tile], lr % TP);
+    auto x_load = [&]() {   // the operands of tile `tile`
+        tl = a.tiles[tile];
+        const size_t mine = static_cast<size_t>(next_row);
+        const uint8_t* x0 = a.xp + mine * K * 4 + 1024 * kb + 16 * lk + (TP == 8 ? 64 * (lr >> 3) : 0);
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) A[d][p] = *reinterpret_cast<const f16x8_t*>(x0 + 128 * d + 64 * p);
+        if constexpr (TYPE == kQ4_K) {   // the minima's terms enter with the high part
+            const float2 s = *reinterpret_cast<const float2*>(a.sx + mine * (K >> 5) + 8 * kb + 2 * lk);
+            As = min_operand(TP == 16 || lr < 8 ? s : make_float2(0.f, 0.f));
+        }
+        if (wv == 0 && lane < TP) exps[tile & 1][lane] = a.ex[mine];
+        next_row = row_of(a.tiles[min(tile + 1, tiles - 1)], lr % TP);   // known when the next tile's turn comes
+    };
+    const int p0 = TP == 8 ? 4 * (lk & 1) : 4 * lk;   // the lane's first pair in the sums
+    auto finish = [&](int turn) {
+        const int row_tile = group * RW + rw, r0 = row_tile * RT;
+        f32x4_t v[WR];
+        int bad = 0;
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) {
+            v[rt] = part[turn & 1][rw * KW][rt][lane];
+#pragma unroll
+            for (int s = 1; s < KW; ++s) v[rt] += part[turn & 1][rw * KW + s][rt][lane];
+            if constexpr (TP == 8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[rt][i] += __shfl_xor(v[rt][i], 32);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = exps[tile & 1][p0 + i];
+            bad |= (e == kRowNonFinite) << i;
+#pragma unroll
+            for (int rt = 0; rt < WR; ++rt) v[rt][i] = ldexpf(v[rt][i], e == kRowNonFinite ? 0 : -e);
+        }
+        if (__ballot(bad != 0)) {   // a row of x with an infinity: its outputs element by element
+#pragma unroll 1
+            for (int q = 0; q < 4 * WR; ++q) {
+                const int i = q & 3, rt = q >> 2, row = r0 + (SWIGLU ? 0 : 16 * rt) + lr;
+                if (!((bad >> i) & 1) || row >= M) continue;
+                replace(v, rt, i, row_dot_per_element(a.w[SWIGLU ? rt : 0], TYPE, (static_cast<uint64_t>(tl.expert) * M + row) * K,
+                                                      a.x + static_cast<size_t>(row_of(tl, p0 + i)) * K, K));
+            }
+        }
+        if ((TP == 8 && lk >= 2) || row_tile >= row_tiles) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (p0 + i >= tl.n) continue;
+            const int pos = tl.first + p0 + i;
+            if constexpr (SWIGLU) {
+                if (r0 + lr < M) a.y[static_cast<size_t>(pos) * M + r0 + lr] = silu(v[0][i]) * v[1][i];
+            } else {
+                float* y = a.y + static_cast<size_t>(pair_at(a.order, pos, a.pairs)) * M;
+#pragma unroll
+                for (int rt = 0; rt < WR; ++rt)
+                    if (r0 + 16 * rt + lr < M) y[r0 + 16 * rt + lr] = v[rt][i];
+            }
+        }
+    };
+    x_load();
+    auto step = [&](WBlock<TYPE> (&wb)[WR], int turn) {
+        f32x4_t C[WR];
+        WScale<TYPE> sc[WR];
+        static_for<8>([&](auto dI) {
+            constexpr int D = decltype(dI)::value, U = D >> 1, J = D & 1;
+#pragma unroll
+            for (int rt = 0; rt < WR; ++rt) {
+                if constexpr (J == 0) sc[rt].template set<U>(wb[rt], lk);
+                f16x8_t B[NB];
+                decode<U, J>(wb[rt], sc[rt], k64, B);
+                C[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[D][0], B[0], D == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : C[rt], 0, 0, 0);
+                if constexpr (NP == 2) C[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[D][1], B[0], C[rt], 0, 0, 0);
+                if constexpr (NB == 2) C[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[D][0], B[NB - 1], C[rt], 0, 0, 0);
+            }
+        });
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) {
+            f32x4_t s;
+            if constexpr (TYPE == kQ4_K) {
+                const float d = opaque(half_bits(wb[rt].hd.x & 0xffffu)), dmin = opaque(-32.0f * half_bits(wb[rt].hd.x >> 16));
+                const f32x4_t pm =
+                    __builtin_amdgcn_mfma_f32_16x16x16f16(As, min_weights(wb[rt].hd, lk), f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(dmin, pm[i], d * C[rt][i]);
+            } else {
+                const float d = opaque(half_bits(wb[rt].d));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] = d * C[rt][i];
+            }
+            part[turn & 1][wv][rt][lane] = active ? s : f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        w_load(wb);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the sums are in LDS (the loads of weights stay in flight)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (turn % KW == kw) finish(turn);
+        if (++group == groups) {
+            group = 0;
+            ++tile;
+            if (turn + 1 < count) x_load();
+        }
+    };
+    // Left from the middle, not skipped over: so that on every way back to the first step the other buffers' loads have been
+    // issued after its own, and it waits for its own alone.
+    for (int u = 0;;) {
+        step(w[0], u);
+        if (++u == count) break;
+        step(w[1], u);
+        if (++u == count) break;
+        step(w[2], u);
+        if (++u == count) break;
+        step(w[3], u);
+        if (++u == count) break;
+    }
+}
+
 // out[t] = sum_j w[t][j] y[t k + j], j in order; NaN for a token one of whose pairs has no expert (y has no row of it).
 __global__ __launch_bounds__(256) void rows_combine(const float* __restrict__ y, const float* __restrict__ w,
                                                     const int* __restrict__ lost, int rows, int k, int dim4,
                                                     float* __restrict__ out) {
-    const int64_t n = static_cast<int64_t>(rows) * dim4;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int t = static_cast<int>(i / dim4), d4 = static_cast<int>(i - static_cast<int64_t>(t) * dim4);
+    const int per = (dim4 + 255) / 256;   // workgroups of a row
+    for (int64_t b = blockIdx.x; b < static_cast<int64_t>(rows) * per; b += gridDim.x) {
+        const int t = static_cast<int>(b / per), d4 = static_cast<int>(b - static_cast<int64_t>(t) * per) * 256 + static_cast<int>(threadIdx.x);
+        if (d4 >= dim4) continue;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         const float* yt = y + (static_cast<size_t>(t) * k * dim4 + d4) * 4;
         for (int j = 0; j < k; ++j) {
@@ -445,17 +651,19 @@ __global__ __launch_bounds__(256) void rows_combine(const float* __restrict__ y,
             o.w = __builtin_fmaf(a, v.w, o.w);
         }
         if (lost[t]) o = make_float4(__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""));
-        st4(out + 4 * i, o);
+        st4(out + (static_cast<size_t>(t) * dim4 + d4) * 4, o);
     }
 }
 
 // ------------------------------------------------------------------ host
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
-// Pairs of a tile by the mean group size.
-int tile_pairs(int64_t pairs, int experts) {
+// Pairs of a tile, and with them the kernel, by the mean size of the groups (those of a routing over all experts):
+// strip_kernel with tiles of 8 or 16 pairs, rows_kernel with 32 or 64.
+int tile_pairs(int64_t pairs, int experts, int width, int inter) {
     const double mean = static_cast<double>(pairs) / std::min<int64_t>(pairs, experts);
-    return mean <= 8 ? 16 : mean <= 20 ? 32 : 64;
+    if (mean <= 8 && std::max(width, inter) <= 2048) return mean <= 1.5 ? 8 : 16;
+    return mean <= 20 ? 32 : 64;
 }
 int64_t tile_bound(int64_t pairs, int experts, int size) { return pairs / size + std::min<int64_t>(pairs, experts); }
 
@@ -466,7 +674,7 @@ struct Layout {
 Layout layout(int rows, int top, int experts, int width, int inter) {
     const size_t pairs = static_cast<size_t>(rows) * top;
     Layout l;
-    l.tiles = tile_bound(pairs, experts, tile_pairs(pairs, experts));
+    l.tiles = tile_bound(pairs, experts, tile_pairs(pairs, experts, width, inter));
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
@@ -494,16 +702,29 @@ void launch_rows(RowsArgs a, int64_t tiles, hipStream_t s) {
     rows_kernel<TYPE, WT, KW, SWIGLU><<<static_cast<unsigned>(tiles * a.column_blocks), 512, 0, s>>>(a);
 }
 
+template <int TYPE, int TP, int KW, bool SWIGLU>
+void launch_strip(const RowsArgs& a, hipStream_t s) {
+    strip_kernel<TYPE, TP, KW, SWIGLU><<<256, 512, 0, s>>>(a);   // one a CU
+}
+
+template <int TYPE, int TP, bool SWIGLU>
+void launch_small(const RowsArgs& a, hipStream_t s) {
+    const int nb = a.K / 256;   // at most 8
+    if (nb > 4)
+        launch_strip<TYPE, TP, 8, SWIGLU>(a, s);
+    else if (nb > 2)
+        launch_strip<TYPE, TP, 4, SWIGLU>(a, s);
+    else
+        launch_strip<TYPE, TP, 2, SWIGLU>(a, s);
+}
+
 template <int TYPE, bool SWIGLU>
 void launch_type(const RowsArgs& a, int size, int64_t tiles, hipStream_t s) {
     const int nb = a.K / 256;
-    if (size == 16) {
-        if (nb % 4 == 0)
-            launch_rows<TYPE, 1, 4, SWIGLU>(a, tiles, s);
-        else if (nb % 2 == 0)
-            launch_rows<TYPE, 1, 2, SWIGLU>(a, tiles, s);
-        else
-            launch_rows<TYPE, 2, 1, SWIGLU>(a, tiles, s);   // half of the tile unused
+    if (size == 8) {
+        launch_small<TYPE, 8, SWIGLU>(a, s);
+    } else if (size == 16) {
+        launch_small<TYPE, 16, SWIGLU>(a, s);
     } else if (size == 32) {
         if (nb % 2 == 0)
             launch_rows<TYPE, 2, 2, SWIGLU>(a, tiles, s);
@@ -564,7 +785,7 @@ int qwen_moe_experts_rows(const void* w_gate, const void* w_up, int type, const 
                "moe_experts_rows: workspace of %zu bytes, need %zu (16-byte aligned)", workspace_bytes, l.bytes);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const hipStream_t s = as_stream(stream);
-    const int pairs = rows * top, size = tile_pairs(pairs, n_experts);
+    const int pairs = rows * top, size = tile_pairs(pairs, n_experts, width, inter);
     Tile* tiles = reinterpret_cast<Tile*>(ws + l.table) + 1;
     int* lost = reinterpret_cast<int*>(ws + l.lost);
     const Grouping gr{order, starts, tiles, lost, n_experts, pairs, top, size, static_cast<int>(l.tiles)};
@@ -598,8 +819,8 @@ int qwen_moe_experts_rows(const void* w_gate, const void* w_up, int type, const 
     a.M = width;
     a.K = inter;
     launch_product<false>(down_type, a, size, l.tiles, s);
-    const int64_t n4 = static_cast<int64_t>(rows) * (width / 4);
-    rows_combine<<<static_cast<unsigned>(std::min<int64_t>((n4 + 255) / 256, 8192)), 256, 0, s>>>(
+    const int64_t strips = static_cast<int64_t>(rows) * blocks_for(width / 4, 256);
+    rows_combine<<<static_cast<unsigned>(std::min<int64_t>(strips, 1 << 16)), 256, 0, s>>>(
         y, weights, lost, rows, top, width / 4, out);
     return check_launch("moe_experts_rows");
 }

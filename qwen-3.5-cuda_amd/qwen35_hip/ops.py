@@ -570,17 +570,22 @@ def kv8_plan(cached, fresh, block_table, free_pages, free_head, page_size, rows,
     if block_table.dim() != 2 or block_table.shape[0] != n:
         raise ValueError("block_table must be [requests, max_pages]")
     _same((1,), free_head)
-    i32 = dict(dtype=torch.int32, device=cached.device)
-    free_head_out = torch.empty(1, **i32) if free_head_out is None else free_head_out
-    row_start = torch.empty(n + 1, **i32) if row_start is None else row_start
-    kv_len = torch.empty(n, **i32) if kv_len is None else kv_len
-    slots = torch.empty(rows, **i32) if slots is None else slots
-    pos = torch.empty(rows, **i32) if pos is None else pos
-    _dev(free_head_out, row_start, kv_len, slots, pos, dtype=torch.int32)
-    _same((1,), free_head_out)
-    _same((n + 1,), row_start)
-    _same((n,), kv_len)
-    _same((rows,), slots, pos)
+    if row_start is None and kv_len is None and slots is None and pos is None and free_head_out is None:
+        # five outputs in one allocation
+        row_start, kv_len, slots, pos, free_head_out = torch.empty(
+            2 * n + 2 * rows + 2, dtype=torch.int32, device=cached.device).split((n + 1, n, rows, rows, 1))
+    else:
+        i32 = dict(dtype=torch.int32, device=cached.device)
+        free_head_out = torch.empty(1, **i32) if free_head_out is None else free_head_out
+        row_start = torch.empty(n + 1, **i32) if row_start is None else row_start
+        kv_len = torch.empty(n, **i32) if kv_len is None else kv_len
+        slots = torch.empty(rows, **i32) if slots is None else slots
+        pos = torch.empty(rows, **i32) if pos is None else pos
+        _dev(free_head_out, row_start, kv_len, slots, pos, dtype=torch.int32)
+        _same((1,), free_head_out)
+        _same((n + 1,), row_start)
+        _same((n,), kv_len)
+        _same((rows,), slots, pos)
     check(load().qwen_kv8_plan(_p(cached), _p(fresh), n, _p(block_table), block_table.shape[1], _p(free_pages),
                                free_pages.numel(), _p(free_head), _p(free_head_out), page_size, rows, _p(row_start),
                                _p(kv_len), _p(slots), _p(pos), _stream(stream)))

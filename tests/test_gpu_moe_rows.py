@@ -143,6 +143,7 @@ def check(layer, idx, w, x, **kw):
 @pytest.mark.parametrize("kind,down", [("Q4_K", "Q4_K"), ("Q6_K", "Q6_K"), ("Q4_K", "Q6_K")])
 @pytest.mark.parametrize("rows,top,experts,inter,width", [
     (1, 1, 1, 256, 256), (1, 8, 16, 512, 2048), (5, 8, 16, 512, 2048), (3, 2, 7, 256, 768),       # groups of a few pairs
+    (2, 3, 40, 1280, 512), (4, 4, 9, 2048, 1024), (3, 2, 4, 256, 2304), (9, 3, 5, 2560, 256),      # and rows past 8 blocks
     (40, 4, 16, 256, 512), (33, 3, 5, 512, 256), (21, 8, 12, 1280, 512),                           # of 10 to 20
     (100, 4, 6, 512, 2048), (130, 1, 2, 256, 256), (67, 2, 3, 768, 768),                           # of 45 and more
 ])
