@@ -12,7 +12,6 @@ torch is used for device memory and streams only.
 from __future__ import annotations
 
 import ctypes
-from typing import NamedTuple
 
 import torch
 
@@ -530,13 +529,31 @@ def attn_decode_noalloc(q, k_cache, v_cache, heads, kv_heads, dim, pos, gate=Non
 
 
 # ------------------------------------------------------------------ several requests: a paged 8-bit KV cache
-class Kv8Cache(NamedTuple):
+def _checked(dtype, *ts) -> None:
+    """_dev with a dtype, for calls of a few microseconds."""
+    for t in ts:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.is_contiguous()):
+            _dev(t, dtype=dtype)
+
+
+class Kv8Cache:
     """int8 codes and float32 scales of a paged cache (qwen35_hip.h): k [pages, kv_heads, page, dim],
-    v [pages, kv_heads, page / 8, dim, 8], k_scale, v_scale [pages, kv_heads]."""
-    k: torch.Tensor
-    v: torch.Tensor
-    k_scale: torch.Tensor
-    v_scale: torch.Tensor
+    v [pages, kv_heads, page / 8, dim, 8], k_scale, v_scale [pages, kv_heads]. Checked once, here."""
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "page", "heads", "dim", "args")
+
+    def __init__(self, k, v, k_scale, v_scale):
+        _checked(torch.int8, k, v)
+        _checked(torch.float32, k_scale, v_scale)
+        if k.dim() != 4:
+            raise ValueError("cache keys must be [pages, kv_heads, page, dim]")
+        pages, heads, page, dim = k.shape
+        if v.shape != (pages, heads, page // 8, dim, 8):
+            _same((pages, heads, page // 8, dim, 8), v)
+        if k_scale.shape != (pages, heads) or v_scale.shape != (pages, heads):
+            _same((pages, heads), k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.page, self.heads, self.dim = pages, page, heads, dim
+        self.args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page, heads, dim)
 
 
 def kv8_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv8Cache:
@@ -548,28 +565,17 @@ def kv8_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv8Cache:
                     torch.zeros((pages, kv_heads), **scales), torch.zeros((pages, kv_heads), **scales))
 
 
-def _kv8_check(cache):
-    _dev(cache.k, cache.v, dtype=torch.int8)
-    _dev(cache.k_scale, cache.v_scale, dtype=torch.float32)
-    if cache.k.dim() != 4:
-        raise ValueError("cache keys must be [pages, kv_heads, page, dim]")
-    pages, heads, page, dim = cache.k.shape
-    _same((pages, heads, page // 8, dim, 8), cache.v)
-    _same((pages, heads), cache.k_scale, cache.v_scale)
-    return pages, page, heads, dim
-
-
 def kv8_plan(cached, fresh, block_table, free_pages, free_head, page_size, rows, free_head_out=None, row_start=None,
              kv_len=None, slots=None, pos=None, stream=None):
     """The bookkeeping of a step of several requests: cached, fresh int32 [requests]; block_table int32
     [requests, max_pages] in place; free_pages int32 [n], free_head int32 [1]
     -> (row_start [requests + 1], kv_len [requests], slots [rows], pos [rows], free_head_out [1])."""
-    _dev(cached, fresh, block_table, free_pages, free_head, dtype=torch.int32)
+    _checked(torch.int32, cached, fresh, block_table, free_pages, free_head)
     n = cached.numel()
-    _same((n,), cached, fresh)
+    if fresh.numel() != n or cached.dim() != 1 or free_head.numel() != 1:
+        raise ValueError("cached and fresh must be [requests], free_head [1]")
     if block_table.dim() != 2 or block_table.shape[0] != n:
         raise ValueError("block_table must be [requests, max_pages]")
-    _same((1,), free_head)
     if row_start is None and kv_len is None and slots is None and pos is None and free_head_out is None:
         # five outputs in one allocation
         row_start, kv_len, slots, pos, free_head_out = torch.empty(
@@ -594,38 +600,43 @@ def kv8_plan(cached, fresh, block_table, free_pages, free_head, page_size, rows,
 
 def _kv_rows(x, heads, dim):
     """Row stride of x [rows, kv_heads, dim]: rows may lie apart (a slice of wider rows), each in one piece."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.float32:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype is not torch.float32:
         raise ValueError("expected a float32 device tensor")
-    if x.dim() != 3 or tuple(x.shape[1:]) != (heads, dim):
+    if x.dim() != 3 or x.shape[1:] != (heads, dim):
         raise ValueError(f"expected [rows, {heads}, {dim}], got {tuple(x.shape)}")
-    if x.shape[0] and (x.stride(2) != 1 or (heads > 1 and x.stride(1) != dim)):
+    if x.is_contiguous():
+        return heads * dim
+    s = x.stride()
+    if s[2] != 1 or (heads > 1 and s[1] != dim):
         raise ValueError("expected rows of kv_heads x dim in one piece")
-    return x.stride(0) if x.shape[0] > 1 else heads * dim
+    return s[0] if x.shape[0] > 1 else heads * dim
 
 
 def kv8_store_rows(k, v, slots, cache: Kv8Cache, stream=None):
     """k, v [rows, kv_heads, dim] (rows may be strided) quantized into `slots` int32 [rows] of the cache, in place."""
-    pages, page, heads, dim = _kv8_check(cache)
-    ks, vs = _kv_rows(k, heads, dim), _kv_rows(v, heads, dim)
-    _dev(slots, dtype=torch.int32)
-    _same((k.shape[0],), slots)
-    _same(k.shape, v)
-    check(load().qwen_kv8_store_rows(_p(k), _p(v), ks, vs, _p(slots), k.shape[0], _p(cache.k), _p(cache.v),
-                                     _p(cache.k_scale), _p(cache.v_scale), pages, page, heads, dim, _stream(stream)))
+    ks, vs = _kv_rows(k, cache.heads, cache.dim), _kv_rows(v, cache.heads, cache.dim)
+    _checked(torch.int32, slots)
+    rows = k.shape[0]
+    if slots.numel() != rows or v.shape[0] != rows:
+        raise ValueError(f"{slots.numel()} slots and {v.shape[0]} value rows for {rows} key rows")
+    check(load().qwen_kv8_store_rows(k.data_ptr(), v.data_ptr(), ks, vs, slots.data_ptr(), rows, *cache.args,
+                                     _stream(stream)))
     return cache
 
 
 def kv8_read_rows(cache: Kv8Cache, slots, k=None, v=None, stream=None):
     """The values of `slots` int32 [rows] -> k, v float32 [rows, kv_heads, dim]."""
-    pages, page, heads, dim = _kv8_check(cache)
-    _dev(slots, dtype=torch.int32)
-    shape = (slots.numel(), heads, dim)
-    k = torch.empty(shape, dtype=torch.float32, device=slots.device) if k is None else k
-    v = torch.empty(shape, dtype=torch.float32, device=slots.device) if v is None else v
-    _dev(k, v, dtype=torch.float32)
-    _same(shape, k, v)
-    check(load().qwen_kv8_read_rows(_p(cache.k), _p(cache.v), _p(cache.k_scale), _p(cache.v_scale), pages, page, heads,
-                                    dim, _p(slots), slots.numel(), _p(k), _p(v), _stream(stream)))
+    _checked(torch.int32, slots)
+    n = slots.numel()
+    shape = (n, cache.heads, cache.dim)
+    if k is None and v is None:
+        k, v = torch.empty((2, *shape), dtype=torch.float32, device=slots.device).unbind()
+    else:
+        k = torch.empty(shape, dtype=torch.float32, device=slots.device) if k is None else k
+        v = torch.empty(shape, dtype=torch.float32, device=slots.device) if v is None else v
+        _dev(k, v, dtype=torch.float32)
+        _same(shape, k, v)
+    check(load().qwen_kv8_read_rows(*cache.args, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _stream(stream)))
     return k, v
 
 
@@ -636,30 +647,30 @@ def attn_kv8_workspace_bytes(rows, requests, heads, kv_heads, dim) -> int:
 def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None, workspace=None, out=None, stream=None):
     """q [rows, heads, dim] of several requests (rows row_start[b] .. row_start[b + 1] - 1 are the last positions of
     request b's kv_len[b] tokens, in the pages block_table[b]) -> out [rows, heads, dim] (x sigmoid(gate)), causal."""
-    pages, page, kv_heads, dim = _kv8_check(cache)
-    _dev(q, dtype=torch.float32)
-    if q.dim() != 3 or q.shape[2] != dim:
-        raise ValueError(f"q must be [rows, heads, {dim}], got {tuple(q.shape)}")
+    _checked(torch.float32, q)
+    if q.dim() != 3 or q.shape[2] != cache.dim:
+        raise ValueError(f"q must be [rows, heads, {cache.dim}], got {tuple(q.shape)}")
     rows, heads, _ = q.shape
-    _dev(block_table, row_start, kv_len, dtype=torch.int32)
+    _checked(torch.int32, block_table, row_start, kv_len)
     n = kv_len.numel()
-    if block_table.dim() != 2 or block_table.shape[0] != n:
-        raise ValueError("block_table must be [requests, max_pages]")
-    _same((n,), kv_len)
-    _same((n + 1,), row_start)
+    if block_table.dim() != 2 or block_table.shape[0] != n or row_start.numel() != n + 1:
+        raise ValueError("block_table must be [requests, max_pages] and row_start [requests + 1]")
     if gate is not None:
-        _dev(gate, dtype=torch.float32)
-        _same(q.shape, gate)
-    out = torch.empty_like(q) if out is None else out
-    _dev(out, dtype=torch.float32)
-    _same(q.shape, out)
+        _checked(torch.float32, gate)
+        if gate.shape != q.shape:
+            _same(q.shape, gate)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _checked(torch.float32, out)
+        if out.shape != q.shape:
+            _same(q.shape, out)
     if workspace is None:
-        workspace = torch.empty(max(16, attn_kv8_workspace_bytes(rows, n, heads, kv_heads, dim)), dtype=torch.uint8,
+        workspace = torch.empty(max(16, attn_kv8_workspace_bytes(rows, n, heads, cache.heads, cache.dim)), dtype=torch.uint8,
                                 device=q.device)
     _dev(workspace)
-    check(load().qwen_attn_kv8_rows(_p(q), _p(cache.k), _p(cache.v), _p(cache.k_scale), _p(cache.v_scale), pages, page,
-                                    _p(block_table), block_table.shape[1], _p(row_start), _p(kv_len), n, _p(gate),
-                                    _p(out), rows, heads, kv_heads, dim, _p(workspace),
+    check(load().qwen_attn_kv8_rows(_p(q), *cache.args[:6], _p(block_table), block_table.shape[1], _p(row_start),
+                                    _p(kv_len), n, _p(gate), _p(out), rows, heads, cache.heads, cache.dim, _p(workspace),
                                     workspace.numel() * workspace.element_size(), _stream(stream)))
     return out
 
@@ -866,13 +877,16 @@ GGML_BLOCK_BYTES = {12: 144, 14: 210}   # of 256 elements: Q4_K, Q6_K
 def moe_group_rows(idx, n_experts: int, order=None, starts=None, stream=None):
     """idx int32 [rows, k] (moe_topk_rows) -> order int32 [rows * k]: the pairs t * k + j sorted by expert, equal ones in
     their order; starts int32 [n_experts + 1]: where each expert's pairs begin."""
-    _dev(idx, dtype=torch.int32)
+    _checked(torch.int32, idx)
     n = idx.numel()
-    order = torch.empty(n, dtype=torch.int32, device=idx.device) if order is None else order
-    starts = torch.empty(n_experts + 1, dtype=torch.int32, device=idx.device) if starts is None else starts
-    _dev(order, starts, dtype=torch.int32)
-    _same((n,), order)
-    _same((n_experts + 1,), starts)
+    if order is None and starts is None:
+        order, starts = torch.empty(n + n_experts + 1, dtype=torch.int32, device=idx.device).split((n, n_experts + 1))
+    else:
+        order = torch.empty(n, dtype=torch.int32, device=idx.device) if order is None else order
+        starts = torch.empty(n_experts + 1, dtype=torch.int32, device=idx.device) if starts is None else starts
+        _dev(order, starts, dtype=torch.int32)
+        _same((n,), order)
+        _same((n_experts + 1,), starts)
     check(load().qwen_moe_group_rows(_p(idx), n, n_experts, _p(order), _p(starts), _stream(stream)))
     return order, starts
 
@@ -885,15 +899,15 @@ def moe_experts_rows(w_gate, w_up, ggml_type, w_down, down_type, n_experts, orde
                      workspace=None, stream=None):
     """x [rows, width], weights [rows, k], order / starts of moe_group_rows -> out [rows, width]:
     out[t] = sum_j weights[t, j] Wd_e (SiLU(Wg_e x_t) * (Wu_e x_t)), e the expert of pair t * k + j."""
-    _dev(w_gate, w_up, w_down, dtype=torch.uint8)
-    _dev(order, starts, dtype=torch.int32)
-    _dev(weights, x, dtype=torch.float32)
+    _checked(torch.uint8, w_gate, w_up, w_down)
+    _checked(torch.int32, order, starts)
+    _checked(torch.float32, weights, x)
     if x.dim() != 2 or weights.dim() != 2 or weights.shape[0] != x.shape[0]:
         raise ValueError("x must be [rows, width] and weights [rows, k]")
     rows, width = x.shape
     top = weights.shape[1]
-    _same((rows * top,), order)
-    _same((n_experts + 1,), starts)
+    if order.numel() != rows * top or starts.numel() != n_experts + 1:
+        raise ValueError(f"order and starts must be [{rows * top}] and [{n_experts + 1}]")
     t, td = (GGML_TYPES[v] if isinstance(v, str) else int(v) for v in (ggml_type, down_type))
     blocks = n_experts * inter * width // 256
     for w, ty in ((w_gate, t), (w_up, t), (w_down, td)):
