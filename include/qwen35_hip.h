@@ -363,8 +363,8 @@ int qwen_kv8_read_rows(const int8_t* k_codes, const int8_t* v_codes, const float
                        int pages, int page_size, int kv_heads, int dim, const int32_t* slots, int rows, float* k,
                        float* v, void* stream);
 
-/* Attention of the step's rows: q, out [rows x heads x dim], gate like out or NULL. Row i of request b's n rows stands at
- * position p = kv_len[b] - n + i and sees keys 0 .. p:
+/* Attention of the step's rows: q, out [rows x heads x dim], gate like out or NULL (16-byte aligned). Row i of
+ * request b's n rows stands at position p = kv_len[b] - n + i and sees keys 0 .. p:
  *   out = sum_t softmax_t(q . k_t / sqrt(dim)) v_t  (* sigmoid(gate)), fp32 accuracy over the codes' exact values.
  * Zeros where p < 0; a page id outside the cache, or a table row too short, makes the rows that see it NaN. Rows behind
  * row_start[requests] are left as they were. heads a multiple of kv_heads, rows * heads <= 2^24; out must not overlap

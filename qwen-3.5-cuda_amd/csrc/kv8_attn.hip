@@ -20,11 +20,13 @@
 // that share a KV head - 16 columns: 8 rows x 2 fp16 parts - and a range of 32-token tiles, its 4 waves every fourth tile,
 // straight from the cache to operand registers. The ranges are cut so that the whole call, ragged requests and all, is
 // about kTargetItems equal pieces; every workgroup works that out from the lengths, so nothing is planned on the host.
-// combine_kernel joins the pieces. prompt_kernel (many rows): bound by the MFMAs. 128 rows per workgroup, both parts of
-// a row in its column, the codes turned to fp16 once per workgroup into LDS.
+// combine_kernel joins the pieces. prompt_kernel (many rows): bound by the MFMAs. 128 rows per workgroup on
+// v_mfma_f32_32x32x16_f16, the codes turned to fp16 once per workgroup into LDS.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
+#include <utility>
 
 #include "capi_common.hpp"
 #include "device_common.hpp"
@@ -44,8 +46,6 @@ constexpr int kTargetItems = 1024;     // pieces of the whole call
 constexpr int kMinTiles = 8;           // of a piece: two steps per wave
 constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take the split kernel;
                                        // a single row always does
-constexpr int kPromptWaves = 8;
-constexpr int kPromptRows = 16 * kPromptWaves;
 constexpr float kMoves = 8.0f;         // a score past the reference by more moves it
 constexpr float kWeightUp = 64.0f;     // weights (up to 2^8) enter fp16 times 2^6
 
@@ -489,17 +489,40 @@ __global__ __launch_bounds__(NW * kWave) void combine_kernel(const AttnArgs a, i
 }
 
 // ------------------------------------------------------------------ many rows
+// 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: an operand of keys or values, 1 KB of LDS, feeds 2
+// products (both parts of 32 rows), 64 cycles, so that the waves' reads take half of the LDS's rate; with 16 rows a wave they
+// took all of it (5000 rows 690 us, now 560). A wave holds its rows' query parts (128 registers at D = 256, pinned in
+// accumulation registers) and sums (128). Its vector work - softmax, turning codes to fp16 - is laid between its own
+// products: while tile t + 1's scores are computed, tile t's are exponentiated; while tile t's values are summed, the codes
+// of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own rows may end one earlier:
+// with a branch around the products the compiler moves the sums between register files at each.
+// The scores^T tile has token rho = 8 b + 4 g + j of the 32 in register 4 b + j of lane half g; key row rho stands for token
+// 16 (b / 2) + 8 g + 4 (b % 2) + j, so that a lane's registers 8 s .. 8 s + 7 are octet 2 s + g, its share of the second
+// product's depth s.
+constexpr int kPromptWaves = 4;
+constexpr int kPromptRows = 32 * kPromptWaves;
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <int S>
+using IC = std::integral_constant<int, S>;
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
+    (f(IC<I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    static_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
 template <int D>
 __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const AttnArgs a) {
-    constexpr int NJ = D / 64, ND = D / 32, NT = D == 64 ? 128 : 64, NTH = kPromptWaves * kWave;
-    constexpr int UK = NT * (D / 16) / NTH;   // 16-byte pieces of keys (and of values) per thread and step
-    static_assert(UK >= 1 && NT * (D / 16) % NTH == 0, "shape");
-    // fp16 operands in the order in which a wave reads them: [16-token tile or 32-token group][depth or dim tile][lane]
-    __shared__ __align__(16) f16x8_t ks[2][NT / 16][2 * NJ][kWave];
-    __shared__ __align__(16) f16x8_t vs[2][NT / 32][2 * ND][kWave];
-    __shared__ float scl[2][2][NT / 8];   // [slot][key, value][octet]
+    constexpr int ND = D / 16, DT = D / 32, NTH = kPromptWaves * kWave;
+    constexpr int UK = D > 128 ? D / 128 : 1;   // a lane's 16-byte pieces of a tile's keys, and of its values
+    __shared__ __align__(16) f16x8_t ks[2][ND][kWave];
+    __shared__ __align__(16) f16x8_t vs[2][DT][2][kWave];
+    __shared__ float scl[2][4][4];   // [key, value][tile % 4][octet]
     // which request, KV head and row tile: the last row tiles (the longest rows) first
-    const int G = a.group, lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4;
+    const int G = a.group, lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
     int b = -1;
     int64_t item = blockIdx.x;
     for (int b0 = 0; b0 < a.requests && b < 0; b0 += kWave) {
@@ -524,165 +547,323 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
     const int unit = __builtin_amdgcn_readfirstlane(static_cast<int>(item));
     const int h = unit % a.c.heads, rt = tiles - 1 - unit / a.c.heads;
     const int wv = wave_in_block(), tid = threadIdx.x;
-    const int mine = rt * kPromptRows + 16 * wv + lr;
-    const int rr = min(mine, pairs - 1);
+    const int row0 = rt * kPromptRows + 32 * wv;             // the wave's first pair
+    const int rr = min(row0 + col, pairs - 1);
     const int ti = rr / G, head = h * G + (rr - ti * G);
     const int limit = r.len - r.n + ti;
-    const int wave_first = r.len - r.n + min(rt * kPromptRows + 16 * wv, pairs - 1) / G;
-    const int wave_seen = r.len - r.n + min(rt * kPromptRows + 16 * wv + 15, pairs - 1) / G + 1;
+    const int wave_first = r.len - r.n + min(row0, pairs - 1) / G;
     const int seen = max(r.len - r.n + min(rt * kPromptRows + kPromptRows - 1, pairs - 1) / G + 1, 0);
-    const int steps = (seen + NT - 1) / NT;
+    const int steps = (seen + 31) / 32;
     const int P = a.c.page;
-    const size_t block = static_cast<size_t>(P) * D;
+    const int block_shift = a.page_shift + (D == 64 ? 6 : D == 128 ? 7 : 8);   // of a page and head, as a power of two
 
+    // A wave brings one octet of tokens of each tile: page, offset and scales are the same for its lanes. A lane's pieces:
+    // keys (token lane % 8, 16 dims), values (pair of dims 2 lane); at D = 64 half of the lanes have one. Octets past the
+    // last are loaded from page 0 and never read from LDS. Page ids are read a tile ahead of the codes they lead to.
     uint4 kr[UK], vr[UK];
-    float sr = 0.f;
-    auto load = [&](int st) {
-        const int t0 = st * NT;
-#pragma unroll
-        for (int i = 0; i < UK; ++i) {
-            const int u = tid + i * NTH;
-            const int tok = u / (D / 16), ch = u % (D / 16);          // keys: token, 16-dim piece
-            const Octet o = octet(a, b, h, (t0 + tok) & ~7, seen);
-            kr[i] = ld16(a.c.k + o.base * block + static_cast<size_t>((t0 + tok) & (P - 1)) * D + 16 * ch);
-            const int oc = u / (D / 2), dp = u % (D / 2);             // values: octet, pair of dims
-            const Octet ov = octet(a, b, h, t0 + 8 * oc, seen);
-            vr[i] = ld16(a.c.v + ov.base * block + (static_cast<size_t>(((t0 + 8 * oc) & (P - 1)) >> 3) * D + 2 * dp) * 8);
-        }
-        if (tid < 2 * (NT / 8)) {
-            const Octet o = octet(a, b, h, t0 + 8 * (tid % (NT / 8)), seen);
-            sr = (tid < NT / 8 ? a.c.ks : a.c.vs)[o.base];
-            if (!o.live) sr = 0.f;
-            if (o.bad) sr = __builtin_nanf("");
-        }
+    float ksr = 0.f, vsr = 0.f;   // the octet's two scales
+    bool sdead = false, sbad = false;
+    const bool some = D > 64 || lane < 32;
+    const uint32_t ko = static_cast<uint32_t>((lane & 7) * D + 16 * (some ? lane >> 3 : 0)), vo = 16 * (some ? lane : 0);
+    int id = 0;
+    size_t off[3];   // of the octet in tiles st + 1, st + 2, st + 3
+    auto next_id = [&](int st) {   // the table's entry for the octet (any in-bounds entry past the row's end)
+        id = a.table[static_cast<size_t>(b) * a.max_pages + min((32 * st + 8 * wv) >> a.page_shift, a.max_pages - 1)];
     };
-    auto store = [&](int slot) {
+    auto k_load = [&](int st) {
+        const int tok = 32 * st + 8 * wv, page = __builtin_amdgcn_readfirstlane(id);
+        sdead = tok >= seen;
+        sbad = !sdead && (page < 0 || page >= a.c.pages);
+        const size_t base = static_cast<size_t>(static_cast<uint32_t>(sdead || sbad ? 0 : page)) * a.c.heads + h;
+        off[0] = off[1];
+        off[1] = off[2];
+        off[2] = (base << block_shift) + static_cast<uint32_t>((tok & (a.c.page - 1)) * D);
+        const int8_t* p = a.c.k + off[2];
 #pragma unroll
-        for (int i = 0; i < UK; ++i) {
-            const int u = tid + i * NTH;
-            const int tok = u / (D / 16), ch = u % (D / 16);
-            // token 8 o + 4 half + x of a 32-token group is row 4 o + x of the group's tile `half`
-            const int tile = 2 * (tok >> 5) + ((tok >> 2) & 1), row = 4 * ((tok >> 3) & 3) + (tok & 3);
-            const int j = ch >> 2, g = ch & 3;
-            ks[slot][tile][2 * j][16 * g + row] = codes8(kr[i].x, kr[i].y);
-            ks[slot][tile][2 * j + 1][16 * g + row] = codes8(kr[i].z, kr[i].w);
-            const int oc = u / (D / 2), dp = u % (D / 2);
-            const int m = dp >> 4;
-            vs[slot][oc >> 2][2 * m][16 * (oc & 3) + (dp & 15)] = codes8(vr[i].x, vr[i].y);
-            vs[slot][oc >> 2][2 * m + 1][16 * (oc & 3) + (dp & 15)] = codes8(vr[i].z, vr[i].w);
-        }
-        if (tid < 2 * (NT / 8)) scl[slot][tid / (NT / 8)][tid % (NT / 8)] = sr;
+        for (int i = 0; i < UK; ++i) kr[i] = ld16(p + ko + 128 * i);
+        ksr = a.c.ks[base];
+        vsr = a.c.vs[base];
     };
-
-    f16x8_t Qh[2 * NJ], Ql[2 * NJ];
+    auto v_load = [&](int n) {   // n: how many tiles behind the keys
+        const int8_t* p = a.c.v + off[2 - n];
+#pragma unroll
+        for (int i = 0; i < UK; ++i) vr[i] = ld16(p + vo + 1024 * i);
+    };
+    // piece 2 i + half of the keys / of the values to LDS; dim 64 m + 2 r + e is row r of value tile 2 m + e
+    constexpr int PIECES = 2 * UK;
+    const int ktok = 8 * wv + (lane & 7), rho = (ktok & 16) + 8 * ((ktok >> 2) & 1) + 4 * ((ktok >> 3) & 1) + (ktok & 3);
+    auto k_put = [&](int st, int piece) {
+        const int i = piece >> 1;
+        const f16x8_t x = piece & 1 ? codes8(kr[i].z, kr[i].w) : codes8(kr[i].x, kr[i].y);
+        if (some) ks[st & 1][(lane >> 3) + 8 * i][32 * (piece & 1) + rho] = x;
+    };
+    auto v_put = [&](int st, int piece) {
+        const int i = piece >> 1;
+        const f16x8_t x = piece & 1 ? codes8(vr[i].z, vr[i].w) : codes8(vr[i].x, vr[i].y);
+        if (some) vs[st & 1][2 * (lane >> 5) + 4 * i + (piece & 1)][wv >> 1][32 * (wv & 1) + (lane & 31)] = x;
+    };
+    auto s_put = [&](int st) {   // (the same values from every lane)
+        scl[0][st & 3][wv] = sbad ? __builtin_nanf("") : sdead ? 0.f : ksr;
+        scl[1][st & 3][wv] = sdead ? 0.f : vsr;
+    };
+    auto k_store = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) k_put(st, i);
+        s_put(st);
+    };
+    auto barrier = []() {   // LDS is written and read; the loads stay in flight
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if (steps > 0) {
+        next_id(0);
+        off[1] = off[2] = 0;
+        k_load(0);
+        next_id(1);
+        v_load(0);
+    }
+    // the row's query, times 2^e, in two parts: dims 16 d + 8 g + 0..7 of depth d
+    f16x8_t Qh[ND], Ql[ND];
     float factor;
     {
-        float f[D / 4];
-        factor = load_query<D>(a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D, lk, a.scale, f);
+        const float* q = a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D + 8 * g;
+        float m = 0.f;
+        bool bad = false;
 #pragma unroll
-        for (int d = 0; d < 2 * NJ; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                Qh[d][i] = static_cast<_Float16>(f[8 * d + i]);
-                Ql[d][i] = static_cast<_Float16>(low_part(f[8 * d + i]));
+                const float v = q[16 * d + i];
+                m = fmaxf(m, fabsf(v));
+                bad |= !(fabsf(v) <= FLT_MAX);
             }
-    }
-    f32x4_t acc[ND][2];
-#pragma unroll
-    for (int m = 0; m < ND; ++m) acc[m][0] = acc[m][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float mu = -FLT_MAX, l = 0.f;
-    if (steps > 0) {
-        load(0);
-        store(0);
-        if (steps > 1) load(1);
-    }
-    for (int st = 0; st < steps; ++st) {
-        __syncthreads();   // slot st % 2 is whole; the other one has been read
-        if (st + 1 < steps) {
-            store((st + 1) & 1);
-            if (st + 2 < steps) load(st + 2);
+        if (bad) m = INFINITY;
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const bool ok = m <= FLT_MAX;
+        int e = 0;
+        if (m > 0.f && ok) {
+            int em;
+            frexpf(m, &em);
+            e = 15 - em;
         }
-        const int slot = st & 1;
-#pragma unroll 1
-        for (int g = 0; g < NT / 32; ++g) {
-            const int t0 = st * NT + 32 * g;
-            if (t0 >= wave_seen) break;   // the wave's rows see nothing from here on
-            f32x4_t S[2];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                S[half] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < ND; ++d) {
 #pragma unroll
-                for (int d = 0; d < 2 * NJ; ++d) {
-                    const f16x8_t A = ks[slot][2 * g + half][d][lane];
-                    S[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Qh[d], S[half], 0, 0, 0);
-                    S[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Ql[d], S[half], 0, 0, 0);
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float v = ok ? ldexpf(q[16 * d + i], e) : 0.f;
+                Qh[d][i] = static_cast<_Float16>(v);
+                Ql[d][i] = static_cast<_Float16>(low_part(v));
             }
-            const float f = factor * scl[slot][0][4 * g + lk];
-            float sv = scl[slot][1][4 * g + lk];
-            float s[8];
+        }
+        factor = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = S[i >> 2][i & 3] * f;
+        for (int d = 0; d < ND; ++d) {   // only products read them: accumulation registers, the others are full
+            asm("" : "+a"(Qh[d]));
+            asm("" : "+a"(Ql[d]));
+        }
+    }
+    f32x16_t acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    float mu = -FLT_MAX, l = 0.f;
+    f32x16_t S, N;          // a tile's scores, scaled; the next tile's
+    f16x8_t Wh[2], Wl[2];   // weights of the last tile
+    // The operands of a step's products are one sequence, the last tile's values (2 DT of them), then the next tile's keys
+    // (ND = 2 DT); each is requested AP products' pairs ahead, into the register that the one before it has left. fill(i) goes
+    // between the two products of an operand and after them.
+    constexpr int AP = 4;
+    f16x8_t A[AP];
+    auto value_at = [&](int slot, int k) { return vs[slot][k >> 1][k & 1][lane]; };
+    auto key_at = [&](int slot, int d) { return ks[slot][d][lane]; };
+    // ahead(d): what to request when operand d has been taken
+    auto scores = [&](auto&& ahead, auto&& fill) {
+        static_for<ND>([&](auto dI) {
+            constexpr int d = decltype(dI)::value;
+            const f16x8_t x = A[d % AP];
+            if constexpr (d == 0) {
+                f32x16_t z;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] = 0.f;
+                N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Qh[d], z, 0, 0, 0);
+            } else {
+                N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Qh[d], N, 0, 0, 0);
+            }
+            fill(IC<2 * d>{});
+            __builtin_amdgcn_sched_barrier(0);
+            N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Ql[d], N, 0, 0, 0);
+            ahead(dI);
+            fill(IC<2 * d + 1>{});
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto values = [&](auto&& ahead, auto&& fill) {
+        static_for<ND>([&](auto kI) {
+            constexpr int k = decltype(kI)::value, d = k >> 1, s = k & 1;
+            const f16x8_t x = A[k % AP];
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Wh[s], acc[d], 0, 0, 0);
+            fill(IC<2 * k>{});
+            __builtin_amdgcn_sched_barrier(0);
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Wl[s], acc[d], 0, 0, 0);
+            ahead(kI);
+            fill(IC<2 * k + 1>{});
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    for (int i = tid; i < DT * 2 * kWave; i += NTH) (&vs[1][0][0][0])[i] = f16x8_t{};   // the values before the first tile
+#pragma unroll
+    for (int s = 0; s < 2; ++s) Wh[s] = Wl[s] = f16x8_t{};
+    if (steps > 0) {
+        k_store(0);
+        k_load(1);
+        next_id(2);
+        barrier();
+        static_for<AP>([&](auto dI) { A[decltype(dI)::value] = key_at(0, decltype(dI)::value); });
+        scores([&](auto dI) {
+            constexpr int d = decltype(dI)::value;
+            if constexpr (d + AP < ND) A[d % AP] = key_at(0, d + AP);
+        }, [](auto) {});
+        k_store(1);
+        k_load(2);
+        next_id(3);
+    }
+    barrier();
+#pragma unroll
+    for (int k = 0; k < AP; ++k) A[k] = value_at(1, k);
+    // Step st: the scores of tile st are in S. Its values and the keys of st + 2 go to LDS (slots whose last readers passed
+    // the barrier before); the values of st - 1 are summed beside that and beside the scaling and maximum of the scores, the
+    // scores of st + 1 beside the exponentials. One step more than tiles; before the first the weights are zero.
+    float f[2], sv[2], top[2], w0 = 0.f;
+    auto scale_max = [&](int i) {
+        S[i] = N[i] * f[i >> 3];
+        top[i >> 3] = (i & 7) ? fmaxf(top[i >> 3], S[i]) : S[i];
+        asm volatile("" : "+v"(S[i]), "+v"(top[i >> 3]));   // here, not where they are used
+    };
+    auto weight = [&](int i) {
+        const float p = __builtin_amdgcn_exp2f(S[i] - mu);
+        l += p;
+        const float w = rounded(p * (sv[i >> 3] * kWeightUp));
+        if (i & 1) {
+            Wh[i >> 3][(i & 7) - 1] = static_cast<_Float16>(w0);
+            Wh[i >> 3][i & 7] = static_cast<_Float16>(w);
+            Wl[i >> 3][(i & 7) - 1] = static_cast<_Float16>(low_part(w0));
+            Wl[i >> 3][i & 7] = static_cast<_Float16>(low_part(w));
+        }
+        w0 = w;
+    };
+    for (int st = 0; steps > 0 && st <= steps; ++st) {
+        {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) f[s] = factor * scl[0][st & 3][2 * s + g];
+            constexpr int SLOTS = 4 * DT, PER = 32 / SLOTS;   // places between products; scores at a place of the second half
+            values([&](auto kI) {
+                constexpr int k = decltype(kI)::value;
+                A[k % AP] = k + AP < ND ? value_at((st + 1) & 1, k + AP) : key_at((st + 1) & 1, k + AP - ND);
+            }, [&](auto kI) {
+                constexpr int k = decltype(kI)::value;
+                constexpr int EVERY = SLOTS / (4 * PIECES);   // a piece to LDS at every so many places of the first half
+                if constexpr (k < SLOTS / 2 && k % EVERY == 0) {
+                    if constexpr ((k / EVERY) & 1)
+                        k_put(st + 2, (k / EVERY) >> 1);
+                    else
+                        v_put(st, (k / EVERY) >> 1);
+                }
+                if constexpr (k == SLOTS / 2) {
+                    s_put(st + 2);
+                    v_load(1);
+                }
+                if constexpr (k == SLOTS / 2 + 2) {
+                    k_load(st + 3);
+                    next_id(st + 4);
+                }
+                if constexpr (k >= SLOTS / 2) {
+#pragma unroll
+                    for (int i = (k - SLOTS / 2) * PER; i < (k - SLOTS / 2 + 1) * PER; ++i) scale_max(i);
+                }
+            });
+        }
+        {
+            const int t0 = 32 * st;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) sv[s] = scl[1][st & 3][2 * s + g];
             if (t0 + 31 > wave_first) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (t0 + 8 * lk + i > limit) s[i] = -INFINITY;
-                if (t0 + 8 * lk > limit) sv = 0.f;
-            }
-            float top = s[0];
+                for (int s = 0; s < 2; ++s) {
 #pragma unroll
-            for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
-            top += __builtin_amdgcn_logf(fmaxf(sv, kKv8Floor));
-            if (__ballot(top > mu + kMoves)) {
-                const float now = fmaxf(mu, max_over_lk(top));
+                    for (int i = 0; i < 8; ++i) {
+                        if (t0 + 16 * s + 8 * g + i > limit) S[8 * s + i] = -INFINITY;
+                        top[s] = i ? fmaxf(top[s], S[8 * s + i]) : S[8 * s];
+                    }
+                    if (t0 + 16 * s + 8 * g > limit) sv[s] = 0.f;   // a page that the row does not see may be marked
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) top[s] += __builtin_amdgcn_logf(fmaxf(sv[s], kKv8Floor));
+            const float hi = fmaxf(top[0], top[1]);
+            if (__ballot(hi > mu + kMoves)) {
+                const float now = fmaxf(mu, fmaxf(hi, __shfl_xor(hi, 32)));
                 const float shrink = __builtin_amdgcn_exp2f(mu - now);
                 mu = now;
                 l *= shrink;
 #pragma unroll
-                for (int m = 0; m < ND; ++m)
+                for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[m][e][i] *= shrink;
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
             }
-            f16x8_t Wh, Wl;
-            const float up = sv * kWeightUp;
+            // (past the wave's last tile these scores are of an old one, and unused)
+            scores([&](auto dI) {
+                constexpr int d = decltype(dI)::value;
+                if constexpr (d + AP < ND) A[d % AP] = key_at((st + 1) & 1, d + AP);
+                // The tile's keys have been read, its values and the next keys are written: the next values can be read.
+                if constexpr (d == ND - 2) {
+                    barrier();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float p = __builtin_amdgcn_exp2f(s[i] - mu);
-                l += p;
-                const float w = rounded(p * up);
-                Wh[i] = static_cast<_Float16>(w);
-                Wl[i] = static_cast<_Float16>(low_part(w));
-            }
-#pragma unroll
-            for (int m = 0; m < ND; ++m)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const f16x8_t A = vs[slot][g][2 * m + e][lane];
-                    acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Wh, acc[m][e], 0, 0, 0);
-                    acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Wl, acc[m][e], 0, 0, 0);
+                    for (int k = 0; k < AP - 1; ++k) A[k] = value_at(st & 1, k);
                 }
+                if constexpr (d == ND - 1) A[AP - 1] = value_at(st & 1, AP - 1);
+            }, [&](auto kI) {
+                constexpr int k = decltype(kI)::value, PLACES = 2 * ND;
+#pragma unroll
+                for (int i = k * 16 / PLACES; i < (k + 1) * 16 / PLACES; ++i) weight(i);
+            });
         }
     }
-    l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (mine >= pairs) return;
+    if (row0 + col >= pairs) return;
     if (r.bad) l = __builtin_nanf("");
     const size_t o = (static_cast<size_t>(r.first + ti) * a.heads + head) * D;
-    const float inv = kWeightUp * l;
+    const float inv = 1.f / (kWeightUp * l);   // (of a sum of at least one: 2^-24 more beside the sums' roundings)
+    // A lane's registers 4 b .. 4 b + 3 of value tiles 2 m and 2 m + 1 are dims 64 m + 16 b + 8 g + 0..7 of its row. (One row's
+    // gates after another's, each load waited for, were a third of the kernel's time.)
 #pragma unroll
-    for (int m = 0; m < ND; ++m)
+    for (int m = 0; m < DT / 2; ++m) {
+        const size_t at = o + 64 * m + 8 * g;
+        float4 gt[4][2];
+        if (a.gate) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)   // dims 32 m + 2 (4 lk + i) + e
+            for (int n = 0; n < 8; ++n) gt[n >> 1][n & 1] = ld4(a.gate + at + 16 * (n >> 1) + 4 * (n & 1));
+        }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int d = 32 * m + 8 * lk + 2 * i + e;
-                float v = l == 0.f ? 0.f : acc[m][e][i] / inv;
-                if (a.gate) v *= sigmoid(a.gate[o + d]);
-                a.out[o + d] = v;
+        for (int n = 0; n < 8; ++n) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = acc[2 * m + (i & 1)][4 * (n >> 1) + 2 * (n & 1) + (i >> 1)];
+                v[i] = l == 0.f ? 0.f : x * inv;
             }
-    if (lk == 0) a.info[o / D] = make_int2(0, 1);
+            if (a.gate) {
+                const float4 x = gt[n >> 1][n & 1];
+                v[0] *= sigmoid(x.x);
+                v[1] *= sigmoid(x.y);
+                v[2] *= sigmoid(x.z);
+                v[3] *= sigmoid(x.w);
+            }
+            st4(a.out + at + 16 * (n >> 1) + 4 * (n & 1), make_float4(v[0], v[1], v[2], v[3]));
+        }
+    }
+    if (g == 0) a.info[o / D] = make_int2(0, 1);
 }
 
 // ------------------------------------------------------------------ host
@@ -752,6 +933,8 @@ int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_co
     QK_REQUIRE(q && out && row_start && kv_len && (block_table || max_pages == 0), "attn_kv8_rows: null pointer");
     QK_REQUIRE(static_cast<int64_t>(rows) * heads <= (int64_t{1} << 24), "attn_kv8_rows: %d rows of %d heads exceed one call",
                rows, heads);
+    QK_REQUIRE(aligned16(q) && aligned16(out) && (!gate || aligned16(gate)),
+               "attn_kv8_rows: q, gate and out must be 16-byte aligned");
     QK_REQUIRE(out != q, "attn_kv8_rows: out is q");
     const Layout l = layout(rows, requests, heads, kv_heads, dim);
     QK_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= l.bytes,

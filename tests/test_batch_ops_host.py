@@ -88,6 +88,8 @@ def test_attention(lib):
     refused(lib, call(max_pages=1 << 30), "table rows")
     refused(lib, call(rows=1 << 21), "exceed one call")
     refused(lib, call(out=P), "out is q")
+    for name in ("q", "out", "gate"):
+        refused(lib, call(**{name: ODD}), "aligned")
     for name in ("q", "out", "start", "len", "table"):
         refused(lib, call(**{name: NUL}), "null")
     refused(lib, call(ws=NUL), "workspace")
