@@ -63,6 +63,7 @@ struct AttnArgs {
     float2* stat;        // [item][kRows] (m, l)
     int2* info;          // [row][head] (first item * kRows + row in item, pieces)
     int items;           // capacity: the split kernel's grid
+    int all_items;       // and with the cut prompts' pieces
     float scale;         // log2(e) / sqrt(D)
 };
 
@@ -409,21 +410,20 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split_kernel(const AttnArgs a)
 }
 
 // ------------------------------------------------------------------ join
-// A workgroup of NW waves joins the pieces of `per` neighbouring (row, head) pairs, one after the other: wave w takes
-// pieces w, w + NW, ...; lanes the dims. Pairs in one piece (and rows of the many-row kernel) are there already: in a
-// prompt's call most workgroups only look, so they look at 16 pairs at once (a workgroup per pair took 29 us at 5000 rows
-// of 16 heads).
+// Joins the pieces of (row, head) pairs. NW > 1: a workgroup of NW waves per pair, wave w takes pieces w, w + NW, ...; NW = 1:
+// a wave per pair, and each wave looks at `per` pairs at once, because in a prompt's call most are there already (a
+// workgroup per pair took 29 us at 5000 rows of 16 heads). Lanes hold the dims.
 template <int D, int NW>
-__global__ __launch_bounds__(NW * kWave) void combine_kernel(const AttnArgs a, int per) {
+__global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kernel(const AttnArgs a, int per) {
     constexpr int V = D / kWave;
-    __shared__ float sums[NW][D], ls[NW], ms[NW];
-    const int wv = wave_in_block(), lane = threadIdx.x & 63;
+    __shared__ float sums[NW][NW == 1 ? 1 : D], ls[NW], ms[NW];
+    const int lane = threadIdx.x & 63, wv = NW == 1 ? 0 : wave_in_block();
     const int live = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;   // pairs of the requests' rows
-    const int pair0 = static_cast<int>(blockIdx.x) * per;
+    const int64_t pair0 = NW == 1 ? (static_cast<int64_t>(blockIdx.x) * 4 + wave_in_block()) * per : blockIdx.x;
     int2 in = make_int2(0, 0);
-    if (lane < per && pair0 + lane < live) in = a.info[pair0 + lane];
-    const bool join = in.y > 1 && in.x >= 0 && in.y <= a.items - in.x / kRows;
-    uint64_t todo = __ballot(join);   // the same in every wave
+    if (lane < (NW == 1 ? per : 1) && pair0 + lane < live) in = a.info[pair0 + lane];
+    const bool join = in.y > 1 && in.x >= 0 && in.y <= a.all_items - in.x / kRows;
+    uint64_t todo = __ballot(join);   // the same in every wave of a pair
     while (todo) {
         const int k = __builtin_ctzll(todo);
         todo &= todo - 1;
@@ -461,29 +461,36 @@ __global__ __launch_bounds__(NW * kWave) void combine_kernel(const AttnArgs a, i
                 for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
             }
         }
-        __syncthreads();   // the last pair's sums have been read
-#pragma unroll
-        for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
-        if (lane == 0) {
-            ms[wv] = m;
-            ls[wv] = l;
-        }
-        __syncthreads();
-        for (int d = threadIdx.x; d < D; d += NW * kWave) {
-            float top = ms[0];
-#pragma unroll
-            for (int w = 1; w < NW; ++w) top = fmaxf(top, ms[w]);
-            float sum = 0.f, tot = 0.f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float f = __builtin_amdgcn_exp2f(ms[w] - top);
-                sum += f * sums[w][d];
-                tot += f * ls[w];
-            }
+        auto put = [&](int d, float sum, float tot) {
             const size_t o = static_cast<size_t>(pair0 + k) * D + d;
             float v = tot == 0.f ? 0.f : sum / kWeightUp / tot;
             if (a.gate) v *= sigmoid(a.gate[o]);
             a.out[o] = v;
+        };
+        if constexpr (NW == 1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) put(V * lane + i, s[i], l);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
+            if (lane == 0) {
+                ms[wv] = m;
+                ls[wv] = l;
+            }
+            __syncthreads();
+            for (int d = threadIdx.x; d < D; d += NW * kWave) {
+                float top = ms[0];
+#pragma unroll
+                for (int w = 1; w < NW; ++w) top = fmaxf(top, ms[w]);
+                float sum = 0.f, tot = 0.f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(ms[w] - top);
+                    sum += f * sums[w][d];
+                    tot += f * ls[w];
+                }
+                put(d, sum, tot);
+            }
         }
     }
 }
@@ -501,6 +508,10 @@ __global__ __launch_bounds__(NW * kWave) void combine_kernel(const AttnArgs a, i
 // product's depth s.
 constexpr int kPromptWaves = 4;
 constexpr int kPromptRows = 32 * kPromptWaves;
+// A workgroup has its CU to itself (registers). If a call has less than half as many of them as the card has CUs, each
+// one's keys are cut into pieces of at least kPromptMinTiles tiles, as many as the card holds at once.
+constexpr int kPromptFill = 256;
+constexpr int kPromptMinTiles = 8;
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 template <int S>
@@ -523,14 +534,22 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
     __shared__ float scl[2][4][4];   // [key, value][tile % 4][octet]
     // which request, KV head and row tile: the last row tiles (the longest rows) first
     const int G = a.group, lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+    auto tiles_here = [&](int b) -> int64_t {   // workgroups of a request, before they are cut
+        if (b >= a.requests) return 0;
+        const Request r = request(a, b);
+        return takes_split(a, r) ? 0 : (static_cast<int64_t>(r.n) * G + kPromptRows - 1) / kPromptRows * a.c.heads;
+    };
+    int64_t total = 0;
+    for (int b0 = 0; b0 < a.requests; b0 += kWave) total += tiles_here(b0 + lane);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
+    if (total == 0) return;   // the whole workgroup
+    const int splits = total < kPromptFill ? static_cast<int>(kPromptFill / total) : 1;
     int b = -1;
-    int64_t item = blockIdx.x;
+    int64_t item = blockIdx.x / static_cast<unsigned>(splits);
+    const int split = static_cast<int>(blockIdx.x % static_cast<unsigned>(splits));
     for (int b0 = 0; b0 < a.requests && b < 0; b0 += kWave) {
-        int64_t n = 0;
-        if (b0 + lane < a.requests) {
-            const Request r = request(a, b0 + lane);
-            if (!takes_split(a, r)) n = (static_cast<int64_t>(r.n) * G + kPromptRows - 1) / kPromptRows * a.c.heads;
-        }
+        const int64_t n = tiles_here(b0 + lane);
         const int64_t upto = wave_prefix(n, lane);
         const uint64_t hit = __ballot(item < upto);
         if (hit) {
@@ -553,8 +572,10 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
     const int limit = r.len - r.n + ti;
     const int wave_first = r.len - r.n + min(row0, pairs - 1) / G;
     const int seen = max(r.len - r.n + min(rt * kPromptRows + kPromptRows - 1, pairs - 1) / G + 1, 0);
-    const int steps = (seen + 31) / 32;
-    const int P = a.c.page;
+    const int all_steps = (seen + 31) / 32, pieces = min(splits, max(all_steps / kPromptMinTiles, 1));
+    if (split >= pieces) return;   // the whole workgroup
+    const int per = (all_steps + pieces - 1) / pieces;
+    const int first_tile = split * per, steps = max(min(per, all_steps - first_tile), 0);   // this piece's tiles
     const int block_shift = a.page_shift + (D == 64 ? 6 : D == 128 ? 7 : 8);   // of a page and head, as a power of two
 
     // A wave brings one octet of tokens of each tile: page, offset and scales are the same for its lanes. A lane's pieces:
@@ -568,10 +589,10 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
     int id = 0;
     size_t off[3];   // of the octet in tiles st + 1, st + 2, st + 3
     auto next_id = [&](int st) {   // the table's entry for the octet (any in-bounds entry past the row's end)
-        id = a.table[static_cast<size_t>(b) * a.max_pages + min((32 * st + 8 * wv) >> a.page_shift, a.max_pages - 1)];
+        id = a.table[static_cast<size_t>(b) * a.max_pages + min((32 * (first_tile + st) + 8 * wv) >> a.page_shift, a.max_pages - 1)];
     };
     auto k_load = [&](int st) {
-        const int tok = 32 * st + 8 * wv, page = __builtin_amdgcn_readfirstlane(id);
+        const int tok = 32 * (first_tile + st) + 8 * wv, page = __builtin_amdgcn_readfirstlane(id);
         sdead = tok >= seen;
         sbad = !sdead && (page < 0 || page >= a.c.pages);
         const size_t base = static_cast<size_t>(static_cast<uint32_t>(sdead || sbad ? 0 : page)) * a.c.heads + h;
@@ -785,18 +806,19 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
             });
         }
         {
-            const int t0 = 32 * st;
+            const int t0 = 32 * (first_tile + st);
 #pragma unroll
             for (int s = 0; s < 2; ++s) sv[s] = scl[1][st & 3][2 * s + g];
-            if (t0 + 31 > wave_first) {
+            if (t0 + 31 > wave_first || st == steps) {   // past the piece's last tile nothing is seen
+                const int last = st == steps ? -1 : limit;
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        if (t0 + 16 * s + 8 * g + i > limit) S[8 * s + i] = -INFINITY;
+                        if (t0 + 16 * s + 8 * g + i > last) S[8 * s + i] = -INFINITY;
                         top[s] = i ? fmaxf(top[s], S[8 * s + i]) : S[8 * s];
                     }
-                    if (t0 + 16 * s + 8 * g > limit) sv[s] = 0.f;   // a page that the row does not see may be marked
+                    if (t0 + 16 * s + 8 * g > last) sv[s] = 0.f;   // a page that the row does not see may be marked
                 }
             }
 #pragma unroll
@@ -834,6 +856,25 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
     if (row0 + col >= pairs) return;
     if (r.bad) l = __builtin_nanf("");
     const size_t o = (static_cast<size_t>(r.first + ti) * a.heads + head) * D;
+    if (pieces > 1) {   // row k of the tile is slot k % kRows of item first + k / kRows * splits + piece, as combine_kernel reads
+        const int k = 32 * wv + col;
+        const int unit_items = static_cast<int>(blockIdx.x) / splits * (kPromptRows / kRows);
+        const int item0 = a.items + (unit_items + k / kRows) * splits;
+        const size_t row = static_cast<size_t>(item0 + split) * kRows + k % kRows;
+#pragma unroll
+        for (int m = 0; m < DT / 2; ++m)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const int q = 4 * (n >> 1) + 2 * (n & 1);
+                st4(a.part + row * D + 64 * m + 8 * g + 16 * (n >> 1) + 4 * (n & 1),
+                    make_float4(acc[2 * m][q], acc[2 * m + 1][q], acc[2 * m][q + 1], acc[2 * m + 1][q + 1]));
+            }
+        if (g == 0) {
+            a.stat[row] = make_float2(mu, l);
+            if (split == 0) a.info[o / D] = make_int2(item0 * kRows + k % kRows, pieces);
+        }
+        return;
+    }
     const float inv = 1.f / (kWeightUp * l);   // (of a sum of at least one: 2^-24 more beside the sums' roundings)
     // A lane's registers 4 b .. 4 b + 3 of value tiles 2 m and 2 m + 1 are dims 64 m + 16 b + 8 g + 0..7 of its row. (One row's
     // gates after another's, each load waited for, were a third of the kernel's time.)
@@ -874,17 +915,20 @@ int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
     const int64_t pairs = static_cast<int64_t>(rows) * group, busy = std::min(rows, requests);
     return std::min(pairs / kRows + busy, busy * blocks_for(std::max(kSplitMax, group), kRows)) * kv_heads;
 }
+bool may_prompt(int rows, int group) { return rows > 1 && static_cast<int64_t>(rows) * group > kSplitMax; }
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
 struct Layout {
-    int64_t items;
+    int64_t items, all;   // pieces of 8 rows: of split_kernel, and with those of prompt_kernel
     size_t stat, info, bytes;
 };
 Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     Layout l;
     l.items = kTargetItems + unit_bound(rows, requests, heads, kv_heads);
-    l.stat = align_up(static_cast<size_t>(l.items) * kRows * dim * 4);
-    l.info = l.stat + align_up(static_cast<size_t>(l.items) * kRows * 8);
+    l.all = l.items;
+    if (may_prompt(rows, heads / kv_heads)) l.all += kPromptFill * (kPromptRows / kRows);
+    l.stat = align_up(static_cast<size_t>(l.all) * kRows * dim * 4);
+    l.info = l.stat + align_up(static_cast<size_t>(l.all) * kRows * 8);
     l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);
     return l;
 }
@@ -895,15 +939,17 @@ void launch(const AttnArgs& a, hipStream_t s) {
     if (!a.split_all) {
         const int64_t pairs = static_cast<int64_t>(a.rows) * a.group;
         const int64_t tiles = (pairs / kPromptRows + std::min<int64_t>(a.requests, pairs / kSplitMax + 1)) * a.c.heads;
-        prompt_kernel<D><<<static_cast<unsigned>(tiles), kPromptWaves * kWave, 0, s>>>(a);
+        prompt_kernel<D><<<static_cast<unsigned>(std::max<int64_t>(tiles, kPromptFill)), kPromptWaves * kWave, 0, s>>>(a);
     }
     const unsigned pairs = static_cast<unsigned>(a.rows) * static_cast<unsigned>(a.heads);
     if (pairs <= 128)   // few rows: many pieces each
         combine_kernel<D, 16><<<pairs, 16 * kWave, 0, s>>>(a, 1);
     else if (pairs <= 2048)
         combine_kernel<D, 4><<<pairs, 4 * kWave, 0, s>>>(a, 1);
+    else if (pairs <= kPromptFill / 2 * kPromptRows)   // a cut prompt's pairs may all have pieces
+        combine_kernel<D, 1><<<blocks_for(pairs, 4), 4 * kWave, 0, s>>>(a, 1);
     else
-        combine_kernel<D, 4><<<blocks_for(pairs, 16), 4 * kWave, 0, s>>>(a, 16);
+        combine_kernel<D, 1><<<blocks_for(pairs, 16), 4 * kWave, 0, s>>>(a, 4);
 }
 
 }  // namespace
@@ -954,11 +1000,12 @@ int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_co
     a.rows = rows;
     a.heads = heads;
     a.group = heads / kv_heads;
-    a.split_all = rows == 1 || static_cast<int64_t>(rows) * a.group <= kSplitMax;   // no request can have more
+    a.split_all = !may_prompt(rows, a.group);
     a.part = reinterpret_cast<float*>(ws);
     a.stat = reinterpret_cast<float2*>(ws + l.stat);
     a.info = reinterpret_cast<int2*>(ws + l.info);
     a.items = static_cast<int>(l.items);
+    a.all_items = static_cast<int>(l.all);
     a.scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(dim)));
     const hipStream_t s = as_stream(stream);
     if (dim == 64)

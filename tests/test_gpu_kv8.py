@@ -282,6 +282,31 @@ def test_attention_long_context_in_pieces():
     attention_case(r, [3000, 1, 700, 2049], [1, 1, 2, 1], 8, 1, 64, 16)
 
 
+@pytest.mark.parametrize("heads,kvh,dim,page", [(16, 2, 256, 64), (6, 2, 64, 8), (8, 8, 128, 16)])
+def test_attention_prompts_in_pieces(heads, kvh, dim, page):
+    """Chunks of prompts behind long prefixes: too few row tiles for the card, so that their keys are cut and joined.
+    Lengths around the pieces' and tiles' ends; two chunks whose pieces differ in number; single tokens beside them."""
+    r = np.random.default_rng(dim)
+    for n, before in ((40, 473), (33, 991), (70, 1500), (36, 220)):
+        attention_case(r, [before + n], [n], heads, kvh, dim, page, gated=n != 33)
+    attention_case(r, [1100, 900, 530, 64], [50, 1, 35, 40], heads, kvh, dim, page, pad=2)
+
+
+def test_attention_prompts_in_pieces_bad_page():
+    """A page outside the cache makes every row of its request NaN that sees it, whichever piece holds it."""
+    r = np.random.default_rng(31)
+    lens, fresh = [900, 700], [60, 50]
+    table, pages = tables(r, lens, 32)
+    table[0, 3] = pages + 5
+    ref = random_cache(r, pages, 2, 32, 128)
+    q = r.standard_normal((110, 16, 128)).astype(F32)
+    got = host(ops.attn_kv8_rows(dev(q), gpu_cache(ref), dev(table), dev([0, 60, 110], I32), dev(lens, I32)))
+    assert np.isnan(got[:60]).all()
+    table[0, 3] = 0
+    want, tol = kv8_ref.attention(q, ref, table, np.array([0, 60, 110]), lens, None)
+    assert np.all(np.abs(got[60:] - want[60:]) <= tol[60:])
+
+
 @pytest.mark.parametrize("n", [3, 40])
 def test_attention_rows_without_keys(n):
     """Positions before the first key (kv_len below the request's rows) give zeros, gated or not."""
