@@ -43,10 +43,16 @@ __global__ __launch_bounds__(kGroupBlock) void group_kernel(const int32_t* __res
         const int e = idx[i];
         return e >= 0 && e < n ? e : n;
     };
-    for (int i = tid; i < pairs; i += kGroupBlock) {
-        const int e = bucket(i);
-        atomicAdd(&all[e], 1);
-        if (i < first) atomicAdd(&before[e], 1);
+    constexpr int AHEAD = 8;   // ids requested before the first is counted
+    for (int i0 = tid; i0 < pairs; i0 += AHEAD * kGroupBlock) {
+        int e[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) e[j] = bucket(min(i0 + j * kGroupBlock, pairs - 1));
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * kGroupBlock;
+            if (i < pairs) atomicAdd(i < first ? &before[e[j]] : &all[e[j]], 1);
+        }
     }
     const int p = first + tid;
     const bool in = p < pairs;
@@ -60,7 +66,7 @@ __global__ __launch_bounds__(kGroupBlock) void group_kernel(const int32_t* __res
     if (in && rank == 0) mine[wv][e] = static_cast<uint16_t>(__popcll(same));
     __syncthreads();
     // exclusive prefix of all[0 .. n], a bucket to a thread (n <= 1024; bucket n needs only the sum before it)
-    const int c = tid < n ? all[tid] : 0;
+    const int c = tid < n ? all[tid] + before[tid] : 0;   // (the pairs before this workgroup's were counted apart)
     int inc = c;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
@@ -102,7 +108,9 @@ __device__ void write_tiles(const int32_t* __restrict__ starts, int experts, int
             s = min(max(starts[e], 0), pairs);
             n = min(max(starts[e + 1], s), pairs) - s;
         }
-        const int k = (n + size - 1) / size;
+        // of several tiles of 16 pairs each: even ones, whole sixteens
+        const int even = (n + size - 1) / size, one = size <= 16 || n == 0 ? size : ((n + even - 1) / even + 15) / 16 * 16;
+        const int k = (n + one - 1) / one;
         int inc = k;
 #pragma unroll
         for (int o = 1; o < kWave; o <<= 1) {
@@ -111,7 +119,7 @@ __device__ void write_tiles(const int32_t* __restrict__ starts, int experts, int
         }
         for (int i = 0; i < k; ++i) {
             const int slot = at + inc - k + i;
-            if (slot < most) tiles[slot] = Tile{e, s + i * size, min(size, n - i * size)};
+            if (slot < most) tiles[slot] = Tile{e, s + i * one, min(one, n - i * one)};
         }
         at += __shfl(inc, 63);
     }
@@ -177,6 +185,47 @@ __device__ __forceinline__ void replace(f32x4_t (&v)[2], int rt, int i, float f)
         if (q == 4 * rt + i) v[q >> 2][q & 3] = f;
 }
 
+// A block of a weight row between memory and the lanes that use it: the 16-byte pieces that it lies in, and a lane's share
+// (WBlock, as load() would bring it) from a copy of them in LDS. Q6_K blocks begin at any even byte.
+template <int TYPE>
+struct Staged;
+template <>
+struct Staged<kQ4_K> {
+    static constexpr int pieces = 9;
+    static __device__ __forceinline__ void take(WBlock<kQ4_K>& w, const uint4* row, uint32_t, int lk) {
+        const uint4* p = row + 1 + 4 * (lk >> 1) + (lk & 1);
+        w.hd = row[0];
+        w.q[0] = p[0];
+        w.q[1] = p[2];
+    }
+};
+template <>
+struct Staged<kQ6_K> {
+    static constexpr int pieces = 14;   // up to 14 bytes before a block's 210
+    static __device__ __forceinline__ void take(WBlock<kQ6_K>& w, const uint4* row, uint32_t skew, int lk) {
+        const uint32_t h = lk >> 1, l = lk & 1;
+        auto words = [&](uint32_t byte, auto n, uint32_t* d) {   // n words from a byte that is 0 or 2 past a word
+            constexpr int N = decltype(n)::value;
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + ((byte + skew) >> 2);
+            uint32_t v[N + 1];
+#pragma unroll
+            for (int i = 0; i <= N; ++i) v[i] = p[i];
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] = __builtin_amdgcn_alignbyte(v[i + 1], v[i], skew & 2u);
+        };
+        uint32_t d[4];
+        words(64u * h + 16u * l, IC<4>{}, d);
+        w.q[0] = make_uint4(d[0], d[1], d[2], d[3]);
+        words(64u * h + 16u * l + 32u, IC<4>{}, d);
+        w.q[1] = make_uint4(d[0], d[1], d[2], d[3]);
+        words(128u + 32u * h + 16u * l, IC<4>{}, d);
+        w.qh = make_uint4(d[0], d[1], d[2], d[3]);
+        words(192u + 8u * h, IC<2>{}, d);
+        w.sc = make_uint2(d[0], d[1]);
+        w.d = reinterpret_cast<const uint16_t*>(row)[(208u + skew) >> 1];
+    }
+};
+
 struct RowsArgs {
     const uint8_t* w[2];   // gate and up, or down
     const Tile* tiles;     // tiles[-1].expert: how many
@@ -189,60 +238,63 @@ struct RowsArgs {
     int M, K, top, pairs, column_blocks;   // M: rows of an expert's matrix; top: pairs per row of x (gate and up)
 };
 
-// 8 waves: RW row groups x KW slices of K; a wave owns 16 WT pairs x 32 weight rows of its slice: 16 gate and the same
-// 16 up rows (SWIGLU), or 32 down rows. Pipeline, operands and epilogue as gemm_kquant's (gemm.hip).
-template <int WT, int KW, bool SWIGLU>
+// 4 waves; a wave owns the tile's 16 WT pairs x 32 weight rows: 16 gate and the same 16 up rows (SWIGLU), or 32 down rows,
+// over the whole of K. Operands, pipeline and fold as gemm_kquant's (gemm.hip), but:
+// A tile has one to kMaxTokenTiles sixteens of pairs and takes the code for its number of them (a group of 24 pairs in the
+// code for 64 spent two thirds of its products on nothing).
+// Loads ask for 64 neighbouring bytes with 4 neighbouring lanes. With the lanes in the operand's order, 16 rows apart from
+// each other, every lane was an access of its own to the first cache, which was then busy 84% of the time (100 accesses a load
+// at Q6_K's odd addresses). So x is laid into LDS by rows, with the 4 pieces of a row turned by its number, because a read
+// takes 16 lanes at once, 8 of two neighbouring lane groups each; and a wave's weights pass through LDS too, where each lane
+// finds its share; nobody else reads them, so that takes no barrier.
+// Two workgroups share a CU, one's start and end beside the other's steps: they are a third of a workgroup's time at K = 512.
+// Together (us, gate and up / down): 777 tokens Q6_K 355 / 237 -> 228 / 140, 4096 tokens Q4_K 585 / 364 -> 475 / 304.
+constexpr int kRowsWaves = 4;
+constexpr int kMaxTokenTiles = 4;   // of 16 pairs, in a tile (5 and 6 do not fit the registers)
+
+template <int WT, bool SWIGLU>
 struct RowsShape {
-    static constexpr int RW = 8 / KW, FR = WT * KW * 4, XF = FR / 8, tokens = 16 * WT, cols = (SWIGLU ? 16 : 32) * RW;
-    static constexpr size_t ring = size_t{4} * FR * 1024, fold = KW > 1 ? size_t{8} * WT * 2 * 1024 : 0;
-    static constexpr size_t lds = ring > fold ? ring : fold;
-    static_assert(FR % 8 == 0, "shape");
+    static constexpr int FR = WT * 4, XF = FR / kRowsWaves, cols = (SWIGLU ? 16 : 32) * kRowsWaves;   // cols divides M
+    static constexpr size_t ring = size_t{3} * FR * 1024;
 };
 
-template <int TYPE, int WT, int KW, bool SWIGLU>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void rows_kernel(const RowsArgs a) {
-    using G = RowsShape<WT, KW, SWIGLU>;
+template <int TYPE, int WT, bool SWIGLU>
+__device__ __forceinline__ void rows_tile(const RowsArgs& a, const Tile& tl, int cb, uint8_t* smem, int* ends) {
+    using G = RowsShape<WT, SWIGLU>;
     constexpr int BB = TYPE == kQ4_K ? 144 : 210, NB = TYPE == kQ4_K ? 1 : 2, WR = 2;
-    __shared__ __align__(16) uint8_t smem[G::lds];
     uint4* xs = reinterpret_cast<uint4*>(smem);
-    const int tile = static_cast<int>(blockIdx.x) / a.column_blocks, cb = static_cast<int>(blockIdx.x) - tile * a.column_blocks;
-    if (tile >= a.tiles[-1].expert) return;   // the whole workgroup
-    const Tile tl = a.tiles[tile];
     const int M = a.M, K = a.K, n = tl.n;
     const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4;
     const int wv = wave_in_block();
-    const int kw = wv / G::RW, rw = wv % G::RW;
-    const int nb = K >> 8, nbk = nb / KW, steps = 4 * nbk, nst = K >> 5;
-    const int c0 = cb * G::cols, r0 = c0 + (SWIGLU ? 16 : 32) * rw;   // the workgroup's and the wave's first row
-    const uint64_t eb = (static_cast<uint64_t>(tl.expert) * M + c0) * nb + static_cast<uint64_t>(kw) * nbk;
+    const int nb = K >> 8, steps = 4 * nb, nst = K >> 5;
+    const int c0 = cb * G::cols, r0 = c0 + (SWIGLU ? 16 : 32) * wv;   // the workgroup's and the wave's first row
+    const uint64_t eb = (static_cast<uint64_t>(tl.expert) * M + c0) * nb;
     const uint8_t* wbase[WR];
-    uint32_t wo[WR];
 #pragma unroll
-    for (int rt = 0; rt < WR; ++rt) {
-        wbase[rt] = a.w[SWIGLU ? rt : 0] + eb * BB;
-        wo[rt] = static_cast<uint32_t>(min(r0 + (SWIGLU ? 0 : 16 * rt) + lr, M - 1) - c0) * static_cast<uint32_t>(nb) * BB;
-    }
+    for (int rt = 0; rt < WR; ++rt) wbase[rt] = a.w[SWIGLU ? rt : 0] + eb * BB;
     auto xrow = [&](int i) {   // row of x of the tile's pair i (the last one again past the end)
         const int pos = tl.first + min(i, n - 1);
         return SWIGLU ? pair_at(a.order, pos, a.pairs) / a.top : pos;
     };
-    const uint8_t* xb[G::XF];   // this wave's fragments of a step: fragment id -> (slice, tile, (depth, part))
+    uint32_t xo[G::XF];   // this wave's fragments of a step: fragment id -> (slice, tile, (depth, part))
 #pragma unroll
     for (int i = 0; i < G::XF; ++i) {
         const int id = wv * G::XF + i;
-        const int ti = id / 4 % WT, ks = id / (4 * WT);
-        xb[i] = a.xp + static_cast<size_t>(xrow(16 * ti + lr)) * K * 4 + ks * nbk * 1024 + 64 * (id % 4) + 16 * lk;
+        const int ti = id / 4;
+        // in pieces of 16 bytes
+        xo[i] = static_cast<uint32_t>(xrow(16 * ti + (lane >> 2))) * static_cast<uint32_t>(K / 4) + 4 * (id % 4) +
+                ((lane & 3) ^ (-(lane >> 4) & 3));
     }
-    uint4 xr[2][G::XF];
+    uint4 xr[1][G::XF];
     auto x_load = [&](uint4 (&d)[G::XF], int st) {
 #pragma unroll
-        for (int i = 0; i < G::XF; ++i) d[i] = ld16(xb[i] + 256u * static_cast<uint32_t>(min(st, steps - 1)));
+        for (int i = 0; i < G::XF; ++i) d[i] = ld16(a.xp + static_cast<size_t>(xo[i]) * 16 + 256u * static_cast<uint32_t>(min(st, steps - 1)));
     };
     auto x_store = [&](const uint4 (&d)[G::XF], int slot) {
 #pragma unroll
         for (int i = 0; i < G::XF; ++i) xs[(slot * G::FR + wv * G::XF + i) * 64 + lane] = d[i];
     };
-    const uint4* as = xs + kw * WT * 4 * 64 + lane;
+    const uint4* as = xs + 4 * lr + (lk ^ (-(lr >> 2) & 3));
     constexpr int PT = WT < 2 ? WT : 2;
     f16x8_t An[PT][2];
     auto a_load = [&](f16x8_t (&d)[PT][2], int slot, int j, int t0) {
@@ -257,9 +309,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    const float* sg_row[WT];
+    uint32_t so[WT];
 #pragma unroll
-    for (int tt = 0; tt < WT; ++tt) sg_row[tt] = a.sx + static_cast<size_t>(xrow(16 * tt + lr)) * nst + 8 * kw * nbk + 2 * lk;
+    for (int tt = 0; tt < WT; ++tt) so[tt] = static_cast<uint32_t>(xrow(16 * tt + lr)) * static_cast<uint32_t>(nst) + 2 * lk;
 
     f32x4_t acc[WT][WR], C[WT][WR];
 #pragma unroll
@@ -268,16 +320,40 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int rt = 0; rt < WR; ++rt) acc[tt][rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     uint32_t k64 = 0x64006400u;
     asm volatile("" : "+v"(k64));
-    WBlock<TYPE> wc[WR], wn[WR];
+    using W = Staged<TYPE>;
+    constexpr int WP = 32 * W::pieces, WI = (WP + 63) / 64;   // 16-byte pieces of the wave's 32 rows of a block
+    uint4 wr[WI];
+    uint32_t wo[WI];
+#pragma unroll
+    for (int i = 0; i < WI; ++i) {
+        const int id = min(64 * i + lane, WP - 1), row = id / W::pieces;
+        wo[i] = static_cast<uint32_t>(r0 - c0 + (SWIGLU ? row & 15 : row)) * static_cast<uint32_t>(nb) * BB;
+    }
+    const uint32_t skew = static_cast<uint32_t>(eb * BB) & 15u;   // of the first row's block in its 16 bytes
+    uint4* wl = reinterpret_cast<uint4*>(smem + G::ring) + wv * WP;
+    WBlock<TYPE> wc[WR];
     WScale<TYPE> sc[WR];
     f16x8_t B[2][WR][NB];
-    auto w_load = [&](int b) {
+    auto w_load = [&](int b) {   // block b of the wave's rows, as it lies in memory
+        const uint32_t at = static_cast<uint32_t>(min(b, nb - 1)) * BB;
 #pragma unroll
-        for (int rt = 0; rt < WR; ++rt) wn[rt].load(wbase[rt] + static_cast<size_t>(min(b, nbk - 1)) * BB, wo[rt], lk);
+        for (int i = 0; i < WI; ++i) {
+            const int id = min(64 * i + lane, WP - 1);
+            const uint8_t* base = SWIGLU && id >= WP / 2 ? wbase[1] : wbase[0];
+            wr[i] = ld16(base - skew + ((wo[i] + at + skew) & ~15u) + 16 * (id % W::pieces));
+        }
     };
-    auto w_take = [&]() {
+    auto w_store = [&]() {
 #pragma unroll
-        for (int rt = 0; rt < WR; ++rt) wc[rt] = wn[rt];
+        for (int i = 0; i < WI; ++i) wl[min(64 * i + lane, WP - 1)] = wr[i];
+    };
+    auto w_take = [&](int b) {   // a lane's share of it
+        const uint32_t at = static_cast<uint32_t>(min(b, nb - 1)) * BB;
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) {
+            const uint32_t row = static_cast<uint32_t>(r0 - c0 + (SWIGLU ? 0 : 16 * rt) + lr) * (static_cast<uint32_t>(nb) * BB);
+            W::take(wc[rt], wl + (16 * rt + lr) * W::pieces, (row + at + skew) & 15u, lk);
+        }
     };
     auto b_make = [&](auto dI) {
         constexpr int D = decltype(dI)::value;
@@ -289,17 +365,23 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     w_load(0);
     x_load(xr[0], 0);
-    x_load(xr[1], 1);
-    w_take();
+    w_store();
     w_load(1);
+    w_take(0);
     x_store(xr[0], 0);
+    x_load(xr[0], 1);
+    x_store(xr[0], 1);
     x_load(xr[0], 2);
-    x_store(xr[1], 1);
-    x_load(xr[1], 3);
     b_make(IC<0>{});
+    if (static_cast<int>(threadIdx.x) < 16 * WT) {   // for the epilogue
+        ends[threadIdx.x] = a.ex[xrow(threadIdx.x)];
+        const int pos = tl.first + min(static_cast<int>(threadIdx.x), n - 1);
+        ends[16 * kMaxTokenTiles + threadIdx.x] = SWIGLU ? 0 : pair_at(a.order, pos, a.pairs);
+    }
     barrier();
     a_load(An, 0, 0, 0);
-    for (int b = 0; b < nbk; ++b) {
+    int s0 = 0, s1 = 1, s2 = 2;   // the ring's slots of steps st, st + 1, st + 2
+    for (int b = 0; b < nb; ++b) {
         f16x4_t Bm[WR];
         float dsc[WR], dmn[WR];
         float2 sg[WT];
@@ -311,7 +393,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 dmn[rt] = opaque(-32.0f * half_bits(wc[rt].hd.x >> 16));
             }
 #pragma unroll
-            for (int tt = 0; tt < WT; ++tt) sg[tt] = *reinterpret_cast<const float2*>(sg_row[tt] + 8 * b);
+            for (int tt = 0; tt < WT; ++tt) sg[tt] = *reinterpret_cast<const float2*>(a.sx + static_cast<size_t>(so[tt]) + 8 * b);
         } else {
 #pragma unroll
             for (int rt = 0; rt < WR; ++rt) dsc[rt] = opaque(half_bits(wc[rt].d));
@@ -319,13 +401,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         static_for<8>([&](auto dI) {
             constexpr int D = decltype(dI)::value, U = D >> 1, J = D & 1;
             const int st = 4 * b + U;
-            if constexpr (D == 7) {
-                w_take();
+            if constexpr (D == 5) {   // the last block's share has been read
+                w_store();
                 w_load(b + 2);
             }
             if constexpr (J == 0) {
-                x_store(xr[U & 1], (U + 2) & 3);
-                x_load(xr[U & 1], st + 4);
+                x_store(xr[0], s2);
+                x_load(xr[0], st + 3);
             }
             __builtin_amdgcn_sched_barrier(0);
             b_make(IC<(D + 1) & 7>{});
@@ -338,9 +420,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     for (int p = 0; p < 2; ++p) A[i][p] = An[i][p];
                 }
                 if constexpr (P0 + 2 < WT)
-                    a_load(An, U, J, P0 + 2);
+                    a_load(An, s0, J, P0 + 2);
                 else
-                    a_load(An, J == 0 ? U : (U + 1) & 3, J ^ 1, 0);
+                    a_load(An, J == 0 ? s0 : s1, J ^ 1, 0);
 #pragma unroll
                 for (int i = 0; i < PN; ++i)
 #pragma unroll
@@ -377,7 +459,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 }
                 __builtin_amdgcn_sched_barrier(0);
             });
-            if constexpr (J == 1) barrier();
+            if constexpr (D == 6) w_take(b + 1);
+            if constexpr (J == 1) {
+                barrier();
+                const int s = s0;
+                s0 = s1;
+                s1 = s2;
+                s2 = s;
+            }
         });
     }
 
@@ -386,7 +475,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         int bad = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int e = a.ex[xrow(16 * tt + 4 * lk + i)];
+            const int e = ends[16 * tt + 4 * lk + i];
             bad |= (e == kRowNonFinite) << i;
 #pragma unroll
             for (int rt = 0; rt < WR; ++rt) v[rt][i] = ldexpf(v[rt][i], e == kRowNonFinite ? 0 : -e);
@@ -404,42 +493,42 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int i = 0; i < 4; ++i) {
             const int t = 16 * tt + 4 * lk + i;
             if (t >= n) continue;
-            const int pos = tl.first + t;
             if constexpr (SWIGLU) {
+                const int pos = tl.first + t;
                 if (r0 + lr < M) a.y[static_cast<size_t>(pos) * M + r0 + lr] = silu(v[0][i]) * v[1][i];
             } else {
-                float* y = a.y + static_cast<size_t>(pair_at(a.order, pos, a.pairs)) * M;
+                float* y = a.y + static_cast<size_t>(ends[16 * (kMaxTokenTiles + tt) + 4 * lk + i]) * M;
 #pragma unroll
                 for (int rt = 0; rt < WR; ++rt)
                     if (r0 + 16 * rt + lr < M) y[r0 + 16 * rt + lr] = v[rt][i];
             }
         }
     };
-    if constexpr (KW == 1) {
 #pragma unroll
-        for (int tt = 0; tt < WT; ++tt) put(tt, acc[tt]);
-    } else {   // every slice's sums to LDS; wave kw of a row group adds the token tiles tt = kw (mod KW) in slice order
-        f32x4_t* part = reinterpret_cast<f32x4_t*>(smem);
-        auto at = [&](int slice, int tt, int rt) { return (((slice * G::RW + rw) * WT + tt) * WR + rt) * 64 + lane; };
-        barrier();
-#pragma unroll
-        for (int tt = 0; tt < WT; ++tt)
-#pragma unroll
-            for (int rt = 0; rt < WR; ++rt) part[at(kw, tt, rt)] = acc[tt][rt];
-        barrier();
-#pragma unroll
-        for (int tt = 0; tt < WT; ++tt) {
-            if (tt % KW != kw) continue;
-            f32x4_t v[WR];
-#pragma unroll
-            for (int rt = 0; rt < WR; ++rt) {
-                v[rt] = part[at(0, tt, rt)];
-#pragma unroll
-                for (int sl = 1; sl < KW; ++sl) v[rt] += part[at(sl, tt, rt)];
-            }
-            put(tt, v);
+    for (int tt = 0; tt < WT; ++tt) put(tt, acc[tt]);
+}
+
+// A workgroup takes a tile and a slice of the expert's rows. Consecutive items go to one XCD (workgroups are handed to the
+// 8 XCDs in turn), so that the slices of a tile find its rows of x, and the tiles of an expert its weights, in one L2.
+template <int TYPE, bool SWIGLU>
+__global__ __launch_bounds__(kRowsWaves* kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) void rows_kernel(const RowsArgs a) {
+    constexpr size_t staged = size_t{kRowsWaves} * 32 * Staged<TYPE>::pieces * 16;
+    __shared__ __align__(16) uint8_t smem[RowsShape<kMaxTokenTiles, SWIGLU>::ring + staged];
+    __shared__ int ends[2 * 16 * kMaxTokenTiles];   // exponents, pairs
+    const int items = a.tiles[-1].expert * a.column_blocks, per = (items + 7) / 8;
+    const int turn = static_cast<int>(blockIdx.x >> 3), item = static_cast<int>(blockIdx.x & 7) * per + turn;
+    if (turn >= per || item >= items) return;   // the whole workgroup
+    const int tile = item / a.column_blocks, cb = item - tile * a.column_blocks;
+    const Tile tl = a.tiles[tile];
+    const int wt = (tl.n + 15) >> 4;
+    bool done = false;
+    static_for<kMaxTokenTiles>([&](auto i) {
+        constexpr int WT = decltype(i)::value + 1;
+        if (!done && (wt == WT || WT == kMaxTokenTiles)) {
+            rows_tile<TYPE, WT, SWIGLU>(a, tl, cb, smem, ends);
+            done = true;
         }
-    }
+    });
 }
 
 // ------------------------------------------------------------------ small groups
@@ -659,11 +748,12 @@ __global__ __launch_bounds__(256) void rows_combine(const float* __restrict__ y,
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
 // Pairs of a tile, and with them the kernel, by the mean size of the groups (those of a routing over all experts):
-// strip_kernel with tiles of 8 or 16 pairs, rows_kernel with 32 or 64.
+// strip_kernel with tiles of 8 or 16 pairs, rows_kernel with up to 64. (All launches of a call, us, strip / rows: 128 tokens
+// of 8 picks among 256 experts Q4_K 153 / 161, Q6_K 224 / 222; 256 tokens 184 / 184 and 274 / 255; 512: 240 / 231, 365 / 303.)
 int tile_pairs(int64_t pairs, int experts, int width, int inter) {
     const double mean = static_cast<double>(pairs) / std::min<int64_t>(pairs, experts);
     if (mean <= 8 && std::max(width, inter) <= 2048) return mean <= 1.5 ? 8 : 16;
-    return mean <= 20 ? 32 : 64;
+    return 16 * kMaxTokenTiles;
 }
 int64_t tile_bound(int64_t pairs, int experts, int size) { return pairs / size + std::min<int64_t>(pairs, experts); }
 
@@ -695,11 +785,11 @@ Layout layout(int rows, int top, int experts, int width, int inter) {
     return l;
 }
 
-template <int TYPE, int WT, int KW, bool SWIGLU>
+template <int TYPE, bool SWIGLU>
 void launch_rows(RowsArgs a, int64_t tiles, hipStream_t s) {
-    using G = RowsShape<WT, KW, SWIGLU>;
-    a.column_blocks = static_cast<int>(blocks_for(a.M, G::cols));
-    rows_kernel<TYPE, WT, KW, SWIGLU><<<static_cast<unsigned>(tiles * a.column_blocks), 512, 0, s>>>(a);
+    a.column_blocks = static_cast<int>(blocks_for(a.M, RowsShape<1, SWIGLU>::cols));
+    const unsigned grid = static_cast<unsigned>((tiles * a.column_blocks + 7) / 8 * 8);
+    rows_kernel<TYPE, SWIGLU><<<grid, kRowsWaves * kWave, 0, s>>>(a);
 }
 
 template <int TYPE, int TP, int KW, bool SWIGLU>
@@ -720,18 +810,12 @@ void launch_small(const RowsArgs& a, hipStream_t s) {
 
 template <int TYPE, bool SWIGLU>
 void launch_type(const RowsArgs& a, int size, int64_t tiles, hipStream_t s) {
-    const int nb = a.K / 256;
     if (size == 8) {
         launch_small<TYPE, 8, SWIGLU>(a, s);
     } else if (size == 16) {
         launch_small<TYPE, 16, SWIGLU>(a, s);
-    } else if (size == 32) {
-        if (nb % 2 == 0)
-            launch_rows<TYPE, 2, 2, SWIGLU>(a, tiles, s);
-        else
-            launch_rows<TYPE, 2, 1, SWIGLU>(a, tiles, s);
     } else {
-        launch_rows<TYPE, 4, 1, SWIGLU>(a, tiles, s);
+        launch_rows<TYPE, SWIGLU>(a, tiles, s);
     }
 }
 
@@ -775,6 +859,8 @@ int qwen_moe_experts_rows(const void* w_gate, const void* w_up, int type, const 
     QK_REQUIRE(n_experts > 0 && n_experts <= kMaxExperts, "moe_experts_rows: %d experts (1 to %d)", n_experts, kMaxExperts);
     QK_REQUIRE(rows >= 0 && top > 0 && static_cast<int64_t>(rows) * top <= (1 << 24), "moe_experts_rows: %d rows of %d picks",
                rows, top);
+    QK_REQUIRE(static_cast<int64_t>(rows) * std::max<int64_t>(width, static_cast<int64_t>(top) * inter) < (int64_t{1} << 34),
+               "moe_experts_rows: %d rows exceed one call", rows);
     if (rows == 0) return ok();
     QK_REQUIRE(order && starts && weights && x && out, "moe_experts_rows: null pointer");
     QK_REQUIRE(aligned16(w_gate) && aligned16(w_up) && aligned16(w_down) && aligned16(x) && aligned16(out),

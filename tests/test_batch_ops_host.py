@@ -117,6 +117,7 @@ def test_experts(lib):
     refused(lib, call(rows=-1), "rows")
     refused(lib, call(top=0), "picks")
     refused(lib, call(rows=1 << 22), "picks")
+    refused(lib, call(rows=1 << 21, inter=1024), "exceed one call")
     for name in ("order", "starts", "w", "x", "out"):
         refused(lib, call(**{name: NUL}), "null")
     for name in ("g", "u", "d", "x", "out"):
