@@ -30,6 +30,11 @@ output projection in `matmul_rows`, the front
 end over all rows (`gdn_frontend_rows`, history carried), the gates of all
 rows, the chunked recurrence (`gdn_recurrent_chunked`) and the gated norm. It
 leaves the history and state where T decode steps leave them.
+
+`MoeLayerDecode.prefill(xs)` runs many tokens through the MoE layer, each
+expert's tokens together, and `AttnLayerBatch.forward(xs, ...)` a step of several
+requests - single tokens and prompts - through an attention layer whose keys and
+values lie in a paged 8-bit cache.
 """
 
 from __future__ import annotations
@@ -212,6 +217,40 @@ class AttnLayerDecode:
         return out
 
 
+class AttnLayerBatch:
+    """An attention layer (the weights of an `AttnLayerDecode`) over a batch of requests, its keys and values in a paged
+    8-bit cache of its own. The pages' bookkeeping is the same for every layer, so a step is planned once:
+
+        plan = ops.kv8_plan(cached, fresh, table, free, head, page_size, rows)
+        for layer in layers: ... x = layer.forward(x, table, plan)
+
+    `forward(xs, block_table, plan)` runs the step's rows (the requests' new tokens, request by request): the three
+    projections in one `matmul_rows_multi`, the split, `attn_qk_norm_rope_rows` at the plan's positions,
+    `kv8_store_rows`, `attn_kv8_rows` with the gate, the output projection. Rows behind the last request's give
+    nothing of use. Nothing leaves the device, so a step of fixed `rows` can be captured in a graph."""
+
+    def __init__(self, layer: AttnLayerDecode, pages, page_size=64):
+        self.layer = layer
+        self.cache = ops.kv8_cache(pages, layer.kvh, layer.hd, page_size, layer.q_norm.device)
+
+    def forward(self, xs, block_table, plan, out=None):
+        a, T = self.layer, xs.shape[0]
+        row_start, kv_len, slots, pos, _ = plan
+        out = torch.empty_like(xs) if out is None else out
+        ws = torch.empty(max(1, ops.matmul_rows_workspace_bytes(T, a.dm), ops.matmul_rows_workspace_bytes(T, a.qd)),
+                         dtype=torch.uint8, device=xs.device)
+        qg, k, v = ops.matmul_rows_multi([(a.w[n][0], a.wtype, a.w[n][1] * a.dm, a.w[n][1], 0, None)
+                                          for n in ("qg", "k", "v")], xs, a.dm, workspace=ws)
+        q, gate = (t.view(T, a.h, a.hd) for t in ops.attn_split_qg(qg, T * a.h, a.hd))
+        k, v = k.view(T, a.kvh, a.hd), v.view(T, a.kvh, a.hd)
+        ops.attn_qk_norm_rope_rows(q, k, a.q_norm, a.k_norm, pos=pos, rope_dim=a.rope_dim, theta=a.theta, eps=a.eps)
+        ops.kv8_store_rows(k, v, slots, self.cache)
+        # zeros in the rows behind the last request's, which attention leaves alone and the projection reads
+        gated = ops.attn_kv8_rows(q, self.cache, block_table, row_start, kv_len, gate=gate, out=torch.zeros_like(q))
+        w, M = a.w["out"]
+        return ops.matmul_rows(w, a.wtype, M * a.qd, gated.view(T, a.qd), M, a.qd, out=out, workspace=ws)
+
+
 class MoeLayerDecode:
     """A MoE layer's decode step (src/layer_moe.cpp:80-159): router, top-k,
     k routed experts (gate, up, SiLU x up, down, weighted add) and the gated
@@ -310,3 +349,22 @@ class MoeLayerDecode:
                              self.hidden_all, I, self.w["sd"][0], self.wtype, dm * S, self.hidden_all[k * I:],
                              self.sgate, dm, out=out, workspace=self.workspace)
         return out
+
+    def prefill(self, xs, out=None):
+        """xs [T, d_model] -> out [T, d_model]: T tokens in one pass (src/layer_moe.cpp:80-159 token by token in the
+        reference): the router and the shared expert's three projections in one `matmul_rows_multi`, the top-k of all
+        rows, the (token, pick) pairs grouped by expert (`moe_group_rows`), every expert's tokens through it together
+        (`moe_experts_rows`), then the shared expert's down projection and its gated add."""
+        T, dm, S = xs.shape[0], self.dm, self.S
+        ws = torch.empty(max(1, ops.matmul_rows_workspace_bytes(T, dm), ops.matmul_rows_workspace_bytes(T, S)),
+                         dtype=torch.uint8, device=xs.device)
+        router, sgate, sg, su = ops.matmul_rows_multi(
+            [(self.w[n][0], self.wtype, self.w[n][1] * dm, self.w[n][1], 0, None) for n in ("router", "sgate", "sg", "su")],
+            xs, dm, workspace=ws)
+        idx, weights = ops.moe_topk_rows(router, self.k)
+        order, starts = ops.moe_group_rows(idx, self.E)
+        e = self.experts_w
+        out = ops.moe_experts_rows(e["gate"], e["up"], self.wtype, e["down"], self.wtype, self.E, order, starts, weights, xs,
+                                   self.I, out=out)
+        shared = ops.matmul_rows(self.w["sd"][0], self.wtype, dm * S, ops.moe_silu_mul(sg, su, out=sg), dm, S, workspace=ws)
+        return ops.moe_shared_add_rows(out, shared, sgate.view(T))
