@@ -44,8 +44,9 @@ constexpr int kSplitBlock = kSplitWaves * kWave;
 constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
 constexpr int kTargetItems = 1024;     // pieces of the whole call
 constexpr int kMinTiles = 8;           // of a piece: two steps per wave
-constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take the split kernel;
-                                       // a single row always does
+constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take the split kernel (100
+                                       // requests of 64 at 1500 keys: 205 us, with the prompt kernel 108); a single row does
+constexpr int kSplitOnly = 1024;       // and of a whole call that has no more rows than requests
 constexpr float kMoves = 8.0f;         // a score past the reference by more moves it
 constexpr float kWeightUp = 64.0f;     // weights (up to 2^8) enter fp16 times 2^6
 
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
 // ------------------------------------------------------------------ many rows
 // 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: an operand of keys or values, 1 KB of LDS, feeds 2
 // products (both parts of 32 rows), 64 cycles, so that the waves' reads take half of the LDS's rate; with 16 rows a wave they
-// took all of it (5000 rows 690 us, now 560). A wave holds its rows' query parts (128 registers at D = 256, pinned in
+// took all of it (5000 rows 690 us, now 485 to 550 with the card's clock). A wave holds its rows' query parts (128 registers at D = 256, pinned in
 // accumulation registers) and sums (128). Its vector work - softmax, turning codes to fp16 - is laid between its own
 // products: while tile t + 1's scores are computed, tile t's are exponentiated; while tile t's values are summed, the codes
 // of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own rows may end one earlier:
@@ -509,9 +510,10 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
 constexpr int kPromptWaves = 4;
 constexpr int kPromptRows = 32 * kPromptWaves;
 // A workgroup has its CU to itself (registers). If a call has less than half as many of them as the card has CUs, each
-// one's keys are cut into pieces of at least kPromptMinTiles tiles, as many as the card holds at once.
+// one's keys are cut into pieces of at least kPromptMinTiles tiles, as many as the card holds at once (777 rows behind 1500
+// keys: 98 workgroups 125 us, 196 pieces 88; a call with 16 rows behind 2500 keys 39 us with pieces of 8 tiles, 35 of 4).
 constexpr int kPromptFill = 256;
-constexpr int kPromptMinTiles = 8;
+constexpr int kPromptMinTiles = 4;
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 template <int S>
@@ -649,15 +651,22 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
     float factor;
     {
         const float* q = a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D + 8 * g;
+        float f[ND][8];   // all of it requested before the first is looked at
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float4 x = ld4(q + 16 * d + 4 * i);
+                f[d][4 * i] = x.x, f[d][4 * i + 1] = x.y, f[d][4 * i + 2] = x.z, f[d][4 * i + 3] = x.w;
+            }
         float m = 0.f;
         bool bad = false;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = q[16 * d + i];
-                m = fmaxf(m, fabsf(v));
-                bad |= !(fabsf(v) <= FLT_MAX);
+                m = fmaxf(m, fabsf(f[d][i]));
+                bad |= !(fabsf(f[d][i]) <= FLT_MAX);
             }
         if (bad) m = INFINITY;
         m = fmaxf(m, __shfl_xor(m, 32));
@@ -672,7 +681,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
         for (int d = 0; d < ND; ++d) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = ok ? ldexpf(q[16 * d + i], e) : 0.f;
+                const float v = ok ? ldexpf(f[d][i], e) : 0.f;
                 Qh[d][i] = static_cast<_Float16>(v);
                 Ql[d][i] = static_cast<_Float16>(low_part(v));
             }
@@ -908,14 +917,24 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
 }
 
 // ------------------------------------------------------------------ host
-// Pieces are at most kTargetItems plus one per unit; units at most one per 8 pairs plus one per request that has rows, and
-// at most one per 8 of the pairs with which a request still takes this kernel.
+// Whether a call can have requests for prompt_kernel; if not, split_kernel takes them all. A call with no more rows than
+// requests is taken for a batch of single tokens, up to kSplitOnly (row, head) pairs of a KV head, and spared the launch
+// (us: 64 tokens at 500 keys 21.1 -> 19.3, 128 31.6 -> 29.9). Should one request have all the rows, split_kernel answers it
+// too (64 rows at 2500 keys among 64 requests: 42, as with prompt_kernel 44), if at long contexts not as fast (33 rows
+// at 30000 keys 138, 67).
+bool may_prompt(int rows, int requests, int group) {
+    const int64_t pairs = static_cast<int64_t>(rows) * group;
+    return rows > 1 && pairs > kSplitMax && (rows > requests || pairs > kSplitOnly);
+}
+// split_kernel's pieces are at most kTargetItems plus one per unit; units at most one per 8 pairs plus one per request that
+// has rows, and, where larger requests go to prompt_kernel, at most one per 8 of the pairs with which one does not.
 int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
     const int group = heads / kv_heads;
     const int64_t pairs = static_cast<int64_t>(rows) * group, busy = std::min(rows, requests);
-    return std::min(pairs / kRows + busy, busy * blocks_for(std::max(kSplitMax, group), kRows)) * kv_heads;
+    int64_t units = pairs / kRows + busy;
+    if (may_prompt(rows, requests, group)) units = std::min(units, busy * blocks_for(std::max(kSplitMax, group), kRows));
+    return units * kv_heads;
 }
-bool may_prompt(int rows, int group) { return rows > 1 && static_cast<int64_t>(rows) * group > kSplitMax; }
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
 struct Layout {
@@ -926,7 +945,7 @@ Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     Layout l;
     l.items = kTargetItems + unit_bound(rows, requests, heads, kv_heads);
     l.all = l.items;
-    if (may_prompt(rows, heads / kv_heads)) l.all += kPromptFill * (kPromptRows / kRows);
+    if (may_prompt(rows, requests, heads / kv_heads)) l.all += kPromptFill * (kPromptRows / kRows);
     l.stat = align_up(static_cast<size_t>(l.all) * kRows * dim * 4);
     l.info = l.stat + align_up(static_cast<size_t>(l.all) * kRows * 8);
     l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);
@@ -1000,7 +1019,7 @@ int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_co
     a.rows = rows;
     a.heads = heads;
     a.group = heads / kv_heads;
-    a.split_all = !may_prompt(rows, a.group);
+    a.split_all = !may_prompt(rows, requests, a.group);
     a.part = reinterpret_cast<float*>(ws);
     a.stat = reinterpret_cast<float2*>(ws + l.stat);
     a.info = reinterpret_cast<int2*>(ws + l.info);
