@@ -96,17 +96,20 @@ struct Tile {
     int expert, first, n;   // pairs order[first .. first + n)
 };
 
-// Tiles of up to `size` pairs, expert by expert; the count in tiles[-1].expert. One wave.
+// Tiles of up to `size` pairs, expert by expert; the count in tiles[-1].expert. One workgroup of 256 threads, an expert to
+// each (one wave took 4 us for 256 experts).
 __device__ void write_tiles(const int32_t* __restrict__ starts, int experts, int pairs, int size, Tile* __restrict__ tiles,
                             int most) {
-    const int lane = threadIdx.x & 63;
+    __shared__ int part[2][4];
+    const int lane = threadIdx.x & 63, wv = wave_in_block();
     int at = 0;
-    for (int e0 = 0; e0 < experts; e0 += kWave) {
-        const int e = e0 + lane;
+    for (int e0 = 0, turn = 0; e0 < experts; e0 += 256, turn ^= 1) {
+        const int e = e0 + static_cast<int>(threadIdx.x);
         int s = 0, n = 0;
         if (e < experts) {
-            s = min(max(starts[e], 0), pairs);
-            n = min(max(starts[e + 1], s), pairs) - s;
+            const int from = starts[e], to = starts[e + 1];
+            s = min(max(from, 0), pairs);
+            n = min(max(to, s), pairs) - s;
         }
         // of several tiles of 16 pairs each: even ones, whole sixteens
         const int even = (n + size - 1) / size, one = size <= 16 || n == 0 ? size : ((n + even - 1) / even + 15) / 16 * 16;
@@ -117,13 +120,18 @@ __device__ void write_tiles(const int32_t* __restrict__ starts, int experts, int
             const int up = __shfl_up(inc, o);
             if (lane >= o) inc += up;
         }
+        if (lane == 63) part[turn][wv] = inc;
+        __syncthreads();   // (two sets of sums: the next turn's are written while a slow wave still reads these)
+        for (int w = 0; w < 4; ++w) {
+            if (w == wv) inc += at;
+            at += part[turn][w];
+        }
         for (int i = 0; i < k; ++i) {
-            const int slot = at + inc - k + i;
+            const int slot = inc - k + i;
             if (slot < most) tiles[slot] = Tile{e, s + i * one, min(one, n - i * one)};
         }
-        at += __shfl(inc, 63);
     }
-    if (lane == 0) tiles[-1] = Tile{min(at, most), 0, 0};
+    if (threadIdx.x == 0) tiles[-1] = Tile{min(at, most), 0, 0};
 }
 
 // Pair at a place of the order, inside the call's pairs whatever the array holds.
@@ -147,7 +155,7 @@ __global__ __launch_bounds__(256) void rows_prep(const float* __restrict__ x, in
     const int wv = wave_in_block(), lane = threadIdx.x & 63;
     if (blockIdx.x == gridDim.x - 1) {
         if constexpr (FIRST) {
-            if (wv == 0) write_tiles(gr.starts, gr.experts, gr.pairs, gr.size, gr.tiles, gr.most);
+            write_tiles(gr.starts, gr.experts, gr.pairs, gr.size, gr.tiles, gr.most);
         } else {
             for (int q = max(gr.starts[gr.experts], 0) + static_cast<int>(threadIdx.x); q < gr.pairs; q += 256)
                 gr.lost[pair_at(gr.order, q, gr.pairs) / gr.top] = 1;
@@ -159,12 +167,14 @@ __global__ __launch_bounds__(256) void rows_prep(const float* __restrict__ x, in
     if (FIRST && lane == 0) gr.lost[r] = 0;
     const float* row = x + static_cast<size_t>(r) * K;
     float m = 0.f;
+#pragma unroll 4
     for (int k = 8 * lane; k < K; k += 512) m = max_abs4(max_abs4(m, ld4(row + k)), ld4(row + k + 4));
     const int e = prep_exponent(wave_max_abs(m)), es = e == kRowNonFinite ? 0 : e;
     if (lane == 0) ex[r] = e;
     const int c = lane & 31;   // chunk of 8 in the block: 16 (lk / 2) + 4 u + 2 (lk % 2) + j, depth 2 u + j
     const int depth = 2 * ((c >> 2) & 3) + (c & 1), lk = 2 * (c >> 4) + ((c >> 1) & 1);
     uint8_t* out = xp + static_cast<size_t>(r) * K * 4 + 128 * depth + 16 * lk;
+#pragma unroll 4
     for (int k = 8 * lane; k < K; k += 512) {
         uint32_t h[4], l[4];
         float s = split8(ld4(row + k), ld4(row + k + 4), es, h, l);
