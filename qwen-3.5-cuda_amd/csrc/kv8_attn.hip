@@ -424,15 +424,26 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
     int2 in = make_int2(0, 0);
     if (lane < (NW == 1 ? per : 1) && pair0 + lane < live) in = a.info[pair0 + lane];
     const bool join = in.y > 1 && in.x >= 0 && in.y <= a.all_items - in.x / kRows;
+    auto load = [](const float* p, float(&f)[V]) {
+        if constexpr (V == 4) {
+            const float4 x = ld4(p);
+            f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = p[i];
+        }
+    };
     uint64_t todo = __ballot(join);   // the same in every wave of a pair
     while (todo) {
         const int k = __builtin_ctzll(todo);
         todo &= todo - 1;
         const int pieces = __builtin_amdgcn_readlane(in.y, k), where = __builtin_amdgcn_readlane(in.x, k);
         const int slot = where % kRows, first = where / kRows;
-        float m = -FLT_MAX, l = 0.f, s[V];
+        float m = -FLT_MAX, l = 0.f, s[V], gt[V];
+        const size_t o = static_cast<size_t>(pair0 + k) * D;
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] = 0.f;
+        for (int i = 0; i < V; ++i) s[i] = 0.f, gt[i] = 0.f;
+        if (NW == 1 && a.gate) load(a.gate + o + V * lane, gt);
         auto at = [&](int p) { return static_cast<size_t>(first + p) * kRows + slot; };
         constexpr int U = 4;   // pieces in flight
         for (int p0 = wv; p0 < pieces; p0 += U * NW) {
@@ -442,13 +453,7 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
             for (int u = 0; u < U; ++u) {
                 const size_t q = at(min(p0 + u * NW, pieces - 1));
                 st[u] = a.stat[q];
-                if constexpr (V == 4) {
-                    const float4 f = ld4(a.part + q * D + 4 * lane);
-                    x[u][0] = f.x, x[u][1] = f.y, x[u][2] = f.z, x[u][3] = f.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) x[u][i] = a.part[q * D + V * lane + i];
-                }
+                load(a.part + q * D + V * lane, x[u]);
             }
             __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
 #pragma unroll
@@ -462,15 +467,19 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
                 for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
             }
         }
-        auto put = [&](int d, float sum, float tot) {
-            const size_t o = static_cast<size_t>(pair0 + k) * D + d;
-            float v = tot == 0.f ? 0.f : sum / kWeightUp / tot;
-            if (a.gate) v *= sigmoid(a.gate[o]);
-            a.out[o] = v;
+        auto done = [&](float sum, float tot, float gate) {
+            const float v = tot == 0.f ? 0.f : sum / kWeightUp / tot;
+            return a.gate ? v * sigmoid(gate) : v;
         };
         if constexpr (NW == 1) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) put(V * lane + i, s[i], l);
+            for (int i = 0; i < V; ++i) s[i] = done(s[i], l, gt[i]);
+            if constexpr (V == 4) {
+                st4(a.out + o + 4 * lane, make_float4(s[0], s[1], s[2], s[3]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) a.out[o + V * lane + i] = s[i];
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
@@ -490,7 +499,7 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
                     sum += f * sums[w][d];
                     tot += f * ls[w];
                 }
-                put(d, sum, tot);
+                a.out[o + d] = done(sum, tot, a.gate ? a.gate[o + d] : 0.f);
             }
         }
     }
