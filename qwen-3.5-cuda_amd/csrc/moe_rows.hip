@@ -866,6 +866,7 @@ int qwen_moe_experts_rows(const void* w_gate, const void* w_up, int type, const 
         return fail(QWEN_STATUS_UNSUPPORTED_TYPE, "moe_experts_rows: GGML types %d, %d (Q4_K and Q6_K)", type, down_type);
     QK_REQUIRE(width > 0 && inter > 0 && width % 256 == 0 && inter % 256 == 0,
                "moe_experts_rows: widths %d and %d are not multiples of 256", width, inter);
+    QK_REQUIRE(width <= (1 << 20) && inter <= (1 << 20), "moe_experts_rows: widths %d and %d exceed 2^20", width, inter);
     QK_REQUIRE(n_experts > 0 && n_experts <= kMaxExperts, "moe_experts_rows: %d experts (1 to %d)", n_experts, kMaxExperts);
     QK_REQUIRE(rows >= 0 && top > 0 && static_cast<int64_t>(rows) * top <= (1 << 24), "moe_experts_rows: %d rows of %d picks",
                rows, top);

@@ -555,6 +555,11 @@ class Kv8Cache:
         self.pages, self.page, self.heads, self.dim = pages, page, heads, dim
         self.args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page, heads, dim)
 
+    def __setattr__(self, name, value):
+        if hasattr(self, "args"):   # its pointers are those of the tensors above
+            raise AttributeError("a Kv8Cache stays over the tensors it was made of")
+        object.__setattr__(self, name, value)
+
 
 def kv8_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv8Cache:
     """An empty cache."""

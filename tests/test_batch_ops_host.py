@@ -112,6 +112,7 @@ def test_experts(lib):
     assert call(type=8) == UNS and call(down=0) == UNS
     refused(lib, call(width=500), "multiples of 256")
     refused(lib, call(inter=0), "multiples of 256")
+    refused(lib, call(width=(1 << 20) + 256), "exceed 2^20")
     refused(lib, call(experts=1025), "experts")
     refused(lib, call(experts=0), "experts")
     refused(lib, call(rows=-1), "rows")

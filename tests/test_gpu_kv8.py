@@ -292,6 +292,19 @@ def test_attention_prompts_in_pieces(heads, kvh, dim, page):
     attention_case(r, [1100, 900, 530, 64], [50, 1, 35, 40], heads, kvh, dim, page, pad=2)
 
 
+def test_attention_no_more_rows_than_requests():
+    """A batch padded to many requests, one of which has most of the rows (the few-row kernel takes them all)."""
+    r = np.random.default_rng(33)
+    attention_case(r, [700, 0, 90, 1] + [0] * 60, [58, 0, 5, 1] + [0] * 60, 16, 2, 128, 16)
+    attention_case(r, [0] * 79 + [130], [0] * 79 + [80], 8, 2, 64, 8, pad=0)
+
+
+def test_a_cache_stays_over_its_tensors():
+    cache = ops.kv8_cache(2, 1, 64, 8)
+    with pytest.raises(AttributeError, match="stays over"):
+        cache.k = cache.k.clone()
+
+
 def test_attention_prompts_in_pieces_bad_page():
     """A page outside the cache makes every row of its request NaN that sees it, whichever piece holds it."""
     r = np.random.default_rng(31)

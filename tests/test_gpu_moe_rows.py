@@ -165,6 +165,16 @@ def test_experts_ragged(kind, sizes):
     check(Layer(len(sizes), 256, 512, kind, kind), idx, w, (0.05 * r.standard_normal((rows, 512))).astype(F32))
 
 
+@pytest.mark.parametrize("kind", ["Q4_K", "Q6_K"])
+def test_experts_tiles_of_every_size(kind):
+    """Groups around each number of sixteens that a tile can have, and the even tiles of larger ones; odd numbers of blocks."""
+    sizes = [24, 47, 48, 49, 63, 79, 80, 81, 96, 97, 112, 145]
+    r = np.random.default_rng(99)
+    rows = sum(sizes)
+    idx, w = routing(r, rows, 1, len(sizes), sizes)
+    check(Layer(len(sizes), 256, 768, kind, kind), idx, w, (0.05 * r.standard_normal((rows, 768))).astype(F32))
+
+
 def test_experts_rows_of_many_sizes():
     """Rows of x from 1e-30 to 1e10, one of zeros, one whose elements span 2^40."""
     r = np.random.default_rng(7)
