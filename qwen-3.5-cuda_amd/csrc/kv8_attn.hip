@@ -43,7 +43,9 @@ constexpr int kSplitWaves = 4;
 constexpr int kSplitBlock = kSplitWaves * kWave;
 constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
 constexpr int kTargetItems = 1024;     // pieces of the whole call
-constexpr int kMinTiles = 8;           // of a piece: two steps per wave
+constexpr int kMinTiles = 8;           // of a piece: two steps per wave; one in calls that then still have at most kFewItems
+constexpr int kFewItems = 256;         // pieces, one a CU (4 tokens at 4000 keys 14.9 us with 4 tiles, 16.2 with 8; one token
+                                       // at 30000 keys 22.7, 19.0)
 constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take the split kernel (100
                                        // requests of 64 at 1500 keys: 205 us, with the prompt kernel 108); a single row does
 constexpr int kSplitOnly = 1024;       // and of a whole call that has no more rows than requests
@@ -111,7 +113,9 @@ __device__ bool find_piece(const AttnArgs& a, int64_t item, Piece& p) {
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
-    const int64_t cut = max(static_cast<int64_t>(kMinTiles), (total + kTargetItems - 1) / kTargetItems);
+    const int64_t least = min(max((total + kFewItems - 1) / kFewItems, static_cast<int64_t>(kSplitWaves)),
+                              static_cast<int64_t>(kMinTiles));
+    const int64_t cut = max(least, (total + kTargetItems - 1) / kTargetItems);
     p.tiles = static_cast<int>(min(cut, static_cast<int64_t>(0x7fffffff)));
     for (int b0 = 0; b0 < a.requests; b0 += kWave) {
         const int b = b0 + lane;
@@ -162,34 +166,6 @@ __device__ __forceinline__ float max_over_lk(float v) {
     return fmaxf(v, __shfl_xor(v, 32));
 }
 
-// A lane's 16 (D / 64) elements of query row `row` (dims 64 j + 16 lk ..), scaled by 2^e so that the row's largest
-// magnitude is in [2^14, 2^15). Returns the factor from products to log2 scores; NaN for a row with infinities or NaNs.
-template <int D>
-__device__ __forceinline__ float load_query(const float* __restrict__ row, int lk, float scale, float (&f)[D / 4]) {
-    float m = 0.f;
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float v = row[64 * j + 16 * lk + i];
-            f[16 * j + i] = v;
-            m = fmaxf(m, fabsf(v));
-            bad |= !(fabsf(v) <= FLT_MAX);
-        }
-    m = max_over_lk(bad ? INFINITY : m);
-    int e = 0;
-    if (m > 0.f && m <= FLT_MAX) {
-        int em;
-        frexpf(m, &em);
-        e = 15 - em;
-    }
-    const bool ok = m <= FLT_MAX;
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) f[i] = ok ? ldexpf(f[i], e) : 0.f;
-    return ok ? ldexpf(scale, -e) : __builtin_nanf("");
-}
-
 // The fp32 product behind a value that is then split in two fp16 parts: kept from being fused into the conversion
 // (v_fma_mixlo_f16 rounds once where the other part's subtraction has rounded twice, and the parts miss by an fp16 ulp
 // of one weight in some thousands).
@@ -221,6 +197,8 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split_kernel(const AttnArgs a)
     constexpr int NJ = D / 64, ND = D / 32, LD = D + 2;
     __shared__ float sums[kSplitWaves][kRows * LD];
     __shared__ float stat[kSplitWaves][kRows][2];
+    __shared__ __align__(16) _Float16 qs[2 * kRows][D + 8];   // the queries' parts; 16 bytes more, and 16 rows meet no bank twice
+    __shared__ float factors[kRows];
     Piece pc;
     if (!find_piece(a, blockIdx.x, pc)) return;   // the whole workgroup
     const Request r = request(a, pc.b);
@@ -229,8 +207,7 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split_kernel(const AttnArgs a)
     const int h = pc.unit / blocks, rb = pc.unit - h * blocks;
     const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4, part = lr & 1;
     const int wv = wave_in_block();
-    const int rr = min(rb * kRows + (lr >> 1), pairs - 1);   // columns past the last pair repeat it
-    const int ti = rr / G, head = h * G + (rr - ti * G);
+    const int ti = min(rb * kRows + (lr >> 1), pairs - 1) / G;   // columns past the last pair repeat it
     const int limit = r.len - r.n + ti;                      // this column's last key
     const int first_limit = r.len - r.n + rb * kRows / G;    // the smallest of the workgroup
     const int seen = max(r.len - r.n + min(rb * kRows + kRows - 1, pairs - 1) / G + 1, 0);   // keys that some column sees
@@ -275,6 +252,20 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split_kernel(const AttnArgs a)
         if (!w.live) ksc = vsc = 0.f;
         if (w.bad) ksc = __builtin_nanf("");
     };
+    // The rows' queries, scaled by 2^e so that a row's largest magnitude is in [2^14, 2^15), as two fp16 parts: 2 rows a wave,
+    // requested before the first tile. (Every wave on its own for all 8 rows: half of the vector work of a short piece.)
+    const int qr = 2 * wv + (lane >> 5), qp = min(rb * kRows + qr, pairs - 1), qt = qp / G;
+    const float* qrow = a.q + (static_cast<size_t>(r.first + qt) * a.heads + h * G + (qp - qt * G)) * D + (lane & 31) * (D / 32);
+    float qf[D / 32];
+    if constexpr (D >= 128) {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+            const float4 x = ld4(qrow + 4 * i);
+            qf[4 * i] = x.x, qf[4 * i + 1] = x.y, qf[4 * i + 2] = x.z, qf[4 * i + 3] = x.w;
+        }
+    } else {
+        qf[0] = qrow[0], qf[1] = qrow[1];
+    }
     const bool any = t < t_end;
     Where next{};
     if (any) {
@@ -283,19 +274,40 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split_kernel(const AttnArgs a)
         load_v(w);
         if (t + kSplitWaves < t_end) next = where(t + kSplitWaves);
     }
-    f16x8_t Q[2 * NJ];
-    float factor;
     {
-        float f[D / 4];
-        factor = load_query<D>(a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D, lk, a.scale, f);
+        float m = 0.f;
+        bool bad = false;
 #pragma unroll
-        for (int d = 0; d < 2 * NJ; ++d)
+        for (int i = 0; i < D / 32; ++i) {
+            m = fmaxf(m, fabsf(qf[i]));
+            bad |= !(fabsf(qf[i]) <= FLT_MAX);
+        }
+        if (bad) m = INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = f[8 * d + i];
-                Q[d][i] = static_cast<_Float16>(part ? low_part(v) : v);
-            }
-    }
+        for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const bool ok = m <= FLT_MAX;
+        int e = 0;
+        if (m > 0.f && ok) {
+            int em;
+            frexpf(m, &em);
+            e = 15 - em;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const float v = ok ? ldexpf(qf[i], e) : 0.f;
+            qs[2 * qr][(lane & 31) * (D / 32) + i] = static_cast<_Float16>(v);
+            qs[2 * qr + 1][(lane & 31) * (D / 32) + i] = static_cast<_Float16>(low_part(v));
+        }
+        if ((lane & 31) == 0) factors[qr] = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");   // products to log2 scores; NaN: a row
+    }                                                                                        // with infinities or NaNs
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile's loads stay in flight
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    f16x8_t Q[2 * NJ];   // dims 64 j + 16 lk + 8 (d % 2) + 0..7 of depth d = 2 j + d % 2
+#pragma unroll
+    for (int d = 0; d < 2 * NJ; ++d)
+        Q[d] = *reinterpret_cast<const f16x8_t*>(&qs[lr][64 * (d >> 1) + 16 * lk + 8 * (d & 1)]);
+    const float factor = factors[lr >> 1];
     f32x4_t acc[ND][2];
 #pragma unroll
     for (int m = 0; m < ND; ++m) acc[m][0] = acc[m][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
