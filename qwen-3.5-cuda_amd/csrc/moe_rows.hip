@@ -554,13 +554,19 @@ __global__ __launch_bounds__(kRowsWaves* kWave) __attribute__((amdgpu_waves_per_
 // rows: two rounds of some 45 us at 77 tokens. Two workgroups a CU of 128 registers, two turns ahead: 92 us against 65.)
 // Of up to 8 pairs both fp16 parts enter one operand, rows 0-7 the high ones and 8-15 the low ones: half the products, and
 // a sum of two lanes at the end (5 tokens 20.5 and 12.4 us for the two products, 22.2 and 13.6 with tiles of 16).
-// Without its arithmetic the kernel takes 57 us at 77 tokens (202 MB), 65 with it; 8 us are the start.
+// A block's rows come as the 16-byte pieces that they lie in, neighbours to neighbouring lanes, and go to the lanes that use
+// them through LDS, the next turn's before the barrier (each lane its own pieces from memory, us in all: 77 tokens 118 -> 114,
+// Q6_K, whose blocks begin at odd places, 186 -> 171, one token of 8 picks 50 -> 36). 77 tokens: 64 us for 202 MB; 8 are the
+// start, and the products, the decode and the moves of a turn add up to three quarters of the rest.
 template <int TYPE, int TP, int KW, bool SWIGLU>
 __global__ __launch_bounds__(512, 2) void strip_kernel(const RowsArgs a) {
     constexpr int BB = TYPE == kQ4_K ? 144 : 210, NB = TYPE == kQ4_K ? 1 : 2, WR = 2, RW = 8 / KW;
     constexpr int RT = SWIGLU ? 16 : 32;              // rows of a row tile
     constexpr int NP = TP == 8 ? 1 : 2;               // operands of x per depth
-    constexpr int AHEAD = 4;                          // turns of weights in flight
+    constexpr int AHEAD = TYPE == kQ4_K ? 4 : 3;   // turns of weights in flight, as the registers allow
+    using W = Staged<TYPE>;
+    constexpr int WP = 32 * W::pieces, WI = (WP + 63) / 64;   // 16-byte pieces of a wave's 32 rows of its block
+    __shared__ uint4 staged[8][WP];
     __shared__ f32x4_t part[2][8][WR][kWave];
     __shared__ int exps[2][TP];                       // of the rows of this tile and the one before
     const int M = a.M, K = a.K, nb = K >> 8;
@@ -583,12 +589,20 @@ __global__ __launch_bounds__(512, 2) void strip_kernel(const RowsArgs a) {
 #pragma unroll
         for (int rt = 0; rt < WR; ++rt) wexp[rt] = a.w[SWIGLU ? rt : 0] + (static_cast<uint64_t>(e) * M * nb + kb) * BB;
     };
-    auto w_load = [&](WBlock<TYPE> (&d)[WR]) {        // past the end the last one again: nothing waits for it
-        const int r0 = min(lg * RW + rw, row_tiles - 1) * RT;
+    uint32_t wo[WI];
 #pragma unroll
-        for (int rt = 0; rt < WR; ++rt) {
-            const uint32_t r = static_cast<uint32_t>(min(r0 + (SWIGLU ? 0 : 16 * rt) + lr, M - 1));
-            d[rt].load(wexp[rt] + static_cast<size_t>(r) * nb * BB, 0u, lk);
+    for (int i = 0; i < WI; ++i) {
+        const int id = min(64 * i + lane, WP - 1), row = id / W::pieces;
+        wo[i] = static_cast<uint32_t>(SWIGLU ? row & 15 : row) * nb * BB + 16 * (id - row * W::pieces);
+    }
+    auto row_offset = [&](int g) { return static_cast<uint32_t>(min(g * RW + rw, row_tiles - 1) * RT) * nb * BB; };
+    auto w_load = [&](uint4 (&d)[WI]) {               // past the end the last one again: nothing waits for it
+        const uint32_t skew = TYPE == kQ4_K ? 0 : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(wexp[0])) & 15u;
+        const uint32_t at = row_offset(lg) + skew;
+#pragma unroll
+        for (int i = 0; i < WI; ++i) {
+            const int id = min(64 * i + lane, WP - 1);
+            d[i] = ld16((SWIGLU && id >= WP / 2 ? wexp[1] : wexp[0]) - skew + ((at + wo[i]) & ~15u));
         }
         if (++ln < count && ++lg == groups) {
             lg = 0;
@@ -596,7 +610,27 @@ __global__ __launch_bounds__(512, 2) void strip_kernel(const RowsArgs a) {
             w_expert();
         }
     };
-    WBlock<TYPE> w[AHEAD][WR];
+    // the weights of the turn that is taken next: where its first row lies in its 16 bytes
+    int tt = tile, tg = group, tn = 0;
+    WBlock<TYPE> wc[WR];
+    auto w_take = [&](const uint4 (&d)[WI]) {
+        uint4* wl = staged[wv];
+#pragma unroll
+        for (int i = 0; i < WI; ++i) wl[min(64 * i + lane, WP - 1)] = d[i];
+        uint32_t base = 0;
+        if constexpr (TYPE != kQ4_K)
+            base = static_cast<uint32_t>((static_cast<uint64_t>(a.tiles[tt].expert) * M * nb + kb) * BB) + row_offset(tg);
+#pragma unroll
+        for (int rt = 0; rt < WR; ++rt) {
+            const uint32_t row = static_cast<uint32_t>((SWIGLU ? 0 : 16 * rt) + lr) * nb * BB;
+            W::take(wc[rt], wl + (16 * rt + lr) * W::pieces, (base + row) & 15u, lk);
+        }
+        if (++tn < count && ++tg == groups) {
+            tg = 0;
+            ++tt;
+        }
+    };
+    uint4 w[AHEAD][WI];
     w_expert();
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
@@ -675,16 +709,18 @@ __global__ __launch_bounds__(512, 2) void strip_kernel(const RowsArgs a) {
         }
     };
     x_load();
-    auto step = [&](WBlock<TYPE> (&wb)[WR], int turn) {
+    w_take(w[0]);
+    w_load(w[0]);
+    auto step = [&](uint4 (&next)[WI], int turn) {   // next: the weights of the turn after this one
         f32x4_t C[WR];
         WScale<TYPE> sc[WR];
         static_for<8>([&](auto dI) {
             constexpr int D = decltype(dI)::value, U = D >> 1, J = D & 1;
 #pragma unroll
             for (int rt = 0; rt < WR; ++rt) {
-                if constexpr (J == 0) sc[rt].template set<U>(wb[rt], lk);
+                if constexpr (J == 0) sc[rt].template set<U>(wc[rt], lk);
                 f16x8_t B[NB];
-                decode<U, J>(wb[rt], sc[rt], k64, B);
+                decode<U, J>(wc[rt], sc[rt], k64, B);
                 C[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[D][0], B[0], D == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : C[rt], 0, 0, 0);
                 if constexpr (NP == 2) C[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[D][1], B[0], C[rt], 0, 0, 0);
                 if constexpr (NB == 2) C[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[D][0], B[NB - 1], C[rt], 0, 0, 0);
@@ -694,19 +730,20 @@ __global__ __launch_bounds__(512, 2) void strip_kernel(const RowsArgs a) {
         for (int rt = 0; rt < WR; ++rt) {
             f32x4_t s;
             if constexpr (TYPE == kQ4_K) {
-                const float d = opaque(half_bits(wb[rt].hd.x & 0xffffu)), dmin = opaque(-32.0f * half_bits(wb[rt].hd.x >> 16));
+                const float d = opaque(half_bits(wc[rt].hd.x & 0xffffu)), dmin = opaque(-32.0f * half_bits(wc[rt].hd.x >> 16));
                 const f32x4_t pm =
-                    __builtin_amdgcn_mfma_f32_16x16x16f16(As, min_weights(wb[rt].hd, lk), f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    __builtin_amdgcn_mfma_f32_16x16x16f16(As, min_weights(wc[rt].hd, lk), f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(dmin, pm[i], d * C[rt][i]);
             } else {
-                const float d = opaque(half_bits(wb[rt].d));
+                const float d = opaque(half_bits(wc[rt].d));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[i] = d * C[rt][i];
             }
             part[turn & 1][wv][rt][lane] = active ? s : f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
-        w_load(wb);
+        w_take(next);
+        w_load(next);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the sums are in LDS (the loads of weights stay in flight)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -720,14 +757,16 @@ __global__ __launch_bounds__(512, 2) void strip_kernel(const RowsArgs a) {
     // Left from the middle, not skipped over: so that on every way back to the first step the other buffers' loads have been
     // issued after its own, and it waits for its own alone.
     for (int u = 0;;) {
-        step(w[0], u);
+        step(w[1 % AHEAD], u);
         if (++u == count) break;
-        step(w[1], u);
+        step(w[2 % AHEAD], u);
         if (++u == count) break;
-        step(w[2], u);
+        step(w[3 % AHEAD], u);
         if (++u == count) break;
-        step(w[3], u);
-        if (++u == count) break;
+        if constexpr (AHEAD == 4) {
+            step(w[0], u);
+            if (++u == count) break;
+        }
     }
 }
 
@@ -759,7 +798,8 @@ size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
 // Pairs of a tile, and with them the kernel, by the mean size of the groups (those of a routing over all experts):
 // strip_kernel with tiles of 8 or 16 pairs, rows_kernel with up to 64. (All launches of a call, us, strip / rows: 128 tokens
-// of 8 picks among 256 experts Q4_K 153 / 161, Q6_K 224 / 222; 256 tokens 184 / 184 and 274 / 255; 512: 240 / 231, 365 / 303.)
+// of 8 picks among 256 experts Q4_K 142 / 161, Q6_K 208 / 222; 256 tokens 175 / 184 and 251 / 255; 512, before the strips'
+// loads by pieces, 240 / 231 and 365 / 303.)
 int tile_pairs(int64_t pairs, int experts, int width, int inter) {
     const double mean = static_cast<double>(pairs) / std::min<int64_t>(pairs, experts);
     if (mean <= 8 && std::max(width, inter) <= 2048) return mean <= 1.5 ? 8 : 16;
