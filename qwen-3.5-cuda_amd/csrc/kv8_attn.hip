@@ -520,11 +520,11 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
 // ------------------------------------------------------------------ many rows
 // 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: an operand of keys or values, 1 KB of LDS, feeds 2
 // products (both parts of 32 rows), 64 cycles, so that the waves' reads take half of the LDS's rate; with 16 rows a wave they
-// took all of it (5000 rows 690 us, now 485 to 550 with the card's clock). A wave holds its rows' query parts (128 registers at D = 256, pinned in
-// accumulation registers) and sums (128). Its vector work - softmax, turning codes to fp16 - is laid between its own
-// products: while tile t + 1's scores are computed, tile t's are exponentiated; while tile t's values are summed, the codes
-// of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own rows may end one earlier:
-// with a branch around the products the compiler moves the sums between register files at each.
+// took all of it (5000 rows 690 us, now 485 to 550 with the card's clock). A wave holds its rows' query parts (128
+// registers at D = 256, pinned in accumulation registers) and sums (128). Its vector work - softmax, turning codes to fp16 -
+// is laid between its own products: while tile t + 1's scores are computed, tile t's are exponentiated; while tile t's
+// values are summed, the codes of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own
+// rows may end one earlier: with a branch around the products the compiler moves the sums between register files at each.
 // The scores^T tile has token rho = 8 b + 4 g + j of the 32 in register 4 b + j of lane half g; key row rho stands for token
 // 16 (b / 2) + 8 g + 4 (b % 2) + j, so that a lane's registers 8 s .. 8 s + 7 are octet 2 s + g, its share of the second
 // product's depth s.
@@ -1014,7 +1014,8 @@ int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_co
     QK_REQUIRE(heads > 0 && heads % kv_heads == 0, "attn_kv8_rows: %d query heads over %d KV heads", heads, kv_heads);
     QK_REQUIRE(rows >= 0 && requests >= 0 && max_pages >= 0, "attn_kv8_rows: negative size");
     QK_REQUIRE(requests <= kKv8MaxRequests, "attn_kv8_rows: %d requests (at most %d)", requests, kKv8MaxRequests);
-    QK_REQUIRE(static_cast<int64_t>(max_pages) * page_size <= 0x7fffffff, "attn_kv8_rows: table rows of %d pages", max_pages);
+    // (tokens a few tiles past a row's end are computed in 32 bits too)
+    QK_REQUIRE(static_cast<int64_t>(max_pages) * page_size <= (1 << 30), "attn_kv8_rows: table rows of %d pages", max_pages);
     if (rows == 0 || requests == 0) return ok();
     QK_REQUIRE(q && out && row_start && kv_len && (block_table || max_pages == 0), "attn_kv8_rows: null pointer");
     QK_REQUIRE(static_cast<int64_t>(rows) * heads <= (int64_t{1} << 24), "attn_kv8_rows: %d rows of %d heads exceed one call",

@@ -555,9 +555,9 @@ __global__ __launch_bounds__(kRowsWaves* kWave) __attribute__((amdgpu_waves_per_
 // Of up to 8 pairs both fp16 parts enter one operand, rows 0-7 the high ones and 8-15 the low ones: half the products, and
 // a sum of two lanes at the end (5 tokens 20.5 and 12.4 us for the two products, 22.2 and 13.6 with tiles of 16).
 // A block's rows come as the 16-byte pieces that they lie in, neighbours to neighbouring lanes, and go to the lanes that use
-// them through LDS, the next turn's before the barrier (each lane its own pieces from memory, us in all: 77 tokens 118 -> 114,
+// them through LDS, the next turn's before the barrier (each lane its own pieces from memory, us in all: 64 tokens 118 -> 114,
 // Q6_K, whose blocks begin at odd places, 186 -> 171, one token of 8 picks 50 -> 36). 77 tokens: 64 us for 202 MB; 8 are the
-// start, and the products, the decode and the moves of a turn add up to three quarters of the rest.
+// start, and the products and the decode of a turn, counted, are three quarters of the rest.
 template <int TYPE, int TP, int KW, bool SWIGLU>
 __global__ __launch_bounds__(512, 2) void strip_kernel(const RowsArgs a) {
     constexpr int BB = TYPE == kQ4_K ? 144 : 210, NB = TYPE == kQ4_K ? 1 : 2, WR = 2, RW = 8 / KW;

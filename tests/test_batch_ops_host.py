@@ -86,6 +86,7 @@ def test_attention(lib):
     refused(lib, call(rows=-1), "negative")
     refused(lib, call(requests=4097), "at most 4096")
     refused(lib, call(max_pages=1 << 30), "table rows")
+    refused(lib, call(max_pages=(1 << 24) + 1), "table rows")
     refused(lib, call(rows=1 << 21), "exceed one call")
     refused(lib, call(out=P), "out is q")
     for name in ("q", "out", "gate"):
