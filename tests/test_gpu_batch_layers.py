@@ -118,3 +118,45 @@ def test_attention_batch_of_layers():
             want = host(ops.matmul_rows(w, a.wtype, M * a.qd, dev(mid.reshape(n, a.qd), F32), M, a.qd))
             close(got[:n], want, (li, fresh))
             assert np.all(np.isfinite(got))
+
+
+def test_a_step_of_both_layers_in_a_graph():
+    """A planned step through an attention and a MoE layer, captured once and replayed over other lengths and rows with eager
+    work between: every replay equals the eager step bit for bit."""
+    r = np.random.default_rng(4)
+    page, pages, rows, requests, width, dm, E, I, S = 16, 24, 20, 3, 6, 512, 16, 256, 512
+    a = attn_layer(r)
+    moe = MoeLayerDecode(q4(E, dm, 60), q4(E * I, dm, 61), q4(E * I, dm, 62), q4(E * dm, I, 63), q4(1, dm, 64), q4(S, dm, 65),
+                         q4(S, dm, 66), q4(dm, S, 67), d_model=dm, experts=E, k=4, inter=I, shared=S)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    free = dev(r.permutation(pages), I32)
+    cached, fresh, xs = torch.zeros(requests, **i32), torch.zeros(requests, **i32), torch.zeros((rows, dm), device="cuda")
+
+    class Side:
+        def __init__(self):
+            self.batch = AttnLayerBatch(a, pages, page)
+            self.table, self.head = torch.zeros((requests, width), **i32), torch.zeros(1, **i32)
+
+        def step(self):
+            plan = ops.kv8_plan(cached, fresh, self.table, free, self.head, page, rows, free_head_out=self.head)
+            return moe.prefill(self.batch.forward(xs, self.table, plan))
+
+    eager, captured = Side(), Side()
+    for side in (eager, captured):
+        side.step()   # idle requests: loads the kernels, takes no page
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = captured.step()
+    lens = np.zeros(requests, int)
+    for new in ([11, 0, 3], [1, 6, 1], [1, 1, 18], [1, 1, 1]):
+        cached.copy_(dev(lens, I32))
+        fresh.copy_(dev(new, I32))
+        xs.copy_(dev((0.5 * r.standard_normal((rows, dm))).astype(F32)))
+        g.replay()
+        torch.cuda.synchronize()
+        want = eager.step()
+        assert torch.equal(out, want), new
+        assert torch.equal(captured.table, eager.table) and torch.equal(captured.head, eager.head)
+        assert torch.equal(captured.batch.cache.k_scale, eager.batch.cache.k_scale)
+        lens += new
