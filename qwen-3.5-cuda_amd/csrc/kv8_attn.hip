@@ -64,14 +64,15 @@ struct AttnArgs {
     int split_all;       // every request takes the split kernel
     float* part;         // [item][kRows][D] sums
     float2* stat;        // [item][kRows] (m, l)
-    int2* info;          // [row][head] (first item * kRows + row in item, pieces)
+    int2* info;          // [row][head] (first item * kRows + row in item, pieces); written for the requests' rows alone
     int items;           // capacity: the split kernel's grid
     int all_items;       // and with the cut prompts' pieces
     float scale;         // log2(e) / sqrt(D)
 };
 
 // A request as the kernels see it, whatever the arrays hold: rows inside q, lengths from 0 to what the table row holds
-// (`bad` marks a longer one, whose rows come out NaN).
+// (`bad` marks a longer one, whose rows come out NaN). Starts that do not decrease give every row between the first and the
+// last one request; of others the rows are not defined, but nothing is read or written out of bounds.
 struct Request {
     int first, n, len;
     bool bad;
@@ -431,10 +432,11 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
     constexpr int V = D / kWave;
     __shared__ float sums[NW][NW == 1 ? 1 : D], ls[NW], ms[NW];
     const int lane = threadIdx.x & 63, wv = NW == 1 ? 0 : wave_in_block();
-    const int live = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;   // pairs of the requests' rows
+    // Pairs of the requests' rows alone: only those have an entry of this call (the workspace may hold an earlier one's).
+    const int from = min(max(a.row_start[0], 0), a.rows) * a.heads, live = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;
     const int64_t pair0 = NW == 1 ? (static_cast<int64_t>(blockIdx.x) * 4 + wave_in_block()) * per : blockIdx.x;
     int2 in = make_int2(0, 0);
-    if (lane < (NW == 1 ? per : 1) && pair0 + lane < live) in = a.info[pair0 + lane];
+    if (lane < (NW == 1 ? per : 1) && pair0 + lane >= from && pair0 + lane < live) in = a.info[pair0 + lane];
     const bool join = in.y > 1 && in.x >= 0 && in.y <= a.all_items - in.x / kRows;
     auto load = [](const float* p, float(&f)[V]) {
         if constexpr (V == 4) {

@@ -1,0 +1,115 @@
+"""Attention over the paged 8-bit cache where its kernels meet their ends: calls with more row tiles than the card takes at
+once, joins of every form, rows that belong to no request, pages of zeros beside others.
+
+The reference is tests/kv8_ref.py's in 64 bits, a request at a time. Its tolerance stands there; here |v - out| in it is
+replaced by |v| + |out|, which needs no array of rows x keys x dims and is never smaller."""
+
+from __future__ import annotations
+
+import kv8_ref
+import numpy as np
+import pytest
+import torch
+
+from qwen35_hip import ops
+
+pytestmark = pytest.mark.gpu
+F32, F64, I32 = np.float32, np.float64, np.int32
+
+
+def dev(a, dtype=None):
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=dtype)).cuda()
+
+
+def host(t):
+    torch.cuda.synchronize()
+    return t.cpu().numpy()
+
+
+def gpu_cache(ref):
+    pages, heads, page, dim = ref.codes[0].shape
+    v = ref.codes[1].reshape(pages, heads, page // 8, 8, dim).swapaxes(3, 4)
+    return ops.Kv8Cache(dev(ref.codes[0], np.int8), dev(v, np.int8), dev(ref.scales[0], F32), dev(ref.scales[1], F32))
+
+
+def random_cache(r, pages, heads, page, dim):
+    ref = kv8_ref.Cache(pages, heads, page, dim)
+    for w in (0, 1):
+        ref.codes[w] = r.integers(-127, 128, ref.codes[w].shape).astype(F64)
+        ref.scales[w] = F64(F32(0.02 * 2.0 ** r.uniform(-3, 1, ref.scales[w].shape)))
+    return ref
+
+
+def tables(r, lens, page):
+    need = [-(-n // page) for n in lens]
+    ids = r.permutation(sum(need) + 2)
+    table = np.full((len(lens), max(max(need), 1)), -5, I32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = ids[at:at + n]
+        at += n
+    return table, sum(need) + 2
+
+
+def attention_wide(q, ref, table, start, lens):
+    """-> (out, tolerance), all rows of a request and KV head as one matrix."""
+    rows, heads, dim = q.shape
+    kvh = ref.codes[0].shape[1]
+    group = heads // kvh
+    out, tol = np.full(q.shape, 7.0), np.zeros(q.shape)
+    for b, total in enumerate(lens):
+        n = start[b + 1] - start[b]
+        if n == 0:
+            continue
+        t = np.arange(total)
+        slots = table[b][t // ref.page] * ref.page + t % ref.page
+        for g in range(kvh):
+            k, v = (ref.values(w, slots)[:, g] for w in (0, 1))
+            codes = np.abs(ref.codes[1][slots // ref.page, g, slots % ref.page]).cumsum(0)
+            scale = ref.scales[1][slots // ref.page, g]
+            for i0 in range(0, n, 256):
+                i1 = min(i0 + 256, n)
+                qq = q[start[b] + i0:start[b] + i1, g * group:(g + 1) * group].astype(F64).reshape(-1, dim)
+                last = np.repeat(total - n + np.arange(i0, i1), group)
+                seen = t[None, :] <= last[:, None]
+                s = qq @ k.T / np.sqrt(dim)
+                a = np.abs(qq) @ np.abs(k).T / np.sqrt(dim)
+                top = np.where(seen, s, -np.inf).max(1, keepdims=True)
+                e = np.where(seen, np.exp(np.minimum(s - top, 0)), 0.0)
+                w = e / e.sum(1, keepdims=True)
+                o = w @ v
+                we = w * (2.0 ** -21 * a + 2.0 ** -22 * (np.abs(s) + np.abs(s - top)) + 2.0 ** -20)
+                d = we @ np.abs(v) + we.sum(1, keepdims=True) * np.abs(o) + 2.0 ** -21 * (w @ np.abs(v))
+                d += 2.0 ** -31 * (w * scale).max(1, keepdims=True) * codes[last]
+                at = (slice(start[b] + i0, start[b] + i1), slice(g * group, (g + 1) * group))
+                out[at], tol[at] = o.reshape(i1 - i0, group, dim), d.reshape(i1 - i0, group, dim)
+    return out, tol
+
+
+@pytest.mark.parametrize("page", [8, 64])
+def test_rows_of_no_request_are_left(page):
+    """A part of a step's starts with all of its rows: the rows before the first request and behind the last stay as they
+    are, whatever an earlier call has left in the workspace."""
+    r = np.random.default_rng(page)
+    heads, kvh, dim = 16, 2, 128
+    lens, fresh = [1500, 900, 700], [40, 1, 3]
+    table, pages = tables(r, lens, page)
+    ref = random_cache(r, pages, kvh, page, dim)
+    cache = gpu_cache(ref)
+    start = np.concatenate([[0], np.cumsum(fresh)]).astype(int)
+    q = r.standard_normal((start[-1] + 4, heads, dim)).astype(F32)
+    ws = torch.zeros(ops.attn_kv8_workspace_bytes(len(q), 3, heads, kvh, dim), dtype=torch.uint8, device="cuda")
+    out = torch.full(q.shape, 7.0, device="cuda")
+    args = dict(workspace=ws, out=out)
+    got = host(ops.attn_kv8_rows(dev(q), cache, dev(table), dev(start, I32), dev(lens, I32), **args))
+    want, tol = attention_wide(q, ref, table, start, lens)
+    assert np.all(np.abs(got - want) <= tol)
+    for first in (1, 2, 3):   # the requests from `first` on, in a call of as many (the last ones idle)
+        part = np.concatenate([start[first:], [start[-1]] * first])
+        some = np.concatenate([table[first:], table[:first]])
+        some_lens = lens[first:] + [0] * first
+        out.fill_(7.0)
+        got = host(ops.attn_kv8_rows(dev(q), cache, dev(some), dev(part, I32), dev(some_lens, I32), **args))
+        want, tol = attention_wide(q, ref, some, part, some_lens)
+        assert np.all(got[:part[0]] == 7.0) and np.all(got[part[-1]:] == 7.0)
+        assert np.all(np.abs(got - want) <= tol)
