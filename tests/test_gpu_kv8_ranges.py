@@ -86,6 +86,54 @@ def attention_wide(q, ref, table, start, lens):
     return out, tol
 
 
+def compare(r, lens, fresh, heads, kvh, dim, page):
+    table, pages = tables(r, lens, page)
+    ref = random_cache(r, pages, kvh, page, dim)
+    start = np.concatenate([[0], np.cumsum(fresh)]).astype(int)
+    q = r.standard_normal((start[-1], heads, dim)).astype(F32)
+    out = torch.full(q.shape, float("nan"), device="cuda")   # a row that nothing writes shows
+    got = host(ops.attn_kv8_rows(dev(q), gpu_cache(ref), dev(table), dev(start, I32), dev(lens, I32), out=out))
+    want, tol = attention_wide(q, ref, table, start, lens)
+    ok = np.abs(got - want) <= tol
+    assert np.all(ok), (np.argwhere(~ok)[0], int((~ok).any(axis=(1, 2)).sum()))
+
+
+def row_tiles(fresh, heads, kvh):
+    """Workgroups of the many-row kernel, before keys are cut."""
+    g = heads // kvh
+    return sum(-(-n * g // 128) for n in fresh if n * g > max(32, g)) * kvh
+
+
+def test_more_row_tiles_than_the_card_takes():
+    """Prompts whose keys are not cut (256 row tiles and more), a second, ragged one and single tokens beside them, whose
+    pieces are joined four pairs to a wave."""
+    r = np.random.default_rng(21)
+    fresh, lens = [1, 2111, 1, 77, 2, 1], [700, 2111, 33, 400, 1500, 1]
+    assert row_tiles(fresh, 16, 2) >= 256 and sum(fresh) * 16 > 16384
+    compare(r, lens, fresh, 16, 2, 64, 64)
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(16, 2, 64), (16, 2, 128), (24, 2, 256)])
+def test_cut_prompts_joined_four_pairs_a_wave(heads, kvh, dim):
+    """Few enough row tiles to be cut, and more than 16384 pairs with the single tokens beside them."""
+    r = np.random.default_rng(dim)
+    fresh = [1] * 120 + [500] + [1] * 110
+    lens = list(r.integers(1, 400, 120)) + [900] + list(r.integers(200, 700, 110))
+    if heads == 16:
+        fresh[120], lens[120] = 860, 1300
+    assert row_tiles(fresh, heads, kvh) <= 128 and sum(fresh) * heads > 16384
+    compare(r, [int(n) for n in lens], fresh, heads, kvh, dim, 16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_cut_prompts_joined_a_pair_a_wave(dim):
+    """2049 to 16384 pairs at the narrower heads; two prompts whose pieces differ in number."""
+    r = np.random.default_rng(dim + 1)
+    fresh, lens = [120, 1, 37, 9], [1200, 2500, 301, 40]
+    assert 2048 < sum(fresh) * 16 <= 16384
+    compare(r, lens, fresh, 16, 2, dim, 32)
+
+
 @pytest.mark.parametrize("page", [8, 64])
 def test_rows_of_no_request_are_left(page):
     """A part of a step's starts with all of its rows: the rows before the first request and behind the last stay as they
