@@ -366,6 +366,8 @@ int qwen_kv8_read_rows(const int8_t* k_codes, const int8_t* v_codes, const float
 /* Attention of the step's rows: q, out [rows x heads x dim], gate like out or NULL (16-byte aligned). Row i of
  * request b's n rows stands at position p = kv_len[b] - n + i and sees keys 0 .. p:
  *   out = sum_t softmax_t(q . k_t / sqrt(dim)) v_t  (* sigmoid(gate)), fp32 accuracy over the codes' exact values.
+ * That accuracy holds while the pages that a row sees have value scales below 2^60 and within 2^60 of each other; a page
+ * of zeros may lie beside any above 2^-49 (values up to about 2e-13).
  * Zeros where p < 0; a page id outside the cache, or a table row too short, makes the rows that see it NaN. row_start must
  * not decrease and may be a part of a step's: rows before row_start[0] and from row_start[requests] on are left as they
  * were. heads a multiple of kv_heads, rows * heads <= 2^24, max_pages * page_size <= 2^30; out must not overlap q.

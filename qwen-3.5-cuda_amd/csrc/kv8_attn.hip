@@ -14,7 +14,11 @@
 // Scales: score = S * (2^-e / sqrt(D) log2(e) * k_scale); the value scale rides on the weights, w = p * v_scale, so that
 // tokens of pages with different scales share one accumulator. The running reference m of the exponentials therefore
 // bounds score + log2(v_scale); it moves, and the sums are rescaled, only when a score passes it by 8 (weights up to
-// 2^8 are as exact as weights up to 1).
+// 2^8 are as exact as weights up to 1). A page of zeros has the smallest scale, 2^-100, and counts there as one of 2^-40:
+// counted as 2^-100 its keys' weights fell below the smallest fp32 number, and out of the softmax's sum, when a page with
+// values came into the same row (512 zeros with weights of 2^-10 beside values of 2^30: outputs off by a hundredth). What is
+// left of that: of two scales 2^d apart the smaller one's keys lose weights below 2^(d - 126), and beside zeros of the
+// same score a scale below 2^-49 loses a bit at each halving.
 //
 // Two kernels. split_kernel (few rows per request): bound by the cache's bytes. A workgroup takes 8 (row, head) pairs
 // that share a KV head - 16 columns: 8 rows x 2 fp16 parts - and a range of 32-token tiles, its 4 waves every fourth tile,
@@ -174,6 +178,10 @@ __device__ __forceinline__ float rounded(float v) {
     asm("" : "+v"(v));
     return v;
 }
+// The value scale that the exponentials' reference counts with (0 where nothing of the octet is seen).
+constexpr float kZerosScale = 0x1p-40f;
+__device__ __forceinline__ float reference_scale(float sv) { return sv > kKv8Floor ? sv : kZerosScale; }
+
 __device__ __forceinline__ float low_part(float v) { return v - static_cast<float>(static_cast<_Float16>(v)); }
 
 // Where the octet of tokens that starts at token t lies: the page's first code (of one head) and the two scales. Tokens
@@ -344,7 +352,7 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split_kernel(const AttnArgs a)
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
-        top += __builtin_amdgcn_logf(fmaxf(sv, kKv8Floor));   // log2
+        top += __builtin_amdgcn_logf(reference_scale(sv));   // log2
         if (__ballot(top > mu + kMoves)) {
             const float now = fmaxf(mu, max_over_lk(top));
             const float shrink = __builtin_amdgcn_exp2f(mu - now);
@@ -854,7 +862,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
                 }
             }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) top[s] += __builtin_amdgcn_logf(fmaxf(sv[s], kKv8Floor));
+            for (int s = 0; s < 2; ++s) top[s] += __builtin_amdgcn_logf(reference_scale(sv[s]));
             const float hi = fmaxf(top[0], top[1]);
             if (__ballot(hi > mu + kMoves)) {
                 const float now = fmaxf(mu, fmaxf(hi, __shfl_xor(hi, 32)));
@@ -907,7 +915,9 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
         }
         return;
     }
-    const float inv = 1.f / (kWeightUp * l);   // (of a sum of at least one: 2^-24 more beside the sums' roundings)
+    // (l is about 1 / value scale a key: from 2^-60 with the largest scales that the header allows to 2^108 a key at the
+    // smallest, where values below 2^-93 come out as 0 once 64 l overflows. 2^-24 more beside the sums' roundings.)
+    const float inv = 1.f / (kWeightUp * l);
     // A lane's registers 4 b .. 4 b + 3 of value tiles 2 m and 2 m + 1 are dims 64 m + 16 b + 8 g + 0..7 of its row. (One row's
     // gates after another's, each load waited for, were a third of the kernel's time.)
 #pragma unroll

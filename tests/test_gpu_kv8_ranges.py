@@ -161,3 +161,28 @@ def test_rows_of_no_request_are_left(page):
         want, tol = attention_wide(q, ref, some, part, some_lens)
         assert np.all(got[:part[0]] == 7.0) and np.all(got[part[-1]:] == 7.0)
         assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("up", [-20, 0, 10, 30])
+@pytest.mark.parametrize("n", [2, 40])
+def test_pages_of_zeros_keep_their_weight(n, up):
+    """Pages whose values are all zero, of a whole tile and more, before and behind ones with values up to 2^up: what they
+    take of the softmax stays, however small a value their scale (the smallest one) stands for."""
+    r = np.random.default_rng(100 + n + up)
+    page, heads, kvh, dim, zeros = 64, 8, 1, 64, 4
+    total = page * (2 * zeros + 1)
+    table, pages = tables(r, [total], page)
+    ref = random_cache(r, pages, kvh, page, dim)
+    for j in range(2 * zeros + 1):
+        p = table[0, j]
+        ref.scales[0][p] = F64(F32(7.0 / 800))
+        if j == zeros:   # the page with values: scores some 7 (a factor of 2^10) above the others'
+            ref.codes[0][p] = 100 + r.integers(-5, 6, ref.codes[0][p].shape)
+            ref.scales[1][p] = 2.0 ** (up - 7)
+        else:
+            ref.codes[0][p] = r.integers(-5, 6, ref.codes[0][p].shape)
+            ref.codes[1][p], ref.scales[1][p] = 0, kv8_ref.FLOOR
+    q = (1 + 0.1 * r.standard_normal((n, heads, dim))).astype(F32)
+    got = host(ops.attn_kv8_rows(dev(q), gpu_cache(ref), dev(table), dev([0, n], I32), dev([total], I32)))
+    want, tol = attention_wide(q, ref, table, [0, n], [total])
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
