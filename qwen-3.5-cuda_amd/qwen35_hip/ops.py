@@ -3,7 +3,9 @@
 Each function checks on the host that every tensor is a contiguous device
 tensor of the dtype and shape the kernel assumes (the C ABI can only check
 sizes, not buffer extents), then enqueues the kernel on `stream` (default: the
-current torch stream) and returns the output tensor(s). Nothing here computes on
+current torch stream) and returns the output tensor(s). Outputs and workspaces that
+a call allocates belong to the stream that it runs on; a caller with `stream` orders
+it behind the inputs, and what reads the outputs behind it. Nothing here computes on
 the CPU: the work is done by libqwen35_hip.so or not at all.
 
 torch is used for device memory and streams only.
@@ -28,6 +30,31 @@ def _stream(stream) -> int:
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
     return stream.cuda_stream
+
+
+# Memory that a call allocates. With `stream` it is that stream's: memory of the current stream could be handed to the
+# current stream's next tensor while the kernels on `stream` still use it (a workspace from the moment the call returns), or
+# still be written by work of the current stream that `stream` does not wait for. An output is also marked as used by the
+# current stream, so that a caller who reads it there may drop it there.
+def _empty(stream, shape, device, dtype=torch.float32) -> torch.Tensor:
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream())
+    return t
+
+
+def _like(stream, x) -> torch.Tensor:
+    return torch.empty_like(x) if stream is None else _empty(stream, x.shape, x.device, x.dtype)
+
+
+def _scratch(stream, nbytes: int, device) -> torch.Tensor:
+    nbytes = max(nbytes, 16)
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _p(t: torch.Tensor | None) -> int | None:
@@ -62,7 +89,7 @@ def rmsnorm_rows(x, weight, out=None, eps=1e-6, stream=None):
     _dev(x, weight, dtype=torch.float32)
     rows, n = _rows(x)
     _same((n,), weight)
-    out = torch.empty_like(x) if out is None else out
+    out = _like(stream, x) if out is None else out
     _dev(out, dtype=torch.float32)
     _same(x.shape, out)
     check(load().qwen_rmsnorm_rows(_p(x), _p(weight), _p(out), rows, n, eps, _stream(stream)))
@@ -74,7 +101,7 @@ def rmsnorm_gated_rows(x, gate, weight, out=None, eps=1e-6, stream=None):
     rows, n = _rows(x)
     _same(x.shape, gate)
     _same((n,), weight)
-    out = torch.empty_like(x) if out is None else out
+    out = _like(stream, x) if out is None else out
     _dev(out, dtype=torch.float32)
     _same(x.shape, out)
     check(load().qwen_rmsnorm_gated_rows(_p(x), _p(gate), _p(weight), _p(out), rows, n, eps, _stream(stream)))
@@ -84,7 +111,7 @@ def rmsnorm_gated_rows(x, gate, weight, out=None, eps=1e-6, stream=None):
 def residual_add(x1, x2, out=None, stream=None):
     _dev(x1, x2, dtype=torch.float32)
     _same(x1.shape, x2)
-    out = torch.empty_like(x1) if out is None else out
+    out = _like(stream, x1) if out is None else out
     _dev(out, dtype=torch.float32)
     _same(x1.shape, out)
     check(load().qwen_residual_add(_p(x1), _p(x2), _p(out), x1.numel(), _stream(stream)))
@@ -101,8 +128,8 @@ def residual_rmsnorm_rows(x, branch, weight, resid=None, normed=None, eps=1e-6, 
     rows, n = _rows(x)
     _same(x.shape, branch)
     _same((n,), weight)
-    resid = torch.empty_like(x) if resid is None else resid
-    normed = torch.empty_like(x) if normed is None else normed
+    resid = _like(stream, x) if resid is None else resid
+    normed = _like(stream, x) if normed is None else normed
     _dev(resid, normed, dtype=dt)
     _same(x.shape, resid, normed)
     fn = load().qwen_residual_rmsnorm_rows_f32 if dt == torch.float32 else load().qwen_residual_rmsnorm_rows_bf16
@@ -115,7 +142,7 @@ def encoder_forward(token_id: int, table, out=None, stream=None):
     vocab, d = table.shape
     if not 0 <= token_id < vocab:
         raise ValueError(f"token {token_id} outside the table of {vocab} rows")
-    out = torch.empty(d, dtype=torch.float32, device=table.device) if out is None else out
+    out = _empty(stream, d, table.device) if out is None else out
     _dev(out, dtype=torch.float32)
     _same((d,), out)
     check(load().qwen_encoder_forward(token_id, _p(table), _p(out), d, _stream(stream)))
@@ -166,8 +193,8 @@ def gdn_frontend_rows(x, weight, hist_in, hist_out=None, y=None, k_heads=16, key
         raise ValueError("weight must be [channels, kernel]")
     kernel = weight.shape[1]
     _same((c, kernel - 1), hist_in)
-    hist_out = torch.empty_like(hist_in) if hist_out is None else hist_out
-    y = torch.empty_like(x) if y is None else y
+    hist_out = _like(stream, hist_in) if hist_out is None else hist_out
+    y = _like(stream, x) if y is None else y
     _dev(hist_out, y, dtype=torch.float32)
     _same(hist_in.shape, hist_out)
     _same(x.shape, y)
@@ -187,10 +214,10 @@ def gdn_frontend_gates_rows(x, weight, hist_in, beta_raw, alpha_raw, a, dt_bias,
     _same((c, kernel - 1), hist_in)
     _same((heads,), dt_bias)
     _same((rows, heads), beta_raw, alpha_raw)
-    hist_out = torch.empty_like(hist_in) if hist_out is None else hist_out
-    y = torch.empty_like(x) if y is None else y
-    beta = torch.empty_like(beta_raw) if beta is None else beta
-    decay = torch.empty_like(beta_raw) if decay is None else decay
+    hist_out = _like(stream, hist_in) if hist_out is None else hist_out
+    y = _like(stream, x) if y is None else y
+    beta = _like(stream, beta_raw) if beta is None else beta
+    decay = _like(stream, beta_raw) if decay is None else decay
     _dev(hist_out, y, beta, decay, dtype=torch.float32)
     _same(hist_in.shape, hist_out)
     _same(x.shape, y)
@@ -208,7 +235,7 @@ def gdn_conv_step(x, weight, history, y=None, stream=None):
     kernel = weight.shape[1]
     _same((c, kernel), weight)
     _same((c, kernel - 1), history)
-    y = torch.empty_like(x) if y is None else y
+    y = _like(stream, x) if y is None else y
     _dev(y, dtype=torch.float32)
     _same(x.shape, y)
     check(load().qwen_gdn_conv_step(_p(x), _p(weight), _p(history), _p(y), c, kernel, _stream(stream)))
@@ -230,7 +257,7 @@ def gdn_norm_gate_rows(x, z, weight, out=None, eps=1e-6, stream=None):
     heads_total, dim = _rows(x)
     _same(x.shape, z)
     _same((dim,), weight)
-    out = torch.empty_like(x) if out is None else out
+    out = _like(stream, x) if out is None else out
     _dev(out, dtype=torch.float32)
     _same(x.shape, out)
     check(load().qwen_gdn_norm_gate_rows(_p(x), _p(z), _p(weight), _p(out), heads_total, 1, dim, eps,
@@ -248,11 +275,11 @@ def gdn_norm_gate_matmul(x, z, norm_weight, weight, ggml_type, num_elements: int
     heads, dim = _rows(x)
     _same(x.shape, z)
     _same((dim,), norm_weight)
-    normed = torch.empty_like(x) if normed is None else normed
+    normed = _like(stream, x) if normed is None else normed
     _dev(normed, dtype=torch.float32)
     _same(x.shape, normed)
     t = GGML_TYPES[ggml_type] if isinstance(ggml_type, str) else int(ggml_type)
-    out = torch.empty(M, dtype=torch.float32, device=x.device) if out is None else out
+    out = _empty(stream, M, x.device) if out is None else out
     _dev(out, dtype=torch.float32)
     if out.numel() < M:
         raise ValueError(f"out has {out.numel()} elements, M = {M}")
@@ -270,8 +297,8 @@ def gdn_gate_values_rows(beta_raw, alpha_raw, a, dt_bias, beta=None, decay=None,
     if beta_raw.numel() % max(heads, 1):
         raise ValueError("beta_raw must hold whole rows of `heads` values")
     rows = beta_raw.numel() // max(heads, 1)
-    beta = torch.empty_like(beta_raw) if beta is None else beta
-    decay = torch.empty_like(beta_raw) if decay is None else decay
+    beta = _like(stream, beta_raw) if beta is None else beta
+    decay = _like(stream, beta_raw) if decay is None else decay
     _dev(beta, decay, dtype=torch.float32)
     _same(beta_raw.shape, beta, decay)
     check(load().qwen_gdn_gate_values_rows(_p(beta_raw), _p(alpha_raw), _p(a), _p(dt_bias), _p(beta), _p(decay), rows,
@@ -290,7 +317,7 @@ def gdn_recurrent_step(state, q, k, v, beta, decay, key_heads, value_heads, key_
                  (beta, value_heads), (decay, value_heads)):
         if t.numel() < n:
             raise ValueError(f"input of {t.numel()} elements, need {n}")
-    out = torch.empty(value_heads * value_dim, dtype=torch.float32, device=state.device) if out is None else out
+    out = _empty(stream, value_heads * value_dim, state.device) if out is None else out
     _dev(out, dtype=torch.float32)
     check(load().qwen_gdn_recurrent_step(_p(state), _p(q), _p(k), _p(v), _p(beta), _p(decay), _p(out), key_heads,
                                          value_heads, key_dim, value_dim, _stream(stream)))
@@ -309,7 +336,7 @@ def gdn_recurrent_rows(state, qkv, beta, decay, key_heads, value_heads, key_dim,
     if state.numel() != value_heads * key_dim * value_dim:
         raise ValueError("state shape does not match the head sizes")
     _same((rows, value_heads), beta, decay)
-    out = torch.empty((rows, value_heads * value_dim), dtype=torch.float32, device=qkv.device) if out is None else out
+    out = _empty(stream, (rows, value_heads * value_dim), qkv.device) if out is None else out
     _dev(out, dtype=torch.float32)
     _same((rows, value_heads * value_dim), out)
     base = qkv.data_ptr()
@@ -333,7 +360,7 @@ def gdn_gated_recurrent_rows(state, qkv, beta_raw, alpha_raw, a, dt_bias, key_he
         raise ValueError("state shape does not match the head sizes")
     _same((rows, value_heads), beta_raw, alpha_raw)
     _same((value_heads,), a, dt_bias)
-    out = torch.empty((rows, value_heads * value_dim), dtype=torch.float32, device=qkv.device) if out is None else out
+    out = _empty(stream, (rows, value_heads * value_dim), qkv.device) if out is None else out
     _dev(out, dtype=torch.float32)
     _same((rows, value_heads * value_dim), out)
     base = qkv.data_ptr()
@@ -356,8 +383,8 @@ def gdn_decode_step(x, conv_w, hist_in, hist_out, state, beta_raw, alpha_raw, a,
     if state.numel() != value_heads * key_dim * value_dim:
         raise ValueError("state must be [value_heads, key_dim, value_dim]")
     _same((value_heads,), beta_raw, alpha_raw, a, dt_bias)
-    y = torch.empty(C, dtype=torch.float32, device=x.device) if y is None else y
-    out = torch.empty(value_heads * value_dim, dtype=torch.float32, device=x.device) if out is None else out
+    y = _empty(stream, C, x.device) if y is None else y
+    out = _empty(stream, value_heads * value_dim, x.device) if out is None else out
     _dev(y, out, dtype=torch.float32)
     if y.numel() != C or out.numel() != value_heads * value_dim:
         raise ValueError("y or out of the wrong size")
@@ -379,12 +406,12 @@ def gdn_recurrent_chunked(state, qkv, beta, decay, key_heads, value_heads, key_d
     if state.numel() != value_heads * key_dim * value_dim:
         raise ValueError("state shape does not match the head sizes")
     _same((rows, value_heads), beta, decay)
-    out = torch.empty((rows, value_heads * value_dim), dtype=torch.float32, device=qkv.device) if out is None else out
+    out = _empty(stream, (rows, value_heads * value_dim), qkv.device) if out is None else out
     _dev(out, dtype=torch.float32)
     _same((rows, value_heads * value_dim), out)
     need = load().qwen_gdn_recurrent_chunked_workspace_bytes(rows, value_heads)
     if workspace is None:
-        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=qkv.device)
+        workspace = _scratch(stream, need, qkv.device)
     _dev(workspace, dtype=torch.uint8)
     base = qkv.data_ptr()
     check(load().qwen_gdn_recurrent_chunked(_p(state), ctypes.c_void_p(base), ctypes.c_void_p(base + 4 * kd),
@@ -400,8 +427,8 @@ def attn_split_qg(qg, heads, dim, q=None, g=None, stream=None):
     _dev(qg, dtype=torch.float32)
     if qg.numel() != 2 * heads * dim:
         raise ValueError("qg must hold heads x 2 x dim values")
-    q = torch.empty(heads * dim, dtype=torch.float32, device=qg.device) if q is None else q
-    g = torch.empty_like(q) if g is None else g
+    q = _empty(stream, heads * dim, qg.device) if q is None else q
+    g = _like(stream, q) if g is None else g
     _dev(q, g, dtype=torch.float32)
     if q.numel() < heads * dim or g.numel() < heads * dim:
         raise ValueError("q / g outputs smaller than heads x dim")
@@ -417,7 +444,7 @@ def _attn_check(q, cache, heads, kv_heads, dim, pos):
 def attn_scores(q, k_cache, heads, kv_heads, dim, pos, out=None, stream=None):
     _dev(q, k_cache, dtype=torch.float32)
     _attn_check(q, k_cache, heads, kv_heads, dim, pos)
-    out = torch.empty(heads * (pos + 1), dtype=torch.float32, device=q.device) if out is None else out
+    out = _empty(stream, heads * (pos + 1), q.device) if out is None else out
     _dev(out, dtype=torch.float32)
     if out.numel() < heads * (pos + 1):
         raise ValueError("scores output too small for the shape")
@@ -437,7 +464,7 @@ def attn_values(scores, v_cache, heads, kv_heads, dim, pos, out=None, stream=Non
     _dev(scores, v_cache, dtype=torch.float32)
     if scores.numel() < heads * (pos + 1) or v_cache.numel() < (pos + 1) * kv_heads * dim:
         raise ValueError("scores or cache too small for the shape")
-    out = torch.empty(heads * dim, dtype=torch.float32, device=scores.device) if out is None else out
+    out = _empty(stream, heads * dim, scores.device) if out is None else out
     _dev(out, dtype=torch.float32)
     if out.numel() < heads * dim:
         raise ValueError("values output too small for the shape")
@@ -448,7 +475,7 @@ def attn_values(scores, v_cache, heads, kv_heads, dim, pos, out=None, stream=Non
 def attn_sigmoid_gate(x, gate, out=None, stream=None):
     _dev(x, gate, dtype=torch.float32)
     _same(x.shape, gate)
-    out = torch.empty_like(x) if out is None else out
+    out = _like(stream, x) if out is None else out
     check(load().qwen_attn_sigmoid_gate(_p(x), _p(gate), _p(out), x.numel(), _stream(stream)))
     return out
 
@@ -475,9 +502,9 @@ def attn_decode(q, k_cache, v_cache, heads, kv_heads, dim, pos, gate=None, works
         _dev(gate, dtype=torch.float32)
     nbytes = attn_decode_workspace_bytes(heads, kv_heads, dim, pos)
     if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        workspace = _scratch(stream, nbytes, q.device)
     _dev(workspace)
-    out = torch.empty(heads * dim, dtype=torch.float32, device=q.device) if out is None else out
+    out = _empty(stream, heads * dim, q.device) if out is None else out
     _dev(out, dtype=torch.float32)
     check(load().qwen_attn_decode(_p(q), _p(k_cache), _p(v_cache), _p(gate), _p(out), heads, kv_heads, dim, pos,
                                   _p(workspace), workspace.numel() * workspace.element_size(), _stream(stream)))
@@ -498,13 +525,13 @@ def attn_decode_norm_rope(q, k_cache, v_cache, heads, kv_heads, dim, pos, q_weig
         _dev(gate, dtype=torch.float32)
     nbytes = attn_decode_workspace_bytes(heads, kv_heads, dim, pos)
     if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        workspace = _scratch(stream, nbytes, q.device)
     _dev(workspace)
-    q_normed = torch.empty(heads * dim, dtype=torch.float32, device=q.device) if q_normed is None else q_normed
+    q_normed = _empty(stream, heads * dim, q.device) if q_normed is None else q_normed
     _dev(q_normed, dtype=torch.float32)
     if q_normed.numel() < heads * dim:
         raise ValueError(f"q_normed has {q_normed.numel()} elements, need {heads * dim}")
-    out = torch.empty(heads * dim, dtype=torch.float32, device=q.device) if out is None else out
+    out = _empty(stream, heads * dim, q.device) if out is None else out
     _dev(out, dtype=torch.float32)
     check(load().qwen_attn_decode_norm_rope(_p(q), _p(q_normed), _p(k_cache), _p(v_cache), _p(gate), _p(out), heads,
                                             kv_heads, dim, pos, _p(q_weight), _p(k_weight), rope_dim, theta, eps,
@@ -521,7 +548,7 @@ def attn_decode_noalloc(q, k_cache, v_cache, heads, kv_heads, dim, pos, gate=Non
     _attn_check(q, v_cache, heads, kv_heads, dim, pos)
     if gate is not None:
         _dev(gate, dtype=torch.float32)
-    out = torch.empty(heads * dim, dtype=torch.float32, device=q.device) if out is None else out
+    out = _empty(stream, heads * dim, q.device) if out is None else out
     _dev(out, dtype=torch.float32)
     check(load().qwen_attn_decode_noalloc(_p(q), _p(k_cache), _p(v_cache), _p(gate), _p(out), heads, kv_heads, dim,
                                           pos, _stream(stream)))
@@ -583,15 +610,15 @@ def kv8_plan(cached, fresh, block_table, free_pages, free_head, page_size, rows,
         raise ValueError("block_table must be [requests, max_pages]")
     if row_start is None and kv_len is None and slots is None and pos is None and free_head_out is None:
         # five outputs in one allocation
-        row_start, kv_len, slots, pos, free_head_out = torch.empty(
-            2 * n + 2 * rows + 2, dtype=torch.int32, device=cached.device).split((n + 1, n, rows, rows, 1))
+        row_start, kv_len, slots, pos, free_head_out = _empty(
+            stream, 2 * n + 2 * rows + 2, cached.device, torch.int32).split((n + 1, n, rows, rows, 1))
     else:
-        i32 = dict(dtype=torch.int32, device=cached.device)
-        free_head_out = torch.empty(1, **i32) if free_head_out is None else free_head_out
-        row_start = torch.empty(n + 1, **i32) if row_start is None else row_start
-        kv_len = torch.empty(n, **i32) if kv_len is None else kv_len
-        slots = torch.empty(rows, **i32) if slots is None else slots
-        pos = torch.empty(rows, **i32) if pos is None else pos
+        i32 = (cached.device, torch.int32)
+        free_head_out = _empty(stream, 1, *i32) if free_head_out is None else free_head_out
+        row_start = _empty(stream, n + 1, *i32) if row_start is None else row_start
+        kv_len = _empty(stream, n, *i32) if kv_len is None else kv_len
+        slots = _empty(stream, rows, *i32) if slots is None else slots
+        pos = _empty(stream, rows, *i32) if pos is None else pos
         _dev(free_head_out, row_start, kv_len, slots, pos, dtype=torch.int32)
         _same((1,), free_head_out)
         _same((n + 1,), row_start)
@@ -635,10 +662,10 @@ def kv8_read_rows(cache: Kv8Cache, slots, k=None, v=None, stream=None):
     n = slots.numel()
     shape = (n, cache.heads, cache.dim)
     if k is None and v is None:
-        k, v = torch.empty((2, *shape), dtype=torch.float32, device=slots.device).unbind()
+        k, v = _empty(stream, (2, *shape), slots.device).unbind()
     else:
-        k = torch.empty(shape, dtype=torch.float32, device=slots.device) if k is None else k
-        v = torch.empty(shape, dtype=torch.float32, device=slots.device) if v is None else v
+        k = _empty(stream, shape, slots.device) if k is None else k
+        v = _empty(stream, shape, slots.device) if v is None else v
         _dev(k, v, dtype=torch.float32)
         _same(shape, k, v)
     check(load().qwen_kv8_read_rows(*cache.args, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _stream(stream)))
@@ -665,14 +692,13 @@ def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None,
         if gate.shape != q.shape:
             _same(q.shape, gate)
     if out is None:
-        out = torch.empty_like(q)
+        out = _like(stream, q)
     else:
         _checked(torch.float32, out)
         if out.shape != q.shape:
             _same(q.shape, out)
     if workspace is None:
-        workspace = torch.empty(max(16, attn_kv8_workspace_bytes(rows, n, heads, cache.heads, cache.dim)), dtype=torch.uint8,
-                                device=q.device)
+        workspace = _scratch(stream, attn_kv8_workspace_bytes(rows, n, heads, cache.heads, cache.dim), q.device)
     _dev(workspace)
     check(load().qwen_attn_kv8_rows(_p(q), *cache.args[:6], _p(block_table), block_table.shape[1], _p(row_start),
                                     _p(kv_len), n, _p(gate), _p(out), rows, heads, cache.heads, cache.dim, _p(workspace),
@@ -686,8 +712,8 @@ def moe_topk_rows(logits, k, idx=None, weights=None, stream=None):
     _dev(logits, dtype=torch.float32)
     n = logits.shape[-1]
     rows = logits.numel() // n
-    idx = torch.empty((rows, k), dtype=torch.int32, device=logits.device) if idx is None else idx
-    weights = torch.empty((rows, k), dtype=torch.float32, device=logits.device) if weights is None else weights
+    idx = _empty(stream, (rows, k), logits.device, torch.int32) if idx is None else idx
+    weights = _empty(stream, (rows, k), logits.device) if weights is None else weights
     _dev(idx, dtype=torch.int32)
     _dev(weights, dtype=torch.float32)
     _same((rows, k), idx, weights)
@@ -722,7 +748,7 @@ def moe_expert_matmul(weight, ggml_type, num_elements, expert_stride, n_experts,
     n_sel = idx.numel()
     if n_sel and x.numel() < (n_sel - 1) * x_stride + K:
         raise ValueError("x too small for n_sel inputs")
-    out = torch.empty((n_sel, M), dtype=torch.float32, device=x.device) if out is None else out
+    out = _empty(stream, (n_sel, M), x.device) if out is None else out
     _dev(out, dtype=torch.float32)
     check(load().qwen_moe_expert_matmul(_p(weight), t, num_elements, expert_stride, n_experts, _p(idx), n_sel, _p(x),
                                         x_stride, _p(out), M, K, _stream(stream)))
@@ -739,8 +765,8 @@ def moe_expert_gate_up(w_gate, w_up, ggml_type, num_elements, expert_stride, n_e
     n_sel = idx.numel()
     if x.numel() < K:
         raise ValueError(f"x has {x.numel()} elements, K = {K}")
-    gate_out = torch.empty((n_sel, M), dtype=torch.float32, device=x.device) if gate_out is None else gate_out
-    up_out = torch.empty((n_sel, M), dtype=torch.float32, device=x.device) if up_out is None else up_out
+    gate_out = _empty(stream, (n_sel, M), x.device) if gate_out is None else gate_out
+    up_out = _empty(stream, (n_sel, M), x.device) if up_out is None else up_out
     _dev(gate_out, up_out, dtype=torch.float32)
     if gate_out.numel() < n_sel * M or up_out.numel() < n_sel * M:
         raise ValueError("outputs smaller than n_sel x M")
@@ -771,19 +797,19 @@ def moe_expert_swiglu(w_gate, w_up, ggml_type, num_elements, expert_stride, n_ex
         ts = GGML_TYPES[shared_type] if isinstance(shared_type, str) else int(shared_type)
     else:
         ts, shared_dim = 0, 0
-    hidden = torch.empty((n_sel, inter), dtype=torch.float32, device=x.device) if hidden is None else hidden
+    hidden = _empty(stream, (n_sel, inter), x.device) if hidden is None else hidden
     _dev(hidden, dtype=torch.float32)
     if hidden.numel() < n_sel * inter:
         raise ValueError("hidden smaller than n_sel x inter")
     if has_shared:
-        shared_hidden = (torch.empty(shared_dim, dtype=torch.float32, device=x.device) if shared_hidden is None
+        shared_hidden = (_empty(stream, shared_dim, x.device) if shared_hidden is None
                          else shared_hidden)
         _dev(shared_hidden, dtype=torch.float32)
         if shared_hidden.numel() < shared_dim:
             raise ValueError("shared_hidden smaller than shared_dim")
     nbytes = moe_expert_swiglu_workspace_bytes(n_sel, inter, shared_dim)
     if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
+        workspace = _scratch(stream, nbytes, x.device)
     _dev(workspace)
     check(load().qwen_moe_expert_swiglu(_p(w_gate), _p(w_up), t, num_elements, expert_stride, n_experts, _p(idx),
                                         n_sel, inter, _p(w_shared_gate) if has_shared else None,
@@ -806,8 +832,8 @@ def moe_route_swiglu(logits, k, w_gate, w_up, ggml_type, num_elements, expert_st
     t = GGML_TYPES[ggml_type] if isinstance(ggml_type, str) else int(ggml_type)
     if x.numel() < K:
         raise ValueError(f"x has {x.numel()} elements, K = {K}")
-    idx = torch.empty(k, dtype=torch.int32, device=x.device) if idx is None else idx
-    weights = torch.empty(k, dtype=torch.float32, device=x.device) if weights is None else weights
+    idx = _empty(stream, k, x.device, torch.int32) if idx is None else idx
+    weights = _empty(stream, k, x.device) if weights is None else weights
     _dev(idx, dtype=torch.int32)
     _dev(weights, dtype=torch.float32)
     _same((k,), idx, weights)
@@ -817,19 +843,19 @@ def moe_route_swiglu(logits, k, w_gate, w_up, ggml_type, num_elements, expert_st
         ts = GGML_TYPES[shared_type] if isinstance(shared_type, str) else int(shared_type)
     else:
         ts, shared_dim = 0, 0
-    hidden = torch.empty((k, inter), dtype=torch.float32, device=x.device) if hidden is None else hidden
+    hidden = _empty(stream, (k, inter), x.device) if hidden is None else hidden
     _dev(hidden, dtype=torch.float32)
     if hidden.numel() < k * inter:
         raise ValueError("hidden smaller than k x inter")
     if has_shared:
-        shared_hidden = (torch.empty(shared_dim, dtype=torch.float32, device=x.device) if shared_hidden is None
+        shared_hidden = (_empty(stream, shared_dim, x.device) if shared_hidden is None
                          else shared_hidden)
         _dev(shared_hidden, dtype=torch.float32)
         if shared_hidden.numel() < shared_dim:
             raise ValueError("shared_hidden smaller than shared_dim")
     nbytes = moe_expert_swiglu_workspace_bytes(k, inter, shared_dim)
     if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
+        workspace = _scratch(stream, nbytes, x.device)
     _dev(workspace)
     check(load().qwen_moe_route_swiglu(_p(logits), _p(idx), _p(weights), k, _p(w_gate), _p(w_up), t, num_elements,
                                        expert_stride, n_experts, inter, _p(w_shared_gate) if has_shared else None,
@@ -862,9 +888,9 @@ def moe_down_combine(w_down, down_type, down_elements, expert_stride, n_experts,
     ts = GGML_TYPES[shared_type] if isinstance(shared_type, str) else int(shared_type)
     nbytes = moe_down_combine_workspace_bytes(n_sel, d_model)
     if workspace is None:
-        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=hidden.device)
+        workspace = _scratch(stream, nbytes, hidden.device)
     _dev(workspace)
-    out = torch.empty(d_model, dtype=torch.float32, device=hidden.device) if out is None else out
+    out = _empty(stream, d_model, hidden.device) if out is None else out
     _dev(out, dtype=torch.float32)
     if out.numel() < d_model:
         raise ValueError("out smaller than d_model")
@@ -885,10 +911,10 @@ def moe_group_rows(idx, n_experts: int, order=None, starts=None, stream=None):
     _checked(torch.int32, idx)
     n = idx.numel()
     if order is None and starts is None:
-        order, starts = torch.empty(n + n_experts + 1, dtype=torch.int32, device=idx.device).split((n, n_experts + 1))
+        order, starts = _empty(stream, n + n_experts + 1, idx.device, torch.int32).split((n, n_experts + 1))
     else:
-        order = torch.empty(n, dtype=torch.int32, device=idx.device) if order is None else order
-        starts = torch.empty(n_experts + 1, dtype=torch.int32, device=idx.device) if starts is None else starts
+        order = _empty(stream, n, idx.device, torch.int32) if order is None else order
+        starts = _empty(stream, n_experts + 1, idx.device, torch.int32) if starts is None else starts
         _dev(order, starts, dtype=torch.int32)
         _same((n,), order)
         _same((n_experts + 1,), starts)
@@ -918,12 +944,11 @@ def moe_experts_rows(w_gate, w_up, ggml_type, w_down, down_type, n_experts, orde
     for w, ty in ((w_gate, t), (w_up, t), (w_down, td)):
         if w.numel() < blocks * GGML_BLOCK_BYTES.get(ty, 0):
             raise ValueError(f"{n_experts} experts of {inter} x {width} exceed a tensor of {w.numel()} bytes")
-    out = torch.empty_like(x) if out is None else out
+    out = _like(stream, x) if out is None else out
     _dev(out, dtype=torch.float32)
     _same(x.shape, out)
     if workspace is None:
-        workspace = torch.empty(max(16, moe_experts_rows_workspace_bytes(rows, top, n_experts, width, inter)),
-                                dtype=torch.uint8, device=x.device)
+        workspace = _scratch(stream, moe_experts_rows_workspace_bytes(rows, top, n_experts, width, inter), x.device)
     _dev(workspace)
     check(load().qwen_moe_experts_rows(_p(w_gate), _p(w_up), t, _p(w_down), td, n_experts, _p(order), _p(starts),
                                        _p(weights), top, _p(x), rows, width, inter, _p(out), _p(workspace),
@@ -935,7 +960,7 @@ def moe_experts_rows(w_gate, w_up, ggml_type, w_down, down_type, n_experts, orde
 def moe_silu_mul(g, u, out=None, stream=None):
     _dev(g, u, dtype=torch.float32)
     _same(g.shape, u)
-    out = torch.empty_like(g) if out is None else out
+    out = _like(stream, g) if out is None else out
     _dev(out, dtype=torch.float32)
     _same(g.shape, out)
     check(load().qwen_moe_silu_mul(_p(g), _p(u), _p(out), g.numel(), _stream(stream)))
@@ -955,7 +980,7 @@ def moe_shared_add_rows(accum, shared_out, gate, stream=None):
 def swiglu_bf16(g, u, out=None, stream=None):
     _dev(g, u, dtype=BF16)
     _same(g.shape, u)
-    out = torch.empty_like(g) if out is None else out
+    out = _like(stream, g) if out is None else out
     _dev(out, dtype=BF16)
     _same(g.shape, out)
     check(load().qwen_swiglu_bf16(_p(g), _p(u), _p(out), g.numel(), _stream(stream)))
@@ -968,7 +993,7 @@ def shared_swiglu_sigmoid_rows_bf16(g, u, logits, out=None, stream=None):
     rows, dim = _rows(g)
     _same(g.shape, u)
     _same((rows,), logits)
-    out = torch.empty_like(g) if out is None else out
+    out = _like(stream, g) if out is None else out
     _dev(out, dtype=BF16)
     _same(g.shape, out)
     check(load().qwen_shared_swiglu_sigmoid_rows_bf16(_p(g), _p(u), _p(logits), _p(out), rows, dim, _stream(stream)))
@@ -985,8 +1010,8 @@ def swiglu_routed_shared_bf16(g, u, sg, su, logits, out=None, shared_out=None, s
     rows, dim = _rows(sg)
     _same(sg.shape, su)
     _same((rows,), logits)
-    out = torch.empty_like(g) if out is None else out
-    shared_out = torch.empty_like(sg) if shared_out is None else shared_out
+    out = _like(stream, g) if out is None else out
+    shared_out = _like(stream, sg) if shared_out is None else shared_out
     _dev(out, shared_out, dtype=BF16)
     _same(g.shape, out)
     _same(sg.shape, shared_out)
@@ -1002,7 +1027,7 @@ def dequant_gather_rows(table, ggml_type, num_elements: int, ids, cols: int, out
     _dev(ids, dtype=torch.int32)
     t = GGML_TYPES[ggml_type] if isinstance(ggml_type, str) else int(ggml_type)
     n = ids.numel()
-    out = torch.empty((n, cols), dtype=torch.float32, device=table.device) if out is None else out
+    out = _empty(stream, (n, cols), table.device) if out is None else out
     _dev(out, dtype=torch.float32)
     _same((n, cols), out)
     check(load().qwen_dequant_gather_rows(_p(table), t, num_elements, _p(ids), n, cols, _p(out), _stream(stream)))
@@ -1012,7 +1037,7 @@ def dequant_gather_rows(table, ggml_type, num_elements: int, ids, cols: int, out
 def dequantize_row(table, ggml_type, num_elements: int, row: int, cols: int, out=None, stream=None):
     _dev(table, dtype=torch.uint8)
     t = GGML_TYPES[ggml_type] if isinstance(ggml_type, str) else int(ggml_type)
-    out = torch.empty(cols, dtype=torch.float32, device=table.device) if out is None else out
+    out = _empty(stream, cols, table.device) if out is None else out
     _dev(out, dtype=torch.float32)
     _same((cols,), out)
     check(load().qwen_dequantize_row(_p(table), t, num_elements, _p(out), row, cols, _stream(stream)))
@@ -1041,7 +1066,7 @@ def matmul_dispatch_multi(jobs, x, K: int, stream=None):
         w, t, ne, M, off, out = job[:6]
         split = job[6] if len(job) > 6 else 0
         _dev(w, dtype=torch.uint8)
-        out = torch.empty(M, dtype=torch.float32, device=x.device) if out is None else out
+        out = _empty(stream, M, x.device) if out is None else out
         _dev(out, dtype=torch.float32)
         if out.numel() < M:
             raise ValueError(f"job {j}: out has {out.numel()} elements, M = {M}")
@@ -1068,12 +1093,12 @@ def matmul_rows(weight, ggml_type, num_elements: int, x, M: int, K: int, element
         raise ValueError(f"x must be [rows, {K}], got {tuple(x.shape)}")
     rows = x.shape[0]
     t = GGML_TYPES[ggml_type] if isinstance(ggml_type, str) else int(ggml_type)
-    out = torch.empty(rows, M, dtype=torch.float32, device=x.device) if out is None else out
+    out = _empty(stream, (rows, M), x.device) if out is None else out
     _dev(out, dtype=torch.float32)
     if out.numel() < rows * M:
         raise ValueError(f"out has {out.numel()} elements, rows * M = {rows * M}")
     if workspace is None:
-        workspace = torch.empty(max(1, matmul_rows_workspace_bytes(rows, K)), dtype=torch.uint8, device=x.device)
+        workspace = _scratch(stream, matmul_rows_workspace_bytes(rows, K), x.device)
     _dev(workspace, dtype=torch.uint8)
     check(load().qwen_matmul_rows(_p(weight), t, num_elements, _p(x), _p(out), rows, M, K, element_offset,
                                   _p(workspace), workspace.numel(), _stream(stream)))
@@ -1092,14 +1117,14 @@ def matmul_rows_multi(jobs, x, K: int, workspace=None, stream=None):
     outs = []
     for j, (w, t, ne, M, off, out) in enumerate(jobs):
         _dev(w, dtype=torch.uint8)
-        out = torch.empty(rows, M, dtype=torch.float32, device=x.device) if out is None else out
+        out = _empty(stream, (rows, M), x.device) if out is None else out
         _dev(out, dtype=torch.float32)
         if out.numel() < rows * M:
             raise ValueError(f"job {j}: out has {out.numel()} elements, rows * M = {rows * M}")
         descs[j] = GemvDesc(w.data_ptr(), GGML_TYPES[t] if isinstance(t, str) else int(t), M, ne, off, out.data_ptr(), 0)
         outs.append(out)
     if workspace is None:
-        workspace = torch.empty(max(1, matmul_rows_workspace_bytes(rows, K)), dtype=torch.uint8, device=x.device)
+        workspace = _scratch(stream, matmul_rows_workspace_bytes(rows, K), x.device)
     _dev(workspace, dtype=torch.uint8)
     check(load().qwen_matmul_rows_multi(ctypes.cast(descs, ctypes.c_void_p), len(jobs), _p(x), rows, K,
                                         _p(workspace), workspace.numel(), _stream(stream)))
@@ -1115,7 +1140,7 @@ def matmul_dispatch(weight, ggml_type, num_elements: int, x, M: int, K: int, ele
     if x.numel() < K:
         raise ValueError(f"x has {x.numel()} elements, K = {K}")
     t = GGML_TYPES[ggml_type] if isinstance(ggml_type, str) else int(ggml_type)
-    out = torch.empty(M, dtype=torch.float32, device=x.device) if out is None else out
+    out = _empty(stream, M, x.device) if out is None else out
     _dev(out, dtype=torch.float32)
     if out.numel() < M:
         raise ValueError(f"out has {out.numel()} elements, M = {M}")
