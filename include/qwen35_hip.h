@@ -372,7 +372,7 @@ int qwen_kv8_read_rows(const int8_t* k_codes, const int8_t* v_codes, const float
  * not decrease and may be a part of a step's: rows before row_start[0] and from row_start[requests] on are left as they
  * were. heads a multiple of kv_heads, rows * heads <= 2^24, max_pages * page_size <= 2^30; out must not overlap q.
  * workspace: device memory, 16-byte aligned, of at least qwen_attn_kv8_workspace_bytes() bytes, for one call at a time;
- * nothing in it is kept between calls. */
+ * nothing in it is kept between calls. One for some rows and requests also serves fewer of either. */
 size_t qwen_attn_kv8_workspace_bytes(int rows, int requests, int heads, int kv_heads, int dim);
 int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
                        const float* v_scale, int pages, int page_size, const int32_t* block_table, int max_pages,

@@ -960,12 +960,13 @@ bool may_prompt(int rows, int requests, int group) {
     return rows > 1 && pairs > kSplitMax && (rows > requests || pairs > kSplitOnly);
 }
 // split_kernel's pieces are at most kTargetItems plus one per unit; units at most one per 8 pairs plus one per request that
-// has rows, and, where larger requests go to prompt_kernel, at most one per 8 of the pairs with which one does not.
+// has rows, and, where larger requests go to prompt_kernel, at most one per 8 of the pairs with which one does not (plus one,
+// so that the bound does not fall where the first request goes there).
 int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
     const int group = heads / kv_heads;
     const int64_t pairs = static_cast<int64_t>(rows) * group, busy = std::min(rows, requests);
     int64_t units = pairs / kRows + busy;
-    if (may_prompt(rows, requests, group)) units = std::min(units, busy * blocks_for(std::max(kSplitMax, group), kRows));
+    if (may_prompt(rows, requests, group)) units = std::min(units, busy * (blocks_for(std::max(kSplitMax, group), kRows) + 1));
     return units * kv_heads;
 }
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
@@ -978,7 +979,9 @@ Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     Layout l;
     l.items = kTargetItems + unit_bound(rows, requests, heads, kv_heads);
     l.all = l.items;
-    if (may_prompt(rows, requests, heads / kv_heads)) l.all += kPromptFill * (kPromptRows / kRows);
+    // Room for cut prompts by the rows alone, though a call with no more rows than requests has none: a workspace for some
+    // rows and requests has to serve fewer of either.
+    if (rows > 1 && static_cast<int64_t>(rows) * (heads / kv_heads) > kSplitMax) l.all += kPromptFill * (kPromptRows / kRows);
     l.stat = align_up(static_cast<size_t>(l.all) * kRows * dim * 4);
     l.info = l.stat + align_up(static_cast<size_t>(l.all) * kRows * 8);
     l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);

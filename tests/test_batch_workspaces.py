@@ -1,0 +1,51 @@
+"""Workspace sizes of the operators of several requests: one sized for a server's largest step serves every smaller one."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from qwen35_hip import _lib, ops
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+ROWS = [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 31, 32, 33, 40, 63, 64, 65, 100, 127, 128, 129, 200, 256, 257, 512, 1000, 1024, 1025,
+        2048, 4095, 4096, 5000, 20000]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 256), (1, 1, 64), (12, 12, 64), (24, 8, 128), (40, 1, 128), (31, 1, 64),
+                                                (64, 2, 256), (33, 1, 64)])
+def test_attention_workspace_serves_smaller_steps(lib, heads, kv_heads, dim):
+    """Never more for fewer rows or fewer requests."""
+    requests = [n for n in ROWS if n <= 4096]
+    size = np.array([[lib.qwen_attn_kv8_workspace_bytes(r, b, heads, kv_heads, dim) for b in requests] for r in ROWS])
+    assert (size > 0).all()
+    assert (np.diff(size, axis=0) >= 0).all(), [ROWS[i] for i in np.argwhere(np.diff(size, axis=0) < 0)[0][:1]]
+    assert (np.diff(size, axis=1) >= 0).all(), [requests[i] for i in np.argwhere(np.diff(size, axis=1) < 0)[0][1:]]
+
+
+@pytest.mark.gpu
+def test_attention_workspace_of_a_larger_step():
+    """Requests leave while the step keeps its padded rows: the same workspace, and what a call of its own size gives."""
+    r = np.random.default_rng(0)
+    heads, kvh, dim, rows = 16, 2, 128, 64
+    cache = ops.kv8_cache(rows, kvh, dim, 16)
+    cache.k.copy_(torch.from_numpy(r.integers(-127, 128, tuple(cache.k.shape), dtype=np.int8)))
+    cache.v.copy_(torch.from_numpy(r.integers(-127, 128, tuple(cache.v.shape), dtype=np.int8)))
+    cache.k_scale.fill_(0.02), cache.v_scale.fill_(0.02)
+    i32 = lambda a: torch.from_numpy(np.asarray(a, np.int32)).cuda()
+    q = torch.from_numpy(r.standard_normal((rows, heads, dim)).astype(np.float32)).cuda()
+    table, lens = np.arange(rows).reshape(rows, 1), r.integers(1, 17, rows)
+    ws = torch.empty(ops.attn_kv8_workspace_bytes(rows, rows, heads, kvh, dim), dtype=torch.uint8, device="cuda")
+    for n in (64, 63, 40, 1):
+        ws.fill_(0x7f)
+        args = (q, cache, i32(table[:n]), i32(np.arange(n + 1)), i32(lens[:n]))
+        outs = [torch.zeros_like(q) for _ in range(2)]
+        ops.attn_kv8_rows(*args, workspace=ws, out=outs[0])
+        ops.attn_kv8_rows(*args, out=outs[1])
+        assert torch.equal(*outs) and bool(outs[0][:n].any()) and not bool(outs[0][n:].any())
