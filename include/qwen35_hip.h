@@ -433,9 +433,10 @@ int qwen_moe_group_rows(const int32_t* idx, int pairs, int n_experts, int32_t* o
  *   out[t] = sum_j weights[t][j] * Wd_e (SiLU(Wg_e x_t) * (Wu_e x_t)),  e = the id of pair t top + j
  * written to out [rows x width]. w_gate and w_up (one type) hold n_experts matrices of inter x width one after the
  * other, w_down n_experts of width x inter: Q4_K or Q6_K, width and inter multiples of 256 up to 2^20; every pointer
- * 16-byte aligned, out apart from x, rows * top <= 2^24, rows * width and rows * top * inter < 2^34. The products have an fp32
- * dot product's accuracy (qwen_matmul_rows). A token with an id outside the experts has a NaN row. workspace: at least
- * qwen_moe_experts_rows_workspace_bytes() bytes (0 for sizes that the call refuses), for one call at a time.
+ * 16-byte aligned, out apart from x, n_experts <= 1024, rows * top <= 2^24, rows * width and rows * top * inter < 2^34.
+ * The products have an fp32 dot product's accuracy (qwen_matmul_rows). A token with an id outside the experts has a NaN
+ * row. workspace: at least qwen_moe_experts_rows_workspace_bytes() bytes (0 for sizes that the call refuses, with its
+ * message), for one call at a time.
  * ref: src/layer_moe.cpp:127-142, token by token there */
 size_t qwen_moe_experts_rows_workspace_bytes(int rows, int top, int n_experts, int width, int inter);
 int qwen_moe_experts_rows(const void* w_gate, const void* w_up, int type, const void* w_down, int down_type,

@@ -835,6 +835,19 @@ Layout layout(int rows, int top, int experts, int width, int inter) {
     return l;
 }
 
+// The sizes that a call takes; the message names the first that it does not.
+int check_sizes(int rows, int top, int n_experts, int width, int inter) {
+    QK_REQUIRE(width > 0 && inter > 0 && width % 256 == 0 && inter % 256 == 0,
+               "moe_experts_rows: widths %d and %d are not multiples of 256", width, inter);
+    QK_REQUIRE(width <= (1 << 20) && inter <= (1 << 20), "moe_experts_rows: widths %d and %d exceed 2^20", width, inter);
+    QK_REQUIRE(n_experts > 0 && n_experts <= kMaxExperts, "moe_experts_rows: %d experts (1 to %d)", n_experts, kMaxExperts);
+    QK_REQUIRE(rows >= 0 && top > 0 && static_cast<int64_t>(rows) * top <= (1 << 24), "moe_experts_rows: %d rows of %d picks",
+               rows, top);
+    QK_REQUIRE(static_cast<int64_t>(rows) * std::max<int64_t>(width, static_cast<int64_t>(top) * inter) < (int64_t{1} << 34),
+               "moe_experts_rows: %d rows exceed one call", rows);
+    return QWEN_STATUS_OK;
+}
+
 template <int TYPE, bool SWIGLU>
 void launch_rows(RowsArgs a, int64_t tiles, hipStream_t s) {
     a.column_blocks = static_cast<int>(blocks_for(a.M, RowsShape<1, SWIGLU>::cols));
@@ -894,7 +907,7 @@ int qwen_moe_group_rows(const int32_t* idx, int pairs, int n_experts, int32_t* o
 }
 
 size_t qwen_moe_experts_rows_workspace_bytes(int rows, int top, int n_experts, int width, int inter) {
-    if (rows <= 0 || top <= 0 || n_experts <= 0 || width <= 0 || inter <= 0 || width % 256 || inter % 256) return 0;
+    if (rows == 0 || check_sizes(rows, top, n_experts, width, inter)) return 0;
     return layout(rows, top, n_experts, width, inter).bytes;
 }
 
@@ -904,14 +917,7 @@ int qwen_moe_experts_rows(const void* w_gate, const void* w_up, int type, const 
     QK_REQUIRE(w_gate && w_up && w_down, "moe_experts_rows: tensor is not loaded");
     if ((type != kQ4_K && type != kQ6_K) || (down_type != kQ4_K && down_type != kQ6_K))
         return fail(QWEN_STATUS_UNSUPPORTED_TYPE, "moe_experts_rows: GGML types %d, %d (Q4_K and Q6_K)", type, down_type);
-    QK_REQUIRE(width > 0 && inter > 0 && width % 256 == 0 && inter % 256 == 0,
-               "moe_experts_rows: widths %d and %d are not multiples of 256", width, inter);
-    QK_REQUIRE(width <= (1 << 20) && inter <= (1 << 20), "moe_experts_rows: widths %d and %d exceed 2^20", width, inter);
-    QK_REQUIRE(n_experts > 0 && n_experts <= kMaxExperts, "moe_experts_rows: %d experts (1 to %d)", n_experts, kMaxExperts);
-    QK_REQUIRE(rows >= 0 && top > 0 && static_cast<int64_t>(rows) * top <= (1 << 24), "moe_experts_rows: %d rows of %d picks",
-               rows, top);
-    QK_REQUIRE(static_cast<int64_t>(rows) * std::max<int64_t>(width, static_cast<int64_t>(top) * inter) < (int64_t{1} << 34),
-               "moe_experts_rows: %d rows exceed one call", rows);
+    if (const int rc = check_sizes(rows, top, n_experts, width, inter)) return rc;
     if (rows == 0) return ok();
     QK_REQUIRE(order && starts && weights && x && out, "moe_experts_rows: null pointer");
     QK_REQUIRE(aligned16(w_gate) && aligned16(w_up) && aligned16(w_down) && aligned16(x) && aligned16(out),

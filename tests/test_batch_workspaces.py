@@ -29,6 +29,22 @@ def test_attention_workspace_serves_smaller_steps(lib, heads, kv_heads, dim):
     assert (np.diff(size, axis=1) >= 0).all(), [requests[i] for i in np.argwhere(np.diff(size, axis=1) < 0)[0][1:]]
 
 
+@pytest.mark.parametrize("rows,top,experts,width,inter,words", [
+    (3, 8, 0, 512, 256, "experts"), (3, 8, 1025, 512, 256, "experts"), (3, 8, 2000, 512, 256, "experts"),
+    (3, 8, 16, (1 << 20) + 256, 256, "2^20"), (3, 8, 16, 512, (1 << 20) + 256, "2^20"), (3, 8, 16, 500, 256, "256"),
+    (3, 8, 16, 512, 0, "256"), (3, 0, 16, 512, 256, "picks"), (-1, 8, 16, 512, 256, "picks"), (1 << 22, 8, 16, 512, 256, "picks"),
+    (1 << 21, 8, 16, 512, 1024, "one call"), (1 << 15, 1, 16, 1 << 19, 256, "one call")])
+def test_experts_workspace_of_refused_sizes(lib, rows, top, experts, width, inter, words):
+    """0, and the message of the call itself."""
+    assert lib.qwen_moe_experts_rows_workspace_bytes(rows, top, experts, width, inter) == 0
+    P = 1 << 20
+    said = lib.qwen_last_error().decode()
+    assert words in said
+    assert lib.qwen_moe_experts_rows(P, P, 12, P, 12, experts, P, P, P, top, P, rows, width, inter, 2 * P, P, 1 << 60,
+                                     None) == _lib.STATUS_INVALID_ARGUMENT
+    assert lib.qwen_last_error().decode() == said
+
+
 @pytest.mark.gpu
 def test_attention_workspace_of_a_larger_step():
     """Requests leave while the step keeps its padded rows: the same workspace, and what a call of its own size gives."""
