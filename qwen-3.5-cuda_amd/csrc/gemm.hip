@@ -1559,7 +1559,7 @@ int qwen_matmul_rows_multi(const qwen_gemv_desc* descs, int n, const float* x, i
             static_cast<uint64_t>(e.M) * static_cast<uint64_t>(K) > e.num_elements - e.element_offset)
             return fail(QWEN_STATUS_OUT_OF_RANGE, "descriptor %d: GEMV shape exceeds tensor (M=%d, K=%d)", j, e.M, K);
         QK_REQUIRE(e.split == 0, "matmul_rows_multi: descriptor %d: split rows are not supported", j);
-        QK_REQUIRE(e.y, "matmul_rows_multi: descriptor %d has a null output", j);
+        QK_REQUIRE(e.y || rows == 0, "matmul_rows_multi: descriptor %d has a null output", j);
     }
     QK_REQUIRE(rows >= 0, "matmul_rows_multi: negative rows %d", rows);
     if (rows == 0) return ok();
