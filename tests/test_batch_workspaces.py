@@ -29,6 +29,14 @@ def test_attention_workspace_serves_smaller_steps(lib, heads, kv_heads, dim):
     assert (np.diff(size, axis=1) >= 0).all(), [requests[i] for i in np.argwhere(np.diff(size, axis=1) < 0)[0][1:]]
 
 
+@pytest.mark.parametrize("experts,top,width,inter", [(256, 8, 2048, 512), (60, 4, 2048, 512), (1024, 1, 256, 256), (8, 2, 512, 256),
+                                                     (1, 1, 2304, 256)])
+def test_experts_workspace_serves_smaller_steps(lib, experts, top, width, inter):
+    """Never more for fewer rows, across the sizes of tiles too."""
+    size = np.array([lib.qwen_moe_experts_rows_workspace_bytes(r, top, experts, width, inter) for r in range(1, 9000)])
+    assert (size > 0).all() and (np.diff(size) >= 0).all(), int(np.argmax(np.diff(size) < 0)) + 1
+
+
 @pytest.mark.parametrize("rows,top,experts,width,inter,words", [
     (3, 8, 0, 512, 256, "experts"), (3, 8, 1025, 512, 256, "experts"), (3, 8, 2000, 512, 256, "experts"),
     (3, 8, 16, (1 << 20) + 256, 256, "2^20"), (3, 8, 16, 512, (1 << 20) + 256, "2^20"), (3, 8, 16, 500, 256, "256"),
