@@ -530,7 +530,7 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
 // ------------------------------------------------------------------ many rows
 // 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: an operand of keys or values, 1 KB of LDS, feeds 2
 // products (both parts of 32 rows), 64 cycles, so that the waves' reads take half of the LDS's rate; with 16 rows a wave they
-// took all of it (5000 rows 690 us, now 485 to 550 with the card's clock). A wave holds its rows' query parts (128
+// took all of it (5000 rows 690 us, now 480 to 550 with the card's clock). A wave holds its rows' query parts (128
 // registers at D = 256, pinned in accumulation registers) and sums (128). Its vector work - softmax, turning codes to fp16 -
 // is laid between its own products: while tile t + 1's scores are computed, tile t's are exponentiated; while tile t's
 // values are summed, the codes of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own
@@ -540,9 +540,10 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void combine_kern
 // product's depth s.
 constexpr int kPromptWaves = 4;
 constexpr int kPromptRows = 32 * kPromptWaves;
-// A workgroup has its CU to itself (registers). If a call has less than half as many of them as the card has CUs, each
-// one's keys are cut into pieces of at least kPromptMinTiles tiles, as many as the card holds at once (777 rows behind 1500
-// keys: 98 workgroups 125 us, 196 pieces 88; a call with 16 rows behind 2500 keys 39 us with pieces of 8 tiles, 35 of 4).
+// A workgroup has its CU to itself at D = 256 (registers; at 128 and 64 two would fit). If a call has less than half as many
+// of them as the card has CUs, each one's keys are cut into pieces of at least kPromptMinTiles tiles, up to one piece a CU
+// (777 rows behind 1500 keys: 98 workgroups 125 us, 196 pieces 88 when this was built, 72 now; a call with 16 rows behind
+// 2500 keys 39 us with pieces of 8 tiles, 35 of 4).
 constexpr int kPromptFill = 256;
 constexpr int kPromptMinTiles = 4;
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -952,9 +953,9 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt_kernel(const At
 // ------------------------------------------------------------------ host
 // Whether a call can have requests for prompt_kernel; if not, split_kernel takes them all. A call with no more rows than
 // requests is taken for a batch of single tokens, up to kSplitOnly (row, head) pairs of a KV head, and spared the launch
-// (us: 64 tokens at 500 keys 21.1 -> 19.3, 128 31.6 -> 29.9). Should one request have all the rows, split_kernel answers it
-// too (64 rows at 2500 keys among 64 requests: 42, as with prompt_kernel 44), if at long contexts not as fast (33 rows
-// at 30000 keys 138, 67).
+// (us: 64 tokens at 500 keys 21.1 -> 19.3, 128 31.6 -> 29.9, before the queries' parts were shared; 17.5 and 28.7 with
+// that). Should one request have all the rows, split_kernel answers it too (64 rows at 2500 keys among 64 requests: 39, with
+// prompt_kernel 44), if at long contexts not as fast (33 rows at 30000 keys 138, 67).
 bool may_prompt(int rows, int requests, int group) {
     const int64_t pairs = static_cast<int64_t>(rows) * group;
     return rows > 1 && pairs > kSplitMax && (rows > requests || pairs > kSplitOnly);

@@ -258,7 +258,7 @@ struct RowsArgs {
 // takes 16 lanes at once, 8 of two neighbouring lane groups each; and a wave's weights pass through LDS too, where each lane
 // finds its share; nobody else reads them, so that takes no barrier.
 // Two workgroups share a CU, one's start and end beside the other's steps: they are a third of a workgroup's time at K = 512.
-// Together (us, gate and up / down): 777 tokens Q6_K 355 / 237 -> 228 / 140, 4096 tokens Q4_K 585 / 364 -> 475 / 304.
+// Together (us, gate and up / down): 777 tokens Q6_K 355 / 237 -> 216 / 135, 4096 tokens Q4_K 585 / 364 -> 477 / 307.
 constexpr int kRowsWaves = 4;
 constexpr int kMaxTokenTiles = 4;   // of 16 pairs, in a tile (5 and 6 do not fit the registers)
 

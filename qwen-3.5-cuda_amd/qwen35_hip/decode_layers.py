@@ -227,7 +227,8 @@ class AttnLayerBatch:
     `forward(xs, block_table, plan)` runs the step's rows (the requests' new tokens, request by request): the three
     projections in one `matmul_rows_multi`, the split, `attn_qk_norm_rope_rows` at the plan's positions,
     `kv8_store_rows`, `attn_kv8_rows` with the gate, the output projection. Rows behind the last request's give
-    nothing of use. Nothing leaves the device, so a step of fixed `rows` can be captured in a graph."""
+    nothing of use. The layer's own fp32 cache is not used: its max_seq_len may be 1. Nothing leaves the device, so a step
+    of fixed `rows` can be captured in a graph."""
 
     def __init__(self, layer: AttnLayerDecode, pages, page_size=64):
         self.layer = layer

@@ -678,7 +678,8 @@ def attn_kv8_workspace_bytes(rows, requests, heads, kv_heads, dim) -> int:
 
 def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None, workspace=None, out=None, stream=None):
     """q [rows, heads, dim] of several requests (rows row_start[b] .. row_start[b + 1] - 1 are the last positions of
-    request b's kv_len[b] tokens, in the pages block_table[b]) -> out [rows, heads, dim] (x sigmoid(gate)), causal."""
+    request b's kv_len[b] tokens, in the pages block_table[b]) -> out [rows, heads, dim] (x sigmoid(gate)), causal. Rows of
+    no request are left as `out` has them (uninitialised if it is allocated here)."""
     _checked(torch.float32, q)
     if q.dim() != 3 or q.shape[2] != cache.dim:
         raise ValueError(f"q must be [rows, heads, {cache.dim}], got {tuple(q.shape)}")
