@@ -2,7 +2,8 @@
 
 Each function checks on the host that every tensor is a contiguous device
 tensor of the dtype and shape the kernel assumes (the C ABI can only check
-sizes, not buffer extents), then enqueues the kernel on `stream` (default: the
+sizes, not buffer extents; that they lie on the current device is the caller's
+part), then enqueues the kernel on `stream` (default: the
 current torch stream) and returns the output tensor(s). Outputs and workspaces that
 a call allocates belong to the stream that it runs on; a caller with `stream` orders
 it behind the inputs, and what reads the outputs behind it. Nothing here computes on
