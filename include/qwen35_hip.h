@@ -425,7 +425,7 @@ int qwen_moe_expert_gate_up(const void* w_gate, const void* w_up, int type, uint
 /* The (token, pick) pairs of many tokens grouped by expert: idx [pairs] holds the experts' ids (moe_topk_rows' idx, pair
  * p = t k + j) -> order [pairs], the pairs sorted by id, equal ids in their order, and starts [n_experts + 1]: expert
  * e's pairs are order[starts[e]] .. order[starts[e + 1] - 1]. Pairs whose id is outside [0, n_experts) come last, behind
- * starts[n_experts]. pairs <= 2^24, n_experts <= 1024. No counterpart in the reference. */
+ * starts[n_experts]. pairs <= 2^24, n_experts <= 1024; the three arrays must not overlap. No counterpart in the reference. */
 int qwen_moe_group_rows(const int32_t* idx, int pairs, int n_experts, int32_t* order, int32_t* starts, void* stream);
 
 /* The routed experts of many tokens: x [rows x width], weights [rows x top], order and starts as qwen_moe_group_rows

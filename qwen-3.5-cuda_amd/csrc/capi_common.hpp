@@ -25,6 +25,12 @@ inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether na bytes from a and nb bytes from b have none in common.
+inline bool apart(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    return na == 0 || nb == 0 || p + na <= q || q + nb <= p;
+}
+
 // Number of blocks for `items` work items at `per_block` per block.
 inline unsigned blocks_for(int64_t items, int64_t per_block) {
     return static_cast<unsigned>((items + per_block - 1) / per_block);

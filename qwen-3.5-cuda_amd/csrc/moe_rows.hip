@@ -901,6 +901,10 @@ int qwen_moe_group_rows(const int32_t* idx, int pairs, int n_experts, int32_t* o
     QK_REQUIRE(pairs >= 0 && pairs <= (1 << 24), "moe_group_rows: %d pairs", pairs);
     QK_REQUIRE(n_experts > 0 && n_experts <= kMaxExperts, "moe_group_rows: %d experts (1 to %d)", n_experts, kMaxExperts);
     QK_REQUIRE(starts && (pairs == 0 || (idx && order)), "moe_group_rows: null pointer");
+    // every workgroup reads all ids: one written over by another's pairs would be counted as another expert's
+    const size_t ids = static_cast<size_t>(pairs) * 4, offsets = static_cast<size_t>(n_experts + 1) * 4;
+    QK_REQUIRE(apart(idx, ids, order, ids) && apart(idx, ids, starts, offsets) && apart(order, ids, starts, offsets),
+               "moe_group_rows: idx, order and starts overlap");
     group_kernel<<<std::max(blocks_for(pairs, kGroupBlock), 1u), kGroupBlock, 0, as_stream(stream)>>>(idx, pairs, n_experts,
                                                                                                    order, starts);
     return check_launch("moe_group_rows");
