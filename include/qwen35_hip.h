@@ -338,7 +338,7 @@ int qwen_attn_decode_noalloc(const float* q, const float* k_cache, const float* 
  *   slots [rows], pos [rows]  slot and position of each row; -1 and 0 behind the last request's rows
  * A request is not granted its step if the free pages do not reach for it (then no later request that needs a page is
  * either), its tokens exceed the table row, or its rows exceed `rows`: it takes no page, its kv_len is 0 and its
- * slots are -1 (pos is still written). max_pages * page_size < 2^31. */
+ * slots are -1 (pos is still written). max_pages * page_size < 2^31. Outputs must not overlap the inputs, but for the head. */
 int qwen_kv8_plan(const int32_t* cached, const int32_t* fresh, int requests, int32_t* block_table, int max_pages,
                   const int32_t* free_pages, int n_free, const int32_t* free_head, int32_t* free_head_out,
                   int page_size, int rows, int32_t* row_start, int32_t* kv_len, int32_t* slots, int32_t* pos,

@@ -332,6 +332,17 @@ int qwen_kv8_plan(const int32_t* cached, const int32_t* fresh, int requests, int
     QK_REQUIRE(requests == 0 || (cached && fresh && kv_len && (block_table || max_pages == 0)), "kv8_plan: null pointer");
     QK_REQUIRE(n_free == 0 || free_pages, "kv8_plan: null free list");
     QK_REQUIRE(rows == 0 || (slots && pos), "kv8_plan: null slots or pos");
+    // every workgroup reads the inputs, at any time beside the outputs' writes
+    const size_t b = static_cast<size_t>(requests) * 4, r = static_cast<size_t>(rows) * 4;
+    const struct {
+        const void* p;
+        size_t n;
+    } in[] = {{cached, b}, {fresh, b}, {free_pages, static_cast<size_t>(n_free) * 4}, {free_head, 4}},
+      out[] = {{block_table, b * static_cast<size_t>(max_pages)}, {row_start, b + 4}, {kv_len, b}, {slots, r}, {pos, r}, {free_head_out, 4}};
+    for (const auto& o : out)
+        for (const auto& i : in)
+            QK_REQUIRE(apart(o.p, o.n, i.p, i.n) || (o.p == free_head_out && free_head_out == free_head && i.p == free_head),
+                       "kv8_plan: an output overlaps an input");
     // one workgroup where the head is updated in place: no other may read it after the write
     const unsigned grid = free_head_out == free_head ? 1u : std::min(std::max(blocks_for(rows, kPlanBlock), 1u), 256u);
     kv8_plan_kernel<<<grid, kPlanBlock, 0, as_stream(stream)>>>(cached, fresh, requests, block_table, max_pages, free_pages,
