@@ -338,7 +338,8 @@ int qwen_attn_decode_noalloc(const float* q, const float* k_cache, const float* 
  *   slots [rows], pos [rows]  slot and position of each row; -1 and 0 behind the last request's rows
  * A request is not granted its step if the free pages do not reach for it (then no later request that needs a page is
  * either), its tokens exceed the table row, or its rows exceed `rows`: it takes no page, its kv_len is 0 and its
- * slots are -1 (pos is still written). max_pages * page_size < 2^31. Outputs must not overlap the inputs, but for the head. */
+ * slots are -1 (pos is still written). max_pages * page_size < 2^31. Outputs must not overlap the inputs, but for the
+ * head. */
 int qwen_kv8_plan(const int32_t* cached, const int32_t* fresh, int requests, int32_t* block_table, int max_pages,
                   const int32_t* free_pages, int n_free, const int32_t* free_head, int32_t* free_head_out,
                   int page_size, int rows, int32_t* row_start, int32_t* kv_len, int32_t* slots, int32_t* pos,
@@ -370,9 +371,9 @@ int qwen_kv8_read_rows(const int8_t* k_codes, const int8_t* v_codes, const float
  * of zeros may lie beside any above 2^-49 (values up to about 2e-13).
  * Zeros where p < 0; a page id outside the cache, or a table row too short, makes the rows that see it NaN. row_start must
  * not decrease and may be a part of a step's: rows before row_start[0] and from row_start[requests] on are left as they
- * were. heads a multiple of kv_heads, rows * heads <= 2^24, max_pages * page_size <= 2^30; out must not overlap q.
- * workspace: device memory, 16-byte aligned, of at least qwen_attn_kv8_workspace_bytes() bytes, for one call at a time;
- * nothing in it is kept between calls. One for some rows and requests also serves fewer of either. */
+ * were. heads a multiple of kv_heads, rows * heads <= 2^24, max_pages * page_size <= 2^30; out must not overlap q, and
+ * gate only in place. workspace: device memory, 16-byte aligned, of at least qwen_attn_kv8_workspace_bytes() bytes, for one
+ * call at a time; nothing in it is kept between calls. One for some rows and requests also serves fewer of either. */
 size_t qwen_attn_kv8_workspace_bytes(int rows, int requests, int heads, int kv_heads, int dim);
 int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
                        const float* v_scale, int pages, int page_size, const int32_t* block_table, int max_pages,

@@ -1038,7 +1038,9 @@ int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_co
                rows, heads);
     QK_REQUIRE(aligned16(q) && aligned16(out) && (!gate || aligned16(gate)),
                "attn_kv8_rows: q, gate and out must be 16-byte aligned");
-    QK_REQUIRE(out != q, "attn_kv8_rows: out is q");
+    const size_t row_bytes = static_cast<size_t>(rows) * heads * dim * 4;
+    QK_REQUIRE(apart(out, row_bytes, q, row_bytes), "attn_kv8_rows: out is q or overlaps it");
+    QK_REQUIRE(!gate || gate == out || apart(out, row_bytes, gate, row_bytes), "attn_kv8_rows: out overlaps gate out of place");
     const Layout l = layout(rows, requests, heads, kv_heads, dim);
     QK_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= l.bytes,
                "attn_kv8_rows: workspace of %zu bytes, need %zu (16-byte aligned)", workspace_bytes, l.bytes);

@@ -37,3 +37,16 @@ def test_plan(lib, over):
     assert lib.qwen_kv8_plan(at["cached"], at["fresh"], 64, at["table"], 32, at["free"], 900, at["head"], at["head_out"], 64, 2000,
                              at["row_start"], at["kv_len"], at["slots"], at["pos"], None) == INV
     assert "overlaps" in lib.qwen_last_error().decode()
+
+
+@pytest.mark.parametrize("over", [dict(out="q"), dict(out="q", by=16), dict(out="q", by=-16), dict(out="gate", by=4096),
+                                  dict(out="gate", by=-64)])
+def test_attention(lib, over):
+    """Rows written beside others that are still to be read."""
+    at = dict(q=BASE, gate=2 * BASE, out=3 * BASE)
+    (out, of), by = list(over.items())[0], over.get("by", 0)
+    at[out] = at[of] + by
+    C = 4 * BASE
+    assert lib.qwen_attn_kv8_rows(at["q"], C, C, C, C, 8, 64, C, 4, C, C, 2, at["gate"], at["out"], 3, 16, 2, 256, C, 1 << 40,
+                                  None) == INV
+    assert "overlaps" in lib.qwen_last_error().decode()

@@ -186,3 +186,16 @@ def test_pages_of_zeros_keep_their_weight(n, up):
     got = host(ops.attn_kv8_rows(dev(q), gpu_cache(ref), dev(table), dev([0, n], I32), dev([total], I32)))
     want, tol = attention_wide(q, ref, table, [0, n], [total])
     assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("fresh,lens", [([1, 3], [900, 40]), ([200, 1, 30], [200, 70, 1500]), ([1100], [1100])])
+def test_output_in_the_place_of_the_gate(fresh, lens):
+    """The same bits as apart, from one piece, several, and prompts cut and uncut."""
+    r = np.random.default_rng(len(fresh))
+    heads, kvh, dim, page = 16, 2, 128, 32
+    table, pages = tables(r, lens, page)
+    start = np.concatenate([[0], np.cumsum(fresh)]).astype(int)
+    q, gate = (dev(r.standard_normal((start[-1], heads, dim)), F32) for _ in range(2))
+    args = (q, gpu_cache(random_cache(r, pages, kvh, page, dim)), dev(table), dev(start, I32), dev(lens, I32))
+    want = ops.attn_kv8_rows(*args, gate=gate)
+    assert ops.attn_kv8_rows(*args, gate=gate, out=gate) is gate and torch.equal(gate, want)
