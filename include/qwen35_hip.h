@@ -104,6 +104,16 @@ int qwen_attn_qk_norm_rope_rows(float* q, float* k, const float* q_weight, const
                                 const int32_t* pos, int pos0, int rows, int q_heads, int k_heads,
                                 int head_dim, int rope_dim, float theta, float eps, void* stream);
 
+/* The same with positions of several axes (1 to 4; image and video tokens stand at a time, a height and a width): pos
+ * [axes x rows] on the device; sections [axes] on the host, pairs of each axis, rope_dim = 2 x their sum (at most 128 pairs,
+ * rope_dim <= head_dim). Pair i turns by pos[axis(i)][t] * theta^(-2 i / rope_dim). interleaved 0: the first sections[0]
+ * pairs are axis 0's, the next sections[1] axis 1's, and so on; otherwise the pairs are dealt to the axes in turns, an axis
+ * that has its pairs being passed over. The angle is reduced in 64 bits, so that far positions keep fp32 accuracy (where
+ * all axes agree, the call above differs by its fp32 angles: 2^-24 of the angle). */
+int qwen_attn_qk_norm_mrope_rows(float* q, float* k, const float* q_weight, const float* k_weight,
+                                 const int32_t* pos, const int32_t* sections, int axes, int interleaved, int rows,
+                                 int q_heads, int k_heads, int head_dim, float theta, float eps, void* stream);
+
 /* ========================================================= Gated DeltaNet
  * One decode step of the causal depthwise conv + SiLU; history [channels x
  * (kernel-1)] is shifted in place.
@@ -380,6 +390,44 @@ int qwen_attn_kv8_rows(const float* q, const int8_t* k_codes, const int8_t* v_co
                        const int32_t* row_start, const int32_t* kv_len, int requests, const float* gate, float* out,
                        int rows, int heads, int kv_heads, int dim, void* workspace, size_t workspace_bytes,
                        void* stream);
+
+/* ====================================================================== the same cache in 4 bits
+ * For contexts that fill the card: 276 bytes a token and KV head of 256 where the 8-bit cache has 512. Pages, slots and
+ * block tables are those above, and qwen_kv8_plan makes them (it sees no codes). A value is min + scale * code, code 0..15;
+ * scale and min are bf16 (uint16_t) for each 64 dims of a token's keys and for all dims of a token's values, per head. All
+ * arrays 16-byte aligned, with 8 codes in a 32-bit word (elements 0, 2, 4, 6 in its nibbles 0..3, elements 1, 3, 5, 7 in
+ * nibbles 4..7) and NG = dim / 64:
+ *   k_codes [pages][kv_heads][page_size][dim / 2 bytes]: a token's words [4][NG][2], word (a, g, h) of dims
+ *     64 g + 16 a + 8 h + 0..7
+ *   v_codes [pages][kv_heads][page_size / 8][dim][4 bytes]: a word of 8 tokens of a dim
+ *   k_scale [pages][kv_heads][page_size / 8][NG][8], k_min [pages][kv_heads][page_size][NG]
+ *   v_scale, v_min [pages][kv_heads][page_size] */
+
+/* Rows of keys and values, [rows] x [kv_heads x dim] with row strides k_stride, v_stride (elements), quantized into the
+ * slots. Rows whose slot is negative or past the cache are skipped. Slots may come in any order; what two rows of one slot
+ * leave in it is not defined. Per group: min = the smallest value rounded down to bf16, scale = the smallest bf16 that is
+ * at least (largest - min) / 15 and 2^-100, code = rne((x - min) / scale) of the 64-bit quotient, 0 to 15. A group with
+ * an infinity or NaN, or with a value whose bf16 below is -infinity, has a NaN for its scale: all of it reads back as NaN.
+ * Magnitudes below 2^127. Tokens that are already there are not touched. */
+int qwen_kv4_store_rows(const float* k, const float* v, int64_t k_stride, int64_t v_stride, const int32_t* slots,
+                        int rows, uint8_t* k_codes, uint8_t* v_codes, uint16_t* k_scale, uint16_t* k_min,
+                        uint16_t* v_scale, uint16_t* v_min, int pages, int page_size, int kv_heads, int dim,
+                        void* stream);
+
+/* Slots back as fp32 rows k, v [rows x kv_heads x dim] (16-byte aligned), min + scale * code rounded once: zeros for a
+ * negative slot, NaN for one past the cache. */
+int qwen_kv4_read_rows(const uint8_t* k_codes, const uint8_t* v_codes, const uint16_t* k_scale, const uint16_t* k_min,
+                       const uint16_t* v_scale, const uint16_t* v_min, int pages, int page_size, int kv_heads, int dim,
+                       const int32_t* slots, int rows, float* k, float* v, void* stream);
+
+/* qwen_attn_kv8_rows over this cache: arguments, rows, lengths, refusals and what a bad page or a short table row gives as
+ * there, with fp32 accuracy over the values min + scale * code. */
+size_t qwen_attn_kv4_workspace_bytes(int rows, int requests, int heads, int kv_heads, int dim);
+int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_codes, const uint16_t* k_scale,
+                       const uint16_t* k_min, const uint16_t* v_scale, const uint16_t* v_min, int pages, int page_size,
+                       const int32_t* block_table, int max_pages, const int32_t* row_start, const int32_t* kv_len,
+                       int requests, const float* gate, float* out, int rows, int heads, int kv_heads, int dim,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* ====================================================================== MoE routing
  * The reference picks experts on the device, copies them to the host and syncs

@@ -46,6 +46,7 @@ SIGNATURES: dict[str, list] = {
     "qwen_attn_head_norm": [_P, _P, _I, _I, _F, _P],
     "qwen_rope_forward": [_P, _I, _I, _I, _I, _F, _P],
     "qwen_attn_qk_norm_rope_rows": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _P],
+    "qwen_attn_qk_norm_mrope_rows": [_P] * 6 + [_I] * 6 + [_F, _F, _P],
     "qwen_gdn_conv_step": [_P, _P, _P, _P, _I, _I, _P],
     "qwen_gdn_qk_normalize": [_P, _P, _I, _I, _F, _P],
     "qwen_gdn_frontend_rows": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P],
@@ -85,6 +86,10 @@ SIGNATURES: dict[str, list] = {
     "qwen_kv8_read_rows": [_P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _P, _P, _P],
     "qwen_attn_kv8_workspace_bytes": [_I, _I, _I, _I, _I],
     "qwen_attn_kv8_rows": [_P] * 5 + [_I, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, ctypes.c_size_t, _P],
+    "qwen_kv4_store_rows": [_P, _P, _I64, _I64, _P, _I] + [_P] * 6 + [_I, _I, _I, _I, _P],
+    "qwen_kv4_read_rows": [_P] * 6 + [_I, _I, _I, _I, _P, _I, _P, _P, _P],
+    "qwen_attn_kv4_workspace_bytes": [_I, _I, _I, _I, _I],
+    "qwen_attn_kv4_rows": [_P] * 7 + [_I, _I, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, ctypes.c_size_t, _P],
     "qwen_moe_topk": [_P, _P, _P, _I, _I, _P],
     "qwen_moe_topk_rows": [_P, _P, _P, _I, _I, _I, _P],
     "qwen_moe_add": [_P, _P, _F, _I, _P],
@@ -126,6 +131,7 @@ SIGNATURES: dict[str, list] = {
 _RESTYPES = {"qwen_last_error": ctypes.c_char_p, "qwen_status_name": ctypes.c_char_p,
              "qwen_attn_decode_workspace_bytes": ctypes.c_size_t,
              "qwen_attn_kv8_workspace_bytes": ctypes.c_size_t,
+             "qwen_attn_kv4_workspace_bytes": ctypes.c_size_t,
              "qwen_attn_decode_noalloc_max_scratch_bytes": ctypes.c_size_t,
              "qwen_matmul_rows_workspace_bytes": ctypes.c_size_t,
              "qwen_gdn_recurrent_chunked_workspace_bytes": ctypes.c_size_t,

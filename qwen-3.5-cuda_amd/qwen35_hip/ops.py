@@ -185,6 +185,23 @@ def attn_qk_norm_rope_rows(q, k, q_weight, k_weight, pos=None, pos0=0, rope_dim=
     return q, k
 
 
+def attn_qk_norm_mrope_rows(q, k, q_weight, k_weight, pos, sections, interleaved=True, theta=1e7, eps=1e-6, stream=None):
+    """In place, as attn_qk_norm_rope_rows with positions of several axes: pos int32 [axes, rows], sections the pairs of each
+    axis (rope_dim = 2 sum(sections)), dealt to the axes in turns (interleaved) or in blocks."""
+    _dev(q, k, q_weight, k_weight, dtype=torch.float32)
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError("q, k must be [rows, heads, head_dim] with equal rows and head_dim")
+    rows, qh, hd = q.shape
+    kh = k.shape[1]
+    _same((hd,), q_weight, k_weight)
+    _dev(pos, dtype=torch.int32)
+    _same((len(sections), rows), pos)
+    check(load().qwen_attn_qk_norm_mrope_rows(_p(q), _p(k), _p(q_weight), _p(k_weight), _p(pos),
+                                              (ctypes.c_int32 * len(sections))(*sections), len(sections),
+                                              int(interleaved), rows, qh, kh, hd, theta, eps, _stream(stream)))
+    return q, k
+
+
 # ------------------------------------------------------------------ Gated DeltaNet
 def gdn_frontend_rows(x, weight, hist_in, hist_out=None, y=None, k_heads=16, key_dim=128, eps=1e-6, stream=None):
     """x [rows, C], weight [C, K], hist [C, K-1] -> (y [rows, C], hist_out)."""
@@ -631,6 +648,12 @@ def kv8_plan(cached, fresh, block_table, free_pages, free_head, page_size, rows,
     return row_start, kv_len, slots, pos, free_head_out
 
 
+def _of(cache, kind) -> None:
+    """The two kinds of cache have other arrays behind their pointers."""
+    if not isinstance(cache, kind):
+        raise ValueError(f"expected a {kind.__name__}, got {type(cache).__name__}")
+
+
 def _kv_rows(x, heads, dim):
     """Row stride of x [rows, kv_heads, dim]: rows may lie apart (a slice of wider rows), each in one piece."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype is not torch.float32:
@@ -647,6 +670,7 @@ def _kv_rows(x, heads, dim):
 
 def kv8_store_rows(k, v, slots, cache: Kv8Cache, stream=None):
     """k, v [rows, kv_heads, dim] (rows may be strided) quantized into `slots` int32 [rows] of the cache, in place."""
+    _of(cache, Kv8Cache)
     ks, vs = _kv_rows(k, cache.heads, cache.dim), _kv_rows(v, cache.heads, cache.dim)
     _checked(torch.int32, slots)
     rows = k.shape[0]
@@ -659,6 +683,7 @@ def kv8_store_rows(k, v, slots, cache: Kv8Cache, stream=None):
 
 def kv8_read_rows(cache: Kv8Cache, slots, k=None, v=None, stream=None):
     """The values of `slots` int32 [rows] -> k, v float32 [rows, kv_heads, dim]."""
+    _of(cache, Kv8Cache)
     _checked(torch.int32, slots)
     n = slots.numel()
     shape = (n, cache.heads, cache.dim)
@@ -677,10 +702,8 @@ def attn_kv8_workspace_bytes(rows, requests, heads, kv_heads, dim) -> int:
     return int(load().qwen_attn_kv8_workspace_bytes(rows, requests, heads, kv_heads, dim))
 
 
-def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None, workspace=None, out=None, stream=None):
-    """q [rows, heads, dim] of several requests (rows row_start[b] .. row_start[b + 1] - 1 are the last positions of
-    request b's kv_len[b] tokens, in the pages block_table[b]) -> out [rows, heads, dim] (x sigmoid(gate)), causal. Rows of
-    no request are left as `out` has them (uninitialised if it is allocated here)."""
+def _attn_paged(q, cache, workspace_bytes, block_table, row_start, kv_len, gate, workspace, out, stream):
+    """Checks of an attention over a paged cache -> (rows, heads, requests, out, workspace)."""
     _checked(torch.float32, q)
     if q.dim() != 3 or q.shape[2] != cache.dim:
         raise ValueError(f"q must be [rows, heads, {cache.dim}], got {tuple(q.shape)}")
@@ -700,9 +723,105 @@ def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None,
         if out.shape != q.shape:
             _same(q.shape, out)
     if workspace is None:
-        workspace = _scratch(stream, attn_kv8_workspace_bytes(rows, n, heads, cache.heads, cache.dim), q.device)
+        workspace = _scratch(stream, workspace_bytes(rows, n, heads, cache.heads, cache.dim), q.device)
     _dev(workspace)
+    return rows, heads, n, out, workspace
+
+
+def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None, workspace=None, out=None, stream=None):
+    """q [rows, heads, dim] of several requests (rows row_start[b] .. row_start[b + 1] - 1 are the last positions of
+    request b's kv_len[b] tokens, in the pages block_table[b]) -> out [rows, heads, dim] (x sigmoid(gate)), causal. Rows of
+    no request are left as `out` has them (uninitialised if it is allocated here)."""
+    _of(cache, Kv8Cache)
+    rows, heads, n, out, workspace = _attn_paged(q, cache, attn_kv8_workspace_bytes, block_table, row_start, kv_len, gate,
+                                                 workspace, out, stream)
     check(load().qwen_attn_kv8_rows(_p(q), *cache.args[:6], _p(block_table), block_table.shape[1], _p(row_start),
+                                    _p(kv_len), n, _p(gate), _p(out), rows, heads, cache.heads, cache.dim, _p(workspace),
+                                    workspace.numel() * workspace.element_size(), _stream(stream)))
+    return out
+
+
+# ------------------------------------------------------------------ the same cache in 4 bits
+class Kv4Cache:
+    """4-bit codes and bfloat16 scales and minima of a paged cache (qwen35_hip.h): k uint8 [pages, kv_heads, page, dim / 2],
+    v uint8 [pages, kv_heads, page / 8, dim, 4], k_scale [pages, kv_heads, page / 8, dim / 64, 8], k_min
+    [pages, kv_heads, page, dim / 64], v_scale, v_min [pages, kv_heads, page]. Checked once, here."""
+    __slots__ = ("k", "v", "k_scale", "k_min", "v_scale", "v_min", "pages", "page", "heads", "dim", "args")
+
+    def __init__(self, k, v, k_scale, k_min, v_scale, v_min):
+        _checked(torch.uint8, k, v)
+        _checked(BF16, k_scale, k_min, v_scale, v_min)
+        if k.dim() != 4:
+            raise ValueError("cache keys must be [pages, kv_heads, page, dim / 2]")
+        pages, heads, page, half = k.shape
+        dim = 2 * half
+        for shape, *ts in (((pages, heads, page // 8, dim, 4), v), ((pages, heads, page // 8, dim // 64, 8), k_scale),
+                           ((pages, heads, page, dim // 64), k_min), ((pages, heads, page), v_scale, v_min)):
+            for t in ts:
+                if t.shape != shape:
+                    _same(shape, t)
+        self.k, self.v, self.k_scale, self.k_min, self.v_scale, self.v_min = k, v, k_scale, k_min, v_scale, v_min
+        self.pages, self.page, self.heads, self.dim = pages, page, heads, dim
+        self.args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), k_min.data_ptr(), v_scale.data_ptr(), v_min.data_ptr(),
+                     pages, page, heads, dim)
+
+    def __setattr__(self, name, value):
+        if hasattr(self, "args"):   # its pointers are those of the tensors above
+            raise AttributeError("a Kv4Cache stays over the tensors it was made of")
+        object.__setattr__(self, name, value)
+
+
+def kv4_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv4Cache:
+    """An empty cache. kv8_plan does its pages' bookkeeping."""
+    codes = dict(dtype=torch.uint8, device=device)
+    bf16 = dict(dtype=BF16, device=device)
+    return Kv4Cache(torch.zeros((pages, kv_heads, page_size, dim // 2), **codes),
+                    torch.zeros((pages, kv_heads, page_size // 8, dim, 4), **codes),
+                    torch.zeros((pages, kv_heads, page_size // 8, dim // 64, 8), **bf16),
+                    torch.zeros((pages, kv_heads, page_size, dim // 64), **bf16),
+                    torch.zeros((pages, kv_heads, page_size), **bf16), torch.zeros((pages, kv_heads, page_size), **bf16))
+
+
+def kv4_store_rows(k, v, slots, cache: Kv4Cache, stream=None):
+    """k, v [rows, kv_heads, dim] (rows may be strided) quantized into `slots` int32 [rows] of the cache, in place."""
+    _of(cache, Kv4Cache)
+    ks, vs = _kv_rows(k, cache.heads, cache.dim), _kv_rows(v, cache.heads, cache.dim)
+    _checked(torch.int32, slots)
+    rows = k.shape[0]
+    if slots.numel() != rows or v.shape[0] != rows:
+        raise ValueError(f"{slots.numel()} slots and {v.shape[0]} value rows for {rows} key rows")
+    check(load().qwen_kv4_store_rows(k.data_ptr(), v.data_ptr(), ks, vs, slots.data_ptr(), rows, *cache.args,
+                                     _stream(stream)))
+    return cache
+
+
+def kv4_read_rows(cache: Kv4Cache, slots, k=None, v=None, stream=None):
+    """The values of `slots` int32 [rows] -> k, v float32 [rows, kv_heads, dim]."""
+    _of(cache, Kv4Cache)
+    _checked(torch.int32, slots)
+    n = slots.numel()
+    shape = (n, cache.heads, cache.dim)
+    if k is None and v is None:
+        k, v = _empty(stream, (2, *shape), slots.device).unbind()
+    else:
+        k = _empty(stream, shape, slots.device) if k is None else k
+        v = _empty(stream, shape, slots.device) if v is None else v
+        _dev(k, v, dtype=torch.float32)
+        _same(shape, k, v)
+    check(load().qwen_kv4_read_rows(*cache.args, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _stream(stream)))
+    return k, v
+
+
+def attn_kv4_workspace_bytes(rows, requests, heads, kv_heads, dim) -> int:
+    return int(load().qwen_attn_kv4_workspace_bytes(rows, requests, heads, kv_heads, dim))
+
+
+def attn_kv4_rows(q, cache: Kv4Cache, block_table, row_start, kv_len, gate=None, workspace=None, out=None, stream=None):
+    """attn_kv8_rows over a Kv4Cache."""
+    _of(cache, Kv4Cache)
+    rows, heads, n, out, workspace = _attn_paged(q, cache, attn_kv4_workspace_bytes, block_table, row_start, kv_len, gate,
+                                                 workspace, out, stream)
+    check(load().qwen_attn_kv4_rows(_p(q), *cache.args[:8], _p(block_table), block_table.shape[1], _p(row_start),
                                     _p(kv_len), n, _p(gate), _p(out), rows, heads, cache.heads, cache.dim, _p(workspace),
                                     workspace.numel() * workspace.element_size(), _stream(stream)))
     return out
