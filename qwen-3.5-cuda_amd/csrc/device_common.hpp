@@ -169,6 +169,31 @@ __device__ __forceinline__ void st16_nt(void* p, uint4 v) {
     __builtin_nontemporal_store(t, reinterpret_cast<u32x4_t*>(p));
 }
 
+// 16 bytes per lane global -> LDS (m0 + 16 lane). As inline assembly the
+// compiler neither counts these loads nor waits for them; the kernel waits on
+// its own vmcnt (only stricter for the compiler's own loads, of which the main
+// loops have none).
+__device__ __forceinline__ void dma16(uint32_t voff, const void* sbase, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+}
+
+// The same from an address of each lane's own.
+__device__ __forceinline__ void dma16(const void* p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "s"(lds) : "memory", "m0");
+}
+
+// LDS address of a wave's object, as m0 wants it.
+__device__ __forceinline__ uint32_t lds_address(const void* l) {
+    return __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const void __attribute__((address_space(3)))*)(l))));
+}
+
 __device__ __forceinline__ float sumsq4(float4 v) { return (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w); }
 
 }  // namespace qk

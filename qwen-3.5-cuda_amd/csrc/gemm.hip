@@ -821,20 +821,6 @@ typedef uint4 Q4QSlot[kQ4R][4];             // one half block's quant bytes: [ro
 typedef uint8_t Q4HSlot[kQ4R][16];          // one block's headers (d, dmin, scales)
 typedef float Q4SSlot[kQ4T][8];             // one block's group sums
 
-// 16 bytes per lane global -> LDS (m0 + 16 lane). As inline assembly the
-// compiler neither counts these loads nor waits for them; the kernel waits on
-// its own vmcnt (only stricter for the compiler's own loads, of which the main
-// loop has none).
-__device__ __forceinline__ void dma16(uint32_t voff, const void* sbase, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
-}
-
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-    static_assert(N >= 0 && N < 64, "vmcnt");
-    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
-}
-
 // This wave's loads in ring group j: 2 (x) + 2 (a half block's quant bytes, j % 4 == 0) +
 // 2 (headers and group sums, a block's first depth).
 __host__ __device__ constexpr int q4_group_loads(int j) {

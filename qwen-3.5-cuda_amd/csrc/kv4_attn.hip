@@ -49,11 +49,10 @@ constexpr int kTile = 32;              // tokens of a step
 constexpr int kSplitWaves = 4;
 constexpr int kSplitBlock = kSplitWaves * kWave;
 constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
-constexpr int kTargetItems = 1024;     // pieces of the whole call
 constexpr int kMinTiles = 4;           // of a piece
 constexpr int kMaxItems = 1 << 24;     // more than any call has
 constexpr float kMoves = 8.0f;         // a token past the reference by more moves it
-constexpr float kWeightUp = 0x1p10f;   // weights (p scale up to 2^4) enter fp16 times this
+constexpr float kWeightUp = 10.0f;     // log2 of what exponentials, and so all sums, are taken times: weights fill fp16
 
 struct Attn4Args {
     const float* q;
@@ -68,6 +67,7 @@ struct Attn4Args {
     float2* stat;        // [item][kRows] (m, l)
     int2* info;          // [row][head] (first item * kRows + row in item, pieces); written for the requests' rows alone
     int items;           // the grid, and what `part` and `stat` hold
+    int places;          // workgroups that the card holds at once
     float scale;         // log2(e) / sqrt(D)
 };
 
@@ -99,36 +99,68 @@ __device__ __forceinline__ int wave_prefix(int v) {
 }
 
 // Piece `item` of the call: request, which of its units (KV head, row block), which piece of the unit's tiles. Every wave
-// finds it by itself from the lengths, 64 requests at a time: the whole call, ragged requests and all, is cut into about
-// kTargetItems pieces of the same number of tiles.
+// finds it by itself from the lengths. All pieces of a call have the same number of tiles, `cut`, but a unit's last: as few
+// as still give each of the card's places one piece at most, since a place that takes a second one makes the call half as
+// long again; with more units than places, four pieces. Lengths are held in registers, 64 requests to one, up to kHeld x 64.
 struct Piece {
     int b, unit, split, splits, tiles;   // tiles: of one piece
     Request4 r;
 };
+constexpr int kHeld = 4;
 __device__ __forceinline__ int tiles_of(const Request4& r) { return max(1, (r.len + kTile - 1) / kTile); }
 __device__ __forceinline__ float units_of(const Attn4Args& a, const Request4& r) {
     return static_cast<float>((static_cast<int64_t>(r.n) * a.group + kRows - 1) / kRows) * static_cast<float>(a.c.heads);
 }
+// n / d, both below 2^26, the quotient below 2^20; inverse within 2^-22 of 1 / d.
+__device__ __forceinline__ int quotient(int n, int d, float inverse) {
+    int q = static_cast<int>(static_cast<float>(n) * inverse);
+    q -= q * d > n;
+    return q + (n - q * d >= d);
+}
 __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
     const int lane = threadIdx.x & 63;
-    Request4 r{0, 0, 0, false};
-    if (lane < a.requests) r = request(a, lane);
-    float total = units_of(a, r) * static_cast<float>(tiles_of(r));
-    for (int b = lane + kWave; b < a.requests; b += kWave) {
-        const Request4 s = request(a, b);
-        total += units_of(a, s) * static_cast<float>(tiles_of(s));
-    }
-    total = group_sum<kWave>(total);
-    // (rounded sums: the pieces may be one or two more than kTargetItems and one for every unit)
-    const int cut = max(static_cast<int>(fminf(ceilf(total * (1.0f / kTargetItems)), 0x1p26f)), kMinTiles);
-    p.tiles = cut;
-    for (int b0 = 0; b0 < a.requests; b0 += kWave) {
-        if (b0) {
-            r = Request4{0, 0, 0, false};
-            if (b0 + lane < a.requests) r = request(a, b0 + lane);
+    auto lane_request = [&](int b) { return b < a.requests ? request(a, b) : Request4{0, 0, 0, false}; };
+    Request4 first{0, 0, 0, false};
+    float units[kHeld];
+    int tiles[kHeld];
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) {
+        units[c] = 0.f;
+        tiles[c] = 0;
+        if (c * kWave < a.requests) {
+            const Request4 r = lane_request(c * kWave + lane);
+            units[c] = units_of(a, r);
+            tiles[c] = tiles_of(r);
+            if (c == 0) first = r;
         }
-        const int splits = (tiles_of(r) + cut - 1) / cut;
-        const int n = static_cast<int>(fminf(units_of(a, r) * static_cast<float>(splits), static_cast<float>(kMaxItems)));
+    }
+    auto sum = [&](auto&& of) {   // rounded, but the same in every wave
+        float v = 0.f;
+#pragma unroll
+        for (int c = 0; c < kHeld; ++c) v += of(units[c], static_cast<float>(tiles[c]));
+        for (int b = kHeld * kWave + lane; b < a.requests; b += kWave) {
+            const Request4 r = lane_request(b);
+            v += of(units_of(a, r), static_cast<float>(tiles_of(r)));
+        }
+        return group_sum<kWave>(v);
+    };
+    const float total = sum([](float u, float t) { return u * t; }), all_units = sum([](float u, float) { return u; });
+    const float want = static_cast<float>(a.places) * (all_units > static_cast<float>(a.places) ? 4.0f : 1.0f);
+    auto limited = [](float t) { return max(static_cast<int>(fminf(ceilf(t), 0x1p26f)), kMinTiles); };
+    int cut = limited(total / want);
+    float step = 1.0f / static_cast<float>(cut);
+    for (int i = 0; i < 3; ++i) {
+        const float pieces = sum([=](float u, float t) { return u * ceilf(t * step); });
+        if (pieces <= want) break;
+        cut = max(limited(static_cast<float>(cut) * pieces / want), cut + 1);
+        step = 1.0f / static_cast<float>(cut);
+    }
+    cut = __builtin_amdgcn_readfirstlane(cut);
+    p.tiles = cut;
+    bool found = false;
+    auto look = [&](int b0, float u, int t) {
+        const int splits = quotient(t + cut - 1, cut, step);
+        const int n = static_cast<int>(fminf(u * static_cast<float>(splits), static_cast<float>(kMaxItems)));
         const int upto = wave_prefix(n);
         const uint64_t hit = __ballot(item < upto);
         if (hit) {
@@ -138,21 +170,39 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
             p.splits = __builtin_amdgcn_readlane(splits, l);
             p.unit = __builtin_amdgcn_readfirstlane(local / p.splits);
             p.split = local - p.unit * p.splits;
-            p.r.first = __builtin_amdgcn_readlane(r.first, l);
-            p.r.n = __builtin_amdgcn_readlane(r.n, l);
-            p.r.len = __builtin_amdgcn_readlane(r.len, l);
-            p.r.bad = __builtin_amdgcn_readlane(static_cast<int>(r.bad), l) != 0;
-            return true;
+            if (b0 == 0) {
+                p.r.first = __builtin_amdgcn_readlane(first.first, l);
+                p.r.n = __builtin_amdgcn_readlane(first.n, l);
+                p.r.len = __builtin_amdgcn_readlane(first.len, l);
+                p.r.bad = __builtin_amdgcn_readlane(static_cast<int>(first.bad), l) != 0;
+            } else {
+                p.r = request(a, p.b);
+            }
+            found = true;
+        } else {
+            item -= __builtin_amdgcn_readlane(upto, 63);
         }
-        item -= __builtin_amdgcn_readlane(upto, 63);
+    };
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c)
+        if (!found && c * kWave < a.requests) look(c * kWave, units[c], tiles[c]);
+    for (int b0 = kHeld * kWave; !found && b0 < a.requests; b0 += kWave) {
+        const Request4 r = lane_request(b0 + lane);
+        look(b0, units_of(a, r), tiles_of(r));
     }
-    return false;
+    return found;
 }
 
 // ------------------------------------------------------------------ codes and numbers
-// A word's 8 codes less LESS as the fp16 operand.
+// A word's 8 codes less LESS as the fp16 operand. `magic` is 0x64006400 from a vector register: v_and_or_b32 takes one
+// constant only, and the compiler makes two instructions of a mask and a literal.
+__device__ __forceinline__ uint32_t code_magic() {
+    uint32_t m = 0x64006400u;
+    asm("" : "+v"(m));
+    return m;
+}
 template <int LESS>
-__device__ __forceinline__ f16x8_t codes8(uint32_t w) {
+__device__ __forceinline__ f16x8_t codes8(uint32_t w, uint32_t magic) {
     const f16x2_t down = {(_Float16)(-1024.0f - LESS), (_Float16)(-1024.0f - LESS)}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     const f16x2_t down16 = {(_Float16)(-64.0f - LESS), (_Float16)(-64.0f - LESS)};
     f16x8_t r;
@@ -161,9 +211,9 @@ __device__ __forceinline__ f16x8_t codes8(uint32_t w) {
         const uint32_t x = i & 2 ? w >> 8 : w;
         f16x2_t h;
         if (i & 1)
-            h = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (x & 0x00f000f0u) | 0x64006400u), sixteenth, down16);
+            h = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (x & 0x00f000f0u) | magic), sixteenth, down16);
         else
-            h = __builtin_bit_cast(f16x2_t, (x & 0x000f000fu) | 0x64006400u) + down;
+            h = __builtin_bit_cast(f16x2_t, (x & 0x000f000fu) | magic) + down;
         r[2 * i] = h[0];
         r[2 * i + 1] = h[1];
     }
@@ -187,7 +237,9 @@ __device__ __forceinline__ float bf16_part(float v, int part) {   // bf16 part 0
     }
     return static_cast<float>(static_cast<__bf16>(v));
 }
-__device__ __forceinline__ float max_over_lk(float v) {
+// The largest over the 8 lanes that share a row: its two columns, four lane groups.
+__device__ __forceinline__ float max_over_row(float v) {
+    v = fmaxf(v, dpp_move<0xB1>(v));
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
 }
@@ -197,7 +249,8 @@ __device__ __forceinline__ uint32_t sizes2(uint32_t scale, uint32_t low) {
     const u16x2_t m = __builtin_bit_cast(u16x2_t, low & 0x7fff7fffu);
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_elementwise_max(s, m), u16x2_t{0x2b80, 0x2b80}));
 }
-__device__ __forceinline__ float log2_of_bits(uint32_t b) { return static_cast<float>(b) * 0x1p-7f - 127.0f; }
+// score + log2(size) + 127
+__device__ __forceinline__ float log2_over(float score, uint32_t b) { return __builtin_fmaf(static_cast<float>(b), 0x1p-7f, score); }
 
 // An output from its sums: zero where no key was seen (a weight may be 0 beside a NaN).
 __device__ __forceinline__ float finished(const Attn4Args& a, float m, float sum, float tot, size_t o) {
@@ -206,113 +259,125 @@ __device__ __forceinline__ float finished(const Attn4Args& a, float m, float sum
 }
 
 // ------------------------------------------------------------------ few rows
-// Bound by the cache's bytes. A workgroup takes 8 (row, head) pairs that share a KV head - 16 columns: 8 rows x 2 fp16 parts -
-// and a range of 32-token tiles, its 4 waves every fourth tile, straight from the cache to operand registers.
-// WIDE: pages of 32 tokens and more, so that a tile lies in one page and its addresses are the wave's.
+// A workgroup takes 8 (row, head) pairs that share a KV head - 16 columns: 8 rows x 2 fp16 parts - and a range of 32-token
+// tiles, its 4 waves every fourth tile. A wave's tiles go straight from the cache to a ring of two places in LDS (no
+// registers wait for them), the next but one requested as soon as a tile has been taken to registers: one and a half tiles, 13 KB at D =
+// 256, are under way per wave. The two columns of a row share the work of the softmax: each of the two lanes takes half of the
+// tokens that both hold.
+// WIDE: pages of 32 tokens and more, so that a tile lies in one page.
+//
+// A tile's place: keys, values, then k_scale, k_min, v_scale, v_min, each with its tokens in order. The keys' 16-byte pieces
+// are exchanged within a token's row (piece q of token t lies where q ^ key_turn(t) would), so that the 8 lanes that LDS
+// serves at once, which read one piece of 8 rows, meet no bank twice.
+template <int D>
+struct Ring {
+    static constexpr int NG = D / 64;
+    static constexpr int keys = 32 * D / 2, values = 32 * D / 2, scales = 32 * 2 * NG;   // bytes
+    static constexpr int at_ks = keys + values, at_km = at_ks + scales, at_vs = at_km + scales, at_vm = at_vs + 64;
+    static constexpr int bytes = at_vm + 64;
+    static constexpr int pieces = keys / 1024;              // loads of 1 KB for the keys, and for the values
+    static constexpr int loads = 2 * pieces + 1;            // of a tile
+    static constexpr int small_lanes = (bytes - at_ks) / 16;
+};
+template <int D>
+__device__ __forceinline__ int key_turn(int t) {
+    if constexpr (D == 256) return (t & 3) | ((t >> 1) & 4);
+    if constexpr (D == 128) return ((t >> 1) & 1) | ((t >> 2) & 2);
+    return (t >> 3) & 1;
+}
+
 template <int D, bool WIDE>
 __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args a) {
     constexpr int NG = D / 64, NV = D / 64, LD = D + 2;
-    __shared__ float sums[kSplitWaves][kRows * LD];
-    __shared__ float stat[kSplitWaves][kRows][2];
+    using R = Ring<D>;
+    static_assert(kRows * LD * 4 <= 2 * R::bytes, "a wave's sums go where its ring was");
+    __shared__ __align__(16) uint8_t ring[kSplitWaves][2][R::bytes];
     __shared__ __align__(16) _Float16 qs[2 * kRows][D + 8];   // the queries' parts; 16 bytes more, and 16 rows meet no bank twice
+    __shared__ float stat[kRows][kSplitWaves][2], join[kRows][kSplitWaves + 2];
     __shared__ float factors[kRows], qsum[kRows][NG];
     Piece pc;
     if (!find_piece(a, static_cast<int>(blockIdx.x), pc)) return;   // the whole workgroup
     const Request4 r = pc.r;
     const int G = a.group, pairs = r.n * G;
+    const float per_g = 1.0f / static_cast<float>(G);
+    auto over_g = [&](int pair) { return quotient(pair, G, per_g); };
     const int blocks = (pairs + kRows - 1) / kRows;
     const int h = pc.unit / blocks, rb = pc.unit - h * blocks;
     const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4, part = lr & 1;
     const int wv = wave_in_block();
-    const int ti = min(rb * kRows + (lr >> 1), pairs - 1) / G;   // columns past the last pair repeat it
-    const int limit = r.len - r.n + ti;                      // this column's last key
-    const int first_limit = r.len - r.n + rb * kRows / G;    // the smallest of the workgroup
-    const int seen = max(r.len - r.n + min(rb * kRows + kRows - 1, pairs - 1) / G + 1, 0);   // keys that some column sees
-    const int t_end = min((pc.split + 1) * pc.tiles, (seen + kTile - 1) / kTile);
+    const uint32_t magic = code_magic();
+    const int limit = r.len - r.n + over_g(min(rb * kRows + (lr >> 1), pairs - 1));   // this column's last key; columns past
+                                                                                      // the last pair repeat it
+    const int first_limit = r.len - r.n + over_g(rb * kRows);    // the smallest of the workgroup
+    const int seen = max(r.len - r.n + over_g(min(rb * kRows + kRows - 1, pairs - 1)) + 1, 0);   // keys that some column sees
+    const int t_end = __builtin_amdgcn_readfirstlane(min((pc.split + 1) * pc.tiles, (seen + kTile - 1) / kTile));
     int t = pc.split * pc.tiles + wv;
     const int P = a.c.page;
 
-    // Where a lane's parts of a tile lie, as tokens of the head's cache: `kt` of its octet of key rows (octet lr / 4), `vt` of
-    // octet lk (values, scales). Octets that no row sees are read from page 0, a page id outside the cache is not followed.
-    struct Where {
-        size_t kt, vt;
-        bool bad;
-    };
+    // The pages of a tile's octets of tokens, requested a tile before they are needed. Octets that no row sees are read from
+    // page 0, a page id outside the cache is not followed.
+    constexpr int OCT = WIDE ? 1 : 4;
     const int32_t* row_table = a.table + static_cast<size_t>(pc.b) * a.max_pages;
-    auto where = [&](int tile) {
-        Where w;
-        const int t0 = tile * kTile;
-        if constexpr (WIDE) {
-            int id = row_table[t0 >> a.page_shift];   // the wave's; below max_pages since t0 < seen
-            w.bad = id < 0 || id >= a.c.pages;
-            id = w.bad ? 0 : id;
-            const size_t at = (static_cast<size_t>(id) * a.c.heads + h) * P + (t0 & (P - 1));
-            w.kt = w.vt = at;
-        } else {
-            auto octet = [&](int tok, bool& bad) {
-                bad = false;
-                int id = 0;
-                if (tok < seen) {
-                    id = row_table[tok >> a.page_shift];
-                    bad = id < 0 || id >= a.c.pages;
-                    id = bad ? 0 : id;
-                }
-                return (static_cast<size_t>(id) * a.c.heads + h) * P + (tok & (P - 1));
-            };
-            bool unused;
-            w.kt = octet(t0 + 8 * (lr >> 2), unused);
-            w.vt = octet(t0 + 8 * lk, w.bad);
+    int ids[OCT];
+    auto request_ids = [&](int tile) {
+#pragma unroll
+        for (int j = 0; j < OCT; ++j) {
+            const int tok = tile * kTile + 8 * j;
+            ids[j] = tile < t_end && tok < seen ? row_table[tok >> a.page_shift] : 0;   // below max_pages since tok < seen
         }
-        return w;
     };
-    constexpr int KW = NG * 2;   // words of a lane's share of a token's keys
-    uint32_t K[2][KW];
-    uint4 V[NV], ksc[NG], vsc, vmn;
-    bf16x8_t kmn[2];
-    bool bad_page = false;
-    auto load_k = [&](const Where& w) {
-        const size_t tok = w.kt + (WIDE ? 8 * (lr >> 2) : 0) + (lr & 3);
+    uint32_t bad_octets[2] = {0, 0};   // of the tiles in the ring
+    const uint32_t ring_at = lds_address(&ring[wv][0][0]);
+    // A lane's part of the keys: token L / PR of a load, 16-byte piece L % PR of its row, exchanged; as offset in its octet.
+    constexpr int PR = D / 32;   // pieces of a row
+    const int ktok = lane / PR;
+    const uint32_t koff = (ktok & 7) * (D / 2) + 16 * ((lane % PR) ^ key_turn<D>(ktok)), voff = 16 * (lane % (D / 4));
+    const int lane_oct = lane / (D / 4);   // the octet that a lane has in a load, after the first of the load
+    // and of the rest: NG pieces of an octet's key scales, as many of its minima, one each of the values'
+    const uint8_t* small_base;
+    int small_oct, small_mul;
+    uint32_t small_off;
+    {
+        const int s = lane < 8 * NG ? lane % (4 * NG) : lane & 3, big = lane < 8 * NG;
+        small_base = reinterpret_cast<const uint8_t*>(lane < 4 * NG ? a.c.ks : big ? a.c.km : lane < 8 * NG + 4 ? a.c.vs : a.c.vm);
+        small_oct = big ? s / NG : s;
+        small_mul = big ? 2 * NG : 2;
+        small_off = big ? 16 * (s % NG) : 0;
+    }
+    auto request_tile = [&](int tile, int slot) {   // from `ids`; for tile < t_end
+        size_t at[OCT];   // the octets' first tokens, in the head's cache
+        uint32_t bad = 0;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint8_t* p = a.c.k + (tok + 4 * x) * (D / 2) + lk * (4 * KW);
-            if constexpr (KW == 8) {
-                const uint4 u = ld16(p), v = ld16(p + 16);
-                K[x][0] = u.x, K[x][1] = u.y, K[x][2] = u.z, K[x][3] = u.w;
-                K[x][4] = v.x, K[x][5] = v.y, K[x][6] = v.z, K[x][7] = v.w;
-            } else if constexpr (KW == 4) {
-                const uint4 u = ld16(p);
-                K[x][0] = u.x, K[x][1] = u.y, K[x][2] = u.z, K[x][3] = u.w;
-            } else {
-                const uint2 u = *reinterpret_cast<const uint2*>(p);
-                K[x][0] = u.x, K[x][1] = u.y;
-            }
-            const uint16_t* m = a.c.km + (tok + 4 * x) * NG;
-            u32x4_t z = {0u, 0u, 0u, 0u};
-            if constexpr (NG == 4) {
-                const uint2 u = *reinterpret_cast<const uint2*>(m);
-                z[0] = u.x, z[1] = u.y;
-            } else if constexpr (NG == 2) {
-                z[0] = *reinterpret_cast<const uint32_t*>(m);
-            } else {
-                z[0] = *m;
-            }
-            kmn[x] = __builtin_bit_cast(bf16x8_t, z);
+        for (int j = 0; j < OCT; ++j) {
+            const bool b = static_cast<uint32_t>(ids[j]) >= static_cast<uint32_t>(a.c.pages);
+            bad |= b ? (WIDE ? 15u : 1u << j) : 0u;
+            at[j] = (static_cast<size_t>(b ? 0u : static_cast<uint32_t>(ids[j])) * a.c.heads + h) * P + ((tile * kTile + 8 * j) & (P - 1));
         }
-        const size_t oct = w.vt + (WIDE ? 8 * lk : 0);   // a multiple of 8
+        bad_octets[slot] = bad;
+        auto octet = [&](int j) {   // for a lane
+            if constexpr (WIDE) return at[0] + 8 * j;
+            else return j == 0 ? at[0] : j == 1 ? at[1] : j == 2 ? at[2] : at[3];
+        };
+        const uint32_t to = ring_at + slot * R::bytes;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) ksc[g] = ld16(a.c.ks + oct * NG + 8 * g);
-        bad_page = w.bad;
-    };
-    auto load_v = [&](const Where& w) {
-        const size_t oct = w.vt + (WIDE ? 8 * lk : 0);
-#pragma unroll
-        for (int m = 0; m < NV; ++m) V[m] = ld16(a.c.v + oct * (D / 2) + (64 * m + 4 * lr) * 4);
-        vsc = ld16(a.c.vs + oct);
-        vmn = ld16(a.c.vm + oct);
+        for (int i = 0; i < R::pieces; ++i) {
+            constexpr int per = 4 / R::pieces;   // octets of a load
+            if constexpr (WIDE || per == 1) {
+                const size_t base = (WIDE ? at[0] + 8 * per * i : at[WIDE ? 0 : i]) * (D / 2);
+                const uint32_t turn = D == 256 ? 64 * (i & 1) : 0;   // key_turn's bit of the octet
+                dma16((koff ^ turn) + lane_oct * (4 * D), a.c.k + base, to + 1024 * i);
+                dma16(voff + lane_oct * (4 * D), a.c.v + base, to + R::keys + 1024 * i);
+            } else {
+                const size_t base = octet(per * i + lane_oct) * (D / 2);
+                dma16(a.c.k + base + koff, to + 1024 * i);
+                dma16(a.c.v + base + voff, to + R::keys + 1024 * i);
+            }
+        }
+        if (lane < R::small_lanes) dma16(small_base + octet(small_oct) * small_mul + small_off, to + R::at_ks);
     };
     // The rows' queries, scaled by 2^e so that a row's largest magnitude is in [2^14, 2^15), as two fp16 parts: 2 rows a wave,
     // requested before the first tile.
-    const int qr = 2 * wv + (lane >> 5), qp = min(rb * kRows + qr, pairs - 1), qt = qp / G;
+    const int qr = 2 * wv + (lane >> 5), qp = min(rb * kRows + qr, pairs - 1), qt = over_g(qp);
     const float* qrow = a.q + (static_cast<size_t>(r.first + qt) * a.heads + h * G + (qp - qt * G)) * D + (lane & 31) * (D / 32);
     constexpr int QN = D / 32;
     float qf[QN];
@@ -325,14 +390,9 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
     } else {
         qf[0] = qrow[0], qf[1] = qrow[1];
     }
-    const bool any = t < t_end;
-    Where next{};
-    if (any) {
-        const Where w = where(t);
-        load_k(w);
-        load_v(w);
-        if (t + kSplitWaves < t_end) next = where(t + kSplitWaves);
-    }
+    request_ids(t);
+    if (t < t_end) request_tile(t, 0);
+    request_ids(t + kSplitWaves);
     {
         float m = 0.f;
         bool bad = false;
@@ -364,7 +424,9 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
         if ((lane & (64 / QN - 1)) == 0) qsum[qr][d0 / 64] = s;
         if ((lane & 31) == 0) factors[qr] = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");   // products to log2 scores; NaN: a row
     }                                                                                        // with infinities or NaNs
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tile's loads stay in flight
+    if (t + kSplitWaves < t_end) request_tile(t + kSplitWaves, 1);
+    request_ids(t + 2 * kSplitWaves);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tiles' loads stay in flight
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     f16x8_t Q[2 * NG];   // dims 64 g + 16 lk + 8 (d % 2) + 0..7 of depth d = 2 g + d % 2
@@ -381,9 +443,48 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
     for (int m = 0; m < NV; ++m)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[m][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float mu = -FLT_MAX, l = 0.f, low = 0.f;
-    for (; t < t_end; t += kSplitWaves) {
-        const bool more = t + kSplitWaves < t_end;
+    float mu = -FLT_MAX, l = 0.f, low = 0.f;   // mu: the reference less kWeightUp
+    const int my_turn = key_turn<D>(8 * (lr >> 2) + (lr & 3));
+    const uint32_t k_at = (8 * (lr >> 2) + (lr & 3)) * (D / 2);
+    for (int slot = 0; t < t_end; t += kSplitWaves, slot ^= 1) {
+        if (t + kSplitWaves < t_end)
+            wait_vm<R::loads>();   // the next tile stays under way
+        else
+            wait_vm<0>();
+        asm volatile("" ::: "memory");
+        const uint8_t* in = ring[wv][slot];
+        constexpr int KW = NG * 2;   // words of a lane's share of a token's keys
+        uint32_t K[2][KW];
+        uint4 V[NV], ksc[NG];
+        bf16x8_t kmn[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint8_t* p = in + k_at + x * (4 * D / 2);
+            if constexpr (KW == 8) {
+                const uint4 u = ld16(p + 16 * ((2 * lk) ^ my_turn)), v = ld16(p + 16 * ((2 * lk + 1) ^ my_turn));
+                K[x][0] = u.x, K[x][1] = u.y, K[x][2] = u.z, K[x][3] = u.w;
+                K[x][4] = v.x, K[x][5] = v.y, K[x][6] = v.z, K[x][7] = v.w;
+            } else if constexpr (KW == 4) {
+                const uint4 u = ld16(p + 16 * (lk ^ my_turn));
+                K[x][0] = u.x, K[x][1] = u.y, K[x][2] = u.z, K[x][3] = u.w;
+            } else {
+                const uint2 u = *reinterpret_cast<const uint2*>(p + 16 * ((lk >> 1) ^ my_turn) + 8 * (lk & 1));
+                K[x][0] = u.x, K[x][1] = u.y;
+            }
+            const uint8_t* m = in + R::at_km + (8 * (lr >> 2) + 4 * x + (lr & 3)) * (2 * NG);
+            u32x4_t z = {0u, 0u, 0u, 0u};
+            if constexpr (NG == 4) {
+                const uint2 u = *reinterpret_cast<const uint2*>(m);
+                z[0] = u.x, z[1] = u.y;
+            } else if constexpr (NG == 2) {
+                z[0] = *reinterpret_cast<const uint32_t*>(m);
+            } else {
+                z[0] = *reinterpret_cast<const uint16_t*>(m);
+            }
+            kmn[x] = __builtin_bit_cast(bf16x8_t, z);
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) ksc[g] = ld16(in + R::at_ks + lk * (16 * NG) + 16 * g);
         f32x4_t S[2];
         const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -393,40 +494,51 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
             const uint32_t w[4] = {ksc[g].x, ksc[g].y, ksc[g].z, ksc[g].w};
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                f32x4_t T = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<0>(K[x][2 * g]), Q[2 * g], zero, 0, 0, 0);
-                T = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<0>(K[x][2 * g + 1]), Q[2 * g + 1], T, 0, 0, 0);
+                f32x4_t T = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<0>(K[x][2 * g], magic), Q[2 * g], zero, 0, 0, 0);
+                T = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<0>(K[x][2 * g + 1], magic), Q[2 * g + 1], T, 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     S[x][i] = __builtin_fmaf(T[i], i & 1 ? bf16_hi(w[2 * x + (i >> 1)]) : bf16_lo(w[2 * x + (i >> 1)]), S[x][i]);
             }
         }
-        const float f = bad_page ? __builtin_nanf("") : factor;
-        if (more) load_k(next);
-        float s[8], sv[8], mv[8];
-        uint32_t size[4];
-        const uint32_t vs[4] = {vsc.x, vsc.y, vsc.z, vsc.w}, vm[4] = {vmn.x, vmn.y, vmn.z, vmn.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = S[i >> 2][i & 3];
-            s[i] = (v + dpp_move<0xB1>(v)) * f;   // both fp16 parts of the query
+        for (int m = 0; m < NV; ++m) V[m] = ld16(in + R::keys + lk * (4 * D) + 256 * m + 16 * lr);
+        const uint2 vsc = *reinterpret_cast<const uint2*>(in + R::at_vs + 16 * lk + 8 * part);
+        const uint2 vmn = *reinterpret_cast<const uint2*>(in + R::at_vm + 16 * lk + 8 * part);
+        const float f = (bad_octets[slot] >> lk) & 1 ? __builtin_nanf("") : factor;
+        if (t + 2 * kSplitWaves < t_end) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the place has been read
+            request_tile(t + 2 * kSplitWaves, slot);
+            request_ids(t + 3 * kSplitWaves);
+        }
+        // This lane's tokens 8 lk + 4 part + 0..3: both fp16 parts of the query, the other one from the lane beside.
+        const int tok = t * kTile + 8 * lk + 4 * part;
+        float s[4], sv[4], mv[4];
+        const uint32_t vs[2] = {vsc.x, vsc.y}, vm[2] = {vmn.x, vmn.y};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float mine = part ? S[1][i] : S[0][i], other = part ? S[0][i] : S[1][i];
+            s[i] = (mine + dpp_move<0xB1>(other)) * f;
             sv[i] = i & 1 ? bf16_hi(vs[i >> 1]) : bf16_lo(vs[i >> 1]);
             mv[i] = __builtin_fmaf(8.0f, sv[i], i & 1 ? bf16_hi(vm[i >> 1]) : bf16_lo(vm[i >> 1]));
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) size[i] = sizes2(vs[i], vm[i]);
         if (t * kTile + kTile - 1 > first_limit) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (t * kTile + 8 * lk + i > limit) {   // what lies there is anything: no 0 * NaN
+            for (int i = 0; i < 4; ++i)
+                if (tok + i > limit) {   // what lies there is anything: no 0 * NaN
                     s[i] = -INFINITY;
                     sv[i] = mv[i] = 0.f;
                 }
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i] + log2_of_bits(i & 1 ? size[i >> 1] >> 16 : size[i >> 1] & 0xffffu));
+        for (int i = 0; i < 4; i += 2) {
+            const uint32_t z = sizes2(vs[i >> 1], vm[i >> 1]);
+            top = fmaxf(top, fmaxf(log2_over(s[i], z & 0xffffu), log2_over(s[i + 1], z >> 16)));
+        }
+        top -= 127.0f + kWeightUp;
         if (__ballot(top > mu + kMoves)) {
-            const float now = fmaxf(mu, max_over_lk(top));
+            const float now = fmaxf(mu, max_over_row(top));
             const float shrink = __builtin_amdgcn_exp2f(mu - now);
             mu = now;
             l *= shrink;
@@ -438,34 +550,41 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[m][e][i] *= shrink;
         }
-        f16x8_t W;
+        f16x2_t high[2], rest[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const float p = __builtin_amdgcn_exp2f(s[i] - mu);
             l += p;
             low = __builtin_fmaf(p, mv[i], low);
-            const float w = rounded(p * (sv[i] * kWeightUp));
-            W[i] = static_cast<_Float16>(part ? low_part(w) : w);
+            const float w = rounded(p * sv[i]);
+            high[i >> 1][i & 1] = static_cast<_Float16>(w);
+            rest[i >> 1][i & 1] = static_cast<_Float16>(low_part(w));
+        }
+        u32x4_t W;   // tokens 8 lk + 0..7 of this column's part: half of them from the lane beside
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t x = __builtin_bit_cast(uint32_t, high[j]), y = __builtin_bit_cast(uint32_t, rest[j]);
+            const uint32_t got = __float_as_uint(dpp_move<0xB1>(__uint_as_float(part ? x : y)));
+            W[j] = part ? got : x;
+            W[2 + j] = part ? y : got;
         }
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
             const uint32_t w[4] = {V[m].x, V[m].y, V[m].z, V[m].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<8>(w[e]), W, acc[m][e], 0, 0, 0);
-        }
-        if (more) {
-            load_v(next);
-            if (t + 2 * kSplitWaves < t_end) next = where(t + 2 * kSplitWaves);
+                acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<8>(w[e], magic), __builtin_bit_cast(f16x8_t, W), acc[m][e], 0, 0, 0);
         }
     }
     // The waves' sums meet in LDS; the two parts of a row are neighbouring columns, each lane of a pair writes every
     // other dim of both. Row 4 lk + i of value tile (m, e) is dim 64 m + 4 (4 lk + i) + e.
+    l += dpp_move<0xB1>(l);
+    low += dpp_move<0xB1>(low);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     low += __shfl_xor(low, 16);
     low += __shfl_xor(low, 32);
-    float* mine = sums[wv] + (lr >> 1) * LD;
+    float* mine = reinterpret_cast<float*>(ring[wv]) + (lr >> 1) * LD;   // the wave's loads have all come
 #pragma unroll
     for (int m = 0; m < NV; ++m)
 #pragma unroll
@@ -474,29 +593,37 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
             for (int e = 0; e < 4; e += 2) {
                 const float u = acc[m][e][i] + dpp_move<0xB1>(acc[m][e][i]);
                 const float v = acc[m][e + 1][i] + dpp_move<0xB1>(acc[m][e + 1][i]);
-                mine[64 * m + 4 * (4 * lk + i) + e + part] = __builtin_fmaf(part ? v : u, 1.0f / kWeightUp, low);
+                mine[64 * m + 4 * (4 * lk + i) + e + part] = (part ? v : u) + low;
             }
     if (lane < 16 && part == 0) {
-        stat[wv][lr >> 1][0] = mu;
-        stat[wv][lr >> 1][1] = l;
+        stat[lr >> 1][wv][0] = mu;
+        stat[lr >> 1][wv][1] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x < kRows) {   // what each wave's sums count of the row's
+        const int row = threadIdx.x;
+        float m = stat[row][0][0], tot = 0.f;
+#pragma unroll
+        for (int w = 1; w < kSplitWaves; ++w) m = fmaxf(m, stat[row][w][0]);
+#pragma unroll
+        for (int w = 0; w < kSplitWaves; ++w) {
+            const float k = __builtin_amdgcn_exp2f(stat[row][w][0] - m);
+            join[row][w] = k;
+            tot += k * stat[row][w][1];
+        }
+        join[row][kSplitWaves] = m;
+        join[row][kSplitWaves + 1] = r.bad ? __builtin_nanf("") : tot;
     }
     __syncthreads();
     const int rows = min(kRows, pairs - rb * kRows);
     for (int i = threadIdx.x; i < rows * D; i += kSplitBlock) {
         const int row = i / D, d = i - row * D;
-        float m = stat[0][row][0];
+        float sum = 0.f;
 #pragma unroll
-        for (int w = 1; w < kSplitWaves; ++w) m = fmaxf(m, stat[w][row][0]);
-        float sum = 0.f, tot = 0.f;
-#pragma unroll
-        for (int w = 0; w < kSplitWaves; ++w) {
-            const float k = __builtin_amdgcn_exp2f(stat[w][row][0] - m);
-            sum += k * sums[w][row * LD + d];
-            tot += k * stat[w][row][1];
-        }
-        if (r.bad) tot = __builtin_nanf("");
-        const int at = rb * kRows + row, tok = at / G;
-        const size_t o = (static_cast<size_t>(r.first + tok) * a.heads + h * G + (at - tok * G)) * D + d;
+        for (int w = 0; w < kSplitWaves; ++w) sum += join[row][w] * reinterpret_cast<const float*>(ring[w])[row * LD + d];
+        const float m = join[row][kSplitWaves], tot = join[row][kSplitWaves + 1];
+        const int at = rb * kRows + row, n = over_g(at);
+        const size_t o = (static_cast<size_t>(r.first + n) * a.heads + h * G + (at - n * G)) * D + d;
         if (pc.splits == 1) {
             a.out[o] = finished(a, m, sum, tot, o);
         } else {
@@ -578,11 +705,15 @@ __global__ __launch_bounds__(NW* kWave) void join4_kernel(const Attn4Args a) {
 }
 
 // ------------------------------------------------------------------ host
-// split4_kernel's pieces are at most kTargetItems (and a few for rounding) plus one per unit; units at most one per 8 pairs
-// plus one per request that has rows.
-int64_t item_bound(int rows, int requests, int heads, int kv_heads) {
-    const int64_t pairs = static_cast<int64_t>(rows) * (heads / kv_heads);
-    return kTargetItems + 8 + (pairs / kRows + std::min(rows, requests)) * kv_heads;
+// split4_kernel's workgroups of 4 waves on a CU, by their registers.
+int places_on_cu(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
+constexpr int kCus = 256;
+// Its pieces are at most as many as wanted (and a few for rounding) plus one per unit; units at most one per 8 pairs plus one
+// per request that has rows.
+int64_t item_bound(int rows, int requests, int heads, int kv_heads, int dim) {
+    const int64_t pairs = static_cast<int64_t>(rows) * (heads / kv_heads), places = kCus * places_on_cu(dim);
+    const int64_t units = (pairs / kRows + std::min(rows, requests)) * kv_heads;
+    return (units > places ? 4 : 1) * places + 8 + units;
 }
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
@@ -592,7 +723,7 @@ struct Layout {
 };
 Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     Layout l;
-    l.items = item_bound(rows, requests, heads, kv_heads);
+    l.items = item_bound(rows, requests, heads, kv_heads, dim);
     l.stat = align_up(static_cast<size_t>(l.items) * kRows * dim * 4);
     l.info = l.stat + align_up(static_cast<size_t>(l.items) * kRows * 8);
     l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);
@@ -668,6 +799,7 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     a.stat = reinterpret_cast<float2*>(ws + l.stat);
     a.info = reinterpret_cast<int2*>(ws + l.info);
     a.items = static_cast<int>(l.items);
+    a.places = kCus * places_on_cu(dim);
     const hipStream_t s = as_stream(stream);
     if (dim == 64)
         launch<64>(a, s);
