@@ -32,6 +32,8 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
+#include <utility>
 
 #include "capi_common.hpp"
 #include "device_common.hpp"
@@ -51,6 +53,8 @@ constexpr int kSplitBlock = kSplitWaves * kWave;
 constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
 constexpr int kMinTiles = 4;           // of a piece
 constexpr int kMaxItems = 1 << 24;     // more than any call has
+constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take split4_kernel; a row does
+constexpr int kSplitOnly = 1024;       // and of a whole call that has no more rows than requests
 constexpr float kMoves = 8.0f;         // a token past the reference by more moves it
 constexpr float kWeightUp = 10.0f;     // log2 of what exponentials, and so all sums, are taken times: weights fill fp16
 
@@ -66,8 +70,10 @@ struct Attn4Args {
     float* part;         // [item][kRows][D] sums of p v
     float2* stat;        // [item][kRows] (m, l)
     int2* info;          // [row][head] (first item * kRows + row in item, pieces); written for the requests' rows alone
-    int items;           // the grid, and what `part` and `stat` hold
-    int places;          // workgroups that the card holds at once
+    int items;           // split4_kernel's grid, and what `part` and `stat` hold of it
+    int all_items;       // and with the cut prompts' pieces
+    int places;          // split4_kernel's workgroups that the card holds at once
+    int split_all;       // every request takes split4_kernel
     float scale;         // log2(e) / sqrt(D)
 };
 
@@ -108,7 +114,11 @@ struct Piece {
 };
 constexpr int kHeld = 4;
 __device__ __forceinline__ int tiles_of(const Request4& r) { return max(1, (r.len + kTile - 1) / kTile); }
+__device__ __forceinline__ bool takes_split(const Attn4Args& a, const Request4& r) {
+    return a.split_all || static_cast<int64_t>(r.n) * a.group <= max(kSplitMax, a.group);
+}
 __device__ __forceinline__ float units_of(const Attn4Args& a, const Request4& r) {
+    if (!takes_split(a, r)) return 0.f;
     return static_cast<float>((static_cast<int64_t>(r.n) * a.group + kRows - 1) / kRows) * static_cast<float>(a.c.heads);
 }
 // n / d, both below 2^26, the quotient below 2^20; inverse within 2^-22 of 1 / d.
@@ -634,98 +644,616 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
     }
 }
 
-// ------------------------------------------------------------------ join
-// Joins the pieces of (row, head) pairs: a workgroup of NW waves per pair, wave w takes pieces w, w + NW, ... Lanes hold the
-// dims.
-template <int D, int NW>
-__global__ __launch_bounds__(NW* kWave) void join4_kernel(const Attn4Args a) {
-    constexpr int V = D / kWave;
-    __shared__ float sums[NW][D], ls[NW], ms[NW];
-    const int lane = threadIdx.x & 63, wv = wave_in_block();
-    // Pairs of the requests' rows alone: only those have an entry of this call (the workspace may hold an earlier one's).
-    const int from = min(max(a.row_start[0], 0), a.rows) * a.heads, live = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;
-    const int pair = static_cast<int>(blockIdx.x);
-    if (pair < from || pair >= live) return;   // the whole workgroup
-    const int2 in = a.info[pair];
-    if (in.y <= 1 || in.x < 0 || in.y > a.items - in.x / kRows) return;   // one piece; or starts that decrease
-    const int slot = in.x % kRows, first = in.x / kRows;
-    float m = -FLT_MAX, l = 0.f, s[V];
+// ------------------------------------------------------------------ many rows
+// Bound by the matrix products. 128 rows a workgroup, 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: codes are
+// turned to fp16 once per workgroup, into LDS, and an operand of keys or values, 1 KB of LDS, feeds 2 products (both parts of
+// 32 rows). A wave holds its rows' query parts (128 registers at D = 256, pinned in accumulation registers) and sums (128).
+// Its vector work - scales, softmax, turning codes to fp16 - is laid between its own products: while tile t + 1's scores are
+// computed, tile t's are exponentiated and each group's products are scaled beside the next group's; while tile t's values
+// are summed, the codes of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own rows may end
+// one earlier: with a branch around the products the compiler moves the sums between register files at each.
+// The scores^T tile has token rho = 8 b + 4 g + j of the 32 in register 4 b + j of lane half g; key row rho stands for token
+// 16 (b / 2) + 8 g + 4 (b % 2) + j, so that a lane's registers 8 s .. 8 s + 7 are octet 2 s + g, its share of the second
+// product's depth s.
+constexpr int kPromptWaves = 4;
+constexpr int kPromptRows = 32 * kPromptWaves;
+// A workgroup has its CU to itself at D = 256 (registers). If a call has less than half as many of them as the card has CUs,
+// each one's keys are cut into pieces of at least kPromptMinTiles tiles, up to one piece a CU.
+constexpr int kPromptFill = 256;
+constexpr int kPromptMinTiles = 4;
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <int S>
+using IC = std::integral_constant<int, S>;
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
+    (f(IC<I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    static_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+template <int D>
+__global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const Attn4Args a) {
+    constexpr int ND = D / 16, DT = D / 32, NG = D / 64, E = D / 64, NTH = kPromptWaves * kWave;   // E: a lane's words of a tile's
+    __shared__ __align__(16) f16x8_t ks[2][ND][kWave];                                             // keys, and of its values
+    __shared__ __align__(16) f16x8_t vs[2][DT][2][kWave];
+    __shared__ __align__(16) float kscale[4][NG][kTile];   // [tile % 4][group][token]
+    __shared__ __align__(16) uint2 kmin[4][kTile];         // [tile % 4][key row]: 4 bf16, of groups past the last 0
+    __shared__ __align__(16) float vtok[4][3][kTile];      // [tile % 4][scale, min + 8 scale, log2 size][token]
+    // which request, KV head and row tile: the last row tiles (the longest rows) first
+    const int G = a.group, lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+    const float per_g = 1.0f / static_cast<float>(G);
+    auto over_g = [&](int pair) { return quotient(pair, G, per_g); };
+    auto tiles_here = [&](int b) {   // workgroups of a request, before they are cut
+        if (b >= a.requests) return 0;
+        const Request4 r = request(a, b);
+        const int64_t n = (static_cast<int64_t>(r.n) * G + kPromptRows - 1) / kPromptRows * a.c.heads;
+        return takes_split(a, r) ? 0 : static_cast<int>(n < kMaxItems ? n : kMaxItems);
+    };
+    float total = 0.f;
+    for (int b0 = 0; b0 < a.requests; b0 += kWave) total += static_cast<float>(tiles_here(b0 + lane));
+    total = group_sum<kWave>(total);
+    if (total == 0.f) return;   // the whole workgroup
+    const int splits = total < kPromptFill ? __builtin_amdgcn_readfirstlane(kPromptFill / static_cast<int>(total)) : 1;
+    int b = -1, item = static_cast<int>(blockIdx.x) / splits;
+    const int split = static_cast<int>(blockIdx.x) - item * splits;
+    for (int b0 = 0; b0 < a.requests && b < 0; b0 += kWave) {
+        const int n = tiles_here(b0 + lane), upto = wave_prefix(n);
+        const uint64_t hit = __ballot(item < upto);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            item -= __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
+            b = b0 + l;
+        } else {
+            item -= __builtin_amdgcn_readlane(upto, 63);
+        }
+    }
+    if (b < 0) return;   // the whole workgroup
+    const Request4 r = request(a, b);
+    const int pairs = r.n * G, tiles = (pairs + kPromptRows - 1) / kPromptRows;
+    const int unit = __builtin_amdgcn_readfirstlane(item);
+    const int h = unit % a.c.heads, rt = tiles - 1 - unit / a.c.heads;
+    const int wv = wave_in_block(), tid = threadIdx.x;
+    const int row0 = rt * kPromptRows + 32 * wv;             // the wave's first pair
+    const int rr = min(row0 + col, pairs - 1);
+    const int ti = over_g(rr), head = h * G + (rr - ti * G);
+    const int limit = r.len - r.n + ti;
+    const int wave_first = r.len - r.n + over_g(min(row0, pairs - 1));
+    const int seen = max(r.len - r.n + over_g(min(rt * kPromptRows + kPromptRows - 1, pairs - 1)) + 1, 0);
+    const int all_steps = (seen + kTile - 1) / kTile, pieces = min(splits, max(all_steps / kPromptMinTiles, 1));
+    if (split >= pieces) return;   // the whole workgroup
+    const int per = (all_steps + pieces - 1) / pieces;
+    const int first_tile = split * per, steps = max(min(per, all_steps - first_tile), 0);   // this piece's tiles
+    const uint32_t magic = code_magic();
+
+    // A wave brings one octet of tokens of each tile: page and offset are the same for its lanes. A lane's words: of keys
+    // (token lane % 8, words E (lane / 8) .. of its row), of values (dims E lane ..). Octets past the last are loaded from page 0 and
+    // never read from LDS. Page ids are read a tile ahead of the codes they lead to.
+    uint32_t kr[E], vr[E];
+    uint32_t ksr, vsr, vmr;   // bf16: key scale (group lane / 8, token lane % 8), value scale and minimum of token lane % 8
+    uint2 kmr;                // key minima of token lane % 8
+    bool sdead = false, sbad = false;
+    int id = 0;
+    size_t at[3];   // the octet in tiles st + 1, st + 2, st + 3: its first token in the head's cache
+    auto words = [](const uint8_t* p, uint32_t(&w)[E]) {
+        if constexpr (E == 4) {
+            const uint4 x = ld16(p);
+            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        } else if constexpr (E == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            w[0] = x.x, w[1] = x.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+    };
+    auto next_id = [&](int st) {   // the table's entry for the octet (any in-bounds entry past the row's end)
+        id = a.table[static_cast<size_t>(b) * a.max_pages + min((kTile * (first_tile + st) + 8 * wv) >> a.page_shift, a.max_pages - 1)];
+    };
+    auto k_load = [&](int st) {
+        const int tok = kTile * (first_tile + st) + 8 * wv, page = __builtin_amdgcn_readfirstlane(id);
+        sdead = tok >= seen;
+        sbad = !sdead && (page < 0 || page >= a.c.pages);
+        at[0] = at[1];
+        at[1] = at[2];
+        at[2] = (static_cast<size_t>(static_cast<uint32_t>(sdead || sbad ? 0 : page)) * a.c.heads + h) * a.c.page +
+                static_cast<uint32_t>(tok & (a.c.page - 1));
+        words(a.c.k + at[2] * (D / 2) + (lane & 7) * (D / 2) + (lane >> 3) * (4 * E), kr);
+        ksr = a.c.ks[at[2] * NG + lane % (8 * NG)];
+        const uint16_t* m = a.c.km + (at[2] + (lane & 7)) * NG;
+        if constexpr (NG == 4)
+            kmr = *reinterpret_cast<const uint2*>(m);
+        else
+            kmr = make_uint2(NG == 2 ? *reinterpret_cast<const uint32_t*>(m) : *m, 0u);
+        vsr = a.c.vs[at[2] + (lane & 7)];
+        vmr = a.c.vm[at[2] + (lane & 7)];
+    };
+    auto v_load = [&](int n) {   // n: how many tiles behind the keys
+        words(a.c.v + at[2 - n] * (D / 2) + lane * (4 * E), vr);
+    };
+    const int ktok = 8 * wv + (lane & 7), rho = (ktok & 16) + 8 * ((ktok >> 2) & 1) + 4 * ((ktok >> 3) & 1) + (ktok & 3);
+    auto k_put = [&](int st, int j) {   // word E (lane / 8) + j of the token's row: its place among [4][NG][2]
+        const int w = E * (lane >> 3) + j, dims = 4 * ((w % (2 * NG)) >> 1) + w / (2 * NG);
+        ks[st & 1][dims][32 * (w & 1) + rho] = codes8<0>(kr[j], magic);
+    };
+    auto v_put = [&](int st, int j) {   // dim 32 E m + E row + j is row `row` of value tile E m + j
+        vs[st & 1][E * g + j][wv >> 1][32 * (wv & 1) + col] = codes8<8>(vr[j], magic);
+    };
+    auto s_put = [&](int st) {
+        const float s = sbad ? __builtin_nanf("") : sdead ? 0.f : bf16_value(static_cast<uint16_t>(ksr));
+        if (lane < 8 * NG) kscale[st & 3][lane >> 3][8 * wv + (lane & 7)] = s;
+        if (lane < 8) {
+            const float scale = sdead ? 0.f : bf16_value(static_cast<uint16_t>(vsr));
+            kmin[st & 3][rho] = sdead ? make_uint2(0u, 0u) : kmr;
+            vtok[st & 3][0][ktok] = scale;
+            vtok[st & 3][1][ktok] = sdead ? 0.f : __builtin_fmaf(8.0f, scale, bf16_value(static_cast<uint16_t>(vmr)));
+            vtok[st & 3][2][ktok] = log2_over(0.f, sizes2(vsr, vmr) & 0xffffu) - (127.0f + kWeightUp);
+        }
+    };
+    auto k_store = [&](int st) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = 0.f;
-    constexpr int U = 4;   // pieces in flight
-    for (int p0 = wv; p0 < in.y; p0 += U * NW) {
-        float2 st[U];
-        float x[U][V];
+        for (int j = 0; j < E; ++j) k_put(st, j);
+        s_put(st);
+    };
+    auto barrier = []() {   // LDS is written and read; the loads stay in flight
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if (steps > 0) {
+        next_id(0);
+        at[1] = at[2] = 0;
+        k_load(0);
+        next_id(1);
+        v_load(0);
+    }
+    // the row's query, times 2^e, in two parts: dims 16 d + 8 g + 0..7 of depth d; and its groups' sums in three bf16 parts:
+    // depth 8 g + e has part 2 g + e / 4 of group e % 4
+    f16x8_t Qh[ND], Ql[ND];
+    bf16x8_t Qs;
+    float factor;
+    {
+        const float* q = a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D + 8 * g;
+        float f[ND][8];   // all of it requested before the first is looked at
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const size_t q = static_cast<size_t>(first + min(p0 + u * NW, in.y - 1)) * kRows + slot;
-            st[u] = a.stat[q];
-            const float* p = a.part + q * D + V * lane;
-            if constexpr (V == 4) {
-                const float4 y = ld4(p);
-                x[u][0] = y.x, x[u][1] = y.y, x[u][2] = y.z, x[u][3] = y.w;
-            } else {
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int i = 0; i < V; ++i) x[u][i] = p[i];
+            for (int i = 0; i < 2; ++i) {
+                const float4 x = ld4(q + 16 * d + 4 * i);
+                f[d][4 * i] = x.x, f[d][4 * i + 1] = x.y, f[d][4 * i + 2] = x.z, f[d][4 * i + 3] = x.w;
+            }
+        float m = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                m = fmaxf(m, fabsf(f[d][i]));
+                bad |= !(fabsf(f[d][i]) <= FLT_MAX);
+            }
+        if (bad) m = INFINITY;
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const bool ok = m <= FLT_MAX;
+        int e = 0;
+        if (m > 0.f && ok) {
+            int em;
+            frexpf(m, &em);
+            e = 15 - em;
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = ok ? ldexpf(f[d][i], e) : 0.f;
+                Qh[d][i] = static_cast<_Float16>(v);
+                Ql[d][i] = static_cast<_Float16>(low_part(v));
+                sum[d >> 2] += v;
             }
         }
-        __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (p0 + u * NW >= in.y) break;
-            const float now = fmaxf(m, st[u].x);
-            const float was = __builtin_amdgcn_exp2f(m - now), f = __builtin_amdgcn_exp2f(st[u].x - now);
-            m = now;
-            l = l * was + st[u].y * f;
+        for (int i = 0; i < 4; ++i) {
+            if (i < NG) sum[i] += __shfl_xor(sum[i], 32);
+            const float p0 = bf16_part(sum[i], 0), p1 = bf16_part(sum[i], 1), p2 = bf16_part(sum[i], 2);
+            Qs[i] = static_cast<__bf16>(g ? p2 : p0);
+            Qs[4 + i] = static_cast<__bf16>(g ? 0.f : p1);
+        }
+        factor = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");
 #pragma unroll
-            for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
+        for (int d = 0; d < ND; ++d) {   // only products read them: accumulation registers, the others are full
+            asm("" : "+a"(Qh[d]));
+            asm("" : "+a"(Ql[d]));
         }
     }
+    f32x16_t acc[DT];
 #pragma unroll
-    for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
-    if (lane == 0) {
-        ms[wv] = m;
-        ls[wv] = l;
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    float mu = -FLT_MAX, l = 0.f, low = 0.f;
+    f32x16_t zero;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+    f32x16_t S, N;          // a tile's scores; the next tile's, so far
+    f32x16_t T[2];          // products of a group, of the one before
+    float kv[2][16];        // their scales
+    f16x8_t Wh[2], Wl[2];   // weights of the last tile
+    // 16 numbers of a lane's tokens, from an array over the tile's tokens
+    auto of_tokens = [&](const float* p, float(&x)[16]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float4 y = ld4(p + 16 * s + 8 * g + 4 * i);
+                float* o = x + 8 * s + 4 * i;
+                o[0] = y.x, o[1] = y.y, o[2] = y.z, o[3] = y.w;
+            }
+    };
+    // The operands of a step's products are one sequence, the last tile's values (2 DT of them), then the next tile's keys
+    // (ND = 2 DT); each is requested AP products' pairs ahead, into the register that the one before it has left. fill(i) goes
+    // between the two products of an operand and after them.
+    constexpr int AP = 4;
+    f16x8_t A[AP];
+    auto value_at = [&](int slot, int k) { return vs[slot][k >> 1][k & 1][lane]; };
+    auto key_at = [&](int slot, int d) { return ks[slot][d][lane]; };
+    auto minima = [&](int tile) {   // depth 8 g + e: group e % 4
+        const uint2 m = kmin[tile & 3][col];
+        return __builtin_bit_cast(bf16x8_t, u32x4_t{m.x, m.y, m.x, m.y});
+    };
+    // Scores of `tile` into N and, of the last group, T and kv. ahead(d): what to request when operand d has been taken.
+    auto scores = [&](int tile, const bf16x8_t mins, auto&& ahead, auto&& fill) {
+        static_for<ND>([&](auto dI) {
+            constexpr int d = decltype(dI)::value, gr = d >> 2;
+            const f16x8_t x = A[d % AP];
+            auto scaled = [&](int place) {   // two of the group before, at each of 8 places
+                if constexpr (gr > 0) {
+#pragma unroll
+                    for (int i = 2 * place; i < 2 * place + 2; ++i) N[i] = __builtin_fmaf(T[(gr - 1) & 1][i], kv[(gr - 1) & 1][i], N[i]);
+                }
+            };
+            if constexpr (d == 0) N = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mins, Qs, zero, 0, 0, 0);
+            T[gr & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Qh[d], (d & 3) == 0 ? zero : T[gr & 1], 0, 0, 0);
+            if constexpr ((d & 3) == 0) of_tokens(kscale[tile & 3][gr], kv[gr & 1]);
+            scaled(2 * (d & 3));
+            fill(IC<2 * d>{});
+            __builtin_amdgcn_sched_barrier(0);
+            T[gr & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Ql[d], T[gr & 1], 0, 0, 0);
+            ahead(dI);
+            scaled(2 * (d & 3) + 1);
+            fill(IC<2 * d + 1>{});
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto values = [&](auto&& ahead, auto&& fill) {
+        static_for<ND>([&](auto kI) {
+            constexpr int k = decltype(kI)::value, d = k >> 1, s = k & 1;
+            const f16x8_t x = A[k % AP];
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Wh[s], acc[d], 0, 0, 0);
+            fill(IC<2 * k>{});
+            __builtin_amdgcn_sched_barrier(0);
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Wl[s], acc[d], 0, 0, 0);
+            ahead(kI);
+            fill(IC<2 * k + 1>{});
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    for (int i = tid; i < DT * 2 * kWave; i += NTH) (&vs[1][0][0][0])[i] = f16x8_t{};   // the values before the first tile
+#pragma unroll
+    for (int s = 0; s < 2; ++s) Wh[s] = Wl[s] = f16x8_t{};
+    if (steps > 0) {
+        k_store(0);
+        k_load(1);
+        next_id(2);
+        barrier();
+        static_for<AP>([&](auto dI) { A[decltype(dI)::value] = key_at(0, decltype(dI)::value); });
+        scores(0, minima(0), [&](auto dI) {
+            constexpr int d = decltype(dI)::value;
+            if constexpr (d + AP < ND) A[d % AP] = key_at(0, d + AP);
+        }, [](auto) {});
+        k_store(1);
+        k_load(2);
+        next_id(3);
     }
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += NW * kWave) {
-        float top = ms[0];
+    barrier();
 #pragma unroll
-        for (int w = 1; w < NW; ++w) top = fmaxf(top, ms[w]);
-        float sum = 0.f, tot = 0.f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = __builtin_amdgcn_exp2f(ms[w] - top);
-            sum += f * sums[w][d];
-            tot += f * ls[w];
+    for (int k = 0; k < AP; ++k) A[k] = value_at(1, k);
+    // Step st: tile st's scores are in N, T and kv. Its values and the keys of st + 2 go to LDS (slots whose last readers passed
+    // the barrier before); the values of st - 1 are summed beside that and beside the last scaling and the maximum of the scores,
+    // the scores of st + 1 beside the exponentials. One step more than tiles; before the first the weights are zero.
+    constexpr int LG = (NG - 1) & 1;
+    float sv[16], mv[16], sz[16], top = 0.f, w0 = 0.f;
+    auto scale_max = [&](int i) {
+        S[i] = __builtin_fmaf(T[LG][i], kv[LG][i], N[i]) * factor;
+        const float z = S[i] + sz[i];
+        top = i ? fmaxf(top, z) : z;
+        asm volatile("" : "+v"(S[i]), "+v"(top));   // here, not where they are used
+    };
+    auto weight = [&](int i) {
+        const float p = __builtin_amdgcn_exp2f(S[i] - mu);
+        l += p;
+        low = __builtin_fmaf(p, mv[i], low);
+        const float w = rounded(p * sv[i]);
+        if (i & 1) {
+            Wh[i >> 3][(i & 7) - 1] = static_cast<_Float16>(w0);
+            Wh[i >> 3][i & 7] = static_cast<_Float16>(w);
+            Wl[i >> 3][(i & 7) - 1] = static_cast<_Float16>(low_part(w0));
+            Wl[i >> 3][i & 7] = static_cast<_Float16>(low_part(w));
         }
-        const size_t o = static_cast<size_t>(pair) * D + d;
-        a.out[o] = finished(a, top, sum, tot, o);
+        w0 = w;
+    };
+    for (int st = 0; steps > 0 && st <= steps; ++st) {
+        bf16x8_t mins;
+        {
+            constexpr int SLOTS = 4 * DT, PER = 32 / SLOTS;   // places between products; scores at a place of the second half
+            values([&](auto kI) {
+                constexpr int k = decltype(kI)::value;
+                A[k % AP] = k + AP < ND ? value_at((st + 1) & 1, k + AP) : key_at((st + 1) & 1, k + AP - ND);
+            }, [&](auto kI) {
+                constexpr int k = decltype(kI)::value;
+                constexpr int EVERY = SLOTS / (4 * E);   // a word to LDS at every so many places of the first half
+                if constexpr (k < SLOTS / 2 && k % EVERY == 0) {
+                    if constexpr ((k / EVERY) & 1)
+                        k_put(st + 2, (k / EVERY) >> 1);
+                    else
+                        v_put(st, (k / EVERY) >> 1);
+                }
+                if constexpr (k == SLOTS / 2 - 1) of_tokens(vtok[st & 3][2], sz);
+                if constexpr (k == SLOTS / 2) {
+                    s_put(st + 2);
+                    v_load(1);
+                }
+                if constexpr (k == SLOTS / 2 + 2) {
+                    k_load(st + 3);
+                    next_id(st + 4);
+                }
+                if constexpr (k >= SLOTS / 2) {
+#pragma unroll
+                    for (int i = (k - SLOTS / 2) * PER; i < (k - SLOTS / 2 + 1) * PER; ++i) scale_max(i);
+                }
+                if constexpr (k == SLOTS - 2) {
+                    of_tokens(vtok[st & 3][0], sv);
+                    of_tokens(vtok[st & 3][1], mv);
+                    mins = minima(st + 1);
+                }
+            });
+        }
+        {
+            const int t0 = kTile * (first_tile + st);
+            if (t0 + kTile - 1 > wave_first || st == steps) {   // past the piece's last tile nothing is seen
+                const int last = st == steps ? -1 : limit;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (t0 + 16 * (i >> 3) + 8 * g + (i & 7) > last) {   // what lies there is anything: no 0 * NaN
+                        S[i] = -INFINITY;
+                        sv[i] = mv[i] = 0.f;
+                    }
+                    const float z = S[i] + sz[i];
+                    top = i ? fmaxf(top, z) : z;
+                }
+            }
+            if (__ballot(top > mu + kMoves)) {
+                const float now = fmaxf(mu, fmaxf(top, __shfl_xor(top, 32)));
+                const float shrink = __builtin_amdgcn_exp2f(mu - now);
+                mu = now;
+                l *= shrink;
+                low *= shrink;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
+            }
+            // (past the wave's last tile these scores are of an old one, and unused)
+            scores(st + 1, mins, [&](auto dI) {
+                constexpr int d = decltype(dI)::value;
+                if constexpr (d + AP < ND) A[d % AP] = key_at((st + 1) & 1, d + AP);
+                // The tile's keys have been read, its values and the next keys are written: the next values can be read.
+                if constexpr (d == ND - 2) {
+                    barrier();
+#pragma unroll
+                    for (int k = 0; k < AP - 1; ++k) A[k] = value_at(st & 1, k);
+                }
+                if constexpr (d == ND - 1) A[AP - 1] = value_at(st & 1, AP - 1);
+            }, [&](auto kI) {
+                constexpr int k = decltype(kI)::value, PLACES = 2 * ND;
+#pragma unroll
+                for (int i = k * 16 / PLACES; i < (k + 1) * 16 / PLACES; ++i) weight(i);
+            });
+        }
+    }
+    l += __shfl_xor(l, 32);
+    low += __shfl_xor(low, 32);
+    if (row0 + col >= pairs) return;
+    if (r.bad) l = __builtin_nanf("");
+    const size_t o = (static_cast<size_t>(r.first + ti) * a.heads + head) * D;
+    // 4 neighbouring dims, the n-th of DT * 4: of E value tiles of one register, or 2 of two, or one of four
+    auto four = [&](int n, int& dim) {
+        const int m = n * 4 / (16 * E), rest = n - m * 4 * E;   // tile group; 4 registers' 16 rows x E dims as 4 E fours
+        float x[4];
+        if constexpr (E == 4) {
+            const int i = rest;   // register
+            dim = 128 * m + 4 * (8 * (i >> 2) + 4 * g + (i & 3));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[4 * m + e][i];
+        } else if constexpr (E == 2) {
+            const int i = 2 * rest;
+            dim = 64 * m + 2 * (8 * (i >> 2) + 4 * g + (i & 3));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[2 * m + (e & 1)][i + (e >> 1)];
+        } else {
+            const int i = 4 * rest;
+            dim = 32 * m + 8 * (i >> 2) + 4 * g;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[m][i + e];
+        }
+        return make_float4(x[0] + low, x[1] + low, x[2] + low, x[3] + low);
+    };
+    constexpr int FOURS = D / 8;   // of a lane: half of its row
+    if (pieces > 1) {   // row k of the tile is slot k % kRows of item first + k / kRows * splits + piece, as the join reads
+        const int k = 32 * wv + col;
+        const int unit_items = static_cast<int>(blockIdx.x) / splits * (kPromptRows / kRows);
+        const int item0 = a.items + (unit_items + k / kRows) * splits;
+        const size_t row = static_cast<size_t>(item0 + split) * kRows + k % kRows;
+#pragma unroll
+        for (int n = 0; n < FOURS; ++n) {
+            int dim;
+            const float4 x = four(n, dim);
+            st4(a.part + row * D + dim, x);
+        }
+        if (g == 0) {
+            a.stat[row] = make_float2(mu, l);
+            if (split == 0) a.info[o / D] = make_int2(item0 * kRows + k % kRows, pieces);
+        }
+        return;
+    }
+    const bool none = mu == -FLT_MAX && l == 0.f;
+    const float inv = 1.f / l;
+    constexpr int BATCH = 8;   // gates requested together
+#pragma unroll
+    for (int n0 = 0; n0 < FOURS; n0 += BATCH) {
+        float4 x[BATCH], gt[BATCH];
+        int dim[BATCH];
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            x[n] = four(n0 + n, dim[n]);
+            if (a.gate) gt[n] = ld4(a.gate + o + dim[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < BATCH; ++n) {
+            float v[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = none ? 0.f : v[i] * inv;
+            if (a.gate) {
+                v[0] *= sigmoid(gt[n].x);
+                v[1] *= sigmoid(gt[n].y);
+                v[2] *= sigmoid(gt[n].z);
+                v[3] *= sigmoid(gt[n].w);
+            }
+            st4(a.out + o + dim[n], make_float4(v[0], v[1], v[2], v[3]));
+        }
+    }
+    if (g == 0) a.info[o / D] = make_int2(0, 1);
+}
+
+// ------------------------------------------------------------------ join
+// Joins the pieces of (row, head) pairs. NW > 1: a workgroup of NW waves per pair, wave w takes pieces w, w + NW, ...; NW = 1: a
+// wave per pair, and each wave looks at `per` pairs at once, because in a prompt's call most are there already. Lanes hold the
+// dims.
+template <int D, int NW>
+__global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel(const Attn4Args a, int per) {
+    constexpr int V = D / kWave;
+    __shared__ float sums[NW][NW == 1 ? 1 : D], ls[NW], ms[NW];
+    const int lane = threadIdx.x & 63, wv = NW == 1 ? 0 : wave_in_block();
+    // Pairs of the requests' rows alone: only those have an entry of this call (the workspace may hold an earlier one's).
+    const int from = min(max(a.row_start[0], 0), a.rows) * a.heads, live = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;
+    const int64_t pair0 = NW == 1 ? (static_cast<int64_t>(blockIdx.x) * 4 + wave_in_block()) * per : blockIdx.x;
+    int2 in = make_int2(0, 0);
+    if (lane < (NW == 1 ? per : 1) && pair0 + lane >= from && pair0 + lane < live) in = a.info[pair0 + lane];
+    // one piece is there already; starts that decrease may leave anything
+    uint64_t todo = __ballot(in.y > 1 && in.x >= 0 && in.y <= a.all_items - in.x / kRows);   // the same in every wave of a pair
+    while (todo) {
+        const int k = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int pieces = __builtin_amdgcn_readlane(in.y, k), where = __builtin_amdgcn_readlane(in.x, k);
+        const int slot = where % kRows, first = where / kRows;
+        float m = -FLT_MAX, l = 0.f, s[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] = 0.f;
+        constexpr int U = NW == 16 ? 16 : 4;   // pieces in flight
+        for (int p0 = wv; p0 < pieces; p0 += U * NW) {
+            float2 st[U];
+            float x[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const size_t q = static_cast<size_t>(first + min(p0 + u * NW, pieces - 1)) * kRows + slot;
+                st[u] = a.stat[q];
+                const float* p = a.part + q * D + V * lane;
+                if constexpr (V == 4) {
+                    const float4 y = ld4(p);
+                    x[u][0] = y.x, x[u][1] = y.y, x[u][2] = y.z, x[u][3] = y.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) x[u][i] = p[i];
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p0 + u * NW >= pieces) break;
+                const float now = fmaxf(m, st[u].x);
+                const float was = __builtin_amdgcn_exp2f(m - now), f = __builtin_amdgcn_exp2f(st[u].x - now);
+                m = now;
+                l = l * was + st[u].y * f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
+            }
+        }
+        const size_t o = static_cast<size_t>(pair0 + k) * D;
+        if constexpr (NW == 1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) a.out[o + V * lane + i] = finished(a, m, s[i], l, o + V * lane + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
+            if (lane == 0) {
+                ms[wv] = m;
+                ls[wv] = l;
+            }
+            __syncthreads();
+            for (int d = threadIdx.x; d < D; d += NW * kWave) {
+                float top = ms[0];
+#pragma unroll
+                for (int w = 1; w < NW; ++w) top = fmaxf(top, ms[w]);
+                float sum = 0.f, tot = 0.f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(ms[w] - top);
+                    sum += f * sums[w][d];
+                    tot += f * ls[w];
+                }
+                a.out[o + d] = finished(a, top, sum, tot, o + d);
+            }
+        }
     }
 }
 
 // ------------------------------------------------------------------ host
+// Whether a call can have requests for prompt4_kernel; if not, split4_kernel takes them all. A call with no more rows than
+// requests is taken for a batch of single tokens, up to kSplitOnly (row, head) pairs of a KV head, and spared the launch;
+// should one request have all the rows, split4_kernel answers it too.
+bool may_prompt(int rows, int requests, int group) {
+    const int64_t pairs = static_cast<int64_t>(rows) * group;
+    return rows > 1 && pairs > kSplitMax && (rows > requests || pairs > kSplitOnly);
+}
 // split4_kernel's workgroups of 4 waves on a CU, by their registers.
 int places_on_cu(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
 constexpr int kCus = 256;
 // Its pieces are at most as many as wanted (and a few for rounding) plus one per unit; units at most one per 8 pairs plus one
-// per request that has rows.
+// per request that has rows, and, where larger requests go to prompt4_kernel, at most one per 8 of the pairs with which one does
+// not (plus one, so that the bound does not fall where the first request goes there).
 int64_t item_bound(int rows, int requests, int heads, int kv_heads, int dim) {
-    const int64_t pairs = static_cast<int64_t>(rows) * (heads / kv_heads), places = kCus * places_on_cu(dim);
-    const int64_t units = (pairs / kRows + std::min(rows, requests)) * kv_heads;
+    const int group = heads / kv_heads;
+    const int64_t pairs = static_cast<int64_t>(rows) * group, places = kCus * places_on_cu(dim), busy = std::min(rows, requests);
+    int64_t units = pairs / kRows + busy;
+    if (may_prompt(rows, requests, group)) units = std::min(units, busy * (blocks_for(std::max(kSplitMax, group), kRows) + 1));
+    units *= kv_heads;
     return (units > places ? 4 : 1) * places + 8 + units;
 }
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
 struct Layout {
-    int64_t items;
+    int64_t items, all;   // pieces of 8 rows: of split4_kernel, and with those of prompt4_kernel
     size_t stat, info, bytes;
 };
 Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     Layout l;
     l.items = item_bound(rows, requests, heads, kv_heads, dim);
-    l.stat = align_up(static_cast<size_t>(l.items) * kRows * dim * 4);
-    l.info = l.stat + align_up(static_cast<size_t>(l.items) * kRows * 8);
+    l.all = l.items;
+    // Room for cut prompts by the rows alone, though a call with no more rows than requests has none: a workspace for some
+    // rows and requests has to serve fewer of either.
+    if (rows > 1 && static_cast<int64_t>(rows) * (heads / kv_heads) > kSplitMax) l.all += kPromptFill * (kPromptRows / kRows);
+    l.stat = align_up(static_cast<size_t>(l.all) * kRows * dim * 4);
+    l.info = l.stat + align_up(static_cast<size_t>(l.all) * kRows * 8);
     l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);
     return l;
 }
@@ -734,11 +1262,20 @@ template <int D>
 void launch(const Attn4Args& a, hipStream_t s) {
     const auto split = a.c.page >= kTile ? split4_kernel<D, true> : split4_kernel<D, false>;
     split<<<static_cast<unsigned>(a.items), kSplitBlock, 0, s>>>(a);
+    if (!a.split_all) {
+        const int64_t pairs = static_cast<int64_t>(a.rows) * a.group;
+        const int64_t tiles = (pairs / kPromptRows + std::min<int64_t>(a.requests, pairs / kSplitMax + 1)) * a.c.heads;
+        prompt4_kernel<D><<<static_cast<unsigned>(std::max<int64_t>(tiles, kPromptFill)), kPromptWaves * kWave, 0, s>>>(a);
+    }
     const unsigned pairs = static_cast<unsigned>(a.rows) * static_cast<unsigned>(a.heads);
     if (pairs <= 128)   // few rows: many pieces each
-        join4_kernel<D, 16><<<pairs, 16 * kWave, 0, s>>>(a);
+        join4_kernel<D, 16><<<pairs, 16 * kWave, 0, s>>>(a, 1);
+    else if (pairs <= 2048)
+        join4_kernel<D, 4><<<pairs, 4 * kWave, 0, s>>>(a, 1);
+    else if (pairs <= kPromptFill / 2 * kPromptRows)   // a cut prompt's pairs may all have pieces
+        join4_kernel<D, 1><<<blocks_for(pairs, 4), 4 * kWave, 0, s>>>(a, 1);
     else
-        join4_kernel<D, 4><<<pairs, 4 * kWave, 0, s>>>(a);
+        join4_kernel<D, 1><<<blocks_for(pairs, 16), 4 * kWave, 0, s>>>(a, 4);
 }
 
 }  // namespace
@@ -799,6 +1336,8 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     a.stat = reinterpret_cast<float2*>(ws + l.stat);
     a.info = reinterpret_cast<int2*>(ws + l.info);
     a.items = static_cast<int>(l.items);
+    a.all_items = static_cast<int>(l.all);
+    a.split_all = !may_prompt(rows, requests, a.group);
     a.places = kCus * places_on_cu(dim);
     const hipStream_t s = as_stream(stream);
     if (dim == 64)
