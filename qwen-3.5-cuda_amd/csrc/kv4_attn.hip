@@ -55,6 +55,7 @@ constexpr int kMinTiles = 4;           // of a piece
 constexpr int kMaxItems = 1 << 24;     // more than any call has
 constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take split4_kernel; a row does
 constexpr int kSplitOnly = 1024;       // and of a whole call that has no more rows than requests
+constexpr int kMaxUp = 110;             // tiny queries are taken times 2^110 at most, so that what undoes it is a normal number
 constexpr float kMoves = 8.0f;         // a token past the reference by more moves it
 constexpr float kWeightUp = 10.0f;     // log2 of what exponentials, and so all sums, are taken times: weights fill fp16
 
@@ -237,7 +238,8 @@ __device__ __forceinline__ float rounded(float v) {
     asm("" : "+v"(v));
     return v;
 }
-__device__ __forceinline__ float low_part(float v) { return v - static_cast<float>(static_cast<_Float16>(v)); }
+// (exact; as an fma of the half number one instruction with its conversion)
+__device__ __forceinline__ float low_part(float v) { return __builtin_fmaf(static_cast<float>(static_cast<_Float16>(v)), -1.0f, v); }
 __device__ __forceinline__ float bf16_part(float v, int part) {   // bf16 part 0, 1, 2 of v, as an fp32 number
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
         if (m > 0.f && ok) {
             int em;
             frexpf(m, &em);
-            e = 15 - em;
+            e = min(15 - em, kMaxUp);
         }
         float s = 0.f;
         const int d0 = (lane & 31) * QN;
@@ -648,10 +650,14 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
 // Bound by the matrix products. 128 rows a workgroup, 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: codes are
 // turned to fp16 once per workgroup, into LDS, and an operand of keys or values, 1 KB of LDS, feeds 2 products (both parts of
 // 32 rows). A wave holds its rows' query parts (128 registers at D = 256, pinned in accumulation registers) and sums (128).
-// Its vector work - scales, softmax, turning codes to fp16 - is laid between its own products: while tile t + 1's scores are
-// computed, tile t's are exponentiated and each group's products are scaled beside the next group's; while tile t's values
-// are summed, the codes of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own rows may end
+// Its vector work - softmax, turning codes to fp16 - is laid between its own products: while tile t + 1's scores are computed,
+// tile t's are exponentiated; while tile t's values are summed, the codes of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own rows may end
 // one earlier: with a branch around the products the compiler moves the sums between register files at each.
+// The keys' scales are in the operand: code - 8 has at most 3 bits and a bf16 scale 8, so scale (code - 8) is an fp16 number, and
+// all dims of a head are one sum. What is left of a key, min + 8 scale of each group times the sum of its queries, is two
+// products more, of bf16 numbers (the minima, 8 scale) with the sums' three parts. A token's numbers are taken times a power of
+// two that brings the largest max(16 scale, |min|) of its groups below 2^16; the scores are multiplied by its inverse. (Each
+// group's products scaled by themselves, in fp32, took 64 fmas a lane and tile and 64 registers: 522 us at 5000 rows.)
 // The scores^T tile has token rho = 8 b + 4 g + j of the 32 in register 4 b + j of lane half g; key row rho stands for token
 // 16 (b / 2) + 8 g + 4 (b % 2) + j, so that a lane's registers 8 s .. 8 s + 7 are octet 2 s + g, its share of the second
 // product's depth s.
@@ -677,11 +683,11 @@ __device__ __forceinline__ void static_for(F&& f) {
 template <int D>
 __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const Attn4Args a) {
     constexpr int ND = D / 16, DT = D / 32, NG = D / 64, E = D / 64, NTH = kPromptWaves * kWave;   // E: a lane's words of a tile's
-    __shared__ __align__(16) f16x8_t ks[2][ND][kWave];                                             // keys, and of its values
+    constexpr int GL = D == 256 ? 2 : 1;                                                           // keys, and of its values;
+    __shared__ __align__(16) f16x8_t ks[2][ND][kWave];                                             // GL: groups of those words
     __shared__ __align__(16) f16x8_t vs[2][DT][2][kWave];
-    __shared__ __align__(16) float kscale[4][NG][kTile];   // [tile % 4][group][token]
-    __shared__ __align__(16) uint2 kmin[4][kTile];         // [tile % 4][key row]: 4 bf16, of groups past the last 0
-    __shared__ __align__(16) float vtok[4][3][kTile];      // [tile % 4][scale, min + 8 scale, log2 size][token]
+    __shared__ __align__(16) uint16_t kmin[4][kTile][8];   // [tile % 4][key row]: bf16, the groups' minima (4) and 8 scale (4)
+    __shared__ __align__(16) float tok[4][4][kTile];       // [tile % 4][key factor, value scale, min + 8 scale, log2 size][token]
     // which request, KV head and row tile: the last row tiles (the longest rows) first
     const int G = a.group, lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
     const float per_g = 1.0f / static_cast<float>(G);
@@ -732,8 +738,11 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     // (token lane % 8, words E (lane / 8) .. of its row), of values (dims E lane ..). Octets past the last are loaded from page 0 and
     // never read from LDS. Page ids are read a tile ahead of the codes they lead to.
     uint32_t kr[E], vr[E];
-    uint32_t ksr, vsr, vmr;   // bf16: key scale (group lane / 8, token lane % 8), value scale and minimum of token lane % 8
-    uint2 kmr;                // key minima of token lane % 8
+    // bf16, of token lane % 8: the key scales of the lane's words, value scale and minimum, and its element of the token's row of
+    // kmin (the minimum of group lane / 8, from lane 32 on the scale of group lane / 8 - 4)
+    uint32_t ksr[GL], vsr, vmr, own;
+    const int piece = lane >> 3, own_group = piece & 3;
+    const uint16_t* own_at = piece < 4 ? a.c.km + (lane & 7) * NG + min(own_group, NG - 1) : a.c.ks + 8 * min(own_group, NG - 1) + (lane & 7);
     bool sdead = false, sbad = false;
     int id = 0;
     size_t at[3];   // the octet in tiles st + 1, st + 2, st + 3: its first token in the head's cache
@@ -760,12 +769,9 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         at[2] = (static_cast<size_t>(static_cast<uint32_t>(sdead || sbad ? 0 : page)) * a.c.heads + h) * a.c.page +
                 static_cast<uint32_t>(tok & (a.c.page - 1));
         words(a.c.k + at[2] * (D / 2) + (lane & 7) * (D / 2) + (lane >> 3) * (4 * E), kr);
-        ksr = a.c.ks[at[2] * NG + lane % (8 * NG)];
-        const uint16_t* m = a.c.km + (at[2] + (lane & 7)) * NG;
-        if constexpr (NG == 4)
-            kmr = *reinterpret_cast<const uint2*>(m);
-        else
-            kmr = make_uint2(NG == 2 ? *reinterpret_cast<const uint32_t*>(m) : *m, 0u);
+#pragma unroll
+        for (int j = 0; j < GL; ++j) ksr[j] = a.c.ks[at[2] * NG + 8 * ((GL * piece + j) % NG) + (lane & 7)];
+        own = own_at[at[2] * NG];
         vsr = a.c.vs[at[2] + (lane & 7)];
         vmr = a.c.vm[at[2] + (lane & 7)];
     };
@@ -773,25 +779,43 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         words(a.c.v + at[2 - n] * (D / 2) + lane * (4 * E), vr);
     };
     const int ktok = 8 * wv + (lane & 7), rho = (ktok & 16) + 8 * ((ktok >> 2) & 1) + 4 * ((ktok >> 3) & 1) + (ktok & 3);
+    // The token's power of two, over its 8 lanes, and the lane's scales with it.
+    int up = 0;
+    _Float16 scale16[GL];
+    auto k_scale = [&]() {
+        uint32_t z = own_group < NG ? (piece < 4 ? own & 0x7fffu : own + 0x0200u) : 0u;   // |min|, 16 scale
+        z = max(z, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(z), 0x128, 0xF, 0xF, false)));   // row_ror 8
+        const auto x = __builtin_amdgcn_permlane16_swap(z, z, false, false);
+        z = max(x[0], x[1]);
+        const auto y = __builtin_amdgcn_permlane32_swap(z, z, false, false);
+        up = 142 - max(static_cast<int>(max(y[0], y[1]) >> 7), 20);
+#pragma unroll
+        for (int j = 0; j < GL; ++j) scale16[j] = static_cast<_Float16>(ldexpf(bf16_value(static_cast<uint16_t>(ksr[j])), up));
+    };
     auto k_put = [&](int st, int j) {   // word E (lane / 8) + j of the token's row: its place among [4][NG][2]
-        const int w = E * (lane >> 3) + j, dims = 4 * ((w % (2 * NG)) >> 1) + w / (2 * NG);
-        ks[st & 1][dims][32 * (w & 1) + rho] = codes8<0>(kr[j], magic);
+        const int w = E * piece + j, dims = 4 * ((w % (2 * NG)) >> 1) + w / (2 * NG);
+        const _Float16 f = scale16[GL == 2 ? j >> 1 : 0];
+        ks[st & 1][dims][32 * (w & 1) + rho] = codes8<8>(kr[j], magic) * f16x8_t{f, f, f, f, f, f, f, f};
     };
     auto v_put = [&](int st, int j) {   // dim 32 E m + E row + j is row `row` of value tile E m + j
         vs[st & 1][E * g + j][wv >> 1][32 * (wv & 1) + col] = codes8<8>(vr[j], magic);
     };
     auto s_put = [&](int st) {
-        const float s = sbad ? __builtin_nanf("") : sdead ? 0.f : bf16_value(static_cast<uint16_t>(ksr));
-        if (lane < 8 * NG) kscale[st & 3][lane >> 3][8 * wv + (lane & 7)] = s;
+        const float mine = own_group < NG ? ldexpf(bf16_value(static_cast<uint16_t>(own)), piece < 4 ? up : up + 3) : 0.f;
+        kmin[st & 3][rho][piece] = static_cast<uint16_t>(__float_as_uint(mine) >> 16);
         if (lane < 8) {
-            const float scale = sdead ? 0.f : bf16_value(static_cast<uint16_t>(vsr));
-            kmin[st & 3][rho] = sdead ? make_uint2(0u, 0u) : kmr;
-            vtok[st & 3][0][ktok] = scale;
-            vtok[st & 3][1][ktok] = sdead ? 0.f : __builtin_fmaf(8.0f, scale, bf16_value(static_cast<uint16_t>(vmr)));
-            vtok[st & 3][2][ktok] = log2_over(0.f, sizes2(vsr, vmr) & 0xffffu) - (127.0f + kWeightUp);
+            // A page outside the cache, or values that are not finite, make the token's scores NaN: of the rows that see it.
+            float scale = bf16_value(static_cast<uint16_t>(vsr)), rest = __builtin_fmaf(8.0f, scale, bf16_value(static_cast<uint16_t>(vmr)));
+            const bool bad = sbad || !(fabsf(rest) <= FLT_MAX);
+            if (sdead || bad) scale = rest = 0.f;
+            tok[st & 3][0][ktok] = bad ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+            tok[st & 3][1][ktok] = scale;
+            tok[st & 3][2][ktok] = rest;
+            tok[st & 3][3][ktok] = log2_over(0.f, sizes2(vsr, vmr) & 0xffffu) - (127.0f + kWeightUp);
         }
     };
     auto k_store = [&](int st) {
+        k_scale();
 #pragma unroll
         for (int j = 0; j < E; ++j) k_put(st, j);
         s_put(st);
@@ -809,9 +833,9 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         v_load(0);
     }
     // the row's query, times 2^e, in two parts: dims 16 d + 8 g + 0..7 of depth d; and its groups' sums in three bf16 parts:
-    // depth 8 g + e has part 2 g + e / 4 of group e % 4
+    // depth 8 g + e has part g of group e % 4, in a second product part 2 + g
     f16x8_t Qh[ND], Ql[ND];
-    bf16x8_t Qs;
+    bf16x8_t Qs[2];
     float factor;
     {
         const float* q = a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D + 8 * g;
@@ -839,7 +863,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         if (m > 0.f && ok) {
             int em;
             frexpf(m, &em);
-            e = 15 - em;
+            e = min(15 - em, kMaxUp);
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -856,8 +880,8 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         for (int i = 0; i < 4; ++i) {
             if (i < NG) sum[i] += __shfl_xor(sum[i], 32);
             const float p0 = bf16_part(sum[i], 0), p1 = bf16_part(sum[i], 1), p2 = bf16_part(sum[i], 2);
-            Qs[i] = static_cast<__bf16>(g ? p2 : p0);
-            Qs[4 + i] = static_cast<__bf16>(g ? 0.f : p1);
+            Qs[0][i] = Qs[0][4 + i] = static_cast<__bf16>(g ? p1 : p0);
+            Qs[1][i] = Qs[1][4 + i] = static_cast<__bf16>(g ? 0.f : p2);
         }
         factor = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");
 #pragma unroll
@@ -875,21 +899,10 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     f32x16_t zero;
 #pragma unroll
     for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-    f32x16_t S, N;          // a tile's scores; the next tile's, so far
-    f32x16_t T[2];          // products of a group, of the one before
-    float kv[2][16];        // their scales
+    f32x16_t S, N;          // a tile's scores over `factor`; the next tile's products
     f16x8_t Wh[2], Wl[2];   // weights of the last tile
-    // 16 numbers of a lane's tokens, from an array over the tile's tokens
-    auto of_tokens = [&](const float* p, float(&x)[16]) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float4 y = ld4(p + 16 * s + 8 * g + 4 * i);
-                float* o = x + 8 * s + 4 * i;
-                o[0] = y.x, o[1] = y.y, o[2] = y.z, o[3] = y.w;
-            }
-    };
+    // the numbers of a lane's tokens 4 j .. 4 j + 3
+    auto of_tokens = [&](const float* p, int j) { return ld4(p + 16 * (j >> 1) + 8 * g + 4 * (j & 1)); };
     // The operands of a step's products are one sequence, the last tile's values (2 DT of them), then the next tile's keys
     // (ND = 2 DT); each is requested AP products' pairs ahead, into the register that the one before it has left. fill(i) goes
     // between the two products of an operand and after them.
@@ -897,30 +910,19 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     f16x8_t A[AP];
     auto value_at = [&](int slot, int k) { return vs[slot][k >> 1][k & 1][lane]; };
     auto key_at = [&](int slot, int d) { return ks[slot][d][lane]; };
-    auto minima = [&](int tile) {   // depth 8 g + e: group e % 4
-        const uint2 m = kmin[tile & 3][col];
-        return __builtin_bit_cast(bf16x8_t, u32x4_t{m.x, m.y, m.x, m.y});
-    };
-    // Scores of `tile` into N and, of the last group, T and kv. ahead(d): what to request when operand d has been taken.
-    auto scores = [&](int tile, const bf16x8_t mins, auto&& ahead, auto&& fill) {
+    auto minima = [&](int tile) { return *reinterpret_cast<const bf16x8_t*>(&kmin[tile & 3][col][0]); };
+    // A tile's products into N. ahead(d): what to request when operand d has been taken.
+    auto scores = [&](const bf16x8_t mins, auto&& ahead, auto&& fill) {
+        N = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mins, Qs[0], zero, 0, 0, 0);
+        N = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mins, Qs[1], N, 0, 0, 0);
         static_for<ND>([&](auto dI) {
-            constexpr int d = decltype(dI)::value, gr = d >> 2;
+            constexpr int d = decltype(dI)::value;
             const f16x8_t x = A[d % AP];
-            auto scaled = [&](int place) {   // two of the group before, at each of 8 places
-                if constexpr (gr > 0) {
-#pragma unroll
-                    for (int i = 2 * place; i < 2 * place + 2; ++i) N[i] = __builtin_fmaf(T[(gr - 1) & 1][i], kv[(gr - 1) & 1][i], N[i]);
-                }
-            };
-            if constexpr (d == 0) N = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mins, Qs, zero, 0, 0, 0);
-            T[gr & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Qh[d], (d & 3) == 0 ? zero : T[gr & 1], 0, 0, 0);
-            if constexpr ((d & 3) == 0) of_tokens(kscale[tile & 3][gr], kv[gr & 1]);
-            scaled(2 * (d & 3));
+            N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Qh[d], N, 0, 0, 0);
             fill(IC<2 * d>{});
             __builtin_amdgcn_sched_barrier(0);
-            T[gr & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Ql[d], T[gr & 1], 0, 0, 0);
+            N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Ql[d], N, 0, 0, 0);
             ahead(dI);
-            scaled(2 * (d & 3) + 1);
             fill(IC<2 * d + 1>{});
             __builtin_amdgcn_sched_barrier(0);
         });
@@ -947,7 +949,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         next_id(2);
         barrier();
         static_for<AP>([&](auto dI) { A[decltype(dI)::value] = key_at(0, decltype(dI)::value); });
-        scores(0, minima(0), [&](auto dI) {
+        scores(minima(0), [&](auto dI) {
             constexpr int d = decltype(dI)::value;
             if constexpr (d + AP < ND) A[d % AP] = key_at(0, d + AP);
         }, [](auto) {});
@@ -958,22 +960,32 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     barrier();
 #pragma unroll
     for (int k = 0; k < AP; ++k) A[k] = value_at(1, k);
-    // Step st: tile st's scores are in N, T and kv. Its values and the keys of st + 2 go to LDS (slots whose last readers passed
-    // the barrier before); the values of st - 1 are summed beside that and beside the last scaling and the maximum of the scores,
+    // Step st: tile st's products are in N. Its values and the keys of st + 2 go to LDS (slots whose last readers passed
+    // the barrier before); the values of st - 1 are summed beside that and beside the scaling and maximum of the scores,
     // the scores of st + 1 beside the exponentials. One step more than tiles; before the first the weights are zero.
-    constexpr int LG = (NG - 1) & 1;
-    float sv[16], mv[16], sz[16], top = 0.f, w0 = 0.f;
-    auto scale_max = [&](int i) {
-        S[i] = __builtin_fmaf(T[LG][i], kv[LG][i], N[i]) * factor;
-        const float z = S[i] + sz[i];
+    float top = 0.f, w0 = 0.f;
+    float4 kf[2], sz[2], sv[2], mv[2];   // of 4 tokens, and the 4 after them, requested when those come up
+    auto pick = [](const float4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; };
+    auto ask_scales = [&](int st, int j) {
+        kf[j & 1] = of_tokens(tok[st & 3][0], j);
+        sz[j & 1] = of_tokens(tok[st & 3][3], j);
+    };
+    auto scale_max = [&](int st, int i) {
+        if (i % 4 == 0 && i < 12) ask_scales(st, i / 4 + 1);
+        S[i] = N[i] * pick(kf[(i / 4) & 1], i & 3);
+        const float z = __builtin_fmaf(S[i], factor, pick(sz[(i / 4) & 1], i & 3));
         top = i ? fmaxf(top, z) : z;
         asm volatile("" : "+v"(S[i]), "+v"(top));   // here, not where they are used
     };
-    auto weight = [&](int i) {
-        const float p = __builtin_amdgcn_exp2f(S[i] - mu);
+    auto weight = [&](int st, int i) {
+        if (i % 4 == 0 && i < 12) {
+            sv[(i / 4 + 1) & 1] = of_tokens(tok[st & 3][1], i / 4 + 1);
+            mv[(i / 4 + 1) & 1] = of_tokens(tok[st & 3][2], i / 4 + 1);
+        }
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], factor, -mu));
         l += p;
-        low = __builtin_fmaf(p, mv[i], low);
-        const float w = rounded(p * sv[i]);
+        low = __builtin_fmaf(p, pick(mv[(i / 4) & 1], i & 3), low);
+        const float w = rounded(p * pick(sv[(i / 4) & 1], i & 3));
         if (i & 1) {
             Wh[i >> 3][(i & 7) - 1] = static_cast<_Float16>(w0);
             Wh[i >> 3][i & 7] = static_cast<_Float16>(w);
@@ -992,13 +1004,17 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
             }, [&](auto kI) {
                 constexpr int k = decltype(kI)::value;
                 constexpr int EVERY = SLOTS / (4 * E);   // a word to LDS at every so many places of the first half
+                if constexpr (k == 0) k_scale();
                 if constexpr (k < SLOTS / 2 && k % EVERY == 0) {
                     if constexpr ((k / EVERY) & 1)
                         k_put(st + 2, (k / EVERY) >> 1);
                     else
                         v_put(st, (k / EVERY) >> 1);
                 }
-                if constexpr (k == SLOTS / 2 - 1) of_tokens(vtok[st & 3][2], sz);
+                if constexpr (k == SLOTS / 2 - 2) {
+                    ask_scales(st, 0);
+                    mins = minima(st + 1);
+                }
                 if constexpr (k == SLOTS / 2) {
                     s_put(st + 2);
                     v_load(1);
@@ -1009,12 +1025,11 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
                 }
                 if constexpr (k >= SLOTS / 2) {
 #pragma unroll
-                    for (int i = (k - SLOTS / 2) * PER; i < (k - SLOTS / 2 + 1) * PER; ++i) scale_max(i);
+                    for (int i = (k - SLOTS / 2) * PER; i < (k - SLOTS / 2 + 1) * PER; ++i) scale_max(st, i);
                 }
                 if constexpr (k == SLOTS - 2) {
-                    of_tokens(vtok[st & 3][0], sv);
-                    of_tokens(vtok[st & 3][1], mv);
-                    mins = minima(st + 1);
+                    sv[0] = of_tokens(tok[st & 3][1], 0);
+                    mv[0] = of_tokens(tok[st & 3][2], 0);
                 }
             });
         }
@@ -1024,11 +1039,9 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
                 const int last = st == steps ? -1 : limit;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    if (t0 + 16 * (i >> 3) + 8 * g + (i & 7) > last) {   // what lies there is anything: no 0 * NaN
-                        S[i] = -INFINITY;
-                        sv[i] = mv[i] = 0.f;
-                    }
-                    const float z = S[i] + sz[i];
+                    const float4 size = of_tokens(tok[st & 3][3], i / 4);
+                    if (t0 + 16 * (i >> 3) + 8 * g + (i & 7) > last) S[i] = -INFINITY;
+                    const float z = __builtin_fmaf(S[i], factor, pick(size, i & 3));
                     top = i ? fmaxf(top, z) : z;
                 }
             }
@@ -1044,7 +1057,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
                     for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
             }
             // (past the wave's last tile these scores are of an old one, and unused)
-            scores(st + 1, mins, [&](auto dI) {
+            scores(mins, [&](auto dI) {
                 constexpr int d = decltype(dI)::value;
                 if constexpr (d + AP < ND) A[d % AP] = key_at((st + 1) & 1, d + AP);
                 // The tile's keys have been read, its values and the next keys are written: the next values can be read.
@@ -1057,7 +1070,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
             }, [&](auto kI) {
                 constexpr int k = decltype(kI)::value, PLACES = 2 * ND;
 #pragma unroll
-                for (int i = k * 16 / PLACES; i < (k + 1) * 16 / PLACES; ++i) weight(i);
+                for (int i = k * 16 / PLACES; i < (k + 1) * 16 / PLACES; ++i) weight(st, i);
             });
         }
     }
