@@ -75,6 +75,8 @@ struct Attn4Args {
     int all_items;       // and with the cut prompts' pieces
     int places;          // split4_kernel's workgroups that the card holds at once
     int split_all;       // every request takes split4_kernel
+    int units;           // at most
+    int whole;           // and every unit's tiles are one piece: nothing is joined
     float scale;         // log2(e) / sqrt(D)
 };
 
@@ -116,13 +118,13 @@ struct Piece {
 constexpr int kHeld = 4;
 __device__ __forceinline__ int tiles_of(const Request4& r) { return max(1, (r.len + kTile - 1) / kTile); }
 __device__ __forceinline__ bool takes_split(const Attn4Args& a, const Request4& r) {
-    return a.split_all || static_cast<int64_t>(r.n) * a.group <= max(kSplitMax, a.group);
+    return a.split_all || r.n * a.group <= max(kSplitMax, a.group);   // rows * heads <= 2^24
 }
 __device__ __forceinline__ float units_of(const Attn4Args& a, const Request4& r) {
     if (!takes_split(a, r)) return 0.f;
-    return static_cast<float>((static_cast<int64_t>(r.n) * a.group + kRows - 1) / kRows) * static_cast<float>(a.c.heads);
+    return static_cast<float>(((static_cast<uint32_t>(r.n) * static_cast<uint32_t>(a.group)) + kRows - 1) / kRows) * static_cast<float>(a.c.heads);
 }
-// n / d, both below 2^26, the quotient below 2^20; inverse within 2^-22 of 1 / d.
+// n / d, both below 2^27, the quotient below 2^20; inverse within 2^-22 of 1 / d.
 __device__ __forceinline__ int quotient(int n, int d, float inverse) {
     int q = static_cast<int>(static_cast<float>(n) * inverse);
     q -= q * d > n;
@@ -155,18 +157,23 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
         }
         return group_sum<kWave>(v);
     };
-    const float total = sum([](float u, float t) { return u * t; }), all_units = sum([](float u, float) { return u; });
-    const float want = static_cast<float>(a.places) * (all_units > static_cast<float>(a.places) ? 4.0f : 1.0f);
-    auto limited = [](float t) { return max(static_cast<int>(fminf(ceilf(t), 0x1p26f)), kMinTiles); };
-    int cut = limited(total / want);
-    float step = 1.0f / static_cast<float>(cut);
-    for (int i = 0; i < 3; ++i) {
-        const float pieces = sum([=](float u, float t) { return u * ceilf(t * step); });
-        if (pieces <= want) break;
-        cut = max(limited(static_cast<float>(cut) * pieces / want), cut + 1);
-        step = 1.0f / static_cast<float>(cut);
+    int cut = 1 << 26;
+    float step = 0x1p-26f;
+    if (!a.whole) {
+        const float total = sum([](float u, float t) { return u * t; }), all_units = sum([](float u, float) { return u; });
+        const float want = static_cast<float>(a.places) * (all_units > static_cast<float>(a.places) ? 4.0f : 1.0f);
+        const float per_want = __builtin_amdgcn_rcpf(want);
+        auto limited = [](float t) { return max(static_cast<int>(fminf(ceilf(t), 0x1p26f)), kMinTiles); };
+        cut = limited(total * per_want);
+        step = __builtin_amdgcn_rcpf(static_cast<float>(cut));
+        for (int i = 0; i < 3; ++i) {
+            const float pieces = sum([=](float u, float t) { return u * ceilf(t * step * 0.99999f); });   // (step may be an ulp high)
+            if (pieces <= want) break;
+            cut = max(limited(static_cast<float>(cut) * pieces * per_want), cut + 1);
+            step = __builtin_amdgcn_rcpf(static_cast<float>(cut));
+        }
+        cut = __builtin_amdgcn_readfirstlane(cut);
     }
-    cut = __builtin_amdgcn_readfirstlane(cut);
     p.tiles = cut;
     bool found = false;
     auto look = [&](int b0, float u, int t) {
@@ -179,7 +186,7 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
             const int local = item - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
             p.b = b0 + l;
             p.splits = __builtin_amdgcn_readlane(splits, l);
-            p.unit = __builtin_amdgcn_readfirstlane(local / p.splits);
+            p.unit = __builtin_amdgcn_readfirstlane(quotient(local, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))));
             p.split = local - p.unit * p.splits;
             if (b0 == 0) {
                 p.r.first = __builtin_amdgcn_readlane(first.first, l);
@@ -265,9 +272,33 @@ __device__ __forceinline__ uint32_t sizes2(uint32_t scale, uint32_t low) {
 __device__ __forceinline__ float log2_over(float score, uint32_t b) { return __builtin_fmaf(static_cast<float>(b), 0x1p-7f, score); }
 
 // An output from its sums: zero where no key was seen (a weight may be 0 beside a NaN).
-__device__ __forceinline__ float finished(const Attn4Args& a, float m, float sum, float tot, size_t o) {
+__device__ __forceinline__ float finished(float m, float sum, float tot, bool gated, float gate) {
     const float v = m == -FLT_MAX && tot == 0.f ? 0.f : sum / tot;
-    return a.gate ? v * sigmoid(a.gate[o]) : v;
+    return gated ? v * sigmoid(gate) : v;
+}
+// 2, 4 or 8 neighbouring floats, as aligned as they are many
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float (&x)[N]) {
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 y = ld4(p + i);
+            x[i] = y.x, x[i + 1] = y.y, x[i + 2] = y.z, x[i + 3] = y.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = p[i];
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_floats(float* p, const float (&x)[N]) {
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) st4(p + i, make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = x[i];
+    }
 }
 
 // ------------------------------------------------------------------ few rows
@@ -300,21 +331,21 @@ __device__ __forceinline__ int key_turn(int t) {
 
 template <int D, bool WIDE>
 __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args a) {
-    constexpr int NG = D / 64, NV = D / 64, LD = D + 2;
+    constexpr int NG = D / 64, NV = D / 64, LD = D + 4;   // rows of sums: 16-byte aligned
     using R = Ring<D>;
     static_assert(kRows * LD * 4 <= 2 * R::bytes, "a wave's sums go where its ring was");
     __shared__ __align__(16) uint8_t ring[kSplitWaves][2][R::bytes];
     __shared__ __align__(16) _Float16 qs[2 * kRows][D + 8];   // the queries' parts; 16 bytes more, and 16 rows meet no bank twice
-    __shared__ float stat[kRows][kSplitWaves][2], join[kRows][kSplitWaves + 2];
+    __shared__ float2 stat[kSplitWaves][kRows];
     __shared__ float factors[kRows], qsum[kRows][NG];
     Piece pc;
     if (!find_piece(a, static_cast<int>(blockIdx.x), pc)) return;   // the whole workgroup
     const Request4 r = pc.r;
     const int G = a.group, pairs = r.n * G;
-    const float per_g = 1.0f / static_cast<float>(G);
+    const float per_g = __builtin_amdgcn_rcpf(static_cast<float>(G));
     auto over_g = [&](int pair) { return quotient(pair, G, per_g); };
     const int blocks = (pairs + kRows - 1) / kRows;
-    const int h = pc.unit / blocks, rb = pc.unit - h * blocks;
+    const int h = __builtin_amdgcn_readfirstlane(quotient(pc.unit, blocks, __builtin_amdgcn_rcpf(static_cast<float>(blocks)))), rb = pc.unit - h * blocks;
     const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4, part = lr & 1;
     const int wv = wave_in_block();
     const uint32_t magic = code_magic();
@@ -393,16 +424,10 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
     const float* qrow = a.q + (static_cast<size_t>(r.first + qt) * a.heads + h * G + (qp - qt * G)) * D + (lane & 31) * (D / 32);
     constexpr int QN = D / 32;
     float qf[QN];
-    if constexpr (QN >= 4) {
-#pragma unroll
-        for (int i = 0; i < QN / 4; ++i) {
-            const float4 x = ld4(qrow + 4 * i);
-            qf[4 * i] = x.x, qf[4 * i + 1] = x.y, qf[4 * i + 2] = x.z, qf[4 * i + 3] = x.w;
-        }
-    } else {
-        qf[0] = qrow[0], qf[1] = qrow[1];
-    }
+    load_floats(qrow, qf);
     request_ids(t);
+#pragma unroll
+    for (int i = 0; i < QN; ++i) asm volatile("" : "+v"(qf[i]));   // here: behind the tile's loads it would wait for those too
     if (t < t_end) request_tile(t, 0);
     request_ids(t + kSplitWaves);
     {
@@ -414,8 +439,12 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
             bad |= !(fabsf(qf[i]) <= FLT_MAX);
         }
         if (bad) m = INFINITY;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        m = fmaxf(m, dpp_move<0xB1>(m));   // over the row's 32 lanes
+        m = fmaxf(m, dpp_move<0x4E>(m));
+        m = fmaxf(m, dpp_move<0x141>(m));
+        m = fmaxf(m, dpp_move<0x140>(m));
+        const auto two = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+        m = fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
         const bool ok = m <= FLT_MAX;
         int e = 0;
         if (m > 0.f && ok) {
@@ -607,43 +636,44 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
                 const float v = acc[m][e + 1][i] + dpp_move<0xB1>(acc[m][e + 1][i]);
                 mine[64 * m + 4 * (4 * lk + i) + e + part] = (part ? v : u) + low;
             }
-    if (lane < 16 && part == 0) {
-        stat[lr >> 1][wv][0] = mu;
-        stat[lr >> 1][wv][1] = l;
-    }
+    if (lane < 16 && part == 0) stat[wv][lr >> 1] = make_float2(mu, l);
     __syncthreads();
-    if (threadIdx.x < kRows) {   // what each wave's sums count of the row's
-        const int row = threadIdx.x;
-        float m = stat[row][0][0], tot = 0.f;
+    // 32 threads a row, D / 32 dims each
+    const int row = threadIdx.x >> 5, at = rb * kRows + row;
+    if (at >= pairs) return;
+    float2 st[kSplitWaves];
 #pragma unroll
-        for (int w = 1; w < kSplitWaves; ++w) m = fmaxf(m, stat[row][w][0]);
+    for (int w = 0; w < kSplitWaves; ++w) st[w] = stat[w][row];
+    float m = st[0].x, tot = 0.f, sum[QN];
 #pragma unroll
-        for (int w = 0; w < kSplitWaves; ++w) {
-            const float k = __builtin_amdgcn_exp2f(stat[row][w][0] - m);
-            join[row][w] = k;
-            tot += k * stat[row][w][1];
-        }
-        join[row][kSplitWaves] = m;
-        join[row][kSplitWaves + 1] = r.bad ? __builtin_nanf("") : tot;
+    for (int w = 1; w < kSplitWaves; ++w) m = fmaxf(m, st[w].x);
+#pragma unroll
+    for (int i = 0; i < QN; ++i) sum[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSplitWaves; ++w) {
+        const float k = __builtin_amdgcn_exp2f(st[w].x - m);
+        tot += k * st[w].y;
+        const float* from = reinterpret_cast<const float*>(ring[w]) + row * LD + (threadIdx.x & 31) * QN;
+        float x[QN];
+        load_floats(from, x);
+#pragma unroll
+        for (int i = 0; i < QN; ++i) sum[i] += k * x[i];
     }
-    __syncthreads();
-    const int rows = min(kRows, pairs - rb * kRows);
-    for (int i = threadIdx.x; i < rows * D; i += kSplitBlock) {
-        const int row = i / D, d = i - row * D;
-        float sum = 0.f;
+    if (r.bad) tot = __builtin_nanf("");
+    const int n = over_g(at);
+    const size_t pair = static_cast<size_t>(r.first + n) * a.heads + h * G + (at - n * G);
+    const size_t o = pair * D + (threadIdx.x & 31) * QN, item = static_cast<size_t>(blockIdx.x) * kRows + row;
+    if (pc.splits == 1) {
+        float gate[QN];
+        if (a.gate) load_floats(a.gate + o, gate);
 #pragma unroll
-        for (int w = 0; w < kSplitWaves; ++w) sum += join[row][w] * reinterpret_cast<const float*>(ring[w])[row * LD + d];
-        const float m = join[row][kSplitWaves], tot = join[row][kSplitWaves + 1];
-        const int at = rb * kRows + row, n = over_g(at);
-        const size_t o = (static_cast<size_t>(r.first + n) * a.heads + h * G + (at - n * G)) * D + d;
-        if (pc.splits == 1) {
-            a.out[o] = finished(a, m, sum, tot, o);
-        } else {
-            a.part[(static_cast<size_t>(blockIdx.x) * kRows + row) * D + d] = sum;
-            if (d == 0) a.stat[static_cast<size_t>(blockIdx.x) * kRows + row] = make_float2(m, tot);
-        }
-        if (d == 0 && pc.split == 0) a.info[o / D] = make_int2(static_cast<int>(blockIdx.x) * kRows + row, pc.splits);
+        for (int i = 0; i < QN; ++i) sum[i] = finished(m, sum[i], tot, a.gate, a.gate ? gate[i] : 0.f);
+        store_floats(a.out + o, sum);
+    } else {
+        store_floats(a.part + item * D + (threadIdx.x & 31) * QN, sum);
+        if ((threadIdx.x & 31) == 0) a.stat[item] = make_float2(m, tot);
     }
+    if ((threadIdx.x & 31) == 0 && pc.split == 0 && !a.whole) a.info[pair] = make_int2(static_cast<int>(item), pc.splits);
 }
 
 // ------------------------------------------------------------------ many rows
@@ -1169,9 +1199,11 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel
         todo &= todo - 1;
         const int pieces = __builtin_amdgcn_readlane(in.y, k), where = __builtin_amdgcn_readlane(in.x, k);
         const int slot = where % kRows, first = where / kRows;
-        float m = -FLT_MAX, l = 0.f, s[V];
+        const size_t o = static_cast<size_t>(pair0 + k) * D;
+        float m = -FLT_MAX, l = 0.f, s[V], gate[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] = 0.f;
+        for (int i = 0; i < V; ++i) s[i] = gate[i] = 0.f;
+        if (NW == 1 && a.gate) load_floats(a.gate + o + V * lane, gate);
         constexpr int U = NW == 16 ? 16 : 4;   // pieces in flight
         for (int p0 = wv; p0 < pieces; p0 += U * NW) {
             float2 st[U];
@@ -1180,14 +1212,7 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel
             for (int u = 0; u < U; ++u) {
                 const size_t q = static_cast<size_t>(first + min(p0 + u * NW, pieces - 1)) * kRows + slot;
                 st[u] = a.stat[q];
-                const float* p = a.part + q * D + V * lane;
-                if constexpr (V == 4) {
-                    const float4 y = ld4(p);
-                    x[u][0] = y.x, x[u][1] = y.y, x[u][2] = y.z, x[u][3] = y.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) x[u][i] = p[i];
-                }
+                load_floats(a.part + q * D + V * lane, x[u]);
             }
             __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
 #pragma unroll
@@ -1201,10 +1226,10 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel
                 for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
             }
         }
-        const size_t o = static_cast<size_t>(pair0 + k) * D;
         if constexpr (NW == 1) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) a.out[o + V * lane + i] = finished(a, m, s[i], l, o + V * lane + i);
+            for (int i = 0; i < V; ++i) s[i] = finished(m, s[i], l, a.gate, gate[i]);
+            store_floats(a.out + o + V * lane, s);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) sums[wv][V * lane + i] = s[i];
@@ -1224,7 +1249,7 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel
                     sum += f * sums[w][d];
                     tot += f * ls[w];
                 }
-                a.out[o + d] = finished(a, top, sum, tot, o + d);
+                a.out[o + d] = finished(top, sum, tot, a.gate, a.gate ? a.gate[o + d] : 0.f);
             }
         }
     }
@@ -1244,12 +1269,15 @@ constexpr int kCus = 256;
 // Its pieces are at most as many as wanted (and a few for rounding) plus one per unit; units at most one per 8 pairs plus one
 // per request that has rows, and, where larger requests go to prompt4_kernel, at most one per 8 of the pairs with which one does
 // not (plus one, so that the bound does not fall where the first request goes there).
-int64_t item_bound(int rows, int requests, int heads, int kv_heads, int dim) {
+int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
     const int group = heads / kv_heads;
-    const int64_t pairs = static_cast<int64_t>(rows) * group, places = kCus * places_on_cu(dim), busy = std::min(rows, requests);
+    const int64_t pairs = static_cast<int64_t>(rows) * group, busy = std::min(rows, requests);
     int64_t units = pairs / kRows + busy;
     if (may_prompt(rows, requests, group)) units = std::min(units, busy * (blocks_for(std::max(kSplitMax, group), kRows) + 1));
-    units *= kv_heads;
+    return units * kv_heads;
+}
+int64_t item_bound(int rows, int requests, int heads, int kv_heads, int dim) {
+    const int64_t places = kCus * places_on_cu(dim), units = unit_bound(rows, requests, heads, kv_heads);
     return (units > places ? 4 : 1) * places + 8 + units;
 }
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
@@ -1271,10 +1299,15 @@ Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     return l;
 }
 
+// Table rows that hold no more tiles than this make calls whose units are not cut: a workgroup's four waves take them in kWhole / 4
+// turns, less than the launch that joins pieces.
+constexpr int kWhole = 16;
+
 template <int D>
 void launch(const Attn4Args& a, hipStream_t s) {
     const auto split = a.c.page >= kTile ? split4_kernel<D, true> : split4_kernel<D, false>;
-    split<<<static_cast<unsigned>(a.items), kSplitBlock, 0, s>>>(a);
+    split<<<static_cast<unsigned>(a.whole ? a.units : a.items), kSplitBlock, 0, s>>>(a);
+    if (a.whole) return;
     if (!a.split_all) {
         const int64_t pairs = static_cast<int64_t>(a.rows) * a.group;
         const int64_t tiles = (pairs / kPromptRows + std::min<int64_t>(a.requests, pairs / kSplitMax + 1)) * a.c.heads;
@@ -1351,6 +1384,8 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     a.items = static_cast<int>(l.items);
     a.all_items = static_cast<int>(l.all);
     a.split_all = !may_prompt(rows, requests, a.group);
+    a.units = static_cast<int>(unit_bound(rows, requests, heads, kv_heads));
+    a.whole = a.split_all && static_cast<int64_t>(max_pages) * page_size <= kWhole * kTile;
     a.places = kCus * places_on_cu(dim);
     const hipStream_t s = as_stream(stream);
     if (dim == 64)
