@@ -49,7 +49,7 @@ typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kTile = 32;              // tokens of a step
 constexpr int kSplitWaves = 4;
-constexpr int kSplitBlock = kSplitWaves * kWave;
+constexpr int kWholeWaves = 8;
 constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
 constexpr int kMinTiles = 4;           // of a piece
 constexpr int kMaxItems = 1 << 24;     // more than any call has
@@ -303,7 +303,7 @@ __device__ __forceinline__ void store_floats(float* p, const float (&x)[N]) {
 
 // ------------------------------------------------------------------ few rows
 // A workgroup takes 8 (row, head) pairs that share a KV head - 16 columns: 8 rows x 2 fp16 parts - and a range of 32-token
-// tiles, its 4 waves every fourth tile. A wave's tiles go straight from the cache to a ring of two places in LDS (no
+// tiles, its NW waves every NW-th tile. A wave's tiles go straight from the cache to a ring of two places in LDS (no
 // registers wait for them), the next but one requested as soon as a tile has been taken to registers: one and a half tiles, 13 KB at D =
 // 256, are under way per wave. The two columns of a row share the work of the softmax: each of the two lanes takes half of the
 // tokens that both hold.
@@ -329,14 +329,15 @@ __device__ __forceinline__ int key_turn(int t) {
     return (t >> 3) & 1;
 }
 
-template <int D, bool WIDE>
-__global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args a) {
+template <int D, bool WIDE, int NW>
+__global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a) {
     constexpr int NG = D / 64, NV = D / 64, LD = D + 4;   // rows of sums: 16-byte aligned
+    constexpr int QL = kWave * NW / kRows, QN = D / QL;   // threads of a row, in its query and in its output, and their dims
     using R = Ring<D>;
     static_assert(kRows * LD * 4 <= 2 * R::bytes, "a wave's sums go where its ring was");
-    __shared__ __align__(16) uint8_t ring[kSplitWaves][2][R::bytes];
+    __shared__ __align__(16) uint8_t ring[NW][2][R::bytes];
     __shared__ __align__(16) _Float16 qs[2 * kRows][D + 8];   // the queries' parts; 16 bytes more, and 16 rows meet no bank twice
-    __shared__ float2 stat[kSplitWaves][kRows];
+    __shared__ float2 stat[NW][kRows];
     __shared__ float factors[kRows], qsum[kRows][NG];
     Piece pc;
     if (!find_piece(a, static_cast<int>(blockIdx.x), pc)) return;   // the whole workgroup
@@ -418,18 +419,17 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
         }
         if (lane < R::small_lanes) dma16(small_base + octet(small_oct) * small_mul + small_off, to + R::at_ks);
     };
-    // The rows' queries, scaled by 2^e so that a row's largest magnitude is in [2^14, 2^15), as two fp16 parts: 2 rows a wave,
-    // requested before the first tile.
-    const int qr = 2 * wv + (lane >> 5), qp = min(rb * kRows + qr, pairs - 1), qt = over_g(qp);
-    const float* qrow = a.q + (static_cast<size_t>(r.first + qt) * a.heads + h * G + (qp - qt * G)) * D + (lane & 31) * (D / 32);
-    constexpr int QN = D / 32;
+    // The rows' queries, scaled by 2^e so that a row's largest magnitude is in [2^14, 2^15), as two fp16 parts: requested
+    // before the first tile.
+    const int qr = static_cast<int>(threadIdx.x) / QL, qp = min(rb * kRows + qr, pairs - 1), qt = over_g(qp);
+    const float* qrow = a.q + (static_cast<size_t>(r.first + qt) * a.heads + h * G + (qp - qt * G)) * D + (threadIdx.x % QL) * QN;
     float qf[QN];
     load_floats(qrow, qf);
     request_ids(t);
 #pragma unroll
     for (int i = 0; i < QN; ++i) asm volatile("" : "+v"(qf[i]));   // here: behind the tile's loads it would wait for those too
     if (t < t_end) request_tile(t, 0);
-    request_ids(t + kSplitWaves);
+    request_ids(t + NW);
     {
         float m = 0.f;
         bool bad = false;
@@ -439,12 +439,16 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
             bad |= !(fabsf(qf[i]) <= FLT_MAX);
         }
         if (bad) m = INFINITY;
-        m = fmaxf(m, dpp_move<0xB1>(m));   // over the row's 32 lanes
+        m = fmaxf(m, dpp_move<0xB1>(m));   // over the row's lanes
         m = fmaxf(m, dpp_move<0x4E>(m));
         m = fmaxf(m, dpp_move<0x141>(m));
         m = fmaxf(m, dpp_move<0x140>(m));
         const auto two = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
         m = fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
+        if constexpr (QL == 64) {
+            const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+            m = fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+        }
         const bool ok = m <= FLT_MAX;
         int e = 0;
         if (m > 0.f && ok) {
@@ -453,7 +457,7 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
             e = min(15 - em, kMaxUp);
         }
         float s = 0.f;
-        const int d0 = (lane & 31) * QN;
+        const int d0 = (threadIdx.x % QL) * QN;
 #pragma unroll
         for (int i = 0; i < QN; ++i) {
             const float v = ok ? ldexpf(qf[i], e) : 0.f;
@@ -463,10 +467,10 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
         }
         s = group_sum<64 / QN>(s);
         if ((lane & (64 / QN - 1)) == 0) qsum[qr][d0 / 64] = s;
-        if ((lane & 31) == 0) factors[qr] = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");   // products to log2 scores; NaN: a row
+        if (d0 == 0) factors[qr] = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");   // products to log2 scores; NaN: a row
     }                                                                                        // with infinities or NaNs
-    if (t + kSplitWaves < t_end) request_tile(t + kSplitWaves, 1);
-    request_ids(t + 2 * kSplitWaves);
+    if (t + NW < t_end) request_tile(t + NW, 1);
+    request_ids(t + 2 * NW);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the tiles' loads stay in flight
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -487,8 +491,8 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
     float mu = -FLT_MAX, l = 0.f, low = 0.f;   // mu: the reference less kWeightUp
     const int my_turn = key_turn<D>(8 * (lr >> 2) + (lr & 3));
     const uint32_t k_at = (8 * (lr >> 2) + (lr & 3)) * (D / 2);
-    for (int slot = 0; t < t_end; t += kSplitWaves, slot ^= 1) {
-        if (t + kSplitWaves < t_end)
+    for (int slot = 0; t < t_end; t += NW, slot ^= 1) {
+        if (t + NW < t_end)
             wait_vm<R::loads>();   // the next tile stays under way
         else
             wait_vm<0>();
@@ -547,10 +551,10 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
         const uint2 vsc = *reinterpret_cast<const uint2*>(in + R::at_vs + 16 * lk + 8 * part);
         const uint2 vmn = *reinterpret_cast<const uint2*>(in + R::at_vm + 16 * lk + 8 * part);
         const float f = (bad_octets[slot] >> lk) & 1 ? __builtin_nanf("") : factor;
-        if (t + 2 * kSplitWaves < t_end) {
+        if (t + 2 * NW < t_end) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the place has been read
-            request_tile(t + 2 * kSplitWaves, slot);
-            request_ids(t + 3 * kSplitWaves);
+            request_tile(t + 2 * NW, slot);
+            request_ids(t + 3 * NW);
         }
         // This lane's tokens 8 lk + 4 part + 0..3: both fp16 parts of the query, the other one from the lane beside.
         const int tok = t * kTile + 8 * lk + 4 * part;
@@ -638,22 +642,21 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
             }
     if (lane < 16 && part == 0) stat[wv][lr >> 1] = make_float2(mu, l);
     __syncthreads();
-    // 32 threads a row, D / 32 dims each
-    const int row = threadIdx.x >> 5, at = rb * kRows + row;
+    const int row = static_cast<int>(threadIdx.x) / QL, d = (threadIdx.x % QL) * QN, at = rb * kRows + row;
     if (at >= pairs) return;
-    float2 st[kSplitWaves];
+    float2 st[NW];
 #pragma unroll
-    for (int w = 0; w < kSplitWaves; ++w) st[w] = stat[w][row];
+    for (int w = 0; w < NW; ++w) st[w] = stat[w][row];
     float m = st[0].x, tot = 0.f, sum[QN];
 #pragma unroll
-    for (int w = 1; w < kSplitWaves; ++w) m = fmaxf(m, st[w].x);
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, st[w].x);
 #pragma unroll
     for (int i = 0; i < QN; ++i) sum[i] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kSplitWaves; ++w) {
+    for (int w = 0; w < NW; ++w) {
         const float k = __builtin_amdgcn_exp2f(st[w].x - m);
         tot += k * st[w].y;
-        const float* from = reinterpret_cast<const float*>(ring[w]) + row * LD + (threadIdx.x & 31) * QN;
+        const float* from = reinterpret_cast<const float*>(ring[w]) + row * LD + d;
         float x[QN];
         load_floats(from, x);
 #pragma unroll
@@ -662,7 +665,7 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
     if (r.bad) tot = __builtin_nanf("");
     const int n = over_g(at);
     const size_t pair = static_cast<size_t>(r.first + n) * a.heads + h * G + (at - n * G);
-    const size_t o = pair * D + (threadIdx.x & 31) * QN, item = static_cast<size_t>(blockIdx.x) * kRows + row;
+    const size_t o = pair * D + d, item = static_cast<size_t>(blockIdx.x) * kRows + row;
     if (pc.splits == 1) {
         float gate[QN];
         if (a.gate) load_floats(a.gate + o, gate);
@@ -670,10 +673,10 @@ __global__ __launch_bounds__(kSplitBlock, 2) void split4_kernel(const Attn4Args 
         for (int i = 0; i < QN; ++i) sum[i] = finished(m, sum[i], tot, a.gate, a.gate ? gate[i] : 0.f);
         store_floats(a.out + o, sum);
     } else {
-        store_floats(a.part + item * D + (threadIdx.x & 31) * QN, sum);
-        if ((threadIdx.x & 31) == 0) a.stat[item] = make_float2(m, tot);
+        store_floats(a.part + item * D + d, sum);
+        if (d == 0) a.stat[item] = make_float2(m, tot);
     }
-    if ((threadIdx.x & 31) == 0 && pc.split == 0 && !a.whole) a.info[pair] = make_int2(static_cast<int>(item), pc.splits);
+    if (d == 0 && pc.split == 0 && !a.whole) a.info[pair] = make_int2(static_cast<int>(item), pc.splits);
 }
 
 // ------------------------------------------------------------------ many rows
@@ -1204,28 +1207,34 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel
 #pragma unroll
         for (int i = 0; i < V; ++i) s[i] = gate[i] = 0.f;
         if (NW == 1 && a.gate) load_floats(a.gate + o + V * lane, gate);
-        constexpr int U = NW == 16 ? 16 : 4;   // pieces in flight
-        for (int p0 = wv; p0 < pieces; p0 += U * NW) {
-            float2 st[U];
-            float x[U][V];
+        auto take = [&](auto uI) {   // so many pieces in flight
+            constexpr int U = decltype(uI)::value;
+            for (int p0 = wv; p0 < pieces; p0 += U * NW) {
+                float2 st[U];
+                float x[U][V];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const size_t q = static_cast<size_t>(first + min(p0 + u * NW, pieces - 1)) * kRows + slot;
-                st[u] = a.stat[q];
-                load_floats(a.part + q * D + V * lane, x[u]);
+                for (int u = 0; u < U; ++u) {
+                    const size_t q = static_cast<size_t>(first + min(p0 + u * NW, pieces - 1)) * kRows + slot;
+                    st[u] = a.stat[q];
+                    load_floats(a.part + q * D + V * lane, x[u]);
+                }
+                __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (p0 + u * NW >= pieces) break;
+                    const float now = fmaxf(m, st[u].x);
+                    const float was = __builtin_amdgcn_exp2f(m - now), f = __builtin_amdgcn_exp2f(st[u].x - now);
+                    m = now;
+                    l = l * was + st[u].y * f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
+                }
             }
-            __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (p0 + u * NW >= pieces) break;
-                const float now = fmaxf(m, st[u].x);
-                const float was = __builtin_amdgcn_exp2f(m - now), f = __builtin_amdgcn_exp2f(st[u].x - now);
-                m = now;
-                l = l * was + st[u].y * f;
-#pragma unroll
-                for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
-            }
-        }
+        };
+        if (NW == 16 && pieces > 4 * NW)   // (one token at 200000 keys: 7.7 us with 4 in flight, 5.9 with 16; at 2000 keys 3.9, 6.6)
+            take(IC<16>{});
+        else
+            take(IC<4>{});
         if constexpr (NW == 1) {
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] = finished(m, s[i], l, a.gate, gate[i]);
@@ -1299,15 +1308,20 @@ Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     return l;
 }
 
-// Table rows that hold no more tiles than this make calls whose units are not cut: a workgroup's four waves take them in kWhole / 4
+// Table rows that hold no more tiles than this make calls whose units are not cut: a workgroup's eight waves take them in kWhole / 8
 // turns, less than the launch that joins pieces.
 constexpr int kWhole = 16;
 
+template <int D, int NW>
+void launch_split(const Attn4Args& a, int grid, hipStream_t s) {
+    const auto split = a.c.page >= kTile ? split4_kernel<D, true, NW> : split4_kernel<D, false, NW>;
+    split<<<static_cast<unsigned>(grid), NW * kWave, 0, s>>>(a);
+}
+
 template <int D>
 void launch(const Attn4Args& a, hipStream_t s) {
-    const auto split = a.c.page >= kTile ? split4_kernel<D, true> : split4_kernel<D, false>;
-    split<<<static_cast<unsigned>(a.whole ? a.units : a.items), kSplitBlock, 0, s>>>(a);
-    if (a.whole) return;
+    if (a.whole) return launch_split<D, kWholeWaves>(a, a.units, s);
+    launch_split<D, kSplitWaves>(a, a.items, s);
     if (!a.split_all) {
         const int64_t pairs = static_cast<int64_t>(a.rows) * a.group;
         const int64_t tiles = (pairs / kPromptRows + std::min<int64_t>(a.requests, pairs / kSplitMax + 1)) * a.c.heads;

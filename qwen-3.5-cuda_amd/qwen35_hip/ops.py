@@ -15,6 +15,7 @@ torch is used for device memory and streams only.
 from __future__ import annotations
 
 import ctypes
+from collections import namedtuple
 
 import torch
 
@@ -742,33 +743,30 @@ def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None,
 
 
 # ------------------------------------------------------------------ the same cache in 4 bits
-class Kv4Cache:
+class Kv4Cache(namedtuple("_Kv4Cache", "k v k_scale k_min v_scale v_min pages page heads dim args")):
     """4-bit codes and bfloat16 scales and minima of a paged cache (qwen35_hip.h): k uint8 [pages, kv_heads, page, dim / 2],
     v uint8 [pages, kv_heads, page / 8, dim, 4], k_scale [pages, kv_heads, page / 8, dim / 64, 8], k_min
-    [pages, kv_heads, page, dim / 64], v_scale, v_min [pages, kv_heads, page]. Checked once, here."""
-    __slots__ = ("k", "v", "k_scale", "k_min", "v_scale", "v_min", "pages", "page", "heads", "dim", "args")
+    [pages, kv_heads, page, dim / 64], v_scale, v_min [pages, kv_heads, page]. Checked once, here; it stays over the tensors
+    it was made of, whose pointers it keeps."""
+    __slots__ = ()
 
-    def __init__(self, k, v, k_scale, k_min, v_scale, v_min):
+    def __new__(cls, k, v, k_scale, k_min, v_scale, v_min):
         _checked(torch.uint8, k, v)
         _checked(BF16, k_scale, k_min, v_scale, v_min)
         if k.dim() != 4:
             raise ValueError("cache keys must be [pages, kv_heads, page, dim / 2]")
         pages, heads, page, half = k.shape
         dim = 2 * half
-        for shape, *ts in (((pages, heads, page // 8, dim, 4), v), ((pages, heads, page // 8, dim // 64, 8), k_scale),
-                           ((pages, heads, page, dim // 64), k_min), ((pages, heads, page), v_scale, v_min)):
-            for t in ts:
-                if t.shape != shape:
-                    _same(shape, t)
-        self.k, self.v, self.k_scale, self.k_min, self.v_scale, self.v_min = k, v, k_scale, k_min, v_scale, v_min
-        self.pages, self.page, self.heads, self.dim = pages, page, heads, dim
-        self.args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), k_min.data_ptr(), v_scale.data_ptr(), v_min.data_ptr(),
-                     pages, page, heads, dim)
-
-    def __setattr__(self, name, value):
-        if hasattr(self, "args"):   # its pointers are those of the tensors above
-            raise AttributeError("a Kv4Cache stays over the tensors it was made of")
-        object.__setattr__(self, name, value)
+        if (v.shape != (pages, heads, page // 8, dim, 4) or k_scale.shape != (pages, heads, page // 8, dim // 64, 8)
+                or k_min.shape != (pages, heads, page, dim // 64) or v_scale.shape != (pages, heads, page)
+                or v_min.shape != (pages, heads, page)):
+            _same((pages, heads, page // 8, dim, 4), v)
+            _same((pages, heads, page // 8, dim // 64, 8), k_scale)
+            _same((pages, heads, page, dim // 64), k_min)
+            _same((pages, heads, page), v_scale, v_min)
+        args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), k_min.data_ptr(), v_scale.data_ptr(), v_min.data_ptr(),
+                pages, page, heads, dim)
+        return tuple.__new__(cls, (k, v, k_scale, k_min, v_scale, v_min, pages, page, heads, dim, args))
 
 
 def kv4_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv4Cache:
