@@ -51,7 +51,6 @@ constexpr int kTile = 32;              // tokens of a step
 constexpr int kSplitWaves = 4;
 constexpr int kWholeWaves = 8;
 constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
-constexpr int kMinTiles = 4;           // of a piece
 constexpr int kMaxItems = 1 << 24;     // more than any call has
 constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take split4_kernel; a row does
 constexpr int kSplitOnly = 1024;       // and of a whole call that has no more rows than requests
@@ -108,9 +107,10 @@ __device__ __forceinline__ int wave_prefix(int v) {
 }
 
 // Piece `item` of the call: request, which of its units (KV head, row block), which piece of the unit's tiles. Every wave
-// finds it by itself from the lengths. All pieces of a call have the same number of tiles, `cut`, but a unit's last: as few
-// as still give each of the card's places one piece at most, since a place that takes a second one makes the call half as
-// long again; with more units than places, four pieces. Lengths are held in registers, 64 requests to one, up to kHeld x 64.
+// finds it by itself from the lengths. No piece has more than `cut` tiles, a unit's pieces are of one size, and both are whole
+// turns of the waves. `cut` is the least that still gives each of the card's places one piece at most, since a place that takes a
+// second one makes the call half as long again; with more units than places, four pieces. Lengths are held in registers, 64
+// requests to one, up to kHeld x 64.
 struct Piece {
     int b, unit, split, splits, tiles;   // tiles: of one piece
     Request4 r;
@@ -163,18 +163,19 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
         const float total = sum([](float u, float t) { return u * t; }), all_units = sum([](float u, float) { return u; });
         const float want = static_cast<float>(a.places) * (all_units > static_cast<float>(a.places) ? 4.0f : 1.0f);
         const float per_want = __builtin_amdgcn_rcpf(want);
-        auto limited = [](float t) { return max(static_cast<int>(fminf(ceilf(t), 0x1p26f)), kMinTiles); };
+        auto limited = [](float t) {   // whole turns
+            return max(static_cast<int>(fminf(ceilf(t * (1.0f / kSplitWaves)), 0x1p24f)), 1) * kSplitWaves;
+        };
         cut = limited(total * per_want);
         step = __builtin_amdgcn_rcpf(static_cast<float>(cut));
         for (int i = 0; i < 3; ++i) {
             const float pieces = sum([=](float u, float t) { return u * ceilf(t * step * 0.99999f); });   // (step may be an ulp high)
             if (pieces <= want) break;
-            cut = max(limited(static_cast<float>(cut) * pieces * per_want), cut + 1);
+            cut = max(limited(static_cast<float>(cut) * pieces * per_want), cut + kSplitWaves);
             step = __builtin_amdgcn_rcpf(static_cast<float>(cut));
         }
         cut = __builtin_amdgcn_readfirstlane(cut);
     }
-    p.tiles = cut;
     bool found = false;
     auto look = [&](int b0, float u, int t) {
         const int splits = quotient(t + cut - 1, cut, step);
@@ -188,6 +189,8 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
             p.splits = __builtin_amdgcn_readlane(splits, l);
             p.unit = __builtin_amdgcn_readfirstlane(quotient(local, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))));
             p.split = local - p.unit * p.splits;
+            const int all = __builtin_amdgcn_readlane(t, l) + (kSplitWaves - 1);
+            p.tiles = a.whole ? cut : (quotient(all / kSplitWaves + p.splits - 1, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits)))) * kSplitWaves;
             if (b0 == 0) {
                 p.r.first = __builtin_amdgcn_readlane(first.first, l);
                 p.r.n = __builtin_amdgcn_readlane(first.n, l);
@@ -1182,21 +1185,102 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
 }
 
 // ------------------------------------------------------------------ join
-// Joins the pieces of (row, head) pairs. NW > 1: a workgroup of NW waves per pair, wave w takes pieces w, w + NW, ...; NW = 1: a
-// wave per pair, and each wave looks at `per` pairs at once, because in a prompt's call most are there already. Lanes hold the
-// dims.
+// Joins the pieces of (row, head) pairs. `entry`: where a pair's pieces are, (0, 0) where nothing is to be joined.
+__device__ __forceinline__ int2 entry(const Attn4Args& a, int64_t pair, bool live) {
+    // Pairs of the requests' rows alone: only those have an entry of this call (the workspace may hold an earlier one's).
+    const int from = min(max(a.row_start[0], 0), a.rows) * a.heads, end = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;
+    int2 in = make_int2(0, 0);
+    if (live && pair >= from && pair < end) in = a.info[pair];
+    // one piece is there already; starts that decrease may leave anything
+    return in.y > 1 && in.x >= 0 && in.y <= a.all_items - in.x / kRows ? in : make_int2(0, 0);
+}
+// The join of two parts of a sum with their references: (m, l, s) takes in (n, k, x).
+template <int V>
+__device__ __forceinline__ void join_in(float& m, float& l, float (&s)[V], float n, float k, const float (&x)[V]) {
+    const float now = fmaxf(m, n);
+    const float was = __builtin_amdgcn_exp2f(m - now), f = __builtin_amdgcn_exp2f(n - now);
+    m = now;
+    l = l * was + k * f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[i] * f;
+}
+
+// Few pairs, each of perhaps hundreds of pieces: a workgroup of 8 waves per pair and 64 dims, 16 lanes a piece. (A workgroup per
+// pair, whole rows: what one CU can read bounded it, 7.7 us for 16 pairs of 256 pieces.)
+constexpr int kJoinWaves = 8;
+template <int D>
+__global__ __launch_bounds__(kJoinWaves* kWave) void join4_few(const Attn4Args a) {
+    __shared__ __align__(16) float sums[kJoinWaves][64];
+    __shared__ float ls[kJoinWaves], ms[kJoinWaves];
+    constexpr int PARTS = D / 64, LANES = 4 * kJoinWaves;   // pieces looked at together
+    const int lane = threadIdx.x & 63, wv = wave_in_block(), mine = static_cast<int>(threadIdx.x) >> 4;
+    const int pair = static_cast<int>(blockIdx.x) / PARTS, d = 64 * (static_cast<int>(blockIdx.x) % PARTS) + 4 * (lane & 15);
+    const int2 in = entry(a, pair, true);
+    if (in.y == 0) return;   // the whole workgroup
+    const int pieces = in.y, slot = in.x % kRows, first = in.x / kRows;
+    float m = -FLT_MAX, l = 0.f, s[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 8;   // in flight
+    for (int p0 = mine; p0 < pieces; p0 += U * LANES) {
+        float2 st[U];
+        float x[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (p0 + u * LANES < pieces) {
+                const size_t q = static_cast<size_t>(first + p0 + u * LANES) * kRows + slot;
+                st[u] = a.stat[q];
+                load_floats(a.part + q * D + d, x[u]);
+            } else {
+                st[u] = make_float2(-FLT_MAX, 0.f);
+                x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.f;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
+#pragma unroll
+        for (int u = 0; u < U; ++u) join_in(m, l, s, st[u].x, st[u].y, x[u]);
+    }
+    // the wave's four pieces, then the waves
+    auto over_rows = [](float v, auto&& op) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+        const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return op(__uint_as_float(q[0]), __uint_as_float(q[1]));
+    };
+    auto add = [](float x, float y) { return x + y; };
+    const float top = over_rows(m, [](float x, float y) { return fmaxf(x, y); }), f = __builtin_amdgcn_exp2f(m - top);
+    l = over_rows(l * f, add);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = over_rows(s[i] * f, add);
+    if (lane < 16) st4(&sums[wv][4 * lane], make_float4(s[0], s[1], s[2], s[3]));
+    if (lane == 0) {
+        ms[wv] = top;
+        ls[wv] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const size_t o = static_cast<size_t>(pair) * D + d - 4 * (lane & 15) + lane;
+    const float gate = a.gate ? a.gate[o] : 0.f;
+    float all = ms[0], sum = 0.f, tot = 0.f;
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w) all = fmaxf(all, ms[w]);
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) {
+        const float k = __builtin_amdgcn_exp2f(ms[w] - all);
+        sum += k * sums[w][lane];
+        tot += k * ls[w];
+    }
+    a.out[o] = finished(all, sum, tot, a.gate, gate);
+}
+
+// Many pairs. NW > 1: a workgroup of NW waves per pair, wave w takes pieces w, w + NW, ...; NW = 1: a wave per pair, and each wave
+// looks at `per` pairs at once, because in a prompt's call most are there already. Lanes hold the dims.
 template <int D, int NW>
 __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel(const Attn4Args a, int per) {
     constexpr int V = D / kWave;
     __shared__ float sums[NW][NW == 1 ? 1 : D], ls[NW], ms[NW];
     const int lane = threadIdx.x & 63, wv = NW == 1 ? 0 : wave_in_block();
-    // Pairs of the requests' rows alone: only those have an entry of this call (the workspace may hold an earlier one's).
-    const int from = min(max(a.row_start[0], 0), a.rows) * a.heads, live = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;
     const int64_t pair0 = NW == 1 ? (static_cast<int64_t>(blockIdx.x) * 4 + wave_in_block()) * per : blockIdx.x;
-    int2 in = make_int2(0, 0);
-    if (lane < (NW == 1 ? per : 1) && pair0 + lane >= from && pair0 + lane < live) in = a.info[pair0 + lane];
-    // one piece is there already; starts that decrease may leave anything
-    uint64_t todo = __ballot(in.y > 1 && in.x >= 0 && in.y <= a.all_items - in.x / kRows);   // the same in every wave of a pair
+    const int2 in = entry(a, pair0 + lane, lane < (NW == 1 ? per : 1));
+    uint64_t todo = __ballot(in.y > 0);   // the same in every wave of a pair
     while (todo) {
         const int k = __builtin_ctzll(todo);
         todo &= todo - 1;
@@ -1207,34 +1291,23 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel
 #pragma unroll
         for (int i = 0; i < V; ++i) s[i] = gate[i] = 0.f;
         if (NW == 1 && a.gate) load_floats(a.gate + o + V * lane, gate);
-        auto take = [&](auto uI) {   // so many pieces in flight
-            constexpr int U = decltype(uI)::value;
-            for (int p0 = wv; p0 < pieces; p0 += U * NW) {
-                float2 st[U];
-                float x[U][V];
+        constexpr int U = 4;   // pieces in flight
+        for (int p0 = wv; p0 < pieces; p0 += U * NW) {
+            float2 st[U];
+            float x[U][V];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const size_t q = static_cast<size_t>(first + min(p0 + u * NW, pieces - 1)) * kRows + slot;
-                    st[u] = a.stat[q];
-                    load_floats(a.part + q * D + V * lane, x[u]);
-                }
-                __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (p0 + u * NW >= pieces) break;
-                    const float now = fmaxf(m, st[u].x);
-                    const float was = __builtin_amdgcn_exp2f(m - now), f = __builtin_amdgcn_exp2f(st[u].x - now);
-                    m = now;
-                    l = l * was + st[u].y * f;
-#pragma unroll
-                    for (int i = 0; i < V; ++i) s[i] = s[i] * was + x[u][i] * f;
-                }
+            for (int u = 0; u < U; ++u) {
+                const size_t q = static_cast<size_t>(first + min(p0 + u * NW, pieces - 1)) * kRows + slot;
+                st[u] = a.stat[q];
+                load_floats(a.part + q * D + V * lane, x[u]);
             }
-        };
-        if (NW == 16 && pieces > 4 * NW)   // (one token at 200000 keys: 7.7 us with 4 in flight, 5.9 with 16; at 2000 keys 3.9, 6.6)
-            take(IC<16>{});
-        else
-            take(IC<4>{});
+            __builtin_amdgcn_sched_barrier(0);   // all U loads before the first use
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p0 + u * NW >= pieces) break;
+                join_in(m, l, s, st[u].x, st[u].y, x[u]);
+            }
+        }
         if constexpr (NW == 1) {
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] = finished(m, s[i], l, a.gate, gate[i]);
@@ -1329,7 +1402,7 @@ void launch(const Attn4Args& a, hipStream_t s) {
     }
     const unsigned pairs = static_cast<unsigned>(a.rows) * static_cast<unsigned>(a.heads);
     if (pairs <= 128)   // few rows: many pieces each
-        join4_kernel<D, 16><<<pairs, 16 * kWave, 0, s>>>(a, 1);
+        join4_few<D><<<pairs * (D / 64), kJoinWaves * kWave, 0, s>>>(a);
     else if (pairs <= 2048)
         join4_kernel<D, 4><<<pairs, 4 * kWave, 0, s>>>(a, 1);
     else if (pairs <= kPromptFill / 2 * kPromptRows)   // a cut prompt's pairs may all have pieces
