@@ -34,7 +34,7 @@ leaves the history and state where T decode steps leave them.
 `MoeLayerDecode.prefill(xs)` runs many tokens through the MoE layer, each
 expert's tokens together, and `AttnLayerBatch.forward(xs, ...)` a step of several
 requests - single tokens and prompts - through an attention layer whose keys and
-values lie in a paged 8-bit cache.
+values lie in a paged cache of 8 or 4 bits, at positions of one axis or several.
 """
 
 from __future__ import annotations
@@ -219,7 +219,8 @@ class AttnLayerDecode:
 
 class AttnLayerBatch:
     """An attention layer (the weights of an `AttnLayerDecode`) over a batch of requests, its keys and values in a paged
-    8-bit cache of its own. The pages' bookkeeping is the same for every layer, so a step is planned once:
+    cache of its own, of 8 bits a number or (`cache_bits=4`) of 4. The pages' bookkeeping is the same for every layer and
+    either cache, so a step is planned once:
 
         plan = ops.kv8_plan(cached, fresh, table, free, head, page_size, rows)
         for layer in layers: ... x = layer.forward(x, table, plan)
@@ -228,15 +229,28 @@ class AttnLayerBatch:
     projections in one `matmul_rows_multi`, the split, `attn_qk_norm_rope_rows` at the plan's positions,
     `kv8_store_rows`, `attn_kv8_rows` with the gate, the output projection. Rows behind the last request's give
     nothing of use. The layer's own fp32 cache is not used: its max_seq_len may be 1. Nothing leaves the device, so a step
-    of fixed `rows` can be captured in a graph."""
+    of fixed `rows` can be captured in a graph.
 
-    def __init__(self, layer: AttnLayerDecode, pages, page_size=64):
-        self.layer = layer
-        self.cache = ops.kv8_cache(pages, layer.kvh, layer.hd, page_size, layer.q_norm.device)
+    With `cache_bits=4` the cache calls are `kv4_store_rows` and `attn_kv4_rows`. With `rope_sections` (pairs of each axis, a
+    sum of rope_dim / 2; dealt in turns unless `rope_interleaved` is False) tokens have a position of several axes, as images'
+    have: `forward` takes them as `positions`, int32 [axes, rows], and `attn_qk_norm_mrope_rows` rotates by them. Which keys a
+    token sees goes by its place in its request either way, the plan's."""
 
-    def forward(self, xs, block_table, plan, out=None):
+    def __init__(self, layer: AttnLayerDecode, pages, page_size=64, cache_bits=8, rope_sections=None, rope_interleaved=True):
+        if cache_bits not in (4, 8):
+            raise ValueError("cache_bits has to be 4 or 8")
+        if rope_sections is not None and 2 * sum(rope_sections) != layer.rope_dim:
+            raise ValueError("rope_sections have to sum to rope_dim / 2")
+        self.layer, self.sections, self.interleaved = layer, rope_sections, rope_interleaved
+        new, self.store, self.attend = ((ops.kv8_cache, ops.kv8_store_rows, ops.attn_kv8_rows) if cache_bits == 8 else
+                                        (ops.kv4_cache, ops.kv4_store_rows, ops.attn_kv4_rows))
+        self.cache = new(pages, layer.kvh, layer.hd, page_size, layer.q_norm.device)
+
+    def forward(self, xs, block_table, plan, out=None, positions=None):
         a, T = self.layer, xs.shape[0]
         row_start, kv_len, slots, pos, _ = plan
+        if (positions is None) != (self.sections is None):
+            raise ValueError("positions of several axes go with rope_sections")
         out = torch.empty_like(xs) if out is None else out
         ws = torch.empty(max(1, ops.matmul_rows_workspace_bytes(T, a.dm), ops.matmul_rows_workspace_bytes(T, a.qd)),
                          dtype=torch.uint8, device=xs.device)
@@ -244,10 +258,13 @@ class AttnLayerBatch:
                                           for n in ("qg", "k", "v")], xs, a.dm, workspace=ws)
         q, gate = (t.view(T, a.h, a.hd) for t in ops.attn_split_qg(qg, T * a.h, a.hd))
         k, v = k.view(T, a.kvh, a.hd), v.view(T, a.kvh, a.hd)
-        ops.attn_qk_norm_rope_rows(q, k, a.q_norm, a.k_norm, pos=pos, rope_dim=a.rope_dim, theta=a.theta, eps=a.eps)
-        ops.kv8_store_rows(k, v, slots, self.cache)
+        if self.sections is None:
+            ops.attn_qk_norm_rope_rows(q, k, a.q_norm, a.k_norm, pos=pos, rope_dim=a.rope_dim, theta=a.theta, eps=a.eps)
+        else:
+            ops.attn_qk_norm_mrope_rows(q, k, a.q_norm, a.k_norm, positions, self.sections, self.interleaved, a.theta, a.eps)
+        self.store(k, v, slots, self.cache)
         # zeros in the rows behind the last request's, which attention leaves alone and the projection reads
-        gated = ops.attn_kv8_rows(q, self.cache, block_table, row_start, kv_len, gate=gate, out=torch.zeros_like(q))
+        gated = self.attend(q, self.cache, block_table, row_start, kv_len, gate=gate, out=torch.zeros_like(q))
         w, M = a.w["out"]
         return ops.matmul_rows(w, a.wtype, M * a.qd, gated.view(T, a.qd), M, a.qd, out=out, workspace=ws)
 
