@@ -67,15 +67,15 @@ struct Attn4Args {
     const int32_t* row_start;
     const int32_t* kv_len;
     int max_pages, page_shift, requests, rows, heads, group;
-    float* part;         // [item][kRows][D] sums of p v
-    float2* stat;        // [item][kRows] (m, l)
-    int2* info;          // [row][head] (first item * kRows + row in item, pieces); written for the requests' rows alone
-    int items;           // split4_kernel's grid, and what `part` and `stat` hold of it
-    int all_items;       // and with the cut prompts' pieces
+    float* part;         // [place][D] sums of p v, where Places says
+    float2* stat;        // [place] (m, l)
+    int2* info;          // [row][head] (place of the first piece, pieces); written for the requests' rows alone
+    int items;           // split4_kernel's grid, each with kRows places
     int places;          // split4_kernel's workgroups that the card holds at once
     int split_all;       // every request takes split4_kernel
     int units;           // at most
     int whole;           // and every unit's tiles are one piece: nothing is joined
+    int prompt_step;     // tiles of a step of prompt4_kernel's line (a power of two)
     float scale;         // log2(e) / sqrt(D)
 };
 
@@ -105,6 +105,7 @@ __device__ __forceinline__ int wave_prefix(int v) {
 #undef QK_STEP
     return v;
 }
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
 
 // Piece `item` of the call: request, which of its units (KV head, row block), which piece of the unit's tiles. Every wave
 // finds it by itself from the lengths. No piece has more than `cut` tiles, a unit's pieces are of one size, and both are whole
@@ -274,10 +275,18 @@ __device__ __forceinline__ uint32_t sizes2(uint32_t scale, uint32_t low) {
 // score + log2(size) + 127
 __device__ __forceinline__ float log2_over(float score, uint32_t b) { return __builtin_fmaf(static_cast<float>(b), 0x1p-7f, score); }
 
+// v / (1 + e^-x). Below kFarGate, where e^-x leaves the range, e^x as the square of e^(x/2): subnormal results too. Without a
+// branch a value, with which the prompts' outputs took 4500 instructions a wave.
+constexpr float kFarGate = -80.0f;
+__device__ __forceinline__ float near_gated(float v, float x) { return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e)); }
+__device__ __forceinline__ float gated_by(float v, float x) {
+    const float t = __builtin_amdgcn_exp2f(x * (0.5f * kLog2e));
+    return x < kFarGate ? v * (t * t) : near_gated(v, x);
+}
 // An output from its sums: zero where no key was seen (a weight may be 0 beside a NaN).
 __device__ __forceinline__ float finished(float m, float sum, float tot, bool gated, float gate) {
     const float v = m == -FLT_MAX && tot == 0.f ? 0.f : sum / tot;
-    return gated ? v * sigmoid(gate) : v;
+    return gated ? gated_by(v, gate) : v;
 }
 // 2, 4 or 8 neighbouring floats, as aligned as they are many
 template <int N>
@@ -697,12 +706,41 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
 // The scores^T tile has token rho = 8 b + 4 g + j of the 32 in register 4 b + j of lane half g; key row rho stands for token
 // 16 (b / 2) + 8 g + 4 (b % 2) + j, so that a lane's registers 8 s .. 8 s + 7 are octet 2 s + g, its share of the second
 // product's depth s.
+
+// A workgroup has its CU to itself at D = 256 (registers). A unit (a row tile and a KV head) costs 20 us beside its tiles' 2.2 us
+// each: its queries, the first tiles' way to the products, its outputs. How a call's units meet the CUs:
+// - pieces: up to kPromptFill units, each cut in pieces of at most so many tiles that all pieces are at most kPromptFill;
+// - a line: all units' tiles one after the other, kPromptCost more in front of each unit, cut in kPromptFill equal parts. A workgroup takes
+//   its part's segments of units in turn. Of fewer than kPromptCut units, where a part is shorter than the longest piece would be;
+// - of more, a workgroup a unit, the longest first.
+// (Only pieces, of one number for all units: 2048 rows 144 us, now 123; 1100 rows 91, now 66.)
+struct Line {
+    int over, parts, base, more;   // steps in front of a unit; the first `more` parts have base + 1 steps, the others base
+    __device__ __forceinline__ Line(int over, int steps, int most) : over(over) {
+        parts = __builtin_amdgcn_readfirstlane(min(most, steps));
+        base = __builtin_amdgcn_readfirstlane(steps / max(parts, 1));
+        more = __builtin_amdgcn_readfirstlane(steps - base * parts);
+    }
+    __device__ __forceinline__ int start(int i) const { return i * base + min(i, more); }
+    __device__ __forceinline__ int part_of(int step) const {
+        const int wide = more * (base + 1);
+        return step < wide ? step / (base + 1) : more + (step - wide) / base;
+    }
+    // The pieces of a unit that starts at `at`.
+    __device__ __forceinline__ int pieces(int at, int steps) const { return part_of(at + over + steps - 1) - part_of(at + over) + 1; }
+};
+// Where the pieces of a unit lie. split4_kernel's are neighbours, kRows places each. A workgroup of prompt4_kernel has kPromptRows places
+// for the piece that ends its first unit, or passes through it, and in a second region as many for the one that begins its last.
+struct Places {
+    int first, rows, second;   // of a row: the first piece's place in the first region; the second region's distance, or 0
+    __device__ __forceinline__ int of(int piece) const { return first + (piece == 0 ? second : piece * rows); }
+};
 constexpr int kPromptWaves = 4;
 constexpr int kPromptRows = 32 * kPromptWaves;
-// A workgroup has its CU to itself at D = 256 (registers). If a call has less than half as many of them as the card has CUs,
-// each one's keys are cut into pieces of at least kPromptMinTiles tiles, up to one piece a CU.
 constexpr int kPromptFill = 256;
-constexpr int kPromptMinTiles = 4;
+constexpr int kPromptMinTiles = 4;   // of a piece
+constexpr int kPromptCut = 2 * kPromptFill;   // units that are still a line
+constexpr int kPromptCost = 10;  // of a unit, in tiles
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 template <int S>
@@ -716,6 +754,10 @@ __device__ __forceinline__ void static_for(F&& f) {
     static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
+__device__ __forceinline__ Request4 uniform(const Request4& r) {
+    return Request4{__builtin_amdgcn_readfirstlane(r.first), __builtin_amdgcn_readfirstlane(r.n), __builtin_amdgcn_readfirstlane(r.len),
+                    __builtin_amdgcn_readfirstlane(static_cast<int>(r.bad)) != 0};
+}
 template <int D>
 __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const Attn4Args a) {
     constexpr int ND = D / 16, DT = D / 32, NG = D / 64, E = D / 64, NTH = kPromptWaves * kWave;   // E: a lane's words of a tile's
@@ -723,51 +765,147 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     __shared__ __align__(16) f16x8_t ks[2][ND][kWave];                                             // GL: groups of those words
     __shared__ __align__(16) f16x8_t vs[2][DT][2][kWave];
     __shared__ __align__(16) uint16_t kmin[4][kTile][8];   // [tile % 4][key row]: bf16, the groups' minima (4) and 8 scale (4)
+    __shared__ __align__(16) float outs[kPromptWaves][32][64 + 4];   // a wave's rows, 64 dims; 4 more, and 8 rows meet no bank twice
+    __shared__ int2 out_rows[kPromptWaves][32];            // what a row's sums are taken times, where they go (-1: nowhere)
     __shared__ __align__(16) float tok[4][4][kTile];       // [tile % 4][key factor, value scale, min + 8 scale, log2 size][token]
     // which request, KV head and row tile: the last row tiles (the longest rows) first
-    const int G = a.group, lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+    const int G = a.group;
     const float per_g = 1.0f / static_cast<float>(G);
     auto over_g = [&](int pair) { return quotient(pair, G, per_g); };
-    auto tiles_here = [&](int b) {   // workgroups of a request, before they are cut
-        if (b >= a.requests) return 0;
-        const Request4 r = request(a, b);
-        const int64_t n = (static_cast<int64_t>(r.n) * G + kPromptRows - 1) / kPromptRows * a.c.heads;
-        return takes_split(a, r) ? 0 : static_cast<int>(n < kMaxItems ? n : kMaxItems);
+    auto row_tiles = [&](const Request4& r) { return takes_split(a, r) ? 0 : (r.n * G + kPromptRows - 1) / kPromptRows; };
+    auto keys_seen = [&](const Request4& r, int rt) {   // by some row of a row tile
+        return max(r.len - r.n + over_g(min(rt * kPromptRows + kPromptRows - 1, r.n * G - 1)) + 1, 0);
     };
-    float total = 0.f;
-    for (int b0 = 0; b0 < a.requests; b0 += kWave) total += static_cast<float>(tiles_here(b0 + lane));
-    total = group_sum<kWave>(total);
-    if (total == 0.f) return;   // the whole workgroup
-    const int splits = total < kPromptFill ? __builtin_amdgcn_readfirstlane(kPromptFill / static_cast<int>(total)) : 1;
-    int b = -1, item = static_cast<int>(blockIdx.x) / splits;
-    const int split = static_cast<int>(blockIdx.x) - item * splits;
-    for (int b0 = 0; b0 < a.requests && b < 0; b0 += kWave) {
-        const int n = tiles_here(b0 + lane), upto = wave_prefix(n);
-        const uint64_t hit = __ballot(item < upto);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            item -= __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
-            b = b0 + l;
-        } else {
-            item -= __builtin_amdgcn_readlane(upto, 63);
+    const int step_bits = __builtin_ctz(a.prompt_step);
+    auto steps_of = [&](int seen) { return max(1, (seen + kTile * a.prompt_step - 1) >> (5 + step_bits)); };
+    // The requests that have row tiles, in turn, until `look` says that it has found what it wants.
+    auto lane_request = [&](int b) { return b < a.requests ? request(a, b) : Request4{0, 0, 0, false}; };
+    const int lane0 = threadIdx.x & 63;
+    const Request4 held = lane_request(lane0);   // every look is at these first
+    auto each_request = [&](auto&& look) {
+        for (int b0 = 0; b0 < a.requests; b0 += kWave) {
+            const Request4 r = b0 ? lane_request(b0 + lane0) : held;
+            uint64_t hit = __ballot(row_tiles(r) > 0);
+            while (hit) {
+                const int l = __builtin_ctzll(hit);
+                hit &= hit - 1;
+                const Request4 one{__builtin_amdgcn_readlane(r.first, l), __builtin_amdgcn_readlane(r.n, l), __builtin_amdgcn_readlane(r.len, l),
+                                   __builtin_amdgcn_readlane(static_cast<int>(r.bad), l) != 0};
+                if (look(b0 + l, one)) return;
+            }
         }
+    };
+    float units = static_cast<float>(row_tiles(held)) * static_cast<float>(a.c.heads);
+    for (int b0 = kWave; b0 < a.requests; b0 += kWave) units += static_cast<float>(row_tiles(lane_request(b0 + lane0))) * static_cast<float>(a.c.heads);
+    units = group_sum<kWave>(units);
+    if (units == 0.f) return;   // the whole workgroup
+    const bool cut = units < static_cast<float>(kPromptCut);
+    Line line(0, 1, 1);
+    int cut_at = 0;   // steps of a piece at most; 0: not in pieces
+    int line_at = 0, line_end = 1;
+    int b = 0, unit = 0, unit_steps = 1, unit_at = 0;   // unit_at: where the line has it
+    Request4 r{0, 0, 0, false};
+    {
+        bool found = false;
+        if (cut) {
+            // A lane a row tile, all of a request's, in the order of the units; `of`: what a row tile of so many steps counts.
+            auto here = [&](const Request4& q, int k, auto&& of) {
+                const int n = row_tiles(q);
+                return k < n ? of(steps_of(keys_seen(q, n - 1 - k))) * a.c.heads : 0;
+            };
+            auto all = [&](auto&& of) {
+                int v = 0;
+                each_request([&](int, const Request4& q) {
+                    for (int k0 = 0; k0 < row_tiles(q); k0 += kWave) v += wave_total(here(q, k0 + lane0, of));
+                    return false;
+                });
+                return v;
+            };
+            int longest = 0;
+            each_request([&](int, const Request4& q) {
+                longest = max(longest, steps_of(keys_seen(q, row_tiles(q) - 1)));
+                return false;
+            });
+            const int steps = all([](int t) { return t; });
+            int pieces = kPromptFill + 1;
+            if (units <= static_cast<float>(kPromptFill)) {
+                cut_at = max((steps + kPromptFill - 1) / kPromptFill, (kPromptMinTiles + a.prompt_step - 1) >> step_bits);
+                for (int i = 0; i < 4; ++i) {
+                    pieces = all([&](int t) { return (t + cut_at - 1) / cut_at; });
+                    if (pieces <= kPromptFill) break;
+                    cut_at = max(static_cast<int>(static_cast<float>(cut_at) * static_cast<float>(pieces) * (1.0f / kPromptFill)), cut_at + 1);
+                }
+                if (pieces > kPromptFill) {
+                    cut_at = longest;
+                    pieces = static_cast<int>(units);
+                }
+            }
+            const int cost = max(kPromptCost >> step_bits, 1), in_line = steps + cost * static_cast<int>(units);
+            if (pieces > kPromptFill || max(in_line / kPromptFill, kPromptMinTiles >> step_bits) < min(cut_at, longest)) cut_at = 0;
+            line = cut_at ? Line(0, pieces, pieces) : Line(cost, in_line, kPromptFill);
+            if (static_cast<int>(blockIdx.x) >= line.parts) return;   // the whole workgroup
+            line_at = line.start(blockIdx.x);
+            line_end = line.start(blockIdx.x + 1);
+            int left = line_at;
+            each_request([&](int q_b, const Request4& q) {
+                for (int k0 = 0; k0 < row_tiles(q); k0 += kWave) {
+                    const int n = here(q, k0 + lane0, [&](int t) { return cut_at ? (t + cut_at - 1) / cut_at : t + line.over; }), upto = wave_prefix(n);
+                    const uint64_t hit = __ballot(left < upto);
+                    if (hit) {
+                        const int l = __builtin_ctzll(hit), each = __builtin_amdgcn_readlane(n, l) / a.c.heads;
+                        const int local = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l)), head = local / each;
+                        b = q_b;
+                        r = q;
+                        unit = (k0 + l) * a.c.heads + head;
+                        unit_steps = each - line.over;
+                        unit_at = line_at - (local - head * each);
+                        return found = true;
+                    }
+                    left -= __builtin_amdgcn_readlane(upto, 63);
+                }
+                return false;
+            });
+        } else {
+            int64_t left = blockIdx.x;
+            each_request([&](int q_b, const Request4& q) {
+                const int64_t n = static_cast<int64_t>(row_tiles(q)) * a.c.heads;
+                if (left >= n) {
+                    left -= n;
+                    return false;
+                }
+                b = q_b;
+                r = q;
+                unit = static_cast<int>(left);
+                return found = true;
+            });
+        }
+        if (!found) return;   // the whole workgroup
     }
-    if (b < 0) return;   // the whole workgroup
-    const Request4 r = request(a, b);
-    const int pairs = r.n * G, tiles = (pairs + kPromptRows - 1) / kPromptRows;
-    const int unit = __builtin_amdgcn_readfirstlane(item);
+    for (;;) {
+    int tid = threadIdx.x;
+    asm("" : "+v"(tid));   // what follows from it is not held from one segment to the next
+    const int lane = tid & 63, col = lane & 31, g = lane >> 5;
+    r = uniform(r);
+    b = __builtin_amdgcn_readfirstlane(b);
+    unit = __builtin_amdgcn_readfirstlane(unit);
+    unit_at = __builtin_amdgcn_readfirstlane(unit_at);
+    unit_steps = __builtin_amdgcn_readfirstlane(unit_steps);
+    const int pairs = r.n * G, tiles = row_tiles(r);
     const int h = unit % a.c.heads, rt = tiles - 1 - unit / a.c.heads;
-    const int wv = wave_in_block(), tid = threadIdx.x;
+    const int wv = wave_in_block();
     const int row0 = rt * kPromptRows + 32 * wv;             // the wave's first pair
     const int rr = min(row0 + col, pairs - 1);
     const int ti = over_g(rr), head = h * G + (rr - ti * G);
     const int limit = r.len - r.n + ti;
     const int wave_first = r.len - r.n + over_g(min(row0, pairs - 1));
-    const int seen = max(r.len - r.n + over_g(min(rt * kPromptRows + kPromptRows - 1, pairs - 1)) + 1, 0);
-    const int all_steps = (seen + kTile - 1) / kTile, pieces = min(splits, max(all_steps / kPromptMinTiles, 1));
-    if (split >= pieces) return;   // the whole workgroup
-    const int per = (all_steps + pieces - 1) / pieces;
-    const int first_tile = split * per, steps = max(min(per, all_steps - first_tile), 0);   // this piece's tiles
+    const int seen = keys_seen(r, rt);
+    const int all_steps = (seen + kTile - 1) / kTile;
+    const int from = max(line_at - unit_at - line.over, 0), to = min(line_end - unit_at - line.over, unit_steps);
+    if (to <= 0) return;   // the part ends before the unit's first step
+    const bool begins = from == 0, whole = begins && to == unit_steps;
+    const int step = (cut_at ? (steps_of(seen) + unit_steps - 1) / unit_steps : 1) * a.prompt_step;   // tiles
+    const int first_tile = whole ? 0 : __builtin_amdgcn_readfirstlane(from * step);
+    const int steps = __builtin_amdgcn_readfirstlane(whole ? all_steps : max(min(to * step, all_steps) - first_tile, 0));   // this segment's tiles
     const uint32_t magic = code_magic();
 
     // A wave brings one octet of tokens of each tile: page and offset are the same for its lanes. A lane's words: of keys
@@ -883,16 +1021,15 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
                 const float4 x = ld4(q + 16 * d + 4 * i);
                 f[d][4 * i] = x.x, f[d][4 * i + 1] = x.y, f[d][4 * i + 2] = x.z, f[d][4 * i + 3] = x.w;
             }
-        float m = 0.f;
-        bool bad = false;
+        float m = 0.f, bad = 0.f;   // 0, or NaN with an infinity or NaN
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 m = fmaxf(m, fabsf(f[d][i]));
-                bad |= !(fabsf(f[d][i]) <= FLT_MAX);
+                bad = __builtin_fmaf(f[d][i], 0.f, bad);
             }
-        if (bad) m = INFINITY;
+        if (bad != 0.f) m = INFINITY;
         m = fmaxf(m, __shfl_xor(m, 32));
         const bool ok = m <= FLT_MAX;
         int e = 0;
@@ -902,11 +1039,12 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
             e = min(15 - em, kMaxUp);
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float by = ldexpf(1.0f, e);   // what a row with infinities or NaNs gives here does not matter: factor is NaN
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = ok ? ldexpf(f[d][i], e) : 0.f;
+                const float v = f[d][i] * by;
                 Qh[d][i] = static_cast<_Float16>(v);
                 Ql[d][i] = static_cast<_Float16>(low_part(v));
                 sum[d >> 2] += v;
@@ -1112,9 +1250,17 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     }
     l += __shfl_xor(l, 32);
     low += __shfl_xor(low, 32);
-    if (row0 + col >= pairs) return;
-    if (r.bad) l = __builtin_nanf("");
-    const size_t o = (static_cast<size_t>(r.first + ti) * a.heads + head) * D;
+    // The outputs, or the sums of a piece, by way of LDS: a lane of the sums has 16 bytes of each of many rows, the lanes that
+    // write have whole lines.
+    if (g == 0) {
+        const bool none = mu == -FLT_MAX && l == 0.f, live = row0 + col < pairs;
+        const int pair = (r.first + ti) * a.heads + head, k = static_cast<int>(blockIdx.x) * kPromptRows + 32 * wv + col;
+        const int first = a.items * kRows + k, place = first + (begins ? kPromptFill * kPromptRows : 0);
+        const float by = !whole ? 1.f : none ? 0.f : 1.f / (r.bad ? __builtin_nanf("") : l);
+        out_rows[wv][col] = make_int2(__float_as_int(by), !live ? -1 : whole ? pair : place);
+        if (live && !whole) a.stat[place] = make_float2(mu, r.bad ? __builtin_nanf("") : l);
+        if (live && begins) a.info[pair] = whole ? make_int2(0, 1) : make_int2(first, line.pieces(unit_at, unit_steps));
+    }
     // 4 neighbouring dims, the n-th of DT * 4: of E value tiles of one register, or 2 of two, or one of four
     auto four = [&](int n, int& dim) {
         const int m = n * 4 / (16 * E), rest = n - m * 4 * E;   // tile group; 4 registers' 16 rows x E dims as 4 E fours
@@ -1137,62 +1283,91 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         }
         return make_float4(x[0] + low, x[1] + low, x[2] + low, x[3] + low);
     };
-    constexpr int FOURS = D / 8;   // of a lane: half of its row
-    if (pieces > 1) {   // row k of the tile is slot k % kRows of item first + k / kRows * splits + piece, as the join reads
-        const int k = 32 * wv + col;
-        const int unit_items = static_cast<int>(blockIdx.x) / splits * (kPromptRows / kRows);
-        const int item0 = a.items + (unit_items + k / kRows) * splits;
-        const size_t row = static_cast<size_t>(item0 + split) * kRows + k % kRows;
+    {
+        auto meet = []() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };   // of one wave
+        meet();
+        float* to_rows = whole ? a.out : a.part;
+        const bool gated = whole && a.gate;
+        const int dim0 = 4 * (lane & 15);
+        float by[8];
+        int64_t goes[8];
 #pragma unroll
-        for (int n = 0; n < FOURS; ++n) {
-            int dim;
-            const float4 x = four(n, dim);
-            st4(a.part + row * D + dim, x);
+        for (int j = 0; j < 8; ++j) {
+            const int2 x = out_rows[wv][4 * j + (lane >> 4)];
+            by[j] = __int_as_float(x.x);
+            goes[j] = x.y < 0 ? -1 : static_cast<int64_t>(x.y) * D + dim0;
         }
-        if (g == 0) {
-            a.stat[row] = make_float2(mu, l);
-            if (split == 0) a.info[o / D] = make_int2(item0 * kRows + k % kRows, pieces);
-        }
-        return;
-    }
-    const bool none = mu == -FLT_MAX && l == 0.f;
-    const float inv = 1.f / l;
-    constexpr int BATCH = 8;   // gates requested together
+        float4 gates[2][8];   // of 64 dims, requested before the 64 before them
+        auto ask_gates = [&](int c) {
 #pragma unroll
-    for (int n0 = 0; n0 < FOURS; n0 += BATCH) {
-        float4 x[BATCH], gt[BATCH];
-        int dim[BATCH];
+            for (int j = 0; j < 8; ++j)
+                if (gated && goes[j] >= 0) gates[c & 1][j] = ld4(a.gate + goes[j] + 64 * c);
+        };
+        ask_gates(0);
 #pragma unroll
-        for (int n = 0; n < BATCH; ++n) {
-            x[n] = four(n0 + n, dim[n]);
-            if (a.gate) gt[n] = ld4(a.gate + o + dim[n]);
-        }
+        for (int c = 0; c < D / 64; ++c) {
+            if (c + 1 < D / 64) ask_gates(c + 1);
 #pragma unroll
-        for (int n = 0; n < BATCH; ++n) {
-            float v[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = none ? 0.f : v[i] * inv;
-            if (a.gate) {
-                v[0] *= sigmoid(gt[n].x);
-                v[1] *= sigmoid(gt[n].y);
-                v[2] *= sigmoid(gt[n].z);
-                v[3] *= sigmoid(gt[n].w);
+            for (int n = 8 * c; n < 8 * c + 8; ++n) {
+                int dim;
+                const float4 x = four(n, dim);
+                st4(&outs[wv][col][dim - 64 * c], x);
             }
-            st4(a.out + o + dim[n], make_float4(v[0], v[1], v[2], v[3]));
+            meet();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float4 x = ld4(&outs[wv][4 * j + (lane >> 4)][dim0]);
+                x = make_float4(x.x * by[j], x.y * by[j], x.z * by[j], x.w * by[j]);
+                if (gated) {
+                    const float4 y = gates[c & 1][j];
+                    if (__ballot(fminf(fminf(y.x, y.y), fminf(y.z, y.w)) < kFarGate))
+                        x = make_float4(gated_by(x.x, y.x), gated_by(x.y, y.y), gated_by(x.z, y.z), gated_by(x.w, y.w));
+                    else
+                        x = make_float4(near_gated(x.x, y.x), near_gated(x.y, y.y), near_gated(x.z, y.z), near_gated(x.w, y.w));
+                }
+                if (goes[j] >= 0) st4(to_rows + goes[j] + 64 * c, x);
+            }
+            meet();
         }
     }
-    if (g == 0) a.info[o / D] = make_int2(0, 1);
+    if (!cut) return;
+    line_at = unit_at = unit_at + line.over + unit_steps;   // the unit's end
+    if (cut_at || line_at >= line_end) return;
+    if (++unit == tiles * a.c.heads) {   // the next request that has row tiles
+        unit = 0;
+        uint64_t hit = 0;
+        for (int b0 = b + 1; b0 < a.requests; b0 += kWave) {
+            const Request4 q = b0 + lane < a.requests ? request(a, b0 + lane) : Request4{0, 0, 0, false};
+            hit = __ballot(row_tiles(q) > 0);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                b = b0 + l;
+                r = Request4{__builtin_amdgcn_readlane(q.first, l), __builtin_amdgcn_readlane(q.n, l), __builtin_amdgcn_readlane(q.len, l),
+                             __builtin_amdgcn_readlane(static_cast<int>(q.bad), l) != 0};
+                break;
+            }
+        }
+        if (!hit) return;
+    }
+    unit_steps = steps_of(keys_seen(r, row_tiles(r) - 1 - unit / a.c.heads));
+    __syncthreads();   // the last tile has been read from LDS
+    }
 }
 
 // ------------------------------------------------------------------ join
 // Joins the pieces of (row, head) pairs. `entry`: where a pair's pieces are, (0, 0) where nothing is to be joined.
+__device__ __forceinline__ Places places(const Attn4Args& a, int first) {
+    return first < a.items * kRows ? Places{first, kRows, 0} : Places{first, kPromptRows, kPromptFill * kPromptRows};
+}
 __device__ __forceinline__ int2 entry(const Attn4Args& a, int64_t pair, bool live) {
     // Pairs of the requests' rows alone: only those have an entry of this call (the workspace may hold an earlier one's).
     const int from = min(max(a.row_start[0], 0), a.rows) * a.heads, end = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;
     int2 in = make_int2(0, 0);
     if (live && pair >= from && pair < end) in = a.info[pair];
     // one piece is there already; starts that decrease may leave anything
-    return in.y > 1 && in.x >= 0 && in.y <= a.all_items - in.x / kRows ? in : make_int2(0, 0);
+    const Places p = places(a, in.x);
+    const int past = a.items * kRows + p.second;
+    return in.y > 1 && in.x >= 0 && in.x < past && in.y <= (past - in.x - 1) / p.rows + 1 ? in : make_int2(0, 0);
 }
 // The join of two parts of a sum with their references: (m, l, s) takes in (n, k, x).
 template <int V>
@@ -1217,7 +1392,8 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void join4_few(const Attn4Args a
     const int pair = static_cast<int>(blockIdx.x) / PARTS, d = 64 * (static_cast<int>(blockIdx.x) % PARTS) + 4 * (lane & 15);
     const int2 in = entry(a, pair, true);
     if (in.y == 0) return;   // the whole workgroup
-    const int pieces = in.y, slot = in.x % kRows, first = in.x / kRows;
+    const int pieces = in.y;
+    const Places place = places(a, in.x);
     float m = -FLT_MAX, l = 0.f, s[4] = {0.f, 0.f, 0.f, 0.f};
     constexpr int U = 8;   // in flight
     for (int p0 = mine; p0 < pieces; p0 += U * LANES) {
@@ -1226,7 +1402,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void join4_few(const Attn4Args a
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (p0 + u * LANES < pieces) {
-                const size_t q = static_cast<size_t>(first + p0 + u * LANES) * kRows + slot;
+                const size_t q = place.of(p0 + u * LANES);
                 st[u] = a.stat[q];
                 load_floats(a.part + q * D + d, x[u]);
             } else {
@@ -1284,8 +1460,8 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel
     while (todo) {
         const int k = __builtin_ctzll(todo);
         todo &= todo - 1;
-        const int pieces = __builtin_amdgcn_readlane(in.y, k), where = __builtin_amdgcn_readlane(in.x, k);
-        const int slot = where % kRows, first = where / kRows;
+        const int pieces = __builtin_amdgcn_readlane(in.y, k);
+        const Places place = places(a, __builtin_amdgcn_readlane(in.x, k));
         const size_t o = static_cast<size_t>(pair0 + k) * D;
         float m = -FLT_MAX, l = 0.f, s[V], gate[V];
 #pragma unroll
@@ -1297,7 +1473,7 @@ __global__ __launch_bounds__(NW == 1 ? 4 * kWave : NW * kWave) void join4_kernel
             float x[U][V];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const size_t q = static_cast<size_t>(first + min(p0 + u * NW, pieces - 1)) * kRows + slot;
+                const size_t q = place.of(min(p0 + u * NW, pieces - 1));
                 st[u] = a.stat[q];
                 load_floats(a.part + q * D + V * lane, x[u]);
             }
@@ -1365,18 +1541,18 @@ int64_t item_bound(int rows, int requests, int heads, int kv_heads, int dim) {
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
 struct Layout {
-    int64_t items, all;   // pieces of 8 rows: of split4_kernel, and with those of prompt4_kernel
+    int64_t items;   // pieces of split4_kernel
     size_t stat, info, bytes;
 };
 Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     Layout l;
     l.items = item_bound(rows, requests, heads, kv_heads, dim);
-    l.all = l.items;
+    int64_t places = l.items * kRows;
     // Room for cut prompts by the rows alone, though a call with no more rows than requests has none: a workspace for some
     // rows and requests has to serve fewer of either.
-    if (rows > 1 && static_cast<int64_t>(rows) * (heads / kv_heads) > kSplitMax) l.all += kPromptFill * (kPromptRows / kRows);
-    l.stat = align_up(static_cast<size_t>(l.all) * kRows * dim * 4);
-    l.info = l.stat + align_up(static_cast<size_t>(l.all) * kRows * 8);
+    if (rows > 1 && static_cast<int64_t>(rows) * (heads / kv_heads) > kSplitMax) places += 2 * kPromptFill * kPromptRows;
+    l.stat = align_up(static_cast<size_t>(places) * dim * 4);
+    l.info = l.stat + align_up(static_cast<size_t>(places) * 8);
     l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);
     return l;
 }
@@ -1469,11 +1645,12 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     a.stat = reinterpret_cast<float2*>(ws + l.stat);
     a.info = reinterpret_cast<int2*>(ws + l.info);
     a.items = static_cast<int>(l.items);
-    a.all_items = static_cast<int>(l.all);
     a.split_all = !may_prompt(rows, requests, a.group);
     a.units = static_cast<int>(unit_bound(rows, requests, heads, kv_heads));
     a.whole = a.split_all && static_cast<int64_t>(max_pages) * page_size <= kWhole * kTile;
     a.places = kCus * places_on_cu(dim);
+    a.prompt_step = 1;   // a line is below 2^30 steps, in 32 bits
+    while (kPromptCut * (static_cast<int64_t>(max_pages) * page_size / (kTile * a.prompt_step) + 1 + kPromptCost) >= (1 << 30)) a.prompt_step *= 2;
     const hipStream_t s = as_stream(stream);
     if (dim == 64)
         launch<64>(a, s);

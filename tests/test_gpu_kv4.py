@@ -298,6 +298,33 @@ def test_attention_prompts_in_pieces(heads, kvh, dim, page):
     attention_case(r, [1100, 900, 530, 64], [50, 1, 35, 40], heads, kvh, dim, page, pad=2)
 
 
+@pytest.mark.parametrize("lens,fresh,heads,kvh", [
+    ([70 + i for i in range(30)], [70] * 30, 16, 2),   # more row tiles than CUs, each short
+    ([1000], [1000], 32, 1),                           # nearly as many as CUs, of 1 to 32 tiles
+    ([500, 1, 0, 1700], [400, 1, 0, 600], 32, 1),
+    ([40] * 60, [40] * 60, 16, 2),
+])
+def test_attention_prompts_as_a_line(lens, fresh, heads, kvh):
+    """Calls whose row tiles and KV heads are cut as one line of tiles: workgroups with the ends and the beginnings of several."""
+    r = np.random.default_rng(len(lens) + heads)
+    attention_case(r, lens, fresh, heads, kvh, 64, 32, gated=len(lens) > 1, pad=1)
+
+
+def test_attention_gate_sizes():
+    """Gates to where e^-x and e^x leave the range of fp32; below it results are subnormal numbers, as near as their step."""
+    r = np.random.default_rng(17)
+    for n in (1, 40):
+        lens = np.array([n + 20])
+        table, pages = tables(r, lens, 16)
+        ref = random_cache(r, pages, 2, 16, 64)
+        start = np.array([0, n], I32)
+        q = r.standard_normal((n, 8, 64)).astype(F32)
+        gate = r.choice(np.array([-200, -104, -100, -95, -90, -88, -87, -81, -80, -79, -1, 0, 60, 90, 200], F32), (n, 8, 64))
+        got = host(ops.attn_kv4_rows(dev(q), gpu_cache(ref), dev(table), dev(start), dev(lens, I32), gate=dev(gate)))
+        want, tol = kv4_ref.attention(q, ref, table, start, lens, gate)
+        close(got, want, tol + 2.0 ** -147)   # two roundings to subnormal numbers
+
+
 def test_attention_no_more_rows_than_requests():
     """A batch padded to many requests, one of which has most of the rows."""
     r = np.random.default_rng(33)
