@@ -249,7 +249,22 @@ __device__ __forceinline__ float rounded(float v) {
     asm("" : "+v"(v));
     return v;
 }
-// (exact; as an fma of the half number one instruction with its conversion)
+// Two values' high parts as a word, and the rest of one of them behind its high part: exact, and in one instruction, which takes
+// the half number as it lies in the word. (The compiler turns that fma to a conversion of its own and a subtraction.)
+__device__ __forceinline__ uint32_t high_parts(float a, float b) {
+    const f16x2_t h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, h);
+}
+template <int HALF>
+__device__ __forceinline__ float rest_of(uint32_t high, float v) {
+    float r;
+    if constexpr (HALF == 0)
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(high), "v"(v));
+    else
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(high), "v"(v));
+    return r;
+}
+// v less its own fp16 part, exact
 __device__ __forceinline__ float low_part(float v) { return __builtin_fmaf(static_cast<float>(static_cast<_Float16>(v)), -1.0f, v); }
 __device__ __forceinline__ float bf16_part(float v, int part) {   // bf16 part 0, 1, 2 of v, as an fp32 number
 #pragma unroll
@@ -607,20 +622,24 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[m][e][i] *= shrink;
         }
-        f16x2_t high[2], rest[2];
+        uint32_t high[2], rest[2];
+        float w0 = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float p = __builtin_amdgcn_exp2f(s[i] - mu);
             l += p;
             low = __builtin_fmaf(p, mv[i], low);
             const float w = rounded(p * sv[i]);
-            high[i >> 1][i & 1] = static_cast<_Float16>(w);
-            rest[i >> 1][i & 1] = static_cast<_Float16>(low_part(w));
+            if (i & 1) {
+                high[i >> 1] = high_parts(w0, w);
+                rest[i >> 1] = high_parts(rest_of<0>(high[i >> 1], w0), rest_of<1>(high[i >> 1], w));
+            }
+            w0 = w;
         }
         u32x4_t W;   // tokens 8 lk + 0..7 of this column's part: half of them from the lane beside
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t x = __builtin_bit_cast(uint32_t, high[j]), y = __builtin_bit_cast(uint32_t, rest[j]);
+            const uint32_t x = high[j], y = rest[j];
             const uint32_t got = __float_as_uint(dpp_move<0xB1>(__uint_as_float(part ? x : y)));
             W[j] = part ? got : x;
             W[2 + j] = part ? y : got;
@@ -1074,7 +1093,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
 #pragma unroll
     for (int i = 0; i < 16; ++i) zero[i] = 0.f;
     f32x16_t S, N;          // a tile's scores over `factor`; the next tile's products
-    f16x8_t Wh[2], Wl[2];   // weights of the last tile
+    u32x4_t Wh[2], Wl[2];   // weights of the last tile, pairs of fp16 numbers
     // the numbers of a lane's tokens 4 j .. 4 j + 3
     auto of_tokens = [&](const float* p, int j) { return ld4(p + 16 * (j >> 1) + 8 * g + 4 * (j & 1)); };
     // The operands of a step's products are one sequence, the last tile's values (2 DT of them), then the next tile's keys
@@ -1105,10 +1124,10 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         static_for<ND>([&](auto kI) {
             constexpr int k = decltype(kI)::value, d = k >> 1, s = k & 1;
             const f16x8_t x = A[k % AP];
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Wh[s], acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8_t, Wh[s]), acc[d], 0, 0, 0);
             fill(IC<2 * k>{});
             __builtin_amdgcn_sched_barrier(0);
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Wl[s], acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8_t, Wl[s]), acc[d], 0, 0, 0);
             ahead(kI);
             fill(IC<2 * k + 1>{});
             __builtin_amdgcn_sched_barrier(0);
@@ -1116,7 +1135,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     };
     for (int i = tid; i < DT * 2 * kWave; i += NTH) (&vs[1][0][0][0])[i] = f16x8_t{};   // the values before the first tile
 #pragma unroll
-    for (int s = 0; s < 2; ++s) Wh[s] = Wl[s] = f16x8_t{};
+    for (int s = 0; s < 2; ++s) Wh[s] = Wl[s] = u32x4_t{};
     if (steps > 0) {
         k_store(0);
         k_load(1);
@@ -1137,7 +1156,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     // Step st: tile st's products are in N. Its values and the keys of st + 2 go to LDS (slots whose last readers passed
     // the barrier before); the values of st - 1 are summed beside that and beside the scaling and maximum of the scores,
     // the scores of st + 1 beside the exponentials. One step more than tiles; before the first the weights are zero.
-    float top = 0.f, w0 = 0.f;
+    float top = 0.f, w0 = 0.f, z0 = 0.f;
     float4 kf[2], sz[2], sv[2], mv[2];   // of 4 tokens, and the 4 after them, requested when those come up
     auto pick = [](const float4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; };
     auto ask_scales = [&](int st, int j) {
@@ -1148,8 +1167,11 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         if (i % 4 == 0 && i < 12) ask_scales(st, i / 4 + 1);
         S[i] = N[i] * pick(kf[(i / 4) & 1], i & 3);
         const float z = __builtin_fmaf(S[i], factor, pick(sz[(i / 4) & 1], i & 3));
-        top = i ? fmaxf(top, z) : z;
-        asm volatile("" : "+v"(S[i]), "+v"(top));   // here, not where they are used
+        if (i & 1)
+            top = i == 1 ? fmaxf(z0, z) : fmaxf(fmaxf(z0, z), top);   // one instruction
+        else
+            z0 = z;
+        asm volatile("" : "+v"(S[i]), "+v"(top), "+v"(z0));   // here, not where they are used
     };
     auto weight = [&](int st, int i) {
         if (i % 4 == 0 && i < 12) {
@@ -1161,10 +1183,9 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         low = __builtin_fmaf(p, pick(mv[(i / 4) & 1], i & 3), low);
         const float w = rounded(p * pick(sv[(i / 4) & 1], i & 3));
         if (i & 1) {
-            Wh[i >> 3][(i & 7) - 1] = static_cast<_Float16>(w0);
-            Wh[i >> 3][i & 7] = static_cast<_Float16>(w);
-            Wl[i >> 3][(i & 7) - 1] = static_cast<_Float16>(low_part(w0));
-            Wl[i >> 3][i & 7] = static_cast<_Float16>(low_part(w));
+            const uint32_t h = high_parts(w0, w);
+            Wh[i >> 3][(i & 7) / 2] = h;
+            Wl[i >> 3][(i & 7) / 2] = high_parts(rest_of<0>(h, w0), rest_of<1>(h, w));
         }
         w0 = w;
     };
