@@ -123,7 +123,8 @@ __device__ __forceinline__ bool takes_split(const Attn4Args& a, const Request4& 
 }
 __device__ __forceinline__ float units_of(const Attn4Args& a, const Request4& r) {
     if (!takes_split(a, r)) return 0.f;
-    return static_cast<float>(((static_cast<uint32_t>(r.n) * static_cast<uint32_t>(a.group)) + kRows - 1) / kRows) * static_cast<float>(a.c.heads);
+    const uint32_t blocks = (static_cast<uint32_t>(r.n) * static_cast<uint32_t>(a.group) + kRows - 1) / kRows;
+    return static_cast<float>(blocks) * static_cast<float>(a.c.heads);
 }
 // n / d, both below 2^27, the quotient below 2^20; inverse within 2^-22 of 1 / d.
 __device__ __forceinline__ int quotient(int n, int d, float inverse) {
@@ -190,8 +191,8 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
             p.splits = __builtin_amdgcn_readlane(splits, l);
             p.unit = __builtin_amdgcn_readfirstlane(quotient(local, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))));
             p.split = local - p.unit * p.splits;
-            const int all = __builtin_amdgcn_readlane(t, l) + (kSplitWaves - 1);
-            p.tiles = a.whole ? cut : (quotient(all / kSplitWaves + p.splits - 1, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits)))) * kSplitWaves;
+            const int turns = (__builtin_amdgcn_readlane(t, l) + kSplitWaves - 1) / kSplitWaves;
+            p.tiles = a.whole ? cut : quotient(turns + p.splits - 1, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))) * kSplitWaves;
             if (b0 == 0) {
                 p.r.first = __builtin_amdgcn_readlane(first.first, l);
                 p.r.n = __builtin_amdgcn_readlane(first.n, l);
@@ -225,7 +226,8 @@ __device__ __forceinline__ uint32_t code_magic() {
 }
 template <int LESS>
 __device__ __forceinline__ f16x8_t codes8(uint32_t w, uint32_t magic) {
-    const f16x2_t down = {(_Float16)(-1024.0f - LESS), (_Float16)(-1024.0f - LESS)}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const f16x2_t down = {(_Float16)(-1024.0f - LESS), (_Float16)(-1024.0f - LESS)};
+    const f16x2_t sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     const f16x2_t down16 = {(_Float16)(-64.0f - LESS), (_Float16)(-64.0f - LESS)};
     f16x8_t r;
 #pragma unroll
@@ -293,7 +295,9 @@ __device__ __forceinline__ float log2_over(float score, uint32_t b) { return __b
 // v / (1 + e^-x). Below kFarGate, where e^-x leaves the range, e^x as the square of e^(x/2): subnormal results too. Without a
 // branch a value, with which the prompts' outputs took 4500 instructions a wave.
 constexpr float kFarGate = -80.0f;
-__device__ __forceinline__ float near_gated(float v, float x) { return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e)); }
+__device__ __forceinline__ float near_gated(float v, float x) {
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
+}
 __device__ __forceinline__ float gated_by(float v, float x) {
     const float t = __builtin_amdgcn_exp2f(x * (0.5f * kLog2e));
     return x < kFarGate ? v * (t * t) : near_gated(v, x);
@@ -329,11 +333,13 @@ __device__ __forceinline__ void store_floats(float* p, const float (&x)[N]) {
 }
 
 // ------------------------------------------------------------------ few rows
+// Bound by bytes and by vector instructions about alike: at 200000 keys the cache comes at 3.9 TB/s (5.8 more keys added to a long
+// call), and 610 instructions a tile and wave, 290 of them from codes to fp16 numbers, take 15 of the 28 us.
 // A workgroup takes 8 (row, head) pairs that share a KV head - 16 columns: 8 rows x 2 fp16 parts - and a range of 32-token
 // tiles, its NW waves every NW-th tile. A wave's tiles go straight from the cache to a ring of two places in LDS (no
-// registers wait for them), the next but one requested as soon as a tile has been taken to registers: one and a half tiles, 13 KB at D =
-// 256, are under way per wave. The two columns of a row share the work of the softmax: each of the two lanes takes half of the
-// tokens that both hold.
+// registers wait for them), the next but one requested as soon as a tile has been taken to registers: one and a half tiles,
+// 13 KB at D = 256, are under way per wave. The two columns of a row share the work of the softmax: each of the two lanes takes
+// half of the tokens that both hold.
 // WIDE: pages of 32 tokens and more, so that a tile lies in one page.
 //
 // A tile's place: keys, values, then k_scale, k_min, v_scale, v_min, each with its tokens in order. The keys' 16-byte pieces
@@ -373,7 +379,8 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
     const float per_g = __builtin_amdgcn_rcpf(static_cast<float>(G));
     auto over_g = [&](int pair) { return quotient(pair, G, per_g); };
     const int blocks = (pairs + kRows - 1) / kRows;
-    const int h = __builtin_amdgcn_readfirstlane(quotient(pc.unit, blocks, __builtin_amdgcn_rcpf(static_cast<float>(blocks)))), rb = pc.unit - h * blocks;
+    const int h = __builtin_amdgcn_readfirstlane(quotient(pc.unit, blocks, __builtin_amdgcn_rcpf(static_cast<float>(blocks))));
+    const int rb = pc.unit - h * blocks;
     const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4, part = lr & 1;
     const int wv = wave_in_block();
     const uint32_t magic = code_magic();
@@ -422,7 +429,8 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
         for (int j = 0; j < OCT; ++j) {
             const bool b = static_cast<uint32_t>(ids[j]) >= static_cast<uint32_t>(a.c.pages);
             bad |= b ? (WIDE ? 15u : 1u << j) : 0u;
-            at[j] = (static_cast<size_t>(b ? 0u : static_cast<uint32_t>(ids[j])) * a.c.heads + h) * P + ((tile * kTile + 8 * j) & (P - 1));
+            at[j] = (static_cast<size_t>(b ? 0u : static_cast<uint32_t>(ids[j])) * a.c.heads + h) * P +
+                    ((tile * kTile + 8 * j) & (P - 1));
         }
         bad_octets[slot] = bad;
         auto octet = [&](int j) {   // for a lane
@@ -649,7 +657,8 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
             const uint32_t w[4] = {V[m].x, V[m].y, V[m].z, V[m].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<8>(w[e], magic), __builtin_bit_cast(f16x8_t, W), acc[m][e], 0, 0, 0);
+                acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<8>(w[e], magic), __builtin_bit_cast(f16x8_t, W),
+                                                                   acc[m][e], 0, 0, 0);
         }
     }
     // The waves' sums meet in LDS; the two parts of a row are neighbouring columns, each lane of a pair writes every
@@ -711,17 +720,20 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
 }
 
 // ------------------------------------------------------------------ many rows
-// Bound by the matrix products. 128 rows a workgroup, 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: codes are
+// Bound by instruction issue: of the 4870 cycles that a wave has a tile of 32 tokens, the matrix products take 2180 and its 470
+// other vector instructions 1900. 128 rows a workgroup, 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: codes are
 // turned to fp16 once per workgroup, into LDS, and an operand of keys or values, 1 KB of LDS, feeds 2 products (both parts of
 // 32 rows). A wave holds its rows' query parts (128 registers at D = 256, pinned in accumulation registers) and sums (128).
 // Its vector work - softmax, turning codes to fp16 - is laid between its own products: while tile t + 1's scores are computed,
-// tile t's are exponentiated; while tile t's values are summed, the codes of the next tiles go to LDS. All waves run all tiles of the workgroup, though a wave's own rows may end
-// one earlier: with a branch around the products the compiler moves the sums between register files at each.
+// tile t's are exponentiated; while tile t's values are summed, the codes of the next tiles go to LDS. All waves run all tiles
+// of the workgroup, though a wave's own rows may end one earlier: with a branch around the products the compiler moves the sums
+// between register files at each. (5000 rows: 492 us; by exponents for each 8 tokens in place of each token's 506; codes to LDS
+// beside the scores 510.)
 // The keys' scales are in the operand: code - 8 has at most 3 bits and a bf16 scale 8, so scale (code - 8) is an fp16 number, and
 // all dims of a head are one sum. What is left of a key, min + 8 scale of each group times the sum of its queries, is two
 // products more, of bf16 numbers (the minima, 8 scale) with the sums' three parts. A token's numbers are taken times a power of
 // two that brings the largest max(16 scale, |min|) of its groups below 2^16; the scores are multiplied by its inverse. (Each
-// group's products scaled by themselves, in fp32, took 64 fmas a lane and tile and 64 registers: 522 us at 5000 rows.)
+// group's products scaled by themselves, in fp32, took 64 fmas a lane and tile and 64 registers: 506 us where this took 490.)
 // The scores^T tile has token rho = 8 b + 4 g + j of the 32 in register 4 b + j of lane half g; key row rho stands for token
 // 16 (b / 2) + 8 g + 4 (b % 2) + j, so that a lane's registers 8 s .. 8 s + 7 are octet 2 s + g, its share of the second
 // product's depth s.
@@ -729,10 +741,12 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
 // A workgroup has its CU to itself at D = 256 (registers). A unit (a row tile and a KV head) costs 20 us beside its tiles' 2.2 us
 // each: its queries, the first tiles' way to the products, its outputs. How a call's units meet the CUs:
 // - pieces: up to kPromptFill units, each cut in pieces of at most so many tiles that all pieces are at most kPromptFill;
-// - a line: all units' tiles one after the other, kPromptCost more in front of each unit, cut in kPromptFill equal parts. A workgroup takes
-//   its part's segments of units in turn. Of fewer than kPromptCut units, where a part is shorter than the longest piece would be;
+// - a line: all units' tiles one after the other, kPromptCost more in front of each unit, cut in kPromptFill equal parts. A
+//   workgroup takes its part's segments of units in turn. Of fewer than kPromptCut units, where a part is shorter than the
+//   longest piece would be;
 // - of more, a workgroup a unit, the longest first.
-// (Only pieces, of one number for all units: 2048 rows 144 us, now 123; 1100 rows 91, now 66.)
+// (Every unit in the same number of pieces, as many as fit: 2048 rows 144 us, now 124; 1100 rows 91, now 66; 777 behind 6000
+// keys 220, now 193. A cost of 5, 7 or 15 tiles in the line: 153, 134, 131 us where 10 takes 124.)
 struct Line {
     int over, parts, base, more;   // steps in front of a unit; the first `more` parts have base + 1 steps, the others base
     __device__ __forceinline__ Line(int over, int steps, int most) : over(over) {
@@ -748,8 +762,9 @@ struct Line {
     // The pieces of a unit that starts at `at`.
     __device__ __forceinline__ int pieces(int at, int steps) const { return part_of(at + over + steps - 1) - part_of(at + over) + 1; }
 };
-// Where the pieces of a unit lie. split4_kernel's are neighbours, kRows places each. A workgroup of prompt4_kernel has kPromptRows places
-// for the piece that ends its first unit, or passes through it, and in a second region as many for the one that begins its last.
+// Where the pieces of a unit lie. split4_kernel's are neighbours, kRows places each. A workgroup of prompt4_kernel has kPromptRows
+// places for the piece that ends its first unit, or passes through it, and in a second region as many for the one that begins its
+// last.
 struct Places {
     int first, rows, second;   // of a row: the first piece's place in the first region; the second region's distance, or 0
     __device__ __forceinline__ int of(int piece) const { return first + (piece == 0 ? second : piece * rows); }
@@ -773,9 +788,9 @@ __device__ __forceinline__ void static_for(F&& f) {
     static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-__device__ __forceinline__ Request4 uniform(const Request4& r) {
-    return Request4{__builtin_amdgcn_readfirstlane(r.first), __builtin_amdgcn_readfirstlane(r.n), __builtin_amdgcn_readfirstlane(r.len),
-                    __builtin_amdgcn_readfirstlane(static_cast<int>(r.bad)) != 0};
+__device__ __forceinline__ Request4 of_lane(const Request4& r, int l) {
+    return Request4{__builtin_amdgcn_readlane(r.first, l), __builtin_amdgcn_readlane(r.n, l), __builtin_amdgcn_readlane(r.len, l),
+                    __builtin_amdgcn_readlane(static_cast<int>(r.bad), l) != 0};
 }
 template <int D>
 __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const Attn4Args a) {
@@ -808,14 +823,14 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
             while (hit) {
                 const int l = __builtin_ctzll(hit);
                 hit &= hit - 1;
-                const Request4 one{__builtin_amdgcn_readlane(r.first, l), __builtin_amdgcn_readlane(r.n, l), __builtin_amdgcn_readlane(r.len, l),
-                                   __builtin_amdgcn_readlane(static_cast<int>(r.bad), l) != 0};
+                const Request4 one = of_lane(r, l);
                 if (look(b0 + l, one)) return;
             }
         }
     };
     float units = static_cast<float>(row_tiles(held)) * static_cast<float>(a.c.heads);
-    for (int b0 = kWave; b0 < a.requests; b0 += kWave) units += static_cast<float>(row_tiles(lane_request(b0 + lane0))) * static_cast<float>(a.c.heads);
+    for (int b0 = kWave; b0 < a.requests; b0 += kWave)
+        units += static_cast<float>(row_tiles(lane_request(b0 + lane0))) * static_cast<float>(a.c.heads);
     units = group_sum<kWave>(units);
     if (units == 0.f) return;   // the whole workgroup
     const bool cut = units < static_cast<float>(kPromptCut);
@@ -852,7 +867,8 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
                 for (int i = 0; i < 4; ++i) {
                     pieces = all([&](int t) { return (t + cut_at - 1) / cut_at; });
                     if (pieces <= kPromptFill) break;
-                    cut_at = max(static_cast<int>(static_cast<float>(cut_at) * static_cast<float>(pieces) * (1.0f / kPromptFill)), cut_at + 1);
+                    const float longer = static_cast<float>(cut_at) * static_cast<float>(pieces) * (1.0f / kPromptFill);
+                    cut_at = max(static_cast<int>(longer), cut_at + 1);
                 }
                 if (pieces > kPromptFill) {
                     cut_at = longest;
@@ -868,11 +884,13 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
             int left = line_at;
             each_request([&](int q_b, const Request4& q) {
                 for (int k0 = 0; k0 < row_tiles(q); k0 += kWave) {
-                    const int n = here(q, k0 + lane0, [&](int t) { return cut_at ? (t + cut_at - 1) / cut_at : t + line.over; }), upto = wave_prefix(n);
+                    const int n = here(q, k0 + lane0, [&](int t) { return cut_at ? (t + cut_at - 1) / cut_at : t + line.over; });
+                    const int upto = wave_prefix(n);
                     const uint64_t hit = __ballot(left < upto);
                     if (hit) {
                         const int l = __builtin_ctzll(hit), each = __builtin_amdgcn_readlane(n, l) / a.c.heads;
-                        const int local = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l)), head = local / each;
+                        const int local = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
+                        const int head = local / each;
                         b = q_b;
                         r = q;
                         unit = (k0 + l) * a.c.heads + head;
@@ -901,477 +919,480 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         if (!found) return;   // the whole workgroup
     }
     for (;;) {
-    int tid = threadIdx.x;
-    asm("" : "+v"(tid));   // what follows from it is not held from one segment to the next
-    const int lane = tid & 63, col = lane & 31, g = lane >> 5;
-    r = uniform(r);
-    b = __builtin_amdgcn_readfirstlane(b);
-    unit = __builtin_amdgcn_readfirstlane(unit);
-    unit_at = __builtin_amdgcn_readfirstlane(unit_at);
-    unit_steps = __builtin_amdgcn_readfirstlane(unit_steps);
-    const int pairs = r.n * G, tiles = row_tiles(r);
-    const int h = unit % a.c.heads, rt = tiles - 1 - unit / a.c.heads;
-    const int wv = wave_in_block();
-    const int row0 = rt * kPromptRows + 32 * wv;             // the wave's first pair
-    const int rr = min(row0 + col, pairs - 1);
-    const int ti = over_g(rr), head = h * G + (rr - ti * G);
-    const int limit = r.len - r.n + ti;
-    const int wave_first = r.len - r.n + over_g(min(row0, pairs - 1));
-    const int seen = keys_seen(r, rt);
-    const int all_steps = (seen + kTile - 1) / kTile;
-    const int from = max(line_at - unit_at - line.over, 0), to = min(line_end - unit_at - line.over, unit_steps);
-    if (to <= 0) return;   // the part ends before the unit's first step
-    const bool begins = from == 0, whole = begins && to == unit_steps;
-    const int step = (cut_at ? (steps_of(seen) + unit_steps - 1) / unit_steps : 1) * a.prompt_step;   // tiles
-    const int first_tile = whole ? 0 : __builtin_amdgcn_readfirstlane(from * step);
-    const int steps = __builtin_amdgcn_readfirstlane(whole ? all_steps : max(min(to * step, all_steps) - first_tile, 0));   // this segment's tiles
-    const uint32_t magic = code_magic();
+        int tid = threadIdx.x;
+        asm("" : "+v"(tid));   // what follows from it is not held from one segment to the next
+        const int lane = tid & 63, col = lane & 31, g = lane >> 5;
+        r = of_lane(r, 0);
+        b = __builtin_amdgcn_readfirstlane(b);
+        unit = __builtin_amdgcn_readfirstlane(unit);
+        unit_at = __builtin_amdgcn_readfirstlane(unit_at);
+        unit_steps = __builtin_amdgcn_readfirstlane(unit_steps);
+        const int pairs = r.n * G, tiles = row_tiles(r);
+        const int h = unit % a.c.heads, rt = tiles - 1 - unit / a.c.heads;
+        const int wv = wave_in_block();
+        const int row0 = rt * kPromptRows + 32 * wv;             // the wave's first pair
+        const int rr = min(row0 + col, pairs - 1);
+        const int ti = over_g(rr), head = h * G + (rr - ti * G);
+        const int limit = r.len - r.n + ti;
+        const int wave_first = r.len - r.n + over_g(min(row0, pairs - 1));
+        const int seen = keys_seen(r, rt);
+        const int all_steps = (seen + kTile - 1) / kTile;
+        const int from = max(line_at - unit_at - line.over, 0), to = min(line_end - unit_at - line.over, unit_steps);
+        if (to <= 0) return;   // the part ends before the unit's first step
+        const bool begins = from == 0, whole = begins && to == unit_steps;
+        const int step = (cut_at ? (steps_of(seen) + unit_steps - 1) / unit_steps : 1) * a.prompt_step;   // tiles
+        const int first_tile = whole ? 0 : __builtin_amdgcn_readfirstlane(from * step);
+        // this segment's tiles
+        const int steps = __builtin_amdgcn_readfirstlane(whole ? all_steps : max(min(to * step, all_steps) - first_tile, 0));
+        const uint32_t magic = code_magic();
 
-    // A wave brings one octet of tokens of each tile: page and offset are the same for its lanes. A lane's words: of keys
-    // (token lane % 8, words E (lane / 8) .. of its row), of values (dims E lane ..). Octets past the last are loaded from page 0 and
-    // never read from LDS. Page ids are read a tile ahead of the codes they lead to.
-    uint32_t kr[E], vr[E];
-    // bf16, of token lane % 8: the key scales of the lane's words, value scale and minimum, and its element of the token's row of
-    // kmin (the minimum of group lane / 8, from lane 32 on the scale of group lane / 8 - 4)
-    uint32_t ksr[GL], vsr, vmr, own;
-    const int piece = lane >> 3, own_group = piece & 3;
-    const uint16_t* own_at = piece < 4 ? a.c.km + (lane & 7) * NG + min(own_group, NG - 1) : a.c.ks + 8 * min(own_group, NG - 1) + (lane & 7);
-    bool sdead = false, sbad = false;
-    int id = 0;
-    size_t at[3];   // the octet in tiles st + 1, st + 2, st + 3: its first token in the head's cache
-    auto words = [](const uint8_t* p, uint32_t(&w)[E]) {
-        if constexpr (E == 4) {
-            const uint4 x = ld16(p);
-            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-        } else if constexpr (E == 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(p);
-            w[0] = x.x, w[1] = x.y;
-        } else {
-            w[0] = *reinterpret_cast<const uint32_t*>(p);
-        }
-    };
-    auto next_id = [&](int st) {   // the table's entry for the octet (any in-bounds entry past the row's end)
-        id = a.table[static_cast<size_t>(b) * a.max_pages + min((kTile * (first_tile + st) + 8 * wv) >> a.page_shift, a.max_pages - 1)];
-    };
-    auto k_load = [&](int st) {
-        const int tok = kTile * (first_tile + st) + 8 * wv, page = __builtin_amdgcn_readfirstlane(id);
-        sdead = tok >= seen;
-        sbad = !sdead && (page < 0 || page >= a.c.pages);
-        at[0] = at[1];
-        at[1] = at[2];
-        at[2] = (static_cast<size_t>(static_cast<uint32_t>(sdead || sbad ? 0 : page)) * a.c.heads + h) * a.c.page +
-                static_cast<uint32_t>(tok & (a.c.page - 1));
-        words(a.c.k + at[2] * (D / 2) + (lane & 7) * (D / 2) + (lane >> 3) * (4 * E), kr);
-#pragma unroll
-        for (int j = 0; j < GL; ++j) ksr[j] = a.c.ks[at[2] * NG + 8 * ((GL * piece + j) % NG) + (lane & 7)];
-        own = own_at[at[2] * NG];
-        vsr = a.c.vs[at[2] + (lane & 7)];
-        vmr = a.c.vm[at[2] + (lane & 7)];
-    };
-    auto v_load = [&](int n) {   // n: how many tiles behind the keys
-        words(a.c.v + at[2 - n] * (D / 2) + lane * (4 * E), vr);
-    };
-    const int ktok = 8 * wv + (lane & 7), rho = (ktok & 16) + 8 * ((ktok >> 2) & 1) + 4 * ((ktok >> 3) & 1) + (ktok & 3);
-    // The token's power of two, over its 8 lanes, and the lane's scales with it.
-    int up = 0;
-    _Float16 scale16[GL];
-    auto k_scale = [&]() {
-        uint32_t z = own_group < NG ? (piece < 4 ? own & 0x7fffu : own + 0x0200u) : 0u;   // |min|, 16 scale
-        z = max(z, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(z), 0x128, 0xF, 0xF, false)));   // row_ror 8
-        const auto x = __builtin_amdgcn_permlane16_swap(z, z, false, false);
-        z = max(x[0], x[1]);
-        const auto y = __builtin_amdgcn_permlane32_swap(z, z, false, false);
-        up = 142 - max(static_cast<int>(max(y[0], y[1]) >> 7), 20);
-#pragma unroll
-        for (int j = 0; j < GL; ++j) scale16[j] = static_cast<_Float16>(ldexpf(bf16_value(static_cast<uint16_t>(ksr[j])), up));
-    };
-    auto k_put = [&](int st, int j) {   // word E (lane / 8) + j of the token's row: its place among [4][NG][2]
-        const int w = E * piece + j, dims = 4 * ((w % (2 * NG)) >> 1) + w / (2 * NG);
-        const _Float16 f = scale16[GL == 2 ? j >> 1 : 0];
-        ks[st & 1][dims][32 * (w & 1) + rho] = codes8<8>(kr[j], magic) * f16x8_t{f, f, f, f, f, f, f, f};
-    };
-    auto v_put = [&](int st, int j) {   // dim 32 E m + E row + j is row `row` of value tile E m + j
-        vs[st & 1][E * g + j][wv >> 1][32 * (wv & 1) + col] = codes8<8>(vr[j], magic);
-    };
-    auto s_put = [&](int st) {
-        const float mine = own_group < NG ? ldexpf(bf16_value(static_cast<uint16_t>(own)), piece < 4 ? up : up + 3) : 0.f;
-        kmin[st & 3][rho][piece] = static_cast<uint16_t>(__float_as_uint(mine) >> 16);
-        if (lane < 8) {
-            // A page outside the cache, or values that are not finite, make the token's scores NaN: of the rows that see it.
-            float scale = bf16_value(static_cast<uint16_t>(vsr)), rest = __builtin_fmaf(8.0f, scale, bf16_value(static_cast<uint16_t>(vmr)));
-            const bool bad = sbad || !(fabsf(rest) <= FLT_MAX);
-            if (sdead || bad) scale = rest = 0.f;
-            tok[st & 3][0][ktok] = bad ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-            tok[st & 3][1][ktok] = scale;
-            tok[st & 3][2][ktok] = rest;
-            tok[st & 3][3][ktok] = log2_over(0.f, sizes2(vsr, vmr) & 0xffffu) - (127.0f + kWeightUp);
-        }
-    };
-    auto k_store = [&](int st) {
-        k_scale();
-#pragma unroll
-        for (int j = 0; j < E; ++j) k_put(st, j);
-        s_put(st);
-    };
-    auto barrier = []() {   // LDS is written and read; the loads stay in flight
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    if (steps > 0) {
-        next_id(0);
-        at[1] = at[2] = 0;
-        k_load(0);
-        next_id(1);
-        v_load(0);
-    }
-    // the row's query, times 2^e, in two parts: dims 16 d + 8 g + 0..7 of depth d; and its groups' sums in three bf16 parts:
-    // depth 8 g + e has part g of group e % 4, in a second product part 2 + g
-    f16x8_t Qh[ND], Ql[ND];
-    bf16x8_t Qs[2];
-    float factor;
-    {
-        const float* q = a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D + 8 * g;
-        float f[ND][8];   // all of it requested before the first is looked at
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float4 x = ld4(q + 16 * d + 4 * i);
-                f[d][4 * i] = x.x, f[d][4 * i + 1] = x.y, f[d][4 * i + 2] = x.z, f[d][4 * i + 3] = x.w;
+        // A wave brings one octet of tokens of each tile: page and offset are the same for its lanes. A lane's words: of keys
+        // (token lane % 8, words E (lane / 8) .. of its row), of values (dims E lane ..). Octets past the last are loaded from
+        // page 0 and never read from LDS. Page ids are read a tile ahead of the codes they lead to.
+        uint32_t kr[E], vr[E];
+        // bf16, of token lane % 8: the key scales of the lane's words, value scale and minimum, and its element of the token's row of
+        // kmin (the minimum of group lane / 8, from lane 32 on the scale of group lane / 8 - 4)
+        uint32_t ksr[GL], vsr, vmr, own;
+        const int piece = lane >> 3, own_group = piece & 3;
+        const uint16_t* own_at = piece < 4 ? a.c.km + (lane & 7) * NG + min(own_group, NG - 1)
+                                           : a.c.ks + 8 * min(own_group, NG - 1) + (lane & 7);
+        bool sdead = false, sbad = false;
+        int id = 0;
+        size_t at[3];   // the octet in tiles st + 1, st + 2, st + 3: its first token in the head's cache
+        auto words = [](const uint8_t* p, uint32_t(&w)[E]) {
+            if constexpr (E == 4) {
+                const uint4 x = ld16(p);
+                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+            } else if constexpr (E == 2) {
+                const uint2 x = *reinterpret_cast<const uint2*>(p);
+                w[0] = x.x, w[1] = x.y;
+            } else {
+                w[0] = *reinterpret_cast<const uint32_t*>(p);
             }
-        float m = 0.f, bad = 0.f;   // 0, or NaN with an infinity or NaN
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                m = fmaxf(m, fabsf(f[d][i]));
-                bad = __builtin_fmaf(f[d][i], 0.f, bad);
-            }
-        if (bad != 0.f) m = INFINITY;
-        m = fmaxf(m, __shfl_xor(m, 32));
-        const bool ok = m <= FLT_MAX;
-        int e = 0;
-        if (m > 0.f && ok) {
-            int em;
-            frexpf(m, &em);
-            e = min(15 - em, kMaxUp);
-        }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        const float by = ldexpf(1.0f, e);   // what a row with infinities or NaNs gives here does not matter: factor is NaN
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = f[d][i] * by;
-                Qh[d][i] = static_cast<_Float16>(v);
-                Ql[d][i] = static_cast<_Float16>(low_part(v));
-                sum[d >> 2] += v;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i < NG) sum[i] += __shfl_xor(sum[i], 32);
-            const float p0 = bf16_part(sum[i], 0), p1 = bf16_part(sum[i], 1), p2 = bf16_part(sum[i], 2);
-            Qs[0][i] = Qs[0][4 + i] = static_cast<__bf16>(g ? p1 : p0);
-            Qs[1][i] = Qs[1][4 + i] = static_cast<__bf16>(g ? 0.f : p2);
-        }
-        factor = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {   // only products read them: accumulation registers, the others are full
-            asm("" : "+a"(Qh[d]));
-            asm("" : "+a"(Ql[d]));
-        }
-    }
-    f32x16_t acc[DT];
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
-    float mu = -FLT_MAX, l = 0.f, low = 0.f;
-    f32x16_t zero;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-    f32x16_t S, N;          // a tile's scores over `factor`; the next tile's products
-    u32x4_t Wh[2], Wl[2];   // weights of the last tile, pairs of fp16 numbers
-    // the numbers of a lane's tokens 4 j .. 4 j + 3
-    auto of_tokens = [&](const float* p, int j) { return ld4(p + 16 * (j >> 1) + 8 * g + 4 * (j & 1)); };
-    // The operands of a step's products are one sequence, the last tile's values (2 DT of them), then the next tile's keys
-    // (ND = 2 DT); each is requested AP products' pairs ahead, into the register that the one before it has left. fill(i) goes
-    // between the two products of an operand and after them.
-    constexpr int AP = 4;
-    f16x8_t A[AP];
-    auto value_at = [&](int slot, int k) { return vs[slot][k >> 1][k & 1][lane]; };
-    auto key_at = [&](int slot, int d) { return ks[slot][d][lane]; };
-    auto minima = [&](int tile) { return *reinterpret_cast<const bf16x8_t*>(&kmin[tile & 3][col][0]); };
-    // A tile's products into N. ahead(d): what to request when operand d has been taken.
-    auto scores = [&](const bf16x8_t mins, auto&& ahead, auto&& fill) {
-        N = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mins, Qs[0], zero, 0, 0, 0);
-        N = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mins, Qs[1], N, 0, 0, 0);
-        static_for<ND>([&](auto dI) {
-            constexpr int d = decltype(dI)::value;
-            const f16x8_t x = A[d % AP];
-            N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Qh[d], N, 0, 0, 0);
-            fill(IC<2 * d>{});
-            __builtin_amdgcn_sched_barrier(0);
-            N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Ql[d], N, 0, 0, 0);
-            ahead(dI);
-            fill(IC<2 * d + 1>{});
-            __builtin_amdgcn_sched_barrier(0);
-        });
-    };
-    auto values = [&](auto&& ahead, auto&& fill) {
-        static_for<ND>([&](auto kI) {
-            constexpr int k = decltype(kI)::value, d = k >> 1, s = k & 1;
-            const f16x8_t x = A[k % AP];
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8_t, Wh[s]), acc[d], 0, 0, 0);
-            fill(IC<2 * k>{});
-            __builtin_amdgcn_sched_barrier(0);
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8_t, Wl[s]), acc[d], 0, 0, 0);
-            ahead(kI);
-            fill(IC<2 * k + 1>{});
-            __builtin_amdgcn_sched_barrier(0);
-        });
-    };
-    for (int i = tid; i < DT * 2 * kWave; i += NTH) (&vs[1][0][0][0])[i] = f16x8_t{};   // the values before the first tile
-#pragma unroll
-    for (int s = 0; s < 2; ++s) Wh[s] = Wl[s] = u32x4_t{};
-    if (steps > 0) {
-        k_store(0);
-        k_load(1);
-        next_id(2);
-        barrier();
-        static_for<AP>([&](auto dI) { A[decltype(dI)::value] = key_at(0, decltype(dI)::value); });
-        scores(minima(0), [&](auto dI) {
-            constexpr int d = decltype(dI)::value;
-            if constexpr (d + AP < ND) A[d % AP] = key_at(0, d + AP);
-        }, [](auto) {});
-        k_store(1);
-        k_load(2);
-        next_id(3);
-    }
-    barrier();
-#pragma unroll
-    for (int k = 0; k < AP; ++k) A[k] = value_at(1, k);
-    // Step st: tile st's products are in N. Its values and the keys of st + 2 go to LDS (slots whose last readers passed
-    // the barrier before); the values of st - 1 are summed beside that and beside the scaling and maximum of the scores,
-    // the scores of st + 1 beside the exponentials. One step more than tiles; before the first the weights are zero.
-    float top = 0.f, w0 = 0.f, z0 = 0.f;
-    float4 kf[2], sz[2], sv[2], mv[2];   // of 4 tokens, and the 4 after them, requested when those come up
-    auto pick = [](const float4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; };
-    auto ask_scales = [&](int st, int j) {
-        kf[j & 1] = of_tokens(tok[st & 3][0], j);
-        sz[j & 1] = of_tokens(tok[st & 3][3], j);
-    };
-    auto scale_max = [&](int st, int i) {
-        if (i % 4 == 0 && i < 12) ask_scales(st, i / 4 + 1);
-        S[i] = N[i] * pick(kf[(i / 4) & 1], i & 3);
-        const float z = __builtin_fmaf(S[i], factor, pick(sz[(i / 4) & 1], i & 3));
-        if (i & 1)
-            top = i == 1 ? fmaxf(z0, z) : fmaxf(fmaxf(z0, z), top);   // one instruction
-        else
-            z0 = z;
-        asm volatile("" : "+v"(S[i]), "+v"(top), "+v"(z0));   // here, not where they are used
-    };
-    auto weight = [&](int st, int i) {
-        if (i % 4 == 0 && i < 12) {
-            sv[(i / 4 + 1) & 1] = of_tokens(tok[st & 3][1], i / 4 + 1);
-            mv[(i / 4 + 1) & 1] = of_tokens(tok[st & 3][2], i / 4 + 1);
-        }
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], factor, -mu));
-        l += p;
-        low = __builtin_fmaf(p, pick(mv[(i / 4) & 1], i & 3), low);
-        const float w = rounded(p * pick(sv[(i / 4) & 1], i & 3));
-        if (i & 1) {
-            const uint32_t h = high_parts(w0, w);
-            Wh[i >> 3][(i & 7) / 2] = h;
-            Wl[i >> 3][(i & 7) / 2] = high_parts(rest_of<0>(h, w0), rest_of<1>(h, w));
-        }
-        w0 = w;
-    };
-    for (int st = 0; steps > 0 && st <= steps; ++st) {
-        bf16x8_t mins;
-        {
-            constexpr int SLOTS = 4 * DT, PER = 32 / SLOTS;   // places between products; scores at a place of the second half
-            values([&](auto kI) {
-                constexpr int k = decltype(kI)::value;
-                A[k % AP] = k + AP < ND ? value_at((st + 1) & 1, k + AP) : key_at((st + 1) & 1, k + AP - ND);
-            }, [&](auto kI) {
-                constexpr int k = decltype(kI)::value;
-                constexpr int EVERY = SLOTS / (4 * E);   // a word to LDS at every so many places of the first half
-                if constexpr (k == 0) k_scale();
-                if constexpr (k < SLOTS / 2 && k % EVERY == 0) {
-                    if constexpr ((k / EVERY) & 1)
-                        k_put(st + 2, (k / EVERY) >> 1);
-                    else
-                        v_put(st, (k / EVERY) >> 1);
-                }
-                if constexpr (k == SLOTS / 2 - 2) {
-                    ask_scales(st, 0);
-                    mins = minima(st + 1);
-                }
-                if constexpr (k == SLOTS / 2) {
-                    s_put(st + 2);
-                    v_load(1);
-                }
-                if constexpr (k == SLOTS / 2 + 2) {
-                    k_load(st + 3);
-                    next_id(st + 4);
-                }
-                if constexpr (k >= SLOTS / 2) {
-#pragma unroll
-                    for (int i = (k - SLOTS / 2) * PER; i < (k - SLOTS / 2 + 1) * PER; ++i) scale_max(st, i);
-                }
-                if constexpr (k == SLOTS - 2) {
-                    sv[0] = of_tokens(tok[st & 3][1], 0);
-                    mv[0] = of_tokens(tok[st & 3][2], 0);
-                }
-            });
-        }
-        {
-            const int t0 = kTile * (first_tile + st);
-            if (t0 + kTile - 1 > wave_first || st == steps) {   // past the piece's last tile nothing is seen
-                const int last = st == steps ? -1 : limit;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float4 size = of_tokens(tok[st & 3][3], i / 4);
-                    if (t0 + 16 * (i >> 3) + 8 * g + (i & 7) > last) S[i] = -INFINITY;
-                    const float z = __builtin_fmaf(S[i], factor, pick(size, i & 3));
-                    top = i ? fmaxf(top, z) : z;
-                }
-            }
-            if (__ballot(top > mu + kMoves)) {
-                const float now = fmaxf(mu, fmaxf(top, __shfl_xor(top, 32)));
-                const float shrink = __builtin_amdgcn_exp2f(mu - now);
-                mu = now;
-                l *= shrink;
-                low *= shrink;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
-            }
-            // (past the wave's last tile these scores are of an old one, and unused)
-            scores(mins, [&](auto dI) {
-                constexpr int d = decltype(dI)::value;
-                if constexpr (d + AP < ND) A[d % AP] = key_at((st + 1) & 1, d + AP);
-                // The tile's keys have been read, its values and the next keys are written: the next values can be read.
-                if constexpr (d == ND - 2) {
-                    barrier();
-#pragma unroll
-                    for (int k = 0; k < AP - 1; ++k) A[k] = value_at(st & 1, k);
-                }
-                if constexpr (d == ND - 1) A[AP - 1] = value_at(st & 1, AP - 1);
-            }, [&](auto kI) {
-                constexpr int k = decltype(kI)::value, PLACES = 2 * ND;
-#pragma unroll
-                for (int i = k * 16 / PLACES; i < (k + 1) * 16 / PLACES; ++i) weight(st, i);
-            });
-        }
-    }
-    l += __shfl_xor(l, 32);
-    low += __shfl_xor(low, 32);
-    // The outputs, or the sums of a piece, by way of LDS: a lane of the sums has 16 bytes of each of many rows, the lanes that
-    // write have whole lines.
-    if (g == 0) {
-        const bool none = mu == -FLT_MAX && l == 0.f, live = row0 + col < pairs;
-        const int pair = (r.first + ti) * a.heads + head, k = static_cast<int>(blockIdx.x) * kPromptRows + 32 * wv + col;
-        const int first = a.items * kRows + k, place = first + (begins ? kPromptFill * kPromptRows : 0);
-        const float by = !whole ? 1.f : none ? 0.f : 1.f / (r.bad ? __builtin_nanf("") : l);
-        out_rows[wv][col] = make_int2(__float_as_int(by), !live ? -1 : whole ? pair : place);
-        if (live && !whole) a.stat[place] = make_float2(mu, r.bad ? __builtin_nanf("") : l);
-        if (live && begins) a.info[pair] = whole ? make_int2(0, 1) : make_int2(first, line.pieces(unit_at, unit_steps));
-    }
-    // 4 neighbouring dims, the n-th of DT * 4: of E value tiles of one register, or 2 of two, or one of four
-    auto four = [&](int n, int& dim) {
-        const int m = n * 4 / (16 * E), rest = n - m * 4 * E;   // tile group; 4 registers' 16 rows x E dims as 4 E fours
-        float x[4];
-        if constexpr (E == 4) {
-            const int i = rest;   // register
-            dim = 128 * m + 4 * (8 * (i >> 2) + 4 * g + (i & 3));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = acc[4 * m + e][i];
-        } else if constexpr (E == 2) {
-            const int i = 2 * rest;
-            dim = 64 * m + 2 * (8 * (i >> 2) + 4 * g + (i & 3));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = acc[2 * m + (e & 1)][i + (e >> 1)];
-        } else {
-            const int i = 4 * rest;
-            dim = 32 * m + 8 * (i >> 2) + 4 * g;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = acc[m][i + e];
-        }
-        return make_float4(x[0] + low, x[1] + low, x[2] + low, x[3] + low);
-    };
-    {
-        auto meet = []() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };   // of one wave
-        meet();
-        float* to_rows = whole ? a.out : a.part;
-        const bool gated = whole && a.gate;
-        const int dim0 = 4 * (lane & 15);
-        float by[8];
-        int64_t goes[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int2 x = out_rows[wv][4 * j + (lane >> 4)];
-            by[j] = __int_as_float(x.x);
-            goes[j] = x.y < 0 ? -1 : static_cast<int64_t>(x.y) * D + dim0;
-        }
-        float4 gates[2][8];   // of 64 dims, requested before the 64 before them
-        auto ask_gates = [&](int c) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (gated && goes[j] >= 0) gates[c & 1][j] = ld4(a.gate + goes[j] + 64 * c);
         };
-        ask_gates(0);
+        auto next_id = [&](int st) {   // the table's entry for the octet (any in-bounds entry past the row's end)
+            const int page = min((kTile * (first_tile + st) + 8 * wv) >> a.page_shift, a.max_pages - 1);
+            id = a.table[static_cast<size_t>(b) * a.max_pages + page];
+        };
+        auto k_load = [&](int st) {
+            const int tok = kTile * (first_tile + st) + 8 * wv, page = __builtin_amdgcn_readfirstlane(id);
+            sdead = tok >= seen;
+            sbad = !sdead && (page < 0 || page >= a.c.pages);
+            at[0] = at[1];
+            at[1] = at[2];
+            at[2] = (static_cast<size_t>(static_cast<uint32_t>(sdead || sbad ? 0 : page)) * a.c.heads + h) * a.c.page +
+                    static_cast<uint32_t>(tok & (a.c.page - 1));
+            words(a.c.k + at[2] * (D / 2) + (lane & 7) * (D / 2) + (lane >> 3) * (4 * E), kr);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-            if (c + 1 < D / 64) ask_gates(c + 1);
+            for (int j = 0; j < GL; ++j) ksr[j] = a.c.ks[at[2] * NG + 8 * ((GL * piece + j) % NG) + (lane & 7)];
+            own = own_at[at[2] * NG];
+            vsr = a.c.vs[at[2] + (lane & 7)];
+            vmr = a.c.vm[at[2] + (lane & 7)];
+        };
+        auto v_load = [&](int n) {   // n: how many tiles behind the keys
+            words(a.c.v + at[2 - n] * (D / 2) + lane * (4 * E), vr);
+        };
+        const int ktok = 8 * wv + (lane & 7), rho = (ktok & 16) + 8 * ((ktok >> 2) & 1) + 4 * ((ktok >> 3) & 1) + (ktok & 3);
+        // The token's power of two, over its 8 lanes, and the lane's scales with it.
+        int up = 0;
+        _Float16 scale16[GL];
+        auto k_scale = [&]() {
+            uint32_t z = own_group < NG ? (piece < 4 ? own & 0x7fffu : own + 0x0200u) : 0u;   // |min|, 16 scale
+            z = max(z, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(z), 0x128, 0xF, 0xF, false)));   // row_ror 8
+            const auto x = __builtin_amdgcn_permlane16_swap(z, z, false, false);
+            z = max(x[0], x[1]);
+            const auto y = __builtin_amdgcn_permlane32_swap(z, z, false, false);
+            up = 142 - max(static_cast<int>(max(y[0], y[1]) >> 7), 20);
 #pragma unroll
-            for (int n = 8 * c; n < 8 * c + 8; ++n) {
-                int dim;
-                const float4 x = four(n, dim);
-                st4(&outs[wv][col][dim - 64 * c], x);
+            for (int j = 0; j < GL; ++j) scale16[j] = static_cast<_Float16>(ldexpf(bf16_value(static_cast<uint16_t>(ksr[j])), up));
+        };
+        auto k_put = [&](int st, int j) {   // word E (lane / 8) + j of the token's row: its place among [4][NG][2]
+            const int w = E * piece + j, dims = 4 * ((w % (2 * NG)) >> 1) + w / (2 * NG);
+            const _Float16 f = scale16[GL == 2 ? j >> 1 : 0];
+            ks[st & 1][dims][32 * (w & 1) + rho] = codes8<8>(kr[j], magic) * f16x8_t{f, f, f, f, f, f, f, f};
+        };
+        auto v_put = [&](int st, int j) {   // dim 32 E m + E row + j is row `row` of value tile E m + j
+            vs[st & 1][E * g + j][wv >> 1][32 * (wv & 1) + col] = codes8<8>(vr[j], magic);
+        };
+        auto s_put = [&](int st) {
+            const float mine = own_group < NG ? ldexpf(bf16_value(static_cast<uint16_t>(own)), piece < 4 ? up : up + 3) : 0.f;
+            kmin[st & 3][rho][piece] = static_cast<uint16_t>(__float_as_uint(mine) >> 16);
+            if (lane < 8) {
+                // A page outside the cache, or values that are not finite, make the token's scores NaN: of the rows that see it.
+                float scale = bf16_value(static_cast<uint16_t>(vsr));
+                float rest = __builtin_fmaf(8.0f, scale, bf16_value(static_cast<uint16_t>(vmr)));
+                const bool bad = sbad || !(fabsf(rest) <= FLT_MAX);
+                if (sdead || bad) scale = rest = 0.f;
+                tok[st & 3][0][ktok] = bad ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+                tok[st & 3][1][ktok] = scale;
+                tok[st & 3][2][ktok] = rest;
+                tok[st & 3][3][ktok] = log2_over(0.f, sizes2(vsr, vmr) & 0xffffu) - (127.0f + kWeightUp);
             }
+        };
+        auto k_store = [&](int st) {
+            k_scale();
+#pragma unroll
+            for (int j = 0; j < E; ++j) k_put(st, j);
+            s_put(st);
+        };
+        auto barrier = []() {   // LDS is written and read; the loads stay in flight
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        if (steps > 0) {
+            next_id(0);
+            at[1] = at[2] = 0;
+            k_load(0);
+            next_id(1);
+            v_load(0);
+        }
+        // the row's query, times 2^e, in two parts: dims 16 d + 8 g + 0..7 of depth d; and its groups' sums in three bf16 parts:
+        // depth 8 g + e has part g of group e % 4, in a second product part 2 + g
+        f16x8_t Qh[ND], Ql[ND];
+        bf16x8_t Qs[2];
+        float factor;
+        {
+            const float* q = a.q + (static_cast<size_t>(r.first + ti) * a.heads + head) * D + 8 * g;
+            float f[ND][8];   // all of it requested before the first is looked at
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 x = ld4(q + 16 * d + 4 * i);
+                    f[d][4 * i] = x.x, f[d][4 * i + 1] = x.y, f[d][4 * i + 2] = x.z, f[d][4 * i + 3] = x.w;
+                }
+            float m = 0.f, bad = 0.f;   // 0, or NaN with an infinity or NaN
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    m = fmaxf(m, fabsf(f[d][i]));
+                    bad = __builtin_fmaf(f[d][i], 0.f, bad);
+                }
+            if (bad != 0.f) m = INFINITY;
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const bool ok = m <= FLT_MAX;
+            int e = 0;
+            if (m > 0.f && ok) {
+                int em;
+                frexpf(m, &em);
+                e = min(15 - em, kMaxUp);
+            }
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const float by = ldexpf(1.0f, e);   // what a row with infinities or NaNs gives here does not matter: factor is NaN
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = f[d][i] * by;
+                    Qh[d][i] = static_cast<_Float16>(v);
+                    Ql[d][i] = static_cast<_Float16>(low_part(v));
+                    sum[d >> 2] += v;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i < NG) sum[i] += __shfl_xor(sum[i], 32);
+                const float p0 = bf16_part(sum[i], 0), p1 = bf16_part(sum[i], 1), p2 = bf16_part(sum[i], 2);
+                Qs[0][i] = Qs[0][4 + i] = static_cast<__bf16>(g ? p1 : p0);
+                Qs[1][i] = Qs[1][4 + i] = static_cast<__bf16>(g ? 0.f : p2);
+            }
+            factor = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {   // only products read them: accumulation registers, the others are full
+                asm("" : "+a"(Qh[d]));
+                asm("" : "+a"(Ql[d]));
+            }
+        }
+        f32x16_t acc[DT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+        float mu = -FLT_MAX, l = 0.f, low = 0.f;
+        f32x16_t zero;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+        f32x16_t S, N;          // a tile's scores over `factor`; the next tile's products
+        u32x4_t Wh[2], Wl[2];   // weights of the last tile, pairs of fp16 numbers
+        // the numbers of a lane's tokens 4 j .. 4 j + 3
+        auto of_tokens = [&](const float* p, int j) { return ld4(p + 16 * (j >> 1) + 8 * g + 4 * (j & 1)); };
+        // The operands of a step's products are one sequence, the last tile's values (2 DT of them), then the next tile's keys
+        // (ND = 2 DT); each is requested AP products' pairs ahead, into the register that the one before it has left. fill(i) goes
+        // between the two products of an operand and after them.
+        constexpr int AP = 4;
+        f16x8_t A[AP];
+        auto value_at = [&](int slot, int k) { return vs[slot][k >> 1][k & 1][lane]; };
+        auto key_at = [&](int slot, int d) { return ks[slot][d][lane]; };
+        auto minima = [&](int tile) { return *reinterpret_cast<const bf16x8_t*>(&kmin[tile & 3][col][0]); };
+        // A tile's products into N. ahead(d): what to request when operand d has been taken.
+        auto scores = [&](const bf16x8_t mins, auto&& ahead, auto&& fill) {
+            N = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mins, Qs[0], zero, 0, 0, 0);
+            N = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mins, Qs[1], N, 0, 0, 0);
+            static_for<ND>([&](auto dI) {
+                constexpr int d = decltype(dI)::value;
+                const f16x8_t x = A[d % AP];
+                N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Qh[d], N, 0, 0, 0);
+                fill(IC<2 * d>{});
+                __builtin_amdgcn_sched_barrier(0);
+                N = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Ql[d], N, 0, 0, 0);
+                ahead(dI);
+                fill(IC<2 * d + 1>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        auto values = [&](auto&& ahead, auto&& fill) {
+            static_for<ND>([&](auto kI) {
+                constexpr int k = decltype(kI)::value, d = k >> 1, s = k & 1;
+                const f16x8_t x = A[k % AP];
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8_t, Wh[s]), acc[d], 0, 0, 0);
+                fill(IC<2 * k>{});
+                __builtin_amdgcn_sched_barrier(0);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8_t, Wl[s]), acc[d], 0, 0, 0);
+                ahead(kI);
+                fill(IC<2 * k + 1>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        for (int i = tid; i < DT * 2 * kWave; i += NTH) (&vs[1][0][0][0])[i] = f16x8_t{};   // the values before the first tile
+#pragma unroll
+        for (int s = 0; s < 2; ++s) Wh[s] = Wl[s] = u32x4_t{};
+        if (steps > 0) {
+            k_store(0);
+            k_load(1);
+            next_id(2);
+            barrier();
+            static_for<AP>([&](auto dI) { A[decltype(dI)::value] = key_at(0, decltype(dI)::value); });
+            scores(minima(0), [&](auto dI) {
+                constexpr int d = decltype(dI)::value;
+                if constexpr (d + AP < ND) A[d % AP] = key_at(0, d + AP);
+            }, [](auto) {});
+            k_store(1);
+            k_load(2);
+            next_id(3);
+        }
+        barrier();
+#pragma unroll
+        for (int k = 0; k < AP; ++k) A[k] = value_at(1, k);
+        // Step st: tile st's products are in N. Its values and the keys of st + 2 go to LDS (slots whose last readers passed
+        // the barrier before); the values of st - 1 are summed beside that and beside the scaling and maximum of the scores,
+        // the scores of st + 1 beside the exponentials. One step more than tiles; before the first the weights are zero.
+        float top = 0.f, w0 = 0.f, z0 = 0.f;
+        float4 kf[2], sz[2], sv[2], mv[2];   // of 4 tokens, and the 4 after them, requested when those come up
+        auto pick = [](const float4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; };
+        auto ask_scales = [&](int st, int j) {
+            kf[j & 1] = of_tokens(tok[st & 3][0], j);
+            sz[j & 1] = of_tokens(tok[st & 3][3], j);
+        };
+        auto scale_max = [&](int st, int i) {
+            if (i % 4 == 0 && i < 12) ask_scales(st, i / 4 + 1);
+            S[i] = N[i] * pick(kf[(i / 4) & 1], i & 3);
+            const float z = __builtin_fmaf(S[i], factor, pick(sz[(i / 4) & 1], i & 3));
+            if (i & 1)
+                top = i == 1 ? fmaxf(z0, z) : fmaxf(fmaxf(z0, z), top);   // one instruction
+            else
+                z0 = z;
+            asm volatile("" : "+v"(S[i]), "+v"(top), "+v"(z0));   // here, not where they are used
+        };
+        auto weight = [&](int st, int i) {
+            if (i % 4 == 0 && i < 12) {
+                sv[(i / 4 + 1) & 1] = of_tokens(tok[st & 3][1], i / 4 + 1);
+                mv[(i / 4 + 1) & 1] = of_tokens(tok[st & 3][2], i / 4 + 1);
+            }
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i], factor, -mu));
+            l += p;
+            low = __builtin_fmaf(p, pick(mv[(i / 4) & 1], i & 3), low);
+            const float w = rounded(p * pick(sv[(i / 4) & 1], i & 3));
+            if (i & 1) {
+                const uint32_t h = high_parts(w0, w);
+                Wh[i >> 3][(i & 7) / 2] = h;
+                Wl[i >> 3][(i & 7) / 2] = high_parts(rest_of<0>(h, w0), rest_of<1>(h, w));
+            }
+            w0 = w;
+        };
+        for (int st = 0; steps > 0 && st <= steps; ++st) {
+            bf16x8_t mins;
+            {
+                constexpr int SLOTS = 4 * DT, PER = 32 / SLOTS;   // places between products; scores at a place of the second half
+                values([&](auto kI) {
+                    constexpr int k = decltype(kI)::value;
+                    A[k % AP] = k + AP < ND ? value_at((st + 1) & 1, k + AP) : key_at((st + 1) & 1, k + AP - ND);
+                }, [&](auto kI) {
+                    constexpr int k = decltype(kI)::value;
+                    constexpr int EVERY = SLOTS / (4 * E);   // a word to LDS at every so many places of the first half
+                    if constexpr (k == 0) k_scale();
+                    if constexpr (k < SLOTS / 2 && k % EVERY == 0) {
+                        if constexpr ((k / EVERY) & 1)
+                            k_put(st + 2, (k / EVERY) >> 1);
+                        else
+                            v_put(st, (k / EVERY) >> 1);
+                    }
+                    if constexpr (k == SLOTS / 2 - 2) {
+                        ask_scales(st, 0);
+                        mins = minima(st + 1);
+                    }
+                    if constexpr (k == SLOTS / 2) {
+                        s_put(st + 2);
+                        v_load(1);
+                    }
+                    if constexpr (k == SLOTS / 2 + 2) {
+                        k_load(st + 3);
+                        next_id(st + 4);
+                    }
+                    if constexpr (k >= SLOTS / 2) {
+#pragma unroll
+                        for (int i = (k - SLOTS / 2) * PER; i < (k - SLOTS / 2 + 1) * PER; ++i) scale_max(st, i);
+                    }
+                    if constexpr (k == SLOTS - 2) {
+                        sv[0] = of_tokens(tok[st & 3][1], 0);
+                        mv[0] = of_tokens(tok[st & 3][2], 0);
+                    }
+                });
+            }
+            {
+                const int t0 = kTile * (first_tile + st);
+                if (t0 + kTile - 1 > wave_first || st == steps) {   // past the piece's last tile nothing is seen
+                    const int last = st == steps ? -1 : limit;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float4 size = of_tokens(tok[st & 3][3], i / 4);
+                        if (t0 + 16 * (i >> 3) + 8 * g + (i & 7) > last) S[i] = -INFINITY;
+                        const float z = __builtin_fmaf(S[i], factor, pick(size, i & 3));
+                        top = i ? fmaxf(top, z) : z;
+                    }
+                }
+                if (__ballot(top > mu + kMoves)) {
+                    const float now = fmaxf(mu, fmaxf(top, __shfl_xor(top, 32)));
+                    const float shrink = __builtin_amdgcn_exp2f(mu - now);
+                    mu = now;
+                    l *= shrink;
+                    low *= shrink;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
+                }
+                // (past the wave's last tile these scores are of an old one, and unused)
+                scores(mins, [&](auto dI) {
+                    constexpr int d = decltype(dI)::value;
+                    if constexpr (d + AP < ND) A[d % AP] = key_at((st + 1) & 1, d + AP);
+                    // The tile's keys have been read, its values and the next keys are written: the next values can be read.
+                    if constexpr (d == ND - 2) {
+                        barrier();
+#pragma unroll
+                        for (int k = 0; k < AP - 1; ++k) A[k] = value_at(st & 1, k);
+                    }
+                    if constexpr (d == ND - 1) A[AP - 1] = value_at(st & 1, AP - 1);
+                }, [&](auto kI) {
+                    constexpr int k = decltype(kI)::value, PLACES = 2 * ND;
+#pragma unroll
+                    for (int i = k * 16 / PLACES; i < (k + 1) * 16 / PLACES; ++i) weight(st, i);
+                });
+            }
+        }
+        l += __shfl_xor(l, 32);
+        low += __shfl_xor(low, 32);
+        // The outputs, or the sums of a piece, by way of LDS: a lane of the sums has 16 bytes of each of many rows, the lanes that
+        // write have whole lines.
+        if (g == 0) {
+            const bool none = mu == -FLT_MAX && l == 0.f, live = row0 + col < pairs;
+            const int pair = (r.first + ti) * a.heads + head, k = static_cast<int>(blockIdx.x) * kPromptRows + 32 * wv + col;
+            const int first = a.items * kRows + k, place = first + (begins ? kPromptFill * kPromptRows : 0);
+            const float by = !whole ? 1.f : none ? 0.f : 1.f / (r.bad ? __builtin_nanf("") : l);
+            out_rows[wv][col] = make_int2(__float_as_int(by), !live ? -1 : whole ? pair : place);
+            if (live && !whole) a.stat[place] = make_float2(mu, r.bad ? __builtin_nanf("") : l);
+            if (live && begins) a.info[pair] = whole ? make_int2(0, 1) : make_int2(first, line.pieces(unit_at, unit_steps));
+        }
+        // 4 neighbouring dims, the n-th of DT * 4: of E value tiles of one register, or 2 of two, or one of four
+        auto four = [&](int n, int& dim) {
+            const int m = n * 4 / (16 * E), rest = n - m * 4 * E;   // tile group; 4 registers' 16 rows x E dims as 4 E fours
+            float x[4];
+            if constexpr (E == 4) {
+                const int i = rest;   // register
+                dim = 128 * m + 4 * (8 * (i >> 2) + 4 * g + (i & 3));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = acc[4 * m + e][i];
+            } else if constexpr (E == 2) {
+                const int i = 2 * rest;
+                dim = 64 * m + 2 * (8 * (i >> 2) + 4 * g + (i & 3));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = acc[2 * m + (e & 1)][i + (e >> 1)];
+            } else {
+                const int i = 4 * rest;
+                dim = 32 * m + 8 * (i >> 2) + 4 * g;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = acc[m][i + e];
+            }
+            return make_float4(x[0] + low, x[1] + low, x[2] + low, x[3] + low);
+        };
+        {
+            auto meet = []() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };   // of one wave
             meet();
+            float* to_rows = whole ? a.out : a.part;
+            const bool gated = whole && a.gate;
+            const int dim0 = 4 * (lane & 15);
+            float by[8];
+            int64_t goes[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float4 x = ld4(&outs[wv][4 * j + (lane >> 4)][dim0]);
-                x = make_float4(x.x * by[j], x.y * by[j], x.z * by[j], x.w * by[j]);
-                if (gated) {
-                    const float4 y = gates[c & 1][j];
-                    if (__ballot(fminf(fminf(y.x, y.y), fminf(y.z, y.w)) < kFarGate))
-                        x = make_float4(gated_by(x.x, y.x), gated_by(x.y, y.y), gated_by(x.z, y.z), gated_by(x.w, y.w));
-                    else
-                        x = make_float4(near_gated(x.x, y.x), near_gated(x.y, y.y), near_gated(x.z, y.z), near_gated(x.w, y.w));
+                const int2 x = out_rows[wv][4 * j + (lane >> 4)];
+                by[j] = __int_as_float(x.x);
+                goes[j] = x.y < 0 ? -1 : static_cast<int64_t>(x.y) * D + dim0;
+            }
+            float4 gates[2][8];   // of 64 dims, requested before the 64 before them
+            auto ask_gates = [&](int c) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (gated && goes[j] >= 0) gates[c & 1][j] = ld4(a.gate + goes[j] + 64 * c);
+            };
+            ask_gates(0);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                if (c + 1 < D / 64) ask_gates(c + 1);
+#pragma unroll
+                for (int n = 8 * c; n < 8 * c + 8; ++n) {
+                    int dim;
+                    const float4 x = four(n, dim);
+                    st4(&outs[wv][col][dim - 64 * c], x);
                 }
-                if (goes[j] >= 0) st4(to_rows + goes[j] + 64 * c, x);
-            }
-            meet();
-        }
-    }
-    if (!cut) return;
-    line_at = unit_at = unit_at + line.over + unit_steps;   // the unit's end
-    if (cut_at || line_at >= line_end) return;
-    if (++unit == tiles * a.c.heads) {   // the next request that has row tiles
-        unit = 0;
-        uint64_t hit = 0;
-        for (int b0 = b + 1; b0 < a.requests; b0 += kWave) {
-            const Request4 q = b0 + lane < a.requests ? request(a, b0 + lane) : Request4{0, 0, 0, false};
-            hit = __ballot(row_tiles(q) > 0);
-            if (hit) {
-                const int l = __builtin_ctzll(hit);
-                b = b0 + l;
-                r = Request4{__builtin_amdgcn_readlane(q.first, l), __builtin_amdgcn_readlane(q.n, l), __builtin_amdgcn_readlane(q.len, l),
-                             __builtin_amdgcn_readlane(static_cast<int>(q.bad), l) != 0};
-                break;
+                meet();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float4 x = ld4(&outs[wv][4 * j + (lane >> 4)][dim0]);
+                    x = make_float4(x.x * by[j], x.y * by[j], x.z * by[j], x.w * by[j]);
+                    if (gated) {
+                        const float4 y = gates[c & 1][j];
+                        if (__ballot(fminf(fminf(y.x, y.y), fminf(y.z, y.w)) < kFarGate))
+                            x = make_float4(gated_by(x.x, y.x), gated_by(x.y, y.y), gated_by(x.z, y.z), gated_by(x.w, y.w));
+                        else
+                            x = make_float4(near_gated(x.x, y.x), near_gated(x.y, y.y), near_gated(x.z, y.z), near_gated(x.w, y.w));
+                    }
+                    if (goes[j] >= 0) st4(to_rows + goes[j] + 64 * c, x);
+                }
+                meet();
             }
         }
-        if (!hit) return;
-    }
-    unit_steps = steps_of(keys_seen(r, row_tiles(r) - 1 - unit / a.c.heads));
-    __syncthreads();   // the last tile has been read from LDS
+        if (!cut) return;
+        line_at = unit_at = unit_at + line.over + unit_steps;   // the unit's end
+        if (cut_at || line_at >= line_end) return;
+        if (++unit == tiles * a.c.heads) {   // the next request that has row tiles
+            unit = 0;
+            uint64_t hit = 0;
+            for (int b0 = b + 1; b0 < a.requests; b0 += kWave) {
+                const Request4 q = b0 + lane < a.requests ? request(a, b0 + lane) : Request4{0, 0, 0, false};
+                hit = __ballot(row_tiles(q) > 0);
+                if (hit) {
+                    const int l = __builtin_ctzll(hit);
+                    b = b0 + l;
+                    r = of_lane(q, l);
+                    break;
+                }
+            }
+            if (!hit) return;
+        }
+        unit_steps = steps_of(keys_seen(r, row_tiles(r) - 1 - unit / a.c.heads));
+        __syncthreads();   // the last tile has been read from LDS
     }
 }
 
@@ -1670,8 +1691,9 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     a.units = static_cast<int>(unit_bound(rows, requests, heads, kv_heads));
     a.whole = a.split_all && static_cast<int64_t>(max_pages) * page_size <= kWhole * kTile;
     a.places = kCus * places_on_cu(dim);
+    const int64_t tiles = static_cast<int64_t>(max_pages) * page_size / kTile;
     a.prompt_step = 1;   // a line is below 2^30 steps, in 32 bits
-    while (kPromptCut * (static_cast<int64_t>(max_pages) * page_size / (kTile * a.prompt_step) + 1 + kPromptCost) >= (1 << 30)) a.prompt_step *= 2;
+    while (kPromptCut * (tiles / a.prompt_step + 1 + kPromptCost) >= (1 << 30)) a.prompt_step *= 2;
     const hipStream_t s = as_stream(stream);
     if (dim == 64)
         launch<64>(a, s);

@@ -397,6 +397,23 @@ def test_attention_scales_far_apart(n):
     close(got, want, tol)
 
 
+@pytest.mark.parametrize("keys,values", [(0, 96), (0, 40), (0, -44), (0, -90), (96, 0), (-90, 0)])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_sizes(n, keys, values):
+    """Keys and values of sizes to both ends of what is held, queries of the keys' inverse size."""
+    r = np.random.default_rng(keys + 2 * values + n + 500)
+    page, heads, kvh, dim, total = 16, 8, 2, 128, 700
+    table, pages = tables(r, [total], page)
+    ref = random_cache(r, pages, kvh, page, dim)
+    for w, e in ((0, keys), (1, values)):
+        ref.scale[w] *= 2.0 ** e
+        ref.low[w] *= 2.0 ** e
+    q = (2.0 ** -keys * r.standard_normal((n, heads, dim))).astype(F32)
+    got = host(ops.attn_kv4_rows(dev(q), gpu_cache(ref), dev(table), dev([0, n], I32), dev([total], I32)))
+    want, tol = kv4_ref.attention(q, ref, table, [0, n], [total])
+    close(got, want, tol)
+
+
 def test_attention_zeros_before_values():
     """Tokens of zeros keep their weight in the sum when larger values come behind them, in any tile."""
     r = np.random.default_rng(1)
