@@ -1623,7 +1623,7 @@ void launch(const Attn4Args& a, hipStream_t s) {
         join4_few<D><<<pairs * (D / 64), kJoinWaves * kWave, 0, s>>>(a);
     else if (pairs <= 2048)
         join4_kernel<D, 4><<<pairs, 4 * kWave, 0, s>>>(a, 1);
-    else if (pairs <= kPromptFill / 2 * kPromptRows)   // a cut prompt's pairs may all have pieces
+    else if (pairs <= kPromptCut * kPromptRows)   // many of them in pieces
         join4_kernel<D, 1><<<blocks_for(pairs, 4), 4 * kWave, 0, s>>>(a, 1);
     else
         join4_kernel<D, 1><<<blocks_for(pairs, 16), 4 * kWave, 0, s>>>(a, 4);
