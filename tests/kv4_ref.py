@@ -94,7 +94,9 @@ def attention(q, cache, table, row_start, kv_len, gate=None):
     made of, scale * code and min, whose magnitudes A = |scale| code + |min| stand for |value|. A score s = q.k / sqrt(D):
     2^-21 sum |q| A / sqrt(D) for the products, their sums and the scaling, and as an fp32 number that is rounded when it is
     scaled and when the reference is subtracted 2^-22 (|s| + |s - max|); its exponential by that and 2^-20. An output: those,
-    weighted with |v - out|, and 2^-21 of sum p A (second product, its sums, the division).
+    weighted with |v - out|, and 2^-21 of sum p A (second product, its sums, the division). Of a weight p scale, its two fp16
+    parts keep 22 bits: 2^-22 of it, times |code - 8| <= 8 as codes are summed, where the rest of a value, p (min + 8 scale), is
+    an fp32 number that does not share that error: 2^-19 of sum p scale, which A does not cover where min and code are small.
     A weight p scale, as two fp16 parts, also has an absolute step, half the spacing of fp16's smallest numbers, 2^-25: times
     2^-6 in units of a reference that the largest p max(|min|, 16 scale, 2^-40) is at least half of. That is 2^-30 of the
     largest w max(..) with the normalised weights w, met by the codes."""
@@ -111,8 +113,8 @@ def attention(q, cache, table, row_start, kv_len, gate=None):
             rep = dim // cache.scale[w].shape[-1]
             c = cache.codes[w][p, :, o] if total else np.zeros((0, kvh, dim))
             sc, low = ((np.repeat(x[w][p, :, o], rep, axis=-1) if total else c) for x in (cache.scale, cache.low))
-            parts.append((low + sc * c, sc * c + np.abs(low), c, np.maximum(np.maximum(16 * sc, np.abs(low)), 2.0 ** -40)))
-        (k, ka, _, _), (v, va, vc, vm) = parts
+            parts.append((low + sc * c, sc * c + np.abs(low), c, np.maximum(np.maximum(16 * sc, np.abs(low)), 2.0 ** -40), sc))
+        (k, ka, _, _, _), (v, va, vc, vm, vs) = parts
         for i in range(n):
             row, pos = row_start[b] + i, total - n + i
             for h in range(heads):
@@ -130,6 +132,7 @@ def attention(q, cache, table, row_start, kv_len, gate=None):
                 eps = 2.0 ** -21 * a + 2.0 ** -22 * (np.abs(s) + np.abs(s - s.max())) + 2.0 ** -20
                 out[row, h] = y
                 tol[row, h] = (w * eps) @ np.abs(v[sl] - y) + 2.0 ** -21 * (w @ va[sl])
+                tol[row, h] += 2.0 ** -19 * (w @ vs[sl])
                 tol[row, h] += 2.0 ** -30 * (w * vm[sl][:, 0]).max() * vc[sl].sum(axis=0)
     if gate is not None:
         live = row_start[len(kv_len)]
