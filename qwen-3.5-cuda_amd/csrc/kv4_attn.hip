@@ -52,8 +52,11 @@ constexpr int kSplitWaves = 4;
 constexpr int kWholeWaves = 8;
 constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
 constexpr int kMaxItems = 1 << 24;     // more than any call has
-constexpr int kSplitMax = 32;          // (row, head) pairs of a request and KV head that still take split4_kernel; a row does
+constexpr int kSplitMax = 64;          // (row, head) pairs of a request and KV head that always take split4_kernel; a row does
 constexpr int kSplitOnly = 1024;       // and of a whole call that has no more rows than requests
+constexpr int kLightUnits = 1024;      // of a light call, see Weight
+constexpr int kLightWork = 28 * 1024;  // its units x (tiles + kUnitCost) at D = 256
+constexpr int kUnitCost = 8;
 constexpr int kMaxUp = 110;             // tiny queries are taken times 2^110 at most, so that what undoes it is a normal number
 constexpr float kMoves = 8.0f;         // a token past the reference by more moves it
 constexpr float kWeightUp = 10.0f;     // log2 of what exponentials, and so all sums, are taken times: weights fill fp16
@@ -70,10 +73,10 @@ struct Attn4Args {
     float* part;         // [place][D] sums of p v, where Places says
     float2* stat;        // [place] (m, l)
     int2* info;          // [row][head] (place of the first piece, pieces); written for the requests' rows alone
-    int items;           // split4_kernel's grid, each with kRows places
+    int items;           // split4_kernel's pieces that have places, kRows each
     int places;          // split4_kernel's workgroups that the card holds at once
     int split_all;       // every request takes split4_kernel
-    int units;           // at most
+    int light_work;      // of a light call at most
     int whole;           // and every unit's tiles are one piece: nothing is joined
     int prompt_step;     // tiles of a step of prompt4_kernel's line (a power of two)
     float scale;         // log2(e) / sqrt(D)
@@ -105,6 +108,17 @@ __device__ __forceinline__ int wave_prefix(int v) {
 #undef QK_STEP
     return v;
 }
+__device__ __forceinline__ int wave_max(int v) {
+#define QK_STEP(ctrl, rows) v = max(v, __builtin_amdgcn_update_dpp(v, v, ctrl, rows, 0xF, false))
+    QK_STEP(0x111, 0xF);
+    QK_STEP(0x112, 0xF);
+    QK_STEP(0x114, 0xF);
+    QK_STEP(0x118, 0xF);
+    QK_STEP(0x142, 0xA);
+    QK_STEP(0x143, 0xC);
+#undef QK_STEP
+    return __builtin_amdgcn_readlane(v, 63);
+}
 __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
 
 // Piece `item` of the call: request, which of its units (KV head, row block), which piece of the unit's tiles. Every wave
@@ -118,14 +132,30 @@ struct Piece {
 };
 constexpr int kHeld = 4;
 __device__ __forceinline__ int tiles_of(const Request4& r) { return max(1, (r.len + kTile - 1) / kTile); }
-__device__ __forceinline__ bool takes_split(const Attn4Args& a, const Request4& r) {
+__device__ __forceinline__ bool is_small(const Attn4Args& a, const Request4& r) {
     return a.split_all || r.n * a.group <= max(kSplitMax, a.group);   // rows * heads <= 2^24
 }
 __device__ __forceinline__ float units_of(const Attn4Args& a, const Request4& r) {
-    if (!takes_split(a, r)) return 0.f;
     const uint32_t blocks = (static_cast<uint32_t>(r.n) * static_cast<uint32_t>(a.group) + kRows - 1) / kRows;
     return static_cast<float>(blocks) * static_cast<float>(a.c.heads);
 }
+// Whether a call is light: whether split4_kernel takes its larger requests too. A unit of 8 pairs and a tile cost a CU 0.3 us
+// there, and the unit's start and end as much as 8 tiles; 128 pairs and a tile 2.2 us in prompt4_kernel, which begins and ends
+// with 20 us and has more pieces to join. (100 rows of a prompt 12 us for 33, 500 rows 33 for 46, 12 rows at 3000 keys 17 for 34, 20
+// requests of 20 rows at 500 keys 33 for 44; past it, 130 rows at 4000 keys 74 for 56, 30 of 12 rows at 2000 keys 71 for 62.) Both
+// kernels weigh a call's requests alike: sums of whole numbers, exact where they matter.
+struct Weight {
+    float work = 0.f, units = 0.f;
+    __device__ __forceinline__ void add(const Attn4Args& a, const Request4& r) {
+        const float u = units_of(a, r);
+        units += u;
+        if (!is_small(a, r)) work += u * static_cast<float>(tiles_of(r) + kUnitCost);
+    }
+    __device__ __forceinline__ bool light(const Attn4Args& a) const {   // over the wave's lanes
+        return a.light_work > 0 && group_sum<kWave>(work) <= static_cast<float>(a.light_work) &&
+               group_sum<kWave>(units) <= static_cast<float>(kLightUnits);
+    }
+};
 // n / d, both below 2^27, the quotient below 2^20; inverse within 2^-22 of 1 / d.
 __device__ __forceinline__ int quotient(int n, int d, float inverse) {
     int q = static_cast<int>(static_cast<float>(n) * inverse);
@@ -138,6 +168,8 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
     Request4 first{0, 0, 0, false};
     float units[kHeld];
     int tiles[kHeld];
+    uint32_t large = 0;
+    Weight weight;
 #pragma unroll
     for (int c = 0; c < kHeld; ++c) {
         units[c] = 0.f;
@@ -146,16 +178,24 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
             const Request4 r = lane_request(c * kWave + lane);
             units[c] = units_of(a, r);
             tiles[c] = tiles_of(r);
+            large |= is_small(a, r) ? 0u : 1u << c;
+            weight.add(a, r);
             if (c == 0) first = r;
         }
     }
+    for (int b = kHeld * kWave + lane; b < a.requests; b += kWave) weight.add(a, lane_request(b));
+    const bool light = !a.split_all && weight.light(a);
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c)
+        if (((large >> c) & 1) && !light) units[c] = 0.f;
+    auto units_here = [&](const Request4& r) { return light || is_small(a, r) ? units_of(a, r) : 0.f; };
     auto sum = [&](auto&& of) {   // rounded, but the same in every wave
         float v = 0.f;
 #pragma unroll
         for (int c = 0; c < kHeld; ++c) v += of(units[c], static_cast<float>(tiles[c]));
         for (int b = kHeld * kWave + lane; b < a.requests; b += kWave) {
             const Request4 r = lane_request(b);
-            v += of(units_of(a, r), static_cast<float>(tiles_of(r)));
+            v += of(units_here(r), static_cast<float>(tiles_of(r)));
         }
         return group_sum<kWave>(v);
     };
@@ -163,7 +203,8 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
     float step = 0x1p-26f;
     if (!a.whole) {
         const float total = sum([](float u, float t) { return u * t; }), all_units = sum([](float u, float) { return u; });
-        const float want = static_cast<float>(a.places) * (all_units > static_cast<float>(a.places) ? 4.0f : 1.0f);
+        const bool many = all_units > static_cast<float>(a.places);
+        const float want = static_cast<float>(a.places) * (many ? 4.0f : 1.0f);
         const float per_want = __builtin_amdgcn_rcpf(want);
         auto limited = [](float t) {   // whole turns
             return max(static_cast<int>(fminf(ceilf(t * (1.0f / kSplitWaves)), 0x1p24f)), 1) * kSplitWaves;
@@ -177,6 +218,10 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
             step = __builtin_amdgcn_rcpf(static_cast<float>(cut));
         }
         cut = __builtin_amdgcn_readfirstlane(cut);
+        if (light && many) {   // whole units: the workspace has no places for more pieces
+            cut = 1 << 26;
+            step = 0x1p-26f;
+        }
     }
     bool found = false;
     auto look = [&](int b0, float u, int t) {
@@ -192,7 +237,7 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
             p.unit = __builtin_amdgcn_readfirstlane(quotient(local, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))));
             p.split = local - p.unit * p.splits;
             const int turns = (__builtin_amdgcn_readlane(t, l) + kSplitWaves - 1) / kSplitWaves;
-            p.tiles = a.whole ? cut : quotient(turns + p.splits - 1, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))) * kSplitWaves;
+            p.tiles = p.splits == 1 ? 1 << 26 : quotient(turns + p.splits - 1, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))) * kSplitWaves;
             if (b0 == 0) {
                 p.r.first = __builtin_amdgcn_readlane(first.first, l);
                 p.r.n = __builtin_amdgcn_readlane(first.n, l);
@@ -211,7 +256,7 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
         if (!found && c * kWave < a.requests) look(c * kWave, units[c], tiles[c]);
     for (int b0 = kHeld * kWave; !found && b0 < a.requests; b0 += kWave) {
         const Request4 r = lane_request(b0 + lane);
-        look(b0, units_of(a, r), tiles_of(r));
+        look(b0, units_here(r), tiles_of(r));
     }
     return found;
 }
@@ -806,33 +851,25 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     const int G = a.group;
     const float per_g = 1.0f / static_cast<float>(G);
     auto over_g = [&](int pair) { return quotient(pair, G, per_g); };
-    auto row_tiles = [&](const Request4& r) { return takes_split(a, r) ? 0 : (r.n * G + kPromptRows - 1) / kPromptRows; };
+    auto row_tiles = [&](const Request4& r) { return is_small(a, r) ? 0 : (r.n * G + kPromptRows - 1) / kPromptRows; };
     auto keys_seen = [&](const Request4& r, int rt) {   // by some row of a row tile
         return max(r.len - r.n + over_g(min(rt * kPromptRows + kPromptRows - 1, r.n * G - 1)) + 1, 0);
     };
     const int step_bits = __builtin_ctz(a.prompt_step);
     auto steps_of = [&](int seen) { return max(1, (seen + kTile * a.prompt_step - 1) >> (5 + step_bits)); };
-    // The requests that have row tiles, in turn, until `look` says that it has found what it wants.
     auto lane_request = [&](int b) { return b < a.requests ? request(a, b) : Request4{0, 0, 0, false}; };
     const int lane0 = threadIdx.x & 63;
     const Request4 held = lane_request(lane0);   // every look is at these first
-    auto each_request = [&](auto&& look) {
-        for (int b0 = 0; b0 < a.requests; b0 += kWave) {
-            const Request4 r = b0 ? lane_request(b0 + lane0) : held;
-            uint64_t hit = __ballot(row_tiles(r) > 0);
-            while (hit) {
-                const int l = __builtin_ctzll(hit);
-                hit &= hit - 1;
-                const Request4 one = of_lane(r, l);
-                if (look(b0 + l, one)) return;
-            }
-        }
-    };
     float units = static_cast<float>(row_tiles(held)) * static_cast<float>(a.c.heads);
-    for (int b0 = kWave; b0 < a.requests; b0 += kWave)
-        units += static_cast<float>(row_tiles(lane_request(b0 + lane0))) * static_cast<float>(a.c.heads);
+    Weight weight;
+    weight.add(a, held);
+    for (int b0 = kWave; b0 < a.requests; b0 += kWave) {
+        const Request4 q = lane_request(b0 + lane0);
+        units += static_cast<float>(row_tiles(q)) * static_cast<float>(a.c.heads);
+        weight.add(a, q);
+    }
     units = group_sum<kWave>(units);
-    if (units == 0.f) return;   // the whole workgroup
+    if (units == 0.f || weight.light(a)) return;   // the whole workgroup
     const bool cut = units < static_cast<float>(kPromptCut);
     Line line(0, 1, 1);
     int cut_at = 0;   // steps of a piece at most; 0: not in pieces
@@ -842,30 +879,51 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     {
         bool found = false;
         if (cut) {
-            // A lane a row tile, all of a request's, in the order of the units; `of`: what a row tile of so many steps counts.
-            auto here = [&](const Request4& q, int k, auto&& of) {
+            // `of`: what a unit of so many steps counts. Of lane's request q, all its units together: the row tiles one after the
+            // other, or, where that is less, request by request with a lane a row tile.
+            auto here = [&](const Request4& q, int k, auto&& of) {   // the units of row tile k, the longest first
                 const int n = row_tiles(q);
                 return k < n ? of(steps_of(keys_seen(q, n - 1 - k))) * a.c.heads : 0;
             };
-            auto all = [&](auto&& of) {
+            auto looks = [&](const Request4& q) {   // of the first way, and of the other
+                return make_int2(wave_max(row_tiles(q)), wave_total((row_tiles(q) + kWave - 1) / kWave));
+            };
+            const int2 held_looks = looks(held);
+            auto of_request = [&](const Request4& q, int2 ways, auto&& of) {
+                const int n = row_tiles(q);
                 int v = 0;
-                each_request([&](int, const Request4& q) {
-                    for (int k0 = 0; k0 < row_tiles(q); k0 += kWave) v += wave_total(here(q, k0 + lane0, of));
-                    return false;
-                });
+                if (ways.y < ways.x) {
+                    for (uint64_t hit = __ballot(n > 0); hit; hit &= hit - 1) {
+                        const int l = __builtin_ctzll(hit);
+                        const Request4 one = of_lane(q, l);
+                        int sum = 0;
+                        for (int k0 = 0; k0 < row_tiles(one); k0 += kWave) sum += wave_total(here(one, k0 + lane0, of));
+                        if (lane0 == l) v = sum;
+                    }
+                } else {
+                    for (int k = 0; k < ways.x; ++k) v += here(q, k, of);
+                }
                 return v;
             };
-            int longest = 0;
-            each_request([&](int, const Request4& q) {
-                longest = max(longest, steps_of(keys_seen(q, row_tiles(q) - 1)));
-                return false;
-            });
+            auto all = [&](auto&& of) {
+                int v = of_request(held, held_looks, of);
+                for (int b0 = kWave; b0 < a.requests; b0 += kWave) {
+                    const Request4 q = lane_request(b0 + lane0);
+                    v += of_request(q, looks(q), of);
+                }
+                return wave_total(v);
+            };
+            auto longest_of = [&](const Request4& q) { return row_tiles(q) ? steps_of(keys_seen(q, row_tiles(q) - 1)) : 0; };
+            int longest = longest_of(held);
+            for (int b0 = kWave; b0 < a.requests; b0 += kWave) longest = max(longest, longest_of(lane_request(b0 + lane0)));
+            longest = wave_max(longest);
             const int steps = all([](int t) { return t; });
             int pieces = kPromptFill + 1;
+            auto pieces_of = [&](int t) { return quotient(t + cut_at - 1, cut_at, __builtin_amdgcn_rcpf(static_cast<float>(cut_at))); };
             if (units <= static_cast<float>(kPromptFill)) {
                 cut_at = max((steps + kPromptFill - 1) / kPromptFill, (kPromptMinTiles + a.prompt_step - 1) >> step_bits);
                 for (int i = 0; i < 4; ++i) {
-                    pieces = all([&](int t) { return (t + cut_at - 1) / cut_at; });
+                    pieces = all(pieces_of);
                     if (pieces <= kPromptFill) break;
                     const float longer = static_cast<float>(cut_at) * static_cast<float>(pieces) * (1.0f / kPromptFill);
                     cut_at = max(static_cast<int>(longer), cut_at + 1);
@@ -882,39 +940,51 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
             line_at = line.start(blockIdx.x);
             line_end = line.start(blockIdx.x + 1);
             int left = line_at;
-            each_request([&](int q_b, const Request4& q) {
-                for (int k0 = 0; k0 < row_tiles(q); k0 += kWave) {
-                    const int n = here(q, k0 + lane0, [&](int t) { return cut_at ? (t + cut_at - 1) / cut_at : t + line.over; });
-                    const int upto = wave_prefix(n);
-                    const uint64_t hit = __ballot(left < upto);
-                    if (hit) {
-                        const int l = __builtin_ctzll(hit), each = __builtin_amdgcn_readlane(n, l) / a.c.heads;
-                        const int local = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
-                        const int head = local / each;
-                        b = q_b;
-                        r = q;
-                        unit = (k0 + l) * a.c.heads + head;
-                        unit_steps = each - line.over;
-                        unit_at = line_at - (local - head * each);
-                        return found = true;
+            auto of = [&](int t) { return cut_at ? pieces_of(t) : t + line.over; };
+            for (int b0 = 0; b0 < a.requests && !found; b0 += kWave) {
+                const Request4 q = b0 ? lane_request(b0 + lane0) : held;
+                const int n = of_request(q, b0 ? looks(q) : held_looks, of), upto = wave_prefix(n);
+                const uint64_t hit = __ballot(left < upto);
+                if (!hit) {
+                    left -= __builtin_amdgcn_readlane(upto, 63);
+                    continue;
+                }
+                const int l = __builtin_ctzll(hit);
+                left -= __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
+                b = b0 + l;
+                r = of_lane(q, l);
+                for (int k0 = 0; k0 < row_tiles(r) && !found; k0 += kWave) {
+                    const int m = here(r, k0 + lane0, of), last = wave_prefix(m);
+                    const uint64_t in = __ballot(left < last);
+                    if (!in) {
+                        left -= __builtin_amdgcn_readlane(last, 63);
+                        continue;
                     }
+                    const int k = __builtin_ctzll(in), each = __builtin_amdgcn_readlane(m, k) / a.c.heads;
+                    left -= __builtin_amdgcn_readlane(last, k) - __builtin_amdgcn_readlane(m, k);
+                    const int head = left / each;
+                    unit = (k0 + k) * a.c.heads + head;
+                    unit_steps = each - line.over;
+                    unit_at = line_at - (left - head * each);
+                    found = true;
+                }
+            }
+        } else {
+            int left = blockIdx.x;
+            for (int b0 = 0; b0 < a.requests && !found; b0 += kWave) {
+                const Request4 q = b0 ? lane_request(b0 + lane0) : held;
+                const int n = row_tiles(q) * a.c.heads, upto = wave_prefix(n);
+                const uint64_t hit = __ballot(left < upto);
+                if (hit) {
+                    const int l = __builtin_ctzll(hit);
+                    unit = left - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
+                    b = b0 + l;
+                    r = of_lane(q, l);
+                    found = true;
+                } else {
                     left -= __builtin_amdgcn_readlane(upto, 63);
                 }
-                return false;
-            });
-        } else {
-            int64_t left = blockIdx.x;
-            each_request([&](int q_b, const Request4& q) {
-                const int64_t n = static_cast<int64_t>(row_tiles(q)) * a.c.heads;
-                if (left >= n) {
-                    left -= n;
-                    return false;
-                }
-                b = q_b;
-                r = q;
-                unit = static_cast<int>(left);
-                return found = true;
-            });
+            }
         }
         if (!found) return;   // the whole workgroup
     }
@@ -1569,30 +1639,34 @@ constexpr int kCus = 256;
 // Its pieces are at most as many as wanted (and a few for rounding) plus one per unit; units at most one per 8 pairs plus one
 // per request that has rows, and, where larger requests go to prompt4_kernel, at most one per 8 of the pairs with which one does
 // not (plus one, so that the bound does not fall where the first request goes there).
+int64_t all_units(int rows, int requests, int heads, int kv_heads) {
+    return (static_cast<int64_t>(rows) * (heads / kv_heads) / kRows + std::min(rows, requests)) * kv_heads;
+}
 int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
     const int group = heads / kv_heads;
-    const int64_t pairs = static_cast<int64_t>(rows) * group, busy = std::min(rows, requests);
-    int64_t units = pairs / kRows + busy;
-    if (may_prompt(rows, requests, group)) units = std::min(units, busy * (blocks_for(std::max(kSplitMax, group), kRows) + 1));
-    return units * kv_heads;
+    const int64_t units = all_units(rows, requests, heads, kv_heads);
+    if (!may_prompt(rows, requests, group)) return units;
+    return std::min(units, static_cast<int64_t>(std::min(rows, requests)) * (blocks_for(std::max(kSplitMax, group), kRows) + 1) * kv_heads);
 }
-int64_t item_bound(int rows, int requests, int heads, int kv_heads, int dim) {
-    const int64_t places = kCus * places_on_cu(dim), units = unit_bound(rows, requests, heads, kv_heads);
+int64_t item_bound(int64_t units, int dim) {
+    const int64_t places = kCus * places_on_cu(dim);
     return (units > places ? 4 : 1) * places + 8 + units;
 }
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
 struct Layout {
-    int64_t items;   // pieces of split4_kernel
+    int64_t items;   // pieces of split4_kernel that have places
     size_t stat, info, bytes;
 };
 Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     Layout l;
-    l.items = item_bound(rows, requests, heads, kv_heads, dim);
-    int64_t places = l.items * kRows;
-    // Room for cut prompts by the rows alone, though a call with no more rows than requests has none: a workspace for some
-    // rows and requests has to serve fewer of either.
-    if (rows > 1 && static_cast<int64_t>(rows) * (heads / kv_heads) > kSplitMax) places += 2 * kPromptFill * kPromptRows;
+    l.items = item_bound(unit_bound(rows, requests, heads, kv_heads), dim);
+    // Room for cut prompts, and for a light call's pieces (which has them only with no more units than the card has places), by the
+    // rows alone, though a call with no more rows than requests has neither: a workspace for some rows and requests has to serve
+    // fewer of either.
+    const bool large = rows > 1 && static_cast<int64_t>(rows) * (heads / kv_heads) > kSplitMax;
+    if (large) l.items = std::max<int64_t>(l.items, 2 * kCus * places_on_cu(dim) + 8);
+    const int64_t places = l.items * kRows + (large ? 2 * kPromptFill * kPromptRows : 0);
     l.stat = align_up(static_cast<size_t>(places) * dim * 4);
     l.info = l.stat + align_up(static_cast<size_t>(places) * 8);
     l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);
@@ -1610,9 +1684,9 @@ void launch_split(const Attn4Args& a, int grid, hipStream_t s) {
 }
 
 template <int D>
-void launch(const Attn4Args& a, hipStream_t s) {
-    if (a.whole) return launch_split<D, kWholeWaves>(a, a.units, s);
-    launch_split<D, kSplitWaves>(a, a.items, s);
+void launch(const Attn4Args& a, int grid, hipStream_t s) {
+    if (a.whole) return launch_split<D, kWholeWaves>(a, grid, s);
+    launch_split<D, kSplitWaves>(a, grid, s);
     if (!a.split_all) {
         const int64_t pairs = static_cast<int64_t>(a.rows) * a.group;
         const int64_t tiles = (pairs / kPromptRows + std::min<int64_t>(a.requests, pairs / kSplitMax + 1)) * a.c.heads;
@@ -1688,19 +1762,23 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     a.info = reinterpret_cast<int2*>(ws + l.info);
     a.items = static_cast<int>(l.items);
     a.split_all = !may_prompt(rows, requests, a.group);
-    a.units = static_cast<int>(unit_bound(rows, requests, heads, kv_heads));
     a.whole = a.split_all && static_cast<int64_t>(max_pages) * page_size <= kWhole * kTile;
     a.places = kCus * places_on_cu(dim);
+    const int64_t units = unit_bound(rows, requests, heads, kv_heads), every = all_units(rows, requests, heads, kv_heads);
+    int64_t grid = a.whole ? units : item_bound(units, dim);
+    a.light_work = a.split_all ? 0 : kLightWork * (256 / dim);
+    if (a.light_work)   // pieces of no more units than places, or whole units
+        grid = std::max({grid, a.places + 8 + std::min<int64_t>(every, a.places), std::min<int64_t>(every, kLightUnits)});
     const int64_t tiles = static_cast<int64_t>(max_pages) * page_size / kTile;
     a.prompt_step = 1;   // a line is below 2^30 steps, in 32 bits
     while (kPromptCut * (tiles / a.prompt_step + 1 + kPromptCost) >= (1 << 30)) a.prompt_step *= 2;
     const hipStream_t s = as_stream(stream);
     if (dim == 64)
-        launch<64>(a, s);
+        launch<64>(a, static_cast<int>(grid), s);
     else if (dim == 128)
-        launch<128>(a, s);
+        launch<128>(a, static_cast<int>(grid), s);
     else
-        launch<256>(a, s);
+        launch<256>(a, static_cast<int>(grid), s);
     return check_launch("attn_kv4_rows");
 }
 

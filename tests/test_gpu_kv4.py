@@ -310,6 +310,15 @@ def test_attention_prompts_as_a_line(lens, fresh, heads, kvh):
     attention_case(r, lens, fresh, heads, kvh, 64, 32, gated=len(lens) > 1, pad=1)
 
 
+@pytest.mark.parametrize("heads,kvh,dim,page,n,total", [(40, 2, 64, 8, 210, 510), (48, 2, 128, 16, 345, 500),
+                                                        (64, 2, 256, 64, 260, 400), (64, 8, 64, 16, 130, 200)])
+def test_attention_chunks_of_many_units(heads, kvh, dim, page, n, total):
+    """A chunk whose row tiles are cut in pieces, in each head dim; and one of more blocks of 8 pairs than the card has places for
+    workgroups of few rows, but few enough for them. Single tokens beside them."""
+    r = np.random.default_rng(dim + heads)
+    attention_case(r, [total, 77, total // 2], [n, 1, 1], heads, kvh, dim, page, pad=1)
+
+
 def test_attention_gate_sizes():
     """Gates to where e^-x and e^x leave the range of fp32; below it results are subnormal numbers, as near as their step."""
     r = np.random.default_rng(17)
