@@ -55,7 +55,7 @@ constexpr int kMaxItems = 1 << 24;     // more than any call has
 constexpr int kSplitMax = 64;          // (row, head) pairs of a request and KV head that always take split4_kernel; a row does
 constexpr int kSplitOnly = 1024;       // and of a whole call that has no more rows than requests
 constexpr int kLightUnits = 1024;      // of a light call, see Weight
-constexpr int kLightWork = 28 * 1024;  // its units x (tiles + kUnitCost) at D = 256
+constexpr int kLightWork = 25 * 1024;  // its units x (tiles + kUnitCost) at D = 256
 constexpr int kUnitCost = 8;
 constexpr int kMaxUp = 110;             // tiny queries are taken times 2^110 at most, so that what undoes it is a normal number
 constexpr float kMoves = 8.0f;         // a token past the reference by more moves it
