@@ -32,6 +32,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <numeric>
 #include <type_traits>
 #include <utility>
 
@@ -77,6 +78,7 @@ struct Attn4Args {
     int places;          // split4_kernel's workgroups that the card holds at once
     int split_all;       // every request takes split4_kernel
     int light_work;      // of a light call at most
+    int light;           // the call is light whatever its lengths are (and split_all)
     int whole;           // and every unit's tiles are one piece: nothing is joined
     int prompt_step;     // tiles of a step of prompt4_kernel's line (a power of two)
     float scale;         // log2(e) / sqrt(D)
@@ -89,10 +91,17 @@ struct Request4 {
     int first, n, len;
     bool bad;
 };
-__device__ __forceinline__ Request4 request(const Attn4Args& a, int b) {
-    const int s = min(max(a.row_start[b], 0), a.rows), e = min(max(a.row_start[b + 1], s), a.rows);
-    const int len = a.kv_len[b], most = a.max_pages << a.page_shift;
+__device__ __forceinline__ Request4 request_of(const Attn4Args& a, int start, int end, int len) {
+    const int s = min(max(start, 0), a.rows), e = min(max(end, s), a.rows), most = a.max_pages << a.page_shift;
     return Request4{s, e - s, min(max(len, 0), most), len > most};
+}
+__device__ __forceinline__ Request4 request(const Attn4Args& a, int b) {
+    return request_of(a, a.row_start[b], a.row_start[b + 1], a.kv_len[b]);
+}
+
+__device__ __forceinline__ Request4 of_lane(const Request4& r, int l) {
+    return Request4{__builtin_amdgcn_readlane(r.first, l), __builtin_amdgcn_readlane(r.n, l), __builtin_amdgcn_readlane(r.len, l),
+                    __builtin_amdgcn_readlane(static_cast<int>(r.bad), l) != 0};
 }
 
 // ------------------------------------------------------------------ pieces of a call
@@ -125,12 +134,11 @@ __device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readl
 // finds it by itself from the lengths. No piece has more than `cut` tiles, a unit's pieces are of one size, and both are whole
 // turns of the waves. `cut` is the least that still gives each of the card's places one piece at most, since a place that takes a
 // second one makes the call half as long again; with more units than places, four pieces. Lengths are held in registers, 64
-// requests to one, up to kHeld x 64.
+// requests to one, up to HELD x 64 (16 for all calls cost one token 1 us, 4 for all 1000 requests 170 us where they take 90).
 struct Piece {
     int b, unit, split, splits, tiles;   // tiles: of one piece
     Request4 r;
 };
-constexpr int kHeld = 4;
 __device__ __forceinline__ int tiles_of(const Request4& r) { return max(1, (r.len + kTile - 1) / kTile); }
 __device__ __forceinline__ bool is_small(const Attn4Args& a, const Request4& r) {
     return a.split_all || r.n * a.group <= max(kSplitMax, a.group);   // rows * heads <= 2^24
@@ -162,39 +170,51 @@ __device__ __forceinline__ int quotient(int n, int d, float inverse) {
     q -= q * d > n;
     return q + (n - q * d >= d);
 }
-__device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
+template <int HELD>
+__device__ __forceinline__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
     const int lane = threadIdx.x & 63;
     auto lane_request = [&](int b) { return b < a.requests ? request(a, b) : Request4{0, 0, 0, false}; };
-    Request4 first{0, 0, 0, false};
-    float units[kHeld];
-    int tiles[kHeld];
+    // The requests' numbers, all loads of a lane in flight together.
+    int start[HELD], end[HELD], len[HELD];
+    auto load = [&](int c) {
+        const int b = min(c * kWave + lane, a.requests - 1);
+        start[c] = a.row_start[b];
+        end[c] = a.row_start[b + 1];
+        len[c] = a.kv_len[b];
+    };
+#pragma unroll
+    for (int c = 0; c < HELD; ++c)
+        if (c * kWave < a.requests) load(c);
+    float units[HELD];
+    int tiles[HELD];
     uint32_t large = 0;
     Weight weight;
 #pragma unroll
-    for (int c = 0; c < kHeld; ++c) {
+    for (int c = 0; c < HELD; ++c) {
         units[c] = 0.f;
         tiles[c] = 0;
         if (c * kWave < a.requests) {
-            const Request4 r = lane_request(c * kWave + lane);
+            const Request4 r = c * kWave + lane < a.requests ? request_of(a, start[c], end[c], len[c]) : Request4{0, 0, 0, false};
             units[c] = units_of(a, r);
             tiles[c] = tiles_of(r);
             large |= is_small(a, r) ? 0u : 1u << c;
             weight.add(a, r);
-            if (c == 0) first = r;
         }
     }
-    for (int b = kHeld * kWave + lane; b < a.requests; b += kWave) weight.add(a, lane_request(b));
-    const bool light = !a.split_all && weight.light(a);
-#pragma unroll
-    for (int c = 0; c < kHeld; ++c)
-        if (((large >> c) & 1) && !light) units[c] = 0.f;
+    if (!a.split_all)
+        for (int b = HELD * kWave + lane; b < a.requests; b += kWave) weight.add(a, request(a, b));
+    const bool light = a.light || (!a.split_all && weight.light(a));
     auto units_here = [&](const Request4& r) { return light || is_small(a, r) ? units_of(a, r) : 0.f; };
+#pragma unroll
+    for (int c = 0; c < HELD; ++c)
+        if (((large >> c) & 1) && !light) units[c] = 0.f;
     auto sum = [&](auto&& of) {   // rounded, but the same in every wave
         float v = 0.f;
 #pragma unroll
-        for (int c = 0; c < kHeld; ++c) v += of(units[c], static_cast<float>(tiles[c]));
-        for (int b = kHeld * kWave + lane; b < a.requests; b += kWave) {
-            const Request4 r = lane_request(b);
+        for (int c = 0; c < HELD; ++c)
+            if (c * kWave < a.requests) v += of(units[c], static_cast<float>(tiles[c]));
+        for (int b = HELD * kWave + lane; b < a.requests; b += kWave) {
+            const Request4 r = request(a, b);
             v += of(units_here(r), static_cast<float>(tiles_of(r)));
         }
         return group_sum<kWave>(v);
@@ -238,23 +258,18 @@ __device__ bool find_piece(const Attn4Args& a, int item, Piece& p) {
             p.split = local - p.unit * p.splits;
             const int turns = (__builtin_amdgcn_readlane(t, l) + kSplitWaves - 1) / kSplitWaves;
             p.tiles = p.splits == 1 ? 1 << 26 : quotient(turns + p.splits - 1, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))) * kSplitWaves;
-            if (b0 == 0) {
-                p.r.first = __builtin_amdgcn_readlane(first.first, l);
-                p.r.n = __builtin_amdgcn_readlane(first.n, l);
-                p.r.len = __builtin_amdgcn_readlane(first.len, l);
-                p.r.bad = __builtin_amdgcn_readlane(static_cast<int>(first.bad), l) != 0;
-            } else {
-                p.r = request(a, p.b);
-            }
+            p.r = b0 == 0 ? request_of(a, __builtin_amdgcn_readlane(start[0], l), __builtin_amdgcn_readlane(end[0], l),
+                                       __builtin_amdgcn_readlane(len[0], l))
+                          : request(a, p.b);
             found = true;
         } else {
             item -= __builtin_amdgcn_readlane(upto, 63);
         }
     };
 #pragma unroll
-    for (int c = 0; c < kHeld; ++c)
+    for (int c = 0; c < HELD; ++c)
         if (!found && c * kWave < a.requests) look(c * kWave, units[c], tiles[c]);
-    for (int b0 = kHeld * kWave; !found && b0 < a.requests; b0 += kWave) {
+    for (int b0 = HELD * kWave; !found && b0 < a.requests; b0 += kWave) {
         const Request4 r = lane_request(b0 + lane);
         look(b0, units_here(r), tiles_of(r));
     }
@@ -418,8 +433,16 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
     __shared__ float2 stat[NW][kRows];
     __shared__ float factors[kRows], qsum[kRows][NG];
     Piece pc;
-    if (!find_piece(a, static_cast<int>(blockIdx.x), pc)) return;   // the whole workgroup
-    const Request4 r = pc.r;
+    const int item = static_cast<int>(blockIdx.x);
+    if (!(a.requests <= kWave       ? find_piece<1>(a, item, pc)
+          : a.requests <= 4 * kWave ? find_piece<4>(a, item, pc)
+                                    : find_piece<16>(a, item, pc)))
+        return;   // the whole workgroup
+    const Request4 r = of_lane(pc.r, 0);
+    pc.b = __builtin_amdgcn_readfirstlane(pc.b);
+    pc.unit = __builtin_amdgcn_readfirstlane(pc.unit);
+    pc.split = __builtin_amdgcn_readfirstlane(pc.split);
+    pc.tiles = __builtin_amdgcn_readfirstlane(pc.tiles);
     const int G = a.group, pairs = r.n * G;
     const float per_g = __builtin_amdgcn_rcpf(static_cast<float>(G));
     auto over_g = [&](int pair) { return quotient(pair, G, per_g); };
@@ -750,7 +773,7 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
     if (r.bad) tot = __builtin_nanf("");
     const int n = over_g(at);
     const size_t pair = static_cast<size_t>(r.first + n) * a.heads + h * G + (at - n * G);
-    const size_t o = pair * D + d, item = static_cast<size_t>(blockIdx.x) * kRows + row;
+    const size_t o = pair * D + d, place = static_cast<size_t>(item) * kRows + row;
     if (pc.splits == 1) {
         float gate[QN];
         if (a.gate) load_floats(a.gate + o, gate);
@@ -758,10 +781,10 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
         for (int i = 0; i < QN; ++i) sum[i] = finished(m, sum[i], tot, a.gate, a.gate ? gate[i] : 0.f);
         store_floats(a.out + o, sum);
     } else {
-        store_floats(a.part + item * D + d, sum);
-        if (d == 0) a.stat[item] = make_float2(m, tot);
+        store_floats(a.part + place * D + d, sum);
+        if (d == 0) a.stat[place] = make_float2(m, tot);
     }
-    if (d == 0 && pc.split == 0 && !a.whole) a.info[pair] = make_int2(static_cast<int>(item), pc.splits);
+    if (d == 0 && pc.split == 0 && !a.whole) a.info[pair] = make_int2(static_cast<int>(place), pc.splits);
 }
 
 // ------------------------------------------------------------------ many rows
@@ -833,10 +856,6 @@ __device__ __forceinline__ void static_for(F&& f) {
     static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-__device__ __forceinline__ Request4 of_lane(const Request4& r, int l) {
-    return Request4{__builtin_amdgcn_readlane(r.first, l), __builtin_amdgcn_readlane(r.n, l), __builtin_amdgcn_readlane(r.len, l),
-                    __builtin_amdgcn_readlane(static_cast<int>(r.bad), l) != 0};
-}
 template <int D>
 __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const Attn4Args a) {
     constexpr int ND = D / 16, DT = D / 32, NG = D / 64, E = D / 64, NTH = kPromptWaves * kWave;   // E: a lane's words of a tile's
@@ -1636,11 +1655,13 @@ bool may_prompt(int rows, int requests, int group) {
 // split4_kernel's workgroups of 4 waves on a CU, by their registers.
 int places_on_cu(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
 constexpr int kCus = 256;
-// Its pieces are at most as many as wanted (and a few for rounding) plus one per unit; units at most one per 8 pairs plus one
-// per request that has rows, and, where larger requests go to prompt4_kernel, at most one per 8 of the pairs with which one does
+// Its pieces are at most as many as wanted (and a few for rounding) plus one per unit; units at most one per 8 pairs and
+// what each request's last one lacks, and, where larger requests go to prompt4_kernel, at most one per 8 of the pairs with which one does
 // not (plus one, so that the bound does not fall where the first request goes there).
 int64_t all_units(int rows, int requests, int heads, int kv_heads) {
-    return (static_cast<int64_t>(rows) * (heads / kv_heads) / kRows + std::min(rows, requests)) * kv_heads;
+    const int group = heads / kv_heads;   // a request's last block lacks a multiple of what group and kRows have in common
+    const int64_t lacking = kRows - std::gcd(group, kRows), busy = std::min(rows, requests);
+    return (static_cast<int64_t>(rows) * group + busy * lacking) / kRows * kv_heads;
 }
 int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
     const int group = heads / kv_heads;
@@ -1761,15 +1782,17 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     a.stat = reinterpret_cast<float2*>(ws + l.stat);
     a.info = reinterpret_cast<int2*>(ws + l.info);
     a.items = static_cast<int>(l.items);
-    a.split_all = !may_prompt(rows, requests, a.group);
-    a.whole = a.split_all && static_cast<int64_t>(max_pages) * page_size <= kWhole * kTile;
     a.places = kCus * places_on_cu(dim);
+    a.light_work = kLightWork * (256 / dim);
+    const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size + kTile - 1) / kTile;
     const int64_t units = unit_bound(rows, requests, heads, kv_heads), every = all_units(rows, requests, heads, kv_heads);
-    int64_t grid = a.whole ? units : item_bound(units, dim);
-    a.light_work = a.split_all ? 0 : kLightWork * (256 / dim);
-    if (a.light_work)   // pieces of no more units than places, or whole units
-        grid = std::max({grid, a.places + 8 + std::min<int64_t>(every, a.places), std::min<int64_t>(every, kLightUnits)});
-    const int64_t tiles = static_cast<int64_t>(max_pages) * page_size / kTile;
+    const bool prompts = may_prompt(rows, requests, a.group);
+    a.light = prompts && every <= kLightUnits && every * (tiles + kUnitCost) <= a.light_work;
+    a.split_all = !prompts || a.light;
+    a.whole = a.split_all && tiles <= kWhole && (!a.light || every <= kCus);   // more units: the card has places for more small ones
+    // pieces of no more units than places, or whole units
+    const int64_t light_grid = std::max(a.places + 8 + std::min<int64_t>(every, a.places), std::min<int64_t>(every, kLightUnits));
+    const int64_t grid = a.whole ? every : prompts ? std::max(item_bound(units, dim), light_grid) : item_bound(units, dim);
     a.prompt_step = 1;   // a line is below 2^30 steps, in 32 bits
     while (kPromptCut * (tiles / a.prompt_step + 1 + kPromptCost) >= (1 << 30)) a.prompt_step *= 2;
     const hipStream_t s = as_stream(stream);

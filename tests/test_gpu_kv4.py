@@ -319,6 +319,15 @@ def test_attention_chunks_of_many_units(heads, kvh, dim, page, n, total):
     attention_case(r, [total, 77, total // 2], [n, 1, 1], heads, kvh, dim, page, pad=1)
 
 
+@pytest.mark.parametrize("heads,kvh,dim,page", [(16, 2, 256, 64), (6, 2, 64, 8), (8, 8, 128, 16)])
+def test_attention_light_calls_of_long_tables(heads, kvh, dim, page):
+    """Tables that could hold long contexts, so that the lengths alone say how much a call is: rows of one request and of several,
+    prompts short and long beside single tokens, more than 256 requests."""
+    r = np.random.default_rng(dim + 1)
+    for lens, fresh in (([41 + 17], [17]), ([33, 900, 60, 1], [33, 12, 30, 1]), ([130, 700], [100, 9]), ([20] * 300, [0, 9, 1] * 100)):
+        attention_case(r, lens, fresh, heads, kvh, dim, page, pad=2, width=70000 // page)
+
+
 def test_attention_gate_sizes():
     """Gates to where e^-x and e^x leave the range of fp32; below it results are subnormal numbers, as near as their step."""
     r = np.random.default_rng(17)
