@@ -257,7 +257,8 @@ __device__ __forceinline__ bool find_piece(const Attn4Args& a, int item, Piece& 
             p.unit = __builtin_amdgcn_readfirstlane(quotient(local, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))));
             p.split = local - p.unit * p.splits;
             const int turns = (__builtin_amdgcn_readlane(t, l) + kSplitWaves - 1) / kSplitWaves;
-            p.tiles = p.splits == 1 ? 1 << 26 : quotient(turns + p.splits - 1, p.splits, __builtin_amdgcn_rcpf(static_cast<float>(p.splits))) * kSplitWaves;
+            const float per_split = __builtin_amdgcn_rcpf(static_cast<float>(p.splits));
+            p.tiles = p.splits == 1 ? 1 << 26 : quotient(turns + p.splits - 1, p.splits, per_split) * kSplitWaves;
             p.r = b0 == 0 ? request_of(a, __builtin_amdgcn_readlane(start[0], l), __builtin_amdgcn_readlane(end[0], l),
                                        __builtin_amdgcn_readlane(len[0], l))
                           : request(a, p.b);
@@ -1655,9 +1656,9 @@ bool may_prompt(int rows, int requests, int group) {
 // split4_kernel's workgroups of 4 waves on a CU, by their registers.
 int places_on_cu(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
 constexpr int kCus = 256;
-// Its pieces are at most as many as wanted (and a few for rounding) plus one per unit; units at most one per 8 pairs and
-// what each request's last one lacks, and, where larger requests go to prompt4_kernel, at most one per 8 of the pairs with which one does
-// not (plus one, so that the bound does not fall where the first request goes there).
+// Its pieces are at most as many as wanted (and a few for rounding) plus one per unit; units at most one per 8 pairs and what each
+// request's last one lacks, and, where larger requests go to prompt4_kernel, at most one per 8 of the pairs with which one does not
+// (plus one, so that the bound does not fall where the first request goes there).
 int64_t all_units(int rows, int requests, int heads, int kv_heads) {
     const int group = heads / kv_heads;   // a request's last block lacks a multiple of what group and kRows have in common
     const int64_t lacking = kRows - std::gcd(group, kRows), busy = std::min(rows, requests);
@@ -1667,7 +1668,8 @@ int64_t unit_bound(int rows, int requests, int heads, int kv_heads) {
     const int group = heads / kv_heads;
     const int64_t units = all_units(rows, requests, heads, kv_heads);
     if (!may_prompt(rows, requests, group)) return units;
-    return std::min(units, static_cast<int64_t>(std::min(rows, requests)) * (blocks_for(std::max(kSplitMax, group), kRows) + 1) * kv_heads);
+    const int64_t busy = std::min(rows, requests);
+    return std::min(units, busy * (blocks_for(std::max(kSplitMax, group), kRows) + 1) * kv_heads);
 }
 int64_t item_bound(int64_t units, int dim) {
     const int64_t places = kCus * places_on_cu(dim);
