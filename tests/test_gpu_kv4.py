@@ -657,6 +657,23 @@ def test_a_workspace_serves_fewer_rows_and_requests():
         close(got, *kv4_ref.attention(q, ref, table, start, lens))
 
 
+@pytest.mark.parametrize("lens,fresh,heads,kvh,dim", [
+    ([9000], [1], 16, 2, 256), ([700] * 150, [1] * 150, 16, 2, 128), ([300, 41], [30, 9], 16, 2, 64), ([1200, 5], [1000, 1], 16, 2, 256),
+    ([90 + i for i in range(40)], [90] * 40, 16, 2, 64), ([900, 800], [900, 700], 32, 4, 128), ([4000] * 3, [12, 1, 300], 24, 8, 128)])
+def test_workspace_ends_where_the_query_says(lens, fresh, heads, kvh, dim):
+    """Calls that cut their keys in every way leave what lies behind the workspace as it was."""
+    r = np.random.default_rng(dim)
+    table, pages = tables(r, lens, 64)
+    cache = ops.kv4_cache(pages, kvh, dim, 64)
+    rows = int(np.sum(fresh))
+    need = ops.attn_kv4_workspace_bytes(rows, len(lens), heads, kvh, dim)
+    memory = torch.full((need + (1 << 20),), 0x5a, dtype=torch.uint8, device="cuda")
+    q = dev(r.standard_normal((rows, heads, dim)).astype(F32))
+    start = np.concatenate([[0], np.cumsum(fresh)])
+    out = ops.attn_kv4_rows(q, cache, dev(table), dev(start, I32), dev(lens, I32), workspace=memory[:need])
+    assert bool((out == 0).all()) and bool((memory[need:] == 0x5a).all())   # a cache of zeros
+
+
 def test_gate_in_place():
     r = np.random.default_rng(14)
     table, pages = tables(r, [50, 90], 16)
