@@ -20,7 +20,6 @@ down to bfloat16, scale the smallest bfloat16 of at least (largest - min) / 15 a
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -34,7 +33,6 @@ FLOOR = 2.0 ** -100   # smallest scale
 THETA, EPS = 1e7, 1e-6
 
 
-@functools.cache
 def _ops():
     path = str(Path.cwd() / "qwen-3.5-cuda_amd")
     if path not in sys.path:
