@@ -1188,7 +1188,8 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
                 Qs[0][i] = Qs[0][4 + i] = static_cast<__bf16>(g ? p1 : p0);
                 Qs[1][i] = Qs[1][4 + i] = static_cast<__bf16>(g ? 0.f : p2);
             }
-            factor = ok ? ldexpf(a.scale, -e) : __builtin_nanf("");
+            // A row that sees no key keeps a factor that is a number, for scores of -inf that it meets.
+            factor = ok || limit < 0 ? ldexpf(a.scale, -e) : __builtin_nanf("");
 #pragma unroll
             for (int d = 0; d < ND; ++d) {   // only products read them: accumulation registers, the others are full
                 asm("" : "+a"(Qh[d]));
