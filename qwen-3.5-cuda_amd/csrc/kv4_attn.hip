@@ -39,6 +39,7 @@
 #include "capi_common.hpp"
 #include "device_common.hpp"
 #include "kv4_common.hpp"
+#include "kv4_places.hpp"
 
 namespace qk {
 namespace {
@@ -51,7 +52,6 @@ typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 constexpr int kTile = 32;              // tokens of a step
 constexpr int kSplitWaves = 4;
 constexpr int kWholeWaves = 8;
-constexpr int kRows = 8;               // (row, head) pairs of a split workgroup
 constexpr int kMaxItems = 1 << 24;     // more than any call has
 constexpr int kSplitMax = 64;          // (row, head) pairs of a request and KV head that always take split4_kernel; a row does
 constexpr int kSplitOnly = 1024;       // and of a whole call that has no more rows than requests
@@ -75,6 +75,7 @@ struct Attn4Args {
     float2* stat;        // [place] (m, l)
     int2* info;          // [row][head] (place of the first piece, pieces); written for the requests' rows alone
     int items;           // split4_kernel's pieces that have places, kRows each
+    int all_places;      // of the workspace
     int places;          // split4_kernel's workgroups that the card holds at once
     int split_all;       // every request takes split4_kernel
     int light_work;      // of a light call at most
@@ -831,16 +832,8 @@ struct Line {
     // The pieces of a unit that starts at `at`.
     __device__ __forceinline__ int pieces(int at, int steps) const { return part_of(at + over + steps - 1) - part_of(at + over) + 1; }
 };
-// Where the pieces of a unit lie. split4_kernel's are neighbours, kRows places each. A workgroup of prompt4_kernel has kPromptRows
-// places for the piece that ends its first unit, or passes through it, and in a second region as many for the one that begins its
-// last.
-struct Places {
-    int first, rows, second;   // of a row: the first piece's place in the first region; the second region's distance, or 0
-    __device__ __forceinline__ int of(int piece) const { return first + (piece == 0 ? second : piece * rows); }
-};
 constexpr int kPromptWaves = 4;
-constexpr int kPromptRows = 32 * kPromptWaves;
-constexpr int kPromptFill = 256;
+static_assert(kPromptRows == 32 * kPromptWaves, "32 rows a wave");
 constexpr int kPromptMinTiles = 4;   // of a piece
 constexpr int kPromptCut = 2 * kPromptFill;   // units that are still a line
 constexpr int kPromptCost = 10;  // of a unit, in tiles
@@ -1389,7 +1382,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
         if (g == 0) {
             const bool none = mu == -FLT_MAX && l == 0.f, live = row0 + col < pairs;
             const int pair = (r.first + ti) * a.heads + head, k = static_cast<int>(blockIdx.x) * kPromptRows + 32 * wv + col;
-            const int first = a.items * kRows + k, place = first + (begins ? kPromptFill * kPromptRows : 0);
+            const int first = a.items * kRows + k, place = first + (begins ? kPromptRegion : 0);
             const float by = !whole ? 1.f : none ? 0.f : 1.f / (r.bad ? __builtin_nanf("") : l);
             out_rows[wv][col] = make_int2(__float_as_int(by), !live ? -1 : whole ? pair : place);
             if (live && !whole) a.stat[place] = make_float2(mu, r.bad ? __builtin_nanf("") : l);
@@ -1489,18 +1482,13 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
 
 // ------------------------------------------------------------------ join
 // Joins the pieces of (row, head) pairs. `entry`: where a pair's pieces are, (0, 0) where nothing is to be joined.
-__device__ __forceinline__ Places places(const Attn4Args& a, int first) {
-    return first < a.items * kRows ? Places{first, kRows, 0} : Places{first, kPromptRows, kPromptFill * kPromptRows};
-}
+__device__ __forceinline__ Places places(const Attn4Args& a, int first) { return places_of(first, a.items * kRows); }
 __device__ __forceinline__ int2 entry(const Attn4Args& a, int64_t pair, bool live) {
     // Pairs of the requests' rows alone: only those have an entry of this call (the workspace may hold an earlier one's).
     const int from = min(max(a.row_start[0], 0), a.rows) * a.heads, end = min(max(a.row_start[a.requests], 0), a.rows) * a.heads;
     int2 in = make_int2(0, 0);
     if (live && pair >= from && pair < end) in = a.info[pair];
-    // one piece is there already; starts that decrease may leave anything
-    const Places p = places(a, in.x);
-    const int past = a.items * kRows + p.second;
-    return in.y > 1 && in.x >= 0 && in.x < past && in.y <= (past - in.x - 1) / p.rows + 1 ? in : make_int2(0, 0);
+    return joinable(in.x, in.y, a.items * kRows, a.all_places) ? in : make_int2(0, 0);
 }
 // The join of two parts of a sum with their references: (m, l, s) takes in (n, k, x).
 template <int V>
@@ -1679,7 +1667,7 @@ int64_t item_bound(int64_t units, int dim) {
 size_t align_up(size_t b) { return (b + 255) & ~size_t{255}; }
 
 struct Layout {
-    int64_t items;   // pieces of split4_kernel that have places
+    int64_t items, places;   // pieces of split4_kernel that have places; places of the workspace
     size_t stat, info, bytes;
 };
 Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
@@ -1690,9 +1678,9 @@ Layout layout(int rows, int requests, int heads, int kv_heads, int dim) {
     // fewer of either.
     const bool large = rows > 1 && static_cast<int64_t>(rows) * (heads / kv_heads) > kSplitMax;
     if (large) l.items = std::max<int64_t>(l.items, 2 * kCus * places_on_cu(dim) + 8);
-    const int64_t places = l.items * kRows + (large ? 2 * kPromptFill * kPromptRows : 0);
-    l.stat = align_up(static_cast<size_t>(places) * dim * 4);
-    l.info = l.stat + align_up(static_cast<size_t>(places) * 8);
+    l.places = l.items * kRows + (large ? 2 * kPromptRegion : 0);
+    l.stat = align_up(static_cast<size_t>(l.places) * dim * 4);
+    l.info = l.stat + align_up(static_cast<size_t>(l.places) * 8);
     l.bytes = l.info + align_up(static_cast<size_t>(rows) * heads * 8);
     return l;
 }
@@ -1785,6 +1773,7 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     a.stat = reinterpret_cast<float2*>(ws + l.stat);
     a.info = reinterpret_cast<int2*>(ws + l.info);
     a.items = static_cast<int>(l.items);
+    a.all_places = static_cast<int>(l.places);
     a.places = kCus * places_on_cu(dim);
     a.light_work = kLightWork * (256 / dim);
     const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size + kTile - 1) / kTile;

@@ -1,4 +1,5 @@
-"""The 4-bit cache and its attention where a documented call meets an end: query rows that are not finite and see no key."""
+"""The 4-bit cache and its attention where a documented call meets an end: query rows that are not finite and see no key,
+starts that fall over a small workspace."""
 
 from __future__ import annotations
 
@@ -40,3 +41,27 @@ def test_rows_without_keys_are_zeros_whatever_their_query_holds(heads, kvh, dim,
                                   [total - n + row + 1 for row in some])
     good = ~bad[some]
     close(got[some][good], want[good], tol[good])
+
+
+def test_what_a_workspace_held_names_no_place_outside_it():
+    """Starts that fall leave rows without an entry of this call, where the workspace may hold anything: a place in the region for
+    cut prompts' pieces, which so small a workspace does not have, is not read. What lies behind the workspace, here memory of this
+    test's own as large as that region, shows in no row."""
+    heads, kvh, dim, page, rows, requests, width = 8, 1, 256, 64, 8, 1000, 20
+    table, lens = np.zeros((requests, width), I32), np.full(requests, page * width, I32)
+    start = np.array([0, 7] * (requests // 2) + [8], I32)   # the last row is the last request's alone, whose pieces never run
+    need = ops.attn_kv4_workspace_bytes(rows, requests, heads, kvh, dim)
+    region = 2 * 256 * 128 * dim * 4
+    memory = torch.full(((need + region) // 4 + 4096,), 3.0, device="cuda")
+    info = memory[(need - 512) // 4:need // 4].view(torch.int32).view(64, 2)   # a place and a number of pieces for each pair
+    places = (need - 512) // (dim * 4 + 8) // 8 * 8   # sums of dim floats and 8 bytes of statistics each
+    out = torch.full((rows, heads, dim), 7.0, device="cuda")
+    q = torch.zeros((rows, heads, dim), device="cuda")
+    cache = ops.kv4_cache(2, kvh, dim, page)
+    for first in (places - 8, places, places + 5, places + 256 * 128 - 1):
+        for pieces in (2, 3, 200):
+            info[:, 0], info[:, 1] = first, pieces
+            memory[need // 4:] = 3.0
+            ops.attn_kv4_rows(q, cache, dev(table), dev(start), dev(lens), out=out, workspace=memory.view(torch.uint8)[:need])
+            torch.cuda.synchronize()
+            assert not bool((out == 3.0).any()) and not bool((out == 1.0).any()), (first, pieces)
