@@ -169,9 +169,9 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4Cache c, const i
             const float km = bf16_value(c.km[tok * ng + (d >> 6)]), vs = bf16_value(c.vs[tok]), vm = bf16_value(c.vm[tok]);
             const uint32_t w[4] = {vw.x, vw.y, vw.z, vw.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {   // scale * code is exact in fp32: one rounding
-                a[j] = km + ks * static_cast<float>((kw >> kv4_shift((d & 4) + j)) & 15u);
-                b[j] = vm + vs * static_cast<float>((w[j] >> kv4_shift(t & 7)) & 15u);
+            for (int j = 0; j < 4; ++j) {   // one rounding; 15 scale by itself may pass the largest number
+                a[j] = __builtin_fmaf(ks, static_cast<float>((kw >> kv4_shift((d & 4) + j)) & 15u), km);
+                b[j] = __builtin_fmaf(vs, static_cast<float>((w[j] >> kv4_shift(t & 7)) & 15u), vm);
             }
         }
         st4(k + 4 * static_cast<size_t>(i), make_float4(a[0], a[1], a[2], a[3]));

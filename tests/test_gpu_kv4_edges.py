@@ -1,5 +1,5 @@
 """The 4-bit cache and its attention where a documented call meets an end: query rows that are not finite and see no key,
-starts that fall over a small workspace."""
+starts that fall over a small workspace, numbers next to 2^127."""
 
 from __future__ import annotations
 
@@ -65,3 +65,21 @@ def test_what_a_workspace_held_names_no_place_outside_it():
             ops.attn_kv4_rows(q, cache, dev(table), dev(start), dev(lens), out=out, workspace=memory.view(torch.uint8)[:need])
             torch.cuda.synchronize()
             assert not bool((out == 3.0).any()) and not bool((out == 1.0).any()), (first, pieces)
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_values_next_to_two_to_the_127_read_back(dim):
+    """15 scale passes the largest fp32 number where a group reaches from -2^127 to 2^127; min + 15 scale does not."""
+    ref = kv4_ref.Cache(1, 1, 8, dim)
+    cache = gpu_cache(ref)
+    most = np.nextafter(F32(2.0 ** 127), F32(0))
+    x = np.random.default_rng(dim).uniform(-1, 1, (3, 1, dim)).astype(F32) * most
+    x[:, :, ::7], x[:, :, 3::7] = -most, most
+    x[1] *= F32(0.99)
+    x[2, 0, 0::64] = 0.5 * most
+    slots = np.arange(3, dtype=I32)
+    ops.kv4_store_rows(dev(x), dev(x), dev(slots), cache)
+    ref.store(0, x, slots)
+    ref.store(1, x, slots)
+    for w, got in enumerate(host(t) for t in ops.kv4_read_rows(cache, dev(slots))):
+        assert np.array_equal(got, ref.values(w, slots).astype(F32)) and np.all(np.isfinite(got))
