@@ -36,6 +36,13 @@ inline unsigned blocks_for(int64_t items, int64_t per_block) {
     return static_cast<unsigned>((items + per_block - 1) / per_block);
 }
 
+// A grid for n workgroups, n below 2^31, of up to 512 threads, along x and, past 2^22 of them, y: one axis of 2^32 threads or more
+// runs short without an error. Kernels number their workgroups blockIdx.y * gridDim.x + blockIdx.x and leave from n on.
+inline dim3 grid_of(int64_t n) {
+    constexpr int64_t kMost = 1 << 22;
+    return dim3(static_cast<unsigned>(n < kMost ? n : kMost), blocks_for(n, kMost));
+}
+
 }  // namespace qk
 
 #define QK_REQUIRE(cond, ...)                                          \

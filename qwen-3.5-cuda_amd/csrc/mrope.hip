@@ -48,8 +48,9 @@ __global__ __launch_bounds__(kMropeBlock) void mrope_vec(const MropeArgs a, cons
     constexpr int HPV = kWave / LPH, HD = 4 * LPH;   // heads of a float4 row of the wave
     const int lane = threadIdx.x & 63, lg = lane % LPH, gbase = lane - lg;
     const int hpr = a.q_heads + a.k_heads, groups = (hpr + HPV * J - 1) / (HPV * J);
-    const int wave = static_cast<int>(blockIdx.x) * (kMropeBlock / kWave) + wave_in_block();
-    if (wave >= a.rows * groups) return;   // the whole wave; the host checks rows * heads < 2^31
+    const uint32_t at = (blockIdx.y * gridDim.x + blockIdx.x) * (kMropeBlock / kWave) + wave_in_block();
+    if (at >= static_cast<uint32_t>(a.rows) * static_cast<uint32_t>(groups)) return;   // the whole wave; the host checks rows * heads < 2^31
+    const int wave = static_cast<int>(at);
     const int t = wave / groups, h0 = (wave - t * groups) * HPV * J + lane / LPH;
     float4 v[J];
     float* ptr[J];
@@ -101,7 +102,10 @@ __global__ __launch_bounds__(kMropeBlock) void mrope_vec(const MropeArgs a, cons
 // Any head dim and alignment: a workgroup per row and head. A thread reads and writes its own pairs and dims alone.
 __global__ __launch_bounds__(kMropeBlock) void mrope_any(const MropeArgs a, const MropeTable tab) {
     __shared__ float lds[kMropeBlock / kWave];
-    const int hpr = a.q_heads + a.k_heads, t = static_cast<int>(blockIdx.x) / hpr, h = static_cast<int>(blockIdx.x) - t * hpr;
+    const int hpr = a.q_heads + a.k_heads;
+    const uint32_t at = blockIdx.y * gridDim.x + blockIdx.x;
+    if (at >= static_cast<uint32_t>(a.rows) * static_cast<uint32_t>(hpr)) return;   // the whole workgroup
+    const int t = static_cast<int>(at) / hpr, h = static_cast<int>(at) - t * hpr;
     const bool is_q = h < a.q_heads;
     float* p = is_q ? a.q + (static_cast<size_t>(t) * a.q_heads + h) * a.head_dim
                     : a.k + (static_cast<size_t>(t) * a.k_heads + (h - a.q_heads)) * a.head_dim;
@@ -132,7 +136,7 @@ void launch_vec(const MropeArgs& a, const MropeTable& tab, hipStream_t s) {
     constexpr int J = LPH == 64 ? 3 : 2;
     const int per = kWave / LPH * J;
     const int64_t waves = static_cast<int64_t>(a.rows) * ((a.q_heads + a.k_heads + per - 1) / per);
-    mrope_vec<LPH, J><<<blocks_for(waves, kMropeBlock / kWave), kMropeBlock, 0, s>>>(a, tab);
+    mrope_vec<LPH, J><<<grid_of(blocks_for(waves, kMropeBlock / kWave)), kMropeBlock, 0, s>>>(a, tab);
 }
 
 }  // namespace
@@ -188,7 +192,7 @@ extern "C" int qwen_attn_qk_norm_mrope_rows(float* q, float* k, const float* q_w
                      (q_heads == 0 || (aligned16(q) && aligned16(q_weight))) &&
                      (k_heads == 0 || (aligned16(k) && aligned16(k_weight)));
     if (!vec)
-        mrope_any<<<static_cast<unsigned>(rows) * static_cast<unsigned>(q_heads + k_heads), kMropeBlock, 0, s>>>(a, tab);
+        mrope_any<<<grid_of(static_cast<int64_t>(rows) * (q_heads + k_heads)), kMropeBlock, 0, s>>>(a, tab);
     else if (lph == 64)
         launch_vec<64>(a, tab, s);
     else if (lph == 32)
