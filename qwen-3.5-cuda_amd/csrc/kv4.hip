@@ -53,7 +53,7 @@ __device__ __forceinline__ void quantize4(const float4 x, Kv4Group& g, uint32_t 
 
 __device__ __forceinline__ uint16_t bf16_bits(float f) { return static_cast<uint16_t>(__float_as_uint(f) >> 16); }
 
-// Grid: x = shares of kStore4Rows rows, y = head, z = keys, values.
+// Grid: x = shares of kStore4Rows rows, y = head, z = keys, values of the first gridDim.x shares, of the next ones, and so on.
 template <int D, bool ALIGNED>
 __global__ __launch_bounds__(kStore4Block) void kv4_store_kernel(const float* __restrict__ k, const float* __restrict__ v,
                                                                  int64_t k_stride, int64_t v_stride,
@@ -62,7 +62,9 @@ __global__ __launch_bounds__(kStore4Block) void kv4_store_kernel(const float* __
     __shared__ uint32_t codes[2 * kStore4Rows][LPR];   // a value row's codes, a byte a dim
     const int lane = threadIdx.x & 63, l = lane % LPR, h = blockIdx.y, P = c.page;
     const int total = c.pages * P;
-    const int base = static_cast<int>(blockIdx.x) * kStore4Rows;
+    const uint32_t share = (blockIdx.z >> 1) * gridDim.x + blockIdx.x;
+    if (static_cast<int64_t>(share) * kStore4Rows >= rows) return;   // the whole workgroup
+    const int base = static_cast<int>(share) * kStore4Rows;
     // Lane i of every wave looks at row base - 1 + i; `cont`: the row goes on with the piece of the one before it.
     const int64_t seen = static_cast<int64_t>(base) - 1 + lane;
     int slot = -1;
@@ -72,7 +74,7 @@ __global__ __launch_bounds__(kStore4Block) void kv4_store_kernel(const float* __
     const uint64_t cont = __ballot(lane > 0 && in && (slot & 7) != 0 && before == slot - 1);
     const uint64_t live = __ballot(in);
     const int wv = wave_in_block();
-    if (blockIdx.z == 0) {
+    if ((blockIdx.z & 1) == 0) {
 #pragma unroll
         for (int i0 = 0; i0 < kStore4Rows; i0 += WAVES * RPW) {
             const int i = i0 + wv * RPW + lane / LPR, s = __shfl(slot, 1 + i);
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4Cache c, const i
 template <int D>
 void launch_store(const float* k, const float* v, int64_t ks, int64_t vs, const int32_t* slots, int rows, const Kv4Cache& c,
                   bool vec, hipStream_t s) {
-    const dim3 grid(blocks_for(rows, kStore4Rows), static_cast<unsigned>(c.heads), 2);
+    const dim3 shares = grid_of(blocks_for(rows, kStore4Rows)), grid(shares.x, static_cast<unsigned>(c.heads), 2 * shares.y);
     const auto kernel = vec ? kv4_store_kernel<D, true> : kv4_store_kernel<D, false>;
     kernel<<<grid, kStore4Block, 0, s>>>(k, v, ks, vs, slots, rows, c);
 }

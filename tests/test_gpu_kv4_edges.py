@@ -1,5 +1,6 @@
 """The 4-bit cache and its attention where a documented call meets an end: query rows that are not finite and see no key,
-starts that fall over a small workspace, numbers next to 2^127."""
+starts that fall over a small workspace, numbers next to 2^127,
+more rows than one axis of a grid has threads for."""
 
 from __future__ import annotations
 
@@ -9,7 +10,7 @@ import torch
 
 import kv4_ref
 from qwen35_hip import ops
-from test_gpu_kv4 import close, dev, gpu_cache, host, random_cache, tables
+from test_gpu_kv4 import close, dev, gpu_cache, host, random_cache, same_cache, tables
 
 pytestmark = pytest.mark.gpu
 F32, I32 = np.float32, np.int32
@@ -83,3 +84,21 @@ def test_values_next_to_two_to_the_127_read_back(dim):
     ref.store(1, x, slots)
     for w, got in enumerate(host(t) for t in ops.kv4_read_rows(cache, dev(slots))):
         assert np.array_equal(got, ref.values(w, slots).astype(F32)) and np.all(np.isfinite(got))
+
+
+def test_store_of_more_rows_than_one_axis_of_a_grid_takes():
+    """2^26 + 20 rows, all but a few without a slot."""
+    rows, dim, page = (1 << 26) + 20, 64, 16
+    ref = kv4_ref.Cache(4, 1, page, dim)
+    cache = gpu_cache(ref)
+    at = np.concatenate([[0, 9, 1 << 20, (1 << 25) + 3, (1 << 26) - 9], np.arange((1 << 26) - 4, rows)])
+    slots = np.concatenate([[40, 1, 7, 50, 33], 8 + np.arange(24)]).astype(I32)
+    small = np.random.default_rng(3).standard_normal((len(at), 1, dim)).astype(F32)
+    x = torch.empty((rows, 1, dim), device="cuda")
+    x[dev(at)] = dev(small)
+    where = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    where[dev(at)] = dev(slots)
+    ops.kv4_store_rows(x, x, where, cache)
+    ref.store(0, small, slots)
+    ref.store(1, small, slots)
+    same_cache(cache, ref)
