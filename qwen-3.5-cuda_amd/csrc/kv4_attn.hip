@@ -1785,6 +1785,8 @@ int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_
     // pieces of no more units than places, or whole units
     const int64_t light_grid = std::max(a.places + 8 + std::min<int64_t>(every, a.places), std::min<int64_t>(every, kLightUnits));
     const int64_t grid = a.whole ? every : prompts ? std::max(item_bound(units, dim), light_grid) : item_bound(units, dim);
+    QK_REQUIRE(grid * (a.whole ? kWholeWaves : kSplitWaves) * kWave < (int64_t{1} << 32),
+               "attn_kv4_rows: %d rows of %d KV heads in %d requests exceed one call", rows, kv_heads, requests);
     a.prompt_step = 1;   // a line is below 2^30 steps, in 32 bits
     while (kPromptCut * (tiles / a.prompt_step + 1 + kPromptCost) >= (1 << 30)) a.prompt_step *= 2;
     const hipStream_t s = as_stream(stream);
