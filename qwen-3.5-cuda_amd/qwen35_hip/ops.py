@@ -768,6 +768,16 @@ class Kv4Cache(namedtuple("_Kv4Cache", "k v k_scale k_min v_scale v_min pages pa
                 pages, page, heads, dim)
         return tuple.__new__(cls, (k, v, k_scale, k_min, v_scale, v_min, pages, page, heads, dim, args))
 
+    def __getnewargs__(self):   # a copy has the pointers of its own tensors
+        return self[:6]
+
+    def _replace(self, **_):
+        raise AttributeError("a Kv4Cache stays over the tensors it was made of")
+
+    @classmethod
+    def _make(cls, _):
+        raise AttributeError("a Kv4Cache is made of its six tensors")
+
 
 def kv4_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv4Cache:
     """An empty cache. kv8_plan does its pages' bookkeeping."""

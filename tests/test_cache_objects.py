@@ -1,0 +1,47 @@
+"""Copies of the paged caches, and objects that stand for one. On the CPU: the checks that ask for a device's tensors are
+left out, everything else is the classes' own."""
+
+from __future__ import annotations
+
+import copy
+import pickle
+
+import pytest
+import torch
+
+from qwen35_hip import ops
+
+PAGES, HEADS, PAGE, DIM = 3, 2, 16, 64
+
+
+@pytest.fixture
+def four(monkeypatch):
+    monkeypatch.setattr(ops, "_checked", lambda dtype, *ts: None)
+    return ops.kv4_cache(PAGES, HEADS, DIM, PAGE, device="cpu")
+
+
+def pointers(cache, names):
+    return tuple(getattr(cache, n).data_ptr() for n in names)
+
+
+FOUR = ("k", "v", "k_scale", "k_min", "v_scale", "v_min")
+
+
+def test_a_kv4_cache_changes_no_part(four):
+    other = torch.zeros_like(four.k)
+    for change in (lambda: four._replace(k=other), lambda: four._replace(args=four.args), lambda: four._replace(),
+                   lambda: ops.Kv4Cache._make(four), lambda: ops.Kv4Cache._make([other] + list(four)[1:]),
+                   lambda: setattr(four, "k", other), lambda: setattr(four, "more", 1), lambda: delattr(four, "k")):
+        with pytest.raises((AttributeError, TypeError)):
+            change()
+    assert four.args[:6] == pointers(four, FOUR)
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c))])
+def test_a_copy_of_a_kv4_cache_has_its_own_tensors_pointers(four, how):
+    four.k.fill_(7)
+    c = how(four)
+    assert type(c) is ops.Kv4Cache
+    assert c.args[:6] == pointers(c, FOUR) and c.args[6:] == four.args[6:] == (PAGES, PAGE, HEADS, DIM)
+    assert (c.pages, c.page, c.heads, c.dim) == (PAGES, PAGE, HEADS, DIM) and bool((c.k == 7).all())
+    assert (c.k.data_ptr() == four.k.data_ptr()) == (how is copy.copy)
