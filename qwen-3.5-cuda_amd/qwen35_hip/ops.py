@@ -606,6 +606,9 @@ class Kv8Cache:
             raise AttributeError("a Kv8Cache stays over the tensors it was made of")
         object.__setattr__(self, name, value)
 
+    def __reduce__(self):   # a copy has the pointers of its own tensors
+        return type(self), (self.k, self.v, self.k_scale, self.v_scale)
+
 
 def kv8_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv8Cache:
     """An empty cache."""

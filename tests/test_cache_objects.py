@@ -45,3 +45,23 @@ def test_a_copy_of_a_kv4_cache_has_its_own_tensors_pointers(four, how):
     assert c.args[:6] == pointers(c, FOUR) and c.args[6:] == four.args[6:] == (PAGES, PAGE, HEADS, DIM)
     assert (c.pages, c.page, c.heads, c.dim) == (PAGES, PAGE, HEADS, DIM) and bool((c.k == 7).all())
     assert (c.k.data_ptr() == four.k.data_ptr()) == (how is copy.copy)
+
+
+EIGHT = ("k", "v", "k_scale", "v_scale")
+
+
+@pytest.fixture
+def eight(monkeypatch):
+    monkeypatch.setattr(ops, "_checked", lambda dtype, *ts: None)
+    return ops.kv8_cache(PAGES, HEADS, DIM, PAGE, device="cpu")
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda c: pickle.loads(pickle.dumps(c))])
+def test_a_copy_of_a_kv8_cache_has_its_own_tensors_pointers(eight, how):
+    eight.k.fill_(7)
+    c = how(eight)
+    assert type(c) is ops.Kv8Cache
+    assert c.args == pointers(c, EIGHT) + (PAGES, PAGE, HEADS, DIM) and bool((c.k == 7).all())
+    assert (c.k.data_ptr() == eight.k.data_ptr()) == (how is copy.copy)
+    with pytest.raises(AttributeError):
+        c.k = eight.k
