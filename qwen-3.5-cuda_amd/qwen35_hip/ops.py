@@ -652,10 +652,15 @@ def kv8_plan(cached, fresh, block_table, free_pages, free_head, page_size, rows,
     return row_start, kv_len, slots, pos, free_head_out
 
 
-def _of(cache, kind) -> None:
-    """The two kinds of cache have other arrays behind their pointers."""
-    if not isinstance(cache, kind):
-        raise ValueError(f"expected a {kind.__name__}, got {type(cache).__name__}")
+def _not_kv4(cache) -> None:
+    """The two kinds of cache have other arrays behind their pointers. The 8-bit calls take any object with a Kv8Cache's fields."""
+    if isinstance(cache, Kv4Cache):
+        raise ValueError("expected a Kv8Cache, got Kv4Cache")
+
+
+def _kv4(cache) -> None:
+    if not isinstance(cache, Kv4Cache):
+        raise ValueError(f"expected a Kv4Cache, got {type(cache).__name__}")
 
 
 def _kv_rows(x, heads, dim):
@@ -674,7 +679,7 @@ def _kv_rows(x, heads, dim):
 
 def kv8_store_rows(k, v, slots, cache: Kv8Cache, stream=None):
     """k, v [rows, kv_heads, dim] (rows may be strided) quantized into `slots` int32 [rows] of the cache, in place."""
-    _of(cache, Kv8Cache)
+    _not_kv4(cache)
     ks, vs = _kv_rows(k, cache.heads, cache.dim), _kv_rows(v, cache.heads, cache.dim)
     _checked(torch.int32, slots)
     rows = k.shape[0]
@@ -687,7 +692,7 @@ def kv8_store_rows(k, v, slots, cache: Kv8Cache, stream=None):
 
 def kv8_read_rows(cache: Kv8Cache, slots, k=None, v=None, stream=None):
     """The values of `slots` int32 [rows] -> k, v float32 [rows, kv_heads, dim]."""
-    _of(cache, Kv8Cache)
+    _not_kv4(cache)
     _checked(torch.int32, slots)
     n = slots.numel()
     shape = (n, cache.heads, cache.dim)
@@ -736,7 +741,7 @@ def attn_kv8_rows(q, cache: Kv8Cache, block_table, row_start, kv_len, gate=None,
     """q [rows, heads, dim] of several requests (rows row_start[b] .. row_start[b + 1] - 1 are the last positions of
     request b's kv_len[b] tokens, in the pages block_table[b]) -> out [rows, heads, dim] (x sigmoid(gate)), causal. Rows of
     no request are left as `out` has them (uninitialised if it is allocated here)."""
-    _of(cache, Kv8Cache)
+    _not_kv4(cache)
     rows, heads, n, out, workspace = _attn_paged(q, cache, attn_kv8_workspace_bytes, block_table, row_start, kv_len, gate,
                                                  workspace, out, stream)
     check(load().qwen_attn_kv8_rows(_p(q), *cache.args[:6], _p(block_table), block_table.shape[1], _p(row_start),
@@ -795,7 +800,7 @@ def kv4_cache(pages, kv_heads, dim, page_size=64, device="cuda") -> Kv4Cache:
 
 def kv4_store_rows(k, v, slots, cache: Kv4Cache, stream=None):
     """k, v [rows, kv_heads, dim] (rows may be strided) quantized into `slots` int32 [rows] of the cache, in place."""
-    _of(cache, Kv4Cache)
+    _kv4(cache)
     ks, vs = _kv_rows(k, cache.heads, cache.dim), _kv_rows(v, cache.heads, cache.dim)
     _checked(torch.int32, slots)
     rows = k.shape[0]
@@ -808,7 +813,7 @@ def kv4_store_rows(k, v, slots, cache: Kv4Cache, stream=None):
 
 def kv4_read_rows(cache: Kv4Cache, slots, k=None, v=None, stream=None):
     """The values of `slots` int32 [rows] -> k, v float32 [rows, kv_heads, dim]."""
-    _of(cache, Kv4Cache)
+    _kv4(cache)
     _checked(torch.int32, slots)
     n = slots.numel()
     shape = (n, cache.heads, cache.dim)
@@ -829,7 +834,7 @@ def attn_kv4_workspace_bytes(rows, requests, heads, kv_heads, dim) -> int:
 
 def attn_kv4_rows(q, cache: Kv4Cache, block_table, row_start, kv_len, gate=None, workspace=None, out=None, stream=None):
     """attn_kv8_rows over a Kv4Cache."""
-    _of(cache, Kv4Cache)
+    _kv4(cache)
     rows, heads, n, out, workspace = _attn_paged(q, cache, attn_kv4_workspace_bytes, block_table, row_start, kv_len, gate,
                                                  workspace, out, stream)
     check(load().qwen_attn_kv4_rows(_p(q), *cache.args[:8], _p(block_table), block_table.shape[1], _p(row_start),

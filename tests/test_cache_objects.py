@@ -65,3 +65,31 @@ def test_a_copy_of_a_kv8_cache_has_its_own_tensors_pointers(eight, how):
     assert (c.k.data_ptr() == eight.k.data_ptr()) == (how is copy.copy)
     with pytest.raises(AttributeError):
         c.k = eight.k
+
+
+class Lookalike:
+    """A program's own object with a Kv8Cache's fields."""
+
+    def __init__(self, cache):
+        for name in ops.Kv8Cache.__slots__:
+            setattr(self, name, getattr(cache, name))
+
+
+def test_the_8_bit_calls_take_any_object_with_a_caches_fields(eight, four):
+    """They refuse a 4-bit cache, which has other arrays behind its pointers, and nothing else by its type: what these calls
+    refuse here are the tensors, which are not a device's."""
+    x, i = torch.zeros((1, HEADS, DIM)), torch.zeros(1, dtype=torch.int32)
+
+    def calls(c):
+        return (lambda: ops.kv8_store_rows(x, x, i, c), lambda: ops.attn_kv8_rows(x, c, i.view(1, 1), i, i))
+    for call in calls(Lookalike(eight)):
+        with pytest.raises(ValueError) as e:
+            call()
+        assert "expected a Kv" not in str(e.value)
+    for call in (*calls(four), lambda: ops.kv8_read_rows(four, i)):
+        with pytest.raises(ValueError, match="expected a Kv8Cache, got Kv4Cache"):
+            call()
+    for call in (lambda: ops.kv4_store_rows(x, x, i, eight), lambda: ops.kv4_read_rows(eight, i),
+                 lambda: ops.attn_kv4_rows(x, eight, i.view(1, 1), i, i)):
+        with pytest.raises(ValueError, match="expected a Kv4Cache, got Kv8Cache"):
+            call()
