@@ -1,6 +1,6 @@
 """The 4-bit cache and its attention where a documented call meets an end: query rows that are not finite and see no key,
-starts that fall over a small workspace, numbers next to 2^127,
-more rows than one axis of a grid has threads for."""
+starts that fall over a small workspace, numbers next to 2^127, more rows than one axis of a grid has threads for, starts that
+leave the step, thousands of requests, tables that could hold a thousand million tokens."""
 
 from __future__ import annotations
 
@@ -10,7 +10,7 @@ import torch
 
 import kv4_ref
 from qwen35_hip import ops
-from test_gpu_kv4 import close, dev, gpu_cache, host, random_cache, same_cache, tables
+from test_gpu_kv4 import attention_case, close, dev, gpu_cache, host, random_cache, same_cache, tables
 
 pytestmark = pytest.mark.gpu
 F32, I32 = np.float32, np.int32
@@ -102,3 +102,86 @@ def test_store_of_more_rows_than_one_axis_of_a_grid_takes():
     ref.store(0, small, slots)
     ref.store(1, small, slots)
     same_cache(cache, ref)
+
+
+@pytest.mark.parametrize("lens,width", [((64, -5, 64, 1000), 4), ((3000, -5, 2500, 1 << 30), 200)])
+def test_rows_of_starts_that_leave_the_step(lens, width):
+    """Starts before the first row and behind the last, a negative length, and a length past the table row of a request that has
+    no rows: the rows of each request, in one launch or by pieces."""
+    r = np.random.default_rng(width)
+    page, heads, kvh, dim = 16, 4, 2, 64
+    true = [lens[0], 0, lens[2], 0]
+    table, pages = tables(r, true, page, width)
+    ref = random_cache(r, pages, kvh, page, dim)
+    q = r.standard_normal((12, heads, dim)).astype(F32)
+    start = [-7, 3, 6, 2 ** 31 - 1, 2 ** 31 - 1]
+    got = host(ops.attn_kv4_rows(dev(q), gpu_cache(ref), dev(table), dev(start, I32), dev(lens, I32)))
+    close(got, *kv4_ref.attention(q, ref, table, [0, 3, 6, 12, 12], true))
+
+
+def test_rows_of_one_request_where_starts_fall():
+    """Requests that share some rows: those that one request alone has are right."""
+    r = np.random.default_rng(12)
+    page, heads, kvh, dim = 16, 4, 2, 64
+    table, pages = tables(r, [64] * 4, page)
+    ref = random_cache(r, pages, kvh, page, dim)
+    q = r.standard_normal((12, heads, dim)).astype(F32)
+    got = host(ops.attn_kv4_rows(dev(q), gpu_cache(ref), dev(table), dev([0, 5, 3, 99, 4], I32), dev([64] * 4, I32)))
+    for b, first, rows in ((0, 0, [0, 1, 2]), (2, 3, [5, 6, 7, 8, 9, 10, 11])):
+        n = 5 if b == 0 else 9
+        close(got[rows], *kv4_ref.attention(q[rows], ref, np.repeat(table[b:b + 1], len(rows), 0), range(len(rows) + 1),
+                                            [64 - n + row - first + 1 for row in rows]))
+
+
+@pytest.mark.parametrize("requests,width", [(1025, 4), (1100, 60), (4096, 4), (4096, 60)])
+@pytest.mark.parametrize("page", [16, 64])
+def test_more_requests_than_are_held_in_registers(requests, width, page):
+    """Most of them idle, some of the live ones past 1024, alone and with a few rows each; short tables and long ones."""
+    r = np.random.default_rng(requests + width)
+    lens, fresh = np.zeros(requests, int), np.zeros(requests, int)
+    live = np.concatenate([[0, 63, 64, requests - 1, 1024], r.choice(np.arange(65, 1023), 20, replace=False)])
+    lens[live] = r.integers(1, width * page, len(live))
+    fresh[live] = np.minimum(lens[live], r.integers(1, 4, len(live)))
+    attention_case(r, lens.tolist(), fresh.tolist(), 8, 2, 64, page, pad=1, width=width)
+
+
+def close_in_some_rows(r, got, q, ref, table, start, lens, some):
+    """`some` random rows of each request (its first and last among them) against the 64-bit form, a row a request."""
+    rows, of, seen = [], [], []
+    for b, total in enumerate(lens):
+        n = start[b + 1] - start[b]
+        for i in sorted({0, n - 1, *r.integers(0, n, some).tolist()}) if n else ():
+            rows.append(start[b] + i)
+            of.append(b)
+            seen.append(total - n + i + 1)
+    close(got[rows], *kv4_ref.attention(q[rows], ref, table[of], range(len(rows) + 1), seen))
+
+
+def prompts(r, lens, fresh, heads, kvh, dim, page, width):
+    table, pages = tables(r, lens, page, width)
+    ref = random_cache(r, pages, kvh, page, dim)
+    start = np.concatenate([[0], np.cumsum(fresh)]).astype(int)
+    q = r.standard_normal((start[-1], heads, dim)).astype(F32)
+    got = host(ops.attn_kv4_rows(dev(q), gpu_cache(ref), dev(table), dev(start, I32), dev(lens, I32)))
+    close_in_some_rows(r, got, q, ref, table, start.tolist(), lens, 6)
+
+
+@pytest.mark.parametrize("at", [1024, 2000, 4095])
+def test_a_prompt_past_the_requests_in_registers(at):
+    """A chunk too heavy to be a light call, one of few rows and single tokens, among 4096 requests."""
+    r = np.random.default_rng(at)
+    lens, fresh = np.zeros(4096, int), np.zeros(4096, int)
+    lens[[3, 1023, 3000, at]], fresh[[3, 1023, 3000, at]] = (700, 90, 64, 640), (1, 12, 1, 600)
+    prompts(r, lens.tolist(), fresh.tolist(), 16, 2, 64, 16, 48)
+
+
+@pytest.mark.parametrize("width", [65535, 65536, 1 << 18, 1 << 20])
+@pytest.mark.parametrize("lens,fresh,heads,kvh,dim", [
+    ([5000, 33], [140, 1], 64, 2, 64),                 # few row tiles, in pieces
+    ([700, 2100, 90], [600, 300, 1], 16, 2, 64),       # row tiles short and long
+    ([4000, 2200], [300, 200], 64, 16, 64),            # hundreds of them, one line
+    ([1500], [170], 48, 3, 256),
+])
+def test_prompts_over_tables_of_up_to_a_thousand_million_tokens(lens, fresh, heads, kvh, dim, width):
+    """A line of tiles counts steps of 2, 8 and 32 tiles there, so that its length stays in 32 bits."""
+    prompts(np.random.default_rng(width + dim), lens, fresh, heads, kvh, dim, 1024, width)
