@@ -15,9 +15,11 @@
 //
 // The parts of a score: the products of each group of 64 dims come out of the matrix core by themselves and are scaled in
 // fp32; sum_g min_tg sum(q)_g is one product more, of the bf16 minima as they lie in the cache with three bf16 parts, 24
-// bits, of each sum. Values are summed as code - 8, with min + 8 scale in the place of min: codes 0..15 would add up to
-// numbers as large as the context is long, of which the mean of thousands of values of either sign keeps few bits
-// (200000 keys: 2e-3 off, now as near as fp32 values).
+// bits, of each sum. Values are summed as code - 8 of even tokens and code - 7 of odd ones, with min + 8 scale and min + 7 scale in
+// the place of min: codes 0..15 would add up to numbers as large as the context is long, of which the mean of thousands of values
+// of either sign keeps few bits (one row at 200000 keys: 2e-3 off). So would code - 8 alone, at half a code a token: where a row's
+// keys come one after the other, 5.7e-6 of the outputs at 5000 of them and 1.5e-5 at 12000, now 0.8e-6 and 1.3e-6 (fp32 values in
+// a library's products: 0.9e-6 and 1.1e-6).
 //
 // Both products are computed transposed, scores^T = K q^T and out^T = V^T p^T, because then the scores that a lane holds (4
 // tokens of one row in each half of a tile) are already the p^T operand of the second product: with key row lr of half `x`
@@ -58,6 +60,7 @@ constexpr int kSplitOnly = 1024;       // and of a whole call that has no more r
 constexpr int kLightUnits = 1024;      // of a light call, see Weight
 constexpr int kLightWork = 25 * 1024;  // its units x (tiles + kUnitCost) at D = 256
 constexpr int kUnitCost = 8;
+constexpr int kEvenLess = 8, kOddLess = 7;   // what a value's code is less when it is summed, see above
 constexpr int kMaxUp = 110;             // tiny queries are taken times 2^110 at most, so that what undoes it is a normal number
 constexpr float kMoves = 8.0f;         // a token past the reference by more moves it
 constexpr float kWeightUp = 10.0f;     // log2 of what exponentials, and so all sums, are taken times: weights fill fp16
@@ -279,18 +282,18 @@ __device__ __forceinline__ bool find_piece(const Attn4Args& a, int item, Piece& 
 }
 
 // ------------------------------------------------------------------ codes and numbers
-// A word's 8 codes less LESS as the fp16 operand. `magic` is 0x64006400 from a vector register: v_and_or_b32 takes one
+// A word's 8 codes as the fp16 operand, the even ones less EVEN, the odd ones less ODD. `magic` is 0x64006400 from a vector register: v_and_or_b32 takes one
 // constant only, and the compiler makes two instructions of a mask and a literal.
 __device__ __forceinline__ uint32_t code_magic() {
     uint32_t m = 0x64006400u;
     asm("" : "+v"(m));
     return m;
 }
-template <int LESS>
+template <int EVEN, int ODD = EVEN>
 __device__ __forceinline__ f16x8_t codes8(uint32_t w, uint32_t magic) {
-    const f16x2_t down = {(_Float16)(-1024.0f - LESS), (_Float16)(-1024.0f - LESS)};
+    const f16x2_t down = {(_Float16)(-1024.0f - EVEN), (_Float16)(-1024.0f - ODD)};
     const f16x2_t sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-    const f16x2_t down16 = {(_Float16)(-64.0f - LESS), (_Float16)(-64.0f - LESS)};
+    const f16x2_t down16 = {(_Float16)(-64.0f - EVEN), (_Float16)(-64.0f - ODD)};
     f16x8_t r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -670,7 +673,7 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
             const float mine = part ? S[1][i] : S[0][i], other = part ? S[0][i] : S[1][i];
             s[i] = (mine + dpp_move<0xB1>(other)) * f;
             sv[i] = i & 1 ? bf16_hi(vs[i >> 1]) : bf16_lo(vs[i >> 1]);
-            mv[i] = __builtin_fmaf(8.0f, sv[i], i & 1 ? bf16_hi(vm[i >> 1]) : bf16_lo(vm[i >> 1]));
+            mv[i] = __builtin_fmaf(i & 1 ? kOddLess : kEvenLess, sv[i], i & 1 ? bf16_hi(vm[i >> 1]) : bf16_lo(vm[i >> 1]));
         }
         if (t * kTile + kTile - 1 > first_limit) {
 #pragma unroll
@@ -727,7 +730,7 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
             const uint32_t w[4] = {V[m].x, V[m].y, V[m].z, V[m].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<8>(w[e], magic), __builtin_bit_cast(f16x8_t, W),
+                acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8<kEvenLess, kOddLess>(w[e], magic), __builtin_bit_cast(f16x8_t, W),
                                                                    acc[m][e], 0, 0, 0);
         }
     }
@@ -859,7 +862,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
     __shared__ __align__(16) uint16_t kmin[4][kTile][8];   // [tile % 4][key row]: bf16, the groups' minima (4) and 8 scale (4)
     __shared__ __align__(16) float outs[kPromptWaves][32][64 + 4];   // a wave's rows, 64 dims; 4 more, and 8 rows meet no bank twice
     __shared__ int2 out_rows[kPromptWaves][32];            // what a row's sums are taken times, where they go (-1: nowhere)
-    __shared__ __align__(16) float tok[4][4][kTile];       // [tile % 4][key factor, value scale, min + 8 scale, log2 size][token]
+    __shared__ __align__(16) float tok[4][4][kTile];       // [tile % 4][key factor, value scale, min + 8 or 7 scale, log2 size][token]
     // which request, KV head and row tile: the last row tiles (the longest rows) first
     const int G = a.group;
     const float per_g = 1.0f / static_cast<float>(G);
@@ -1095,7 +1098,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
             ks[st & 1][dims][32 * (w & 1) + rho] = codes8<8>(kr[j], magic) * f16x8_t{f, f, f, f, f, f, f, f};
         };
         auto v_put = [&](int st, int j) {   // dim 32 E m + E row + j is row `row` of value tile E m + j
-            vs[st & 1][E * g + j][wv >> 1][32 * (wv & 1) + col] = codes8<8>(vr[j], magic);
+            vs[st & 1][E * g + j][wv >> 1][32 * (wv & 1) + col] = codes8<kEvenLess, kOddLess>(vr[j], magic);
         };
         auto s_put = [&](int st) {
             const float mine = own_group < NG ? ldexpf(bf16_value(static_cast<uint16_t>(own)), piece < 4 ? up : up + 3) : 0.f;
@@ -1103,7 +1106,7 @@ __global__ __launch_bounds__(kPromptWaves* kWave, 1) void prompt4_kernel(const A
             if (lane < 8) {
                 // A page outside the cache, or values that are not finite, make the token's scores NaN: of the rows that see it.
                 float scale = bf16_value(static_cast<uint16_t>(vsr));
-                float rest = __builtin_fmaf(8.0f, scale, bf16_value(static_cast<uint16_t>(vmr)));
+                float rest = __builtin_fmaf(lane & 1 ? kOddLess : kEvenLess, scale, bf16_value(static_cast<uint16_t>(vmr)));
                 const bool bad = sbad || !(fabsf(rest) <= FLT_MAX);
                 if (sdead || bad) scale = rest = 0.f;
                 tok[st & 3][0][ktok] = bad ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
