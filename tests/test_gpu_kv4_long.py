@@ -39,3 +39,16 @@ def test_means_of_values_of_either_sign(total):
     got, want, _ = outputs(r, ref, table, total, 0.5)
     rms = lambda x: float(np.sqrt((x ** 2).mean()))
     assert rms(got - want) <= (2.0 ** -20 + np.sqrt(total / 8) * 2.0 ** -24) * rms(want)
+
+
+@pytest.mark.parametrize("total", [3000, 12000, 40000])
+@pytest.mark.parametrize("scale", [0.125, 0.111328125, 0.140625, 0.1015625])
+def test_equal_weights(total, scale):
+    """Queries of zeros: every key has the same weight, so that every addition to a row's sum of weights is of the same number
+    and rounds the same way. Values above zero, whose sums err by as much as they are large."""
+    r = np.random.default_rng(total)
+    table, pages = tables(r, [total], PAGE)
+    ref = random_cache(r, pages, HEADS, PAGE, DIM)
+    ref.scale[1][:], ref.low[1][:] = scale, 1.0
+    got, want, tol = outputs(r, ref, table, total, 0.0, some=8)
+    close(got, want, tol)
