@@ -13,7 +13,7 @@ namespace qk {
 namespace {
 
 // ------------------------------------------------------------------ store
-// A row of a head lies on D / 4 lanes, 4 dims each: the groups' smallest and largest values by DPP, every lane its 4 codes.
+// A row of a head lies on D / 4 lanes, 4 dims each: the groups' smallest and largest values by lane exchanges, every lane its 4 codes.
 // Keys: the row's words, one per pair of lanes. Values lie 8 tokens to a word, so a workgroup takes the pieces that begin in
 // its 8 rows (a piece: neighbouring rows with neighbouring slots of an octet of tokens; of a prompt one whole octet), hands
 // the codes over in LDS and writes an octet's words whole. A piece that fills only a part of them clears and sets its own

@@ -153,9 +153,9 @@ __device__ __forceinline__ float units_of(const Attn4Args& a, const Request4& r)
 }
 // Whether a call is light: whether split4_kernel takes its larger requests too. A unit of 8 pairs and a tile cost a CU 0.3 us
 // there, and the unit's start and end as much as 8 tiles; 128 pairs and a tile 2.2 us in prompt4_kernel, which begins and ends
-// with 20 us and has more pieces to join. (100 rows of a prompt 12 us for 33, 500 rows 33 for 46, 12 rows at 3000 keys 17 for 34, 20
-// requests of 20 rows at 500 keys 33 for 44; past it, 130 rows at 4000 keys 74 for 56, 30 of 12 rows at 2000 keys 71 for 62.) Both
-// kernels weigh a call's requests alike: sums of whole numbers, exact where they matter.
+// with 20 us and has more pieces to join. (100 rows of a prompt 7 us for 33, 11 with a table row of 200 pages, 500 rows 30 for 44, 12
+// rows at 3000 keys 15 for 33, 20 requests of 20 rows at 500 keys 36 for 47; past it, 130 rows at 4000 keys 69 for 52, 30 of 12 rows
+// at 2000 keys 76 for 66.) Both kernels weigh a call's requests alike: sums of whole numbers, exact where they matter.
 struct Weight {
     float work = 0.f, units = 0.f;
     __device__ __forceinline__ void add(const Attn4Args& a, const Request4& r) {
@@ -415,7 +415,7 @@ __device__ __forceinline__ void store_floats(float* p, const float (&x)[N]) {
 
 // ------------------------------------------------------------------ few rows
 // Bound by bytes and by vector instructions about alike: at 200000 keys the cache comes at 3.9 TB/s (5.8 more keys added to a long
-// call), and 610 instructions a tile and wave, 290 of them from codes to fp16 numbers, take 15 of the 28 us.
+// call), and 600 instructions a tile and wave, 290 of them from codes to fp16 numbers, take 15 of the 29 us.
 // A workgroup takes 8 (row, head) pairs that share a KV head - 16 columns: 8 rows x 2 fp16 parts - and a range of 32-token
 // tiles, its NW waves every NW-th tile. A wave's tiles go straight from the cache to a ring of two places in LDS (no
 // registers wait for them), the next but one requested as soon as a tile has been taken to registers: one and a half tiles,
@@ -813,15 +813,15 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
 }
 
 // ------------------------------------------------------------------ many rows
-// Bound by instruction issue: of the 4870 cycles that a wave has a tile of 32 tokens, the matrix products take 2180 and its 470
-// other vector instructions 1900. 128 rows a workgroup, 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: codes are
+// Bound by instruction issue: of the 4990 cycles that a wave has a tile of 32 tokens, the matrix products take 2180 and its 430
+// other vector instructions 1820. 128 rows a workgroup, 4 waves, one a SIMD, of 32 rows each, on v_mfma_f32_32x32x16_f16: codes are
 // turned to fp16 once per workgroup, into LDS, and an operand of keys or values, 1 KB of LDS, feeds 2 products (both parts of
 // 32 rows). A wave holds its rows' query parts (128 registers at D = 256, pinned in accumulation registers) and sums (128).
 // Its vector work - softmax, turning codes to fp16 - is laid between its own products: while tile t + 1's scores are computed,
 // tile t's are exponentiated; while tile t's values are summed, the codes of the next tiles go to LDS. All waves run all tiles
 // of the workgroup, though a wave's own rows may end one earlier: with a branch around the products the compiler moves the sums
-// between register files at each. (5000 rows: 492 us; by exponents for each 8 tokens in place of each token's 506; codes to LDS
-// beside the scores 510.)
+// between register files at each. (5000 rows by exponents for each 8 tokens in place of each token's 506 us, codes to LDS beside
+// the scores 510, where this took 492; with the roundings of `Sum` and the values' middle 500.)
 // The keys' scales are in the operand: code - 8 has at most 3 bits and a bf16 scale 8, so scale (code - 8) is an fp16 number, and
 // all dims of a head are one sum. What is left of a key, min + 8 scale of each group times the sum of its queries, is two
 // products more, of bf16 numbers (the minima, 8 scale) with the sums' three parts. A token's numbers are taken times a power of
@@ -838,8 +838,8 @@ __global__ __launch_bounds__(NW* kWave, 2) void split4_kernel(const Attn4Args a)
 //   workgroup takes its part's segments of units in turn. Of fewer than kPromptCut units, where a part is shorter than the
 //   longest piece would be;
 // - of more, a workgroup a unit, the longest first.
-// (Every unit in the same number of pieces, as many as fit: 2048 rows 144 us, now 124; 1100 rows 91, now 66; 777 behind 6000
-// keys 220, now 193. A cost of 5, 7 or 15 tiles in the line: 153, 134, 131 us where 10 takes 124.)
+// (Every unit in the same number of pieces, as many as fit: 2048 rows 144 us where this took 124; 1100 rows 91 for 66; 777 behind
+// 6000 keys 220 for 193. A cost of 5, 7 or 15 tiles in the line: 153, 134, 131 us where 10 took 124.)
 struct Line {
     int over, parts, base, more;   // steps in front of a unit; the first `more` parts have base + 1 steps, the others base
     __device__ __forceinline__ Line(int over, int steps, int most) : over(over) {
