@@ -421,11 +421,11 @@ int qwen_kv4_read_rows(const uint8_t* k_codes, const uint8_t* v_codes, const uin
                        const int32_t* slots, int rows, float* k, float* v, void* stream);
 
 /* qwen_attn_kv8_rows over this cache: arguments, rows, lengths, refusals, the workspace's use and what a bad page or a short
- * table row gives as there, with fp32 accuracy over the values min + scale * code: an error counts beside the ranges of the groups that a row sees,
- * 15 scale + |min|, times their weights, not beside each value. It holds for queries of any size whose scores are fp32 numbers
- * (times 1.45), for keys and values below 2^100, and between a token's key groups up to 2^28 apart; where all values are below 2^-40, outputs are good to 2^-66. A
- * NaN scale makes the rows that see its token NaN. Requests of few rows each that have some 2^23 rows * kv_heads together are
- * refused. */
+ * table row gives as there, with fp32 accuracy over the values min + scale * code: an error counts beside the ranges of the
+ * groups that a row sees, 15 scale + |min|, times their weights, not beside each value. It holds for queries of any size whose
+ * scores are fp32 numbers (times 1.45), for keys and values below 2^100, and between a token's key groups up to 2^28 apart;
+ * where all values are below 2^-40, outputs are good to 2^-66. A NaN scale makes the rows that see its token NaN. Requests of
+ * few rows each that have some 2^23 rows * kv_heads together are refused. */
 size_t qwen_attn_kv4_workspace_bytes(int rows, int requests, int heads, int kv_heads, int dim);
 int qwen_attn_kv4_rows(const float* q, const uint8_t* k_codes, const uint8_t* v_codes, const uint16_t* k_scale,
                        const uint16_t* k_min, const uint16_t* v_scale, const uint16_t* v_min, int pages, int page_size,

@@ -282,8 +282,8 @@ __device__ __forceinline__ bool find_piece(const Attn4Args& a, int item, Piece& 
 }
 
 // ------------------------------------------------------------------ codes and numbers
-// A word's 8 codes as the fp16 operand, the even ones less EVEN, the odd ones less ODD. `magic` is 0x64006400 from a vector register: v_and_or_b32 takes one
-// constant only, and the compiler makes two instructions of a mask and a literal.
+// A word's 8 codes as the fp16 operand, the even ones less EVEN, the odd ones less ODD. `magic` is 0x64006400 from a vector
+// register: v_and_or_b32 takes one constant only, and the compiler makes two instructions of a mask and a literal.
 __device__ __forceinline__ uint32_t code_magic() {
     uint32_t m = 0x64006400u;
     asm("" : "+v"(m));
